@@ -60,6 +60,10 @@ extern "C" {
 #define IRIS_NEXT_NORM_MODULATE 1 /* next_out = rms_norm(res) * w * (1 + scale[b]) + shift[b] */
 #define IRIS_NEXT_SILU_ADD 2      /* next_out = silu(shift[b] + res)  (timestep re-fuse)   */
 
+/* Rotary pairs (iris_rope layout) */
+#define IRIS_ROPE_INTERLEAVED 0 /* (2i, 2i + 1)                    */
+#define IRIS_ROPE_HALF 1        /* (i, i + rotary / 2)             */
+
 /* ---- library ---------------------------------------------------------- */
 const char* iris_last_error(void);
 int iris_abi_version(void);
@@ -141,6 +145,40 @@ int iris_qkv_heads(const void* qkv, int64_t batch, int64_t tokens, int64_t row_s
                    int64_t heads_kv, const float* q_weight, const float* k_weight, const float* cos, const float* sin,
                    float eps, void* q_out, void* k_out, void* v_out, int64_t n_out, int64_t n_out_kv, int64_t offset,
                    int head_major, void* stream);
+
+/* Rotary positions on their own (the text side's heads; no QK norm), in any
+ * strides: x and out hold rows [batch, heads, n, head_dim] (element strides of the
+ * first three, head_dim contiguous; out may be x). The first `rotary` columns
+ * turn by pairs (IRIS_ROPE_*) through row p of the fp32 tables [table_rows,
+ * rotary / 2], the others are copied; p = positions[b * positions_stride + t]
+ * (int32, or int64 with positions_64 != 0), or t where positions is null.
+ * inverse != 0 turns back. A position outside the table gives a NaN row and sets
+ * bit 1 of the device error word. The reference's counterpart is apply_rope,
+ * src/iris3b/nn/rope.py:92-101 (interleaved, whole head, positions in order). */
+int iris_rope(const void* x, int dtype, int64_t batch, int64_t heads, int64_t n, int64_t head_dim, int64_t x_stride_b,
+              int64_t x_stride_h, int64_t x_stride_n, void* out, int64_t out_stride_b, int64_t out_stride_h,
+              int64_t out_stride_n, const float* cos, const float* sin, int64_t rotary, int64_t table_rows,
+              const void* positions, int positions_64, int64_t positions_stride, int layout, int inverse,
+              void* stream);
+
+/* The same rotation of q and k with the append of k and v to a cache
+ * [batch, heads_kv, capacity, head_dim] of the same type, in one launch (no
+ * reference counterpart: it keeps no cache). Row t < counts[b] (all n where
+ * counts is null) of sample b is at position p = starts[b] + t; q goes to out, k
+ * (rotated) and v to slot p, or with sinks >= 0 (a rolling cache: the first
+ * `sinks` positions and the latest capacity - sinks) to slot
+ * p < sinks ? p : sinks + (p - sinks) % (capacity - sinks); of two rows of the call
+ * for one slot the later is kept. Rows from counts[b] on are left as they are. A
+ * position outside the table (NaN row, nothing appended) or past the end of a
+ * plain cache (nothing appended) sets bit 1 of the device error word. */
+int iris_rope_append(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads_q,
+                     int64_t heads_kv, int64_t n, int64_t head_dim, int64_t q_stride_b, int64_t q_stride_h,
+                     int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b,
+                     int64_t v_stride_h, int64_t v_stride_n, void* out, int64_t out_stride_b, int64_t out_stride_h,
+                     int64_t out_stride_n, void* k_cache, int64_t kc_stride_b, int64_t kc_stride_h, int64_t kc_stride_n,
+                     void* v_cache, int64_t vc_stride_b, int64_t vc_stride_h, int64_t vc_stride_n, int64_t capacity,
+                     int64_t sinks, const float* cos, const float* sin, int64_t rotary, int64_t table_rows,
+                     const int* starts, const int* counts, int layout, void* stream);
 
 /* ---- tensor-core kernels ------------------------------------------------ */
 /* F.linear in the step (src/iris_metal/model.py:46-52): C = epi(A W^T).
@@ -250,6 +288,23 @@ int iris_flash_attn_fwd_peers(const void* q, const void* k, const void* v, int64
                               float score_bound, void* const* o_peers, int world, int64_t tokens_per_rank,
                               int64_t col0, int64_t row_stride, void* stream);
 
+/* Attention with a window and first tokens that stay visible (a text side's
+ * prompts, chunks and single tokens; the reference's scaled_dot_product,
+ * src/iris3b/nn/attention.py:61-91, has no mask). Query i of sample b is at position
+ * p = starts[b] + i (null: n_kv - n + i) and sees key j < lengths[b] (null: n_kv;
+ * clamped to [0, n_kv]) where j <= p + right and (j >= p - left or j < sinks); -1 is
+ * no bound. out[b, i, h * head_dim + d] = sum_j softmax_j(scale q . k_j) v_j over the
+ * visible keys, 0 where there is none; what lies in other keys' rows, NaN
+ * included, does not reach a row. q [batch, heads_q, n, head_dim], k / v [batch,
+ * heads_kv, n_kv, head_dim], bf16 or f16, element strides of the first three
+ * dimensions (multiples of 8; 0 repeats), head_dim 64 or 128 contiguous. */
+int iris_window_attn_fwd(const void* q, const void* k, const void* v, void* out, int dtype, int64_t batch,
+                         int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv, int64_t head_dim,
+                         int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
+                         int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
+                         int64_t v_stride_n, int64_t out_stride_b, int64_t out_stride_n, const int* starts,
+                         const int* lengths, int64_t left, int64_t right, int64_t sinks, float scale, void* stream);
+
 /* ---- peer memory (sequence parallelism across processes) ---------------- */
 /* No reference counterpart. iris_ipc_export: the IPC handle (IRIS_IPC_HANDLE_BYTES)
  * of the allocation holding device pointer ptr and ptr's offset in it;
@@ -341,6 +396,17 @@ int iris_timestep_embedding(const float* t, float* out, int64_t batch, int64_t f
  * out[m, n] = act_out(sum_k act_in(x[m, k]) w[n, k] + bias[n]); act 0 = none, 1 = silu. */
 int iris_gemv(const float* x, int64_t M, int64_t K, const void* w, int w_dtype, const float* bias, float* out,
               int64_t N, int act_in, int act_out, void* stream);
+
+/* The small-M linear over 4-bit weights (iris_gemv with a quarter of the BF16
+ * weights' bytes): w[n, k] = scale[n, k / group] (q[n, k] - zero[n, k / group]), q the
+ * low (k even) or high nibble of packed[n, k / 2], scale bf16 [N, K / group], zero
+ * uint8 [N, K / group] or null (8 everywhere), group 32, 64 or 128;
+ * out[m, n] = act_out(sum_k act_in(x[m, k]) w[n, k] + bias[n]), the activations silu
+ * where asked for, bias fp32 or null. x [M, K] with row stride ldx, M <= 64; fp32
+ * sums; out [M, N] contiguous. */
+int iris_gemv_q4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const void* packed, const void* scale,
+                 const void* zero, int64_t group, const float* bias, void* out, int out_dtype, int64_t N, int silu_in,
+                 int silu_out, void* stream);
 
 /* Per-block modulation rows, SharedCoreBias.forward (src/iris3b/nn/modulation.py:284-285):
  * out[j, b, :] = core[b, :] + bias[j, :] for j < n_blocks. */

@@ -18,6 +18,7 @@ EPI_STORE, EPI_SWIGLU, EPI_GATE, EPI_HEADS, EPI_ADD, EPI_SILU = 0, 1, 2, 3, 4, 5
 HEADS_LOCAL, HEADS_PEER_SCATTER, HEADS_PEER_BROADCAST_KV = 0, 1, 2
 MAX_PEERS = 8  # IRIS_MAX_PEERS
 IPC_HANDLE_BYTES = 64
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}  # IRIS_ROPE_*
 NEXT_NONE, NEXT_NORM_MODULATE, NEXT_SILU_ADD = 0, 1, 2
 
 P, I64, I32, F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
@@ -98,6 +99,12 @@ SIGNATURES["iris_ipc_import"] = [P, ctypes.POINTER(P)]
 SIGNATURES["iris_ipc_close"] = [P]
 SIGNATURES["iris_peer_barrier"] = [P, P, I32, I32, ctypes.c_uint, I64, P]
 SIGNATURES["iris_flash_attn_fwd_split"] = [P, P, P, I64, I64, I64, I64, I64, I64, F, F, I64, P, P, P, P, I64, P]
+
+SIGNATURES["iris_rope"] = [P, I32, *[I64] * 7, P, *[I64] * 3, P, P, I64, I64, P, I32, I64, I32, I32, P]
+SIGNATURES["iris_rope_append"] = [P, P, P, I32, *[I64] * 14, P, *[I64] * 3, P, *[I64] * 3, P, *[I64] * 5, P, P, I64, I64,
+                                  P, P, I32, P]  # fmt: skip
+SIGNATURES["iris_window_attn_fwd"] = [P, P, P, P, I32, *[I64] * 17, P, P, I64, I64, I64, F, P]
+SIGNATURES["iris_gemv_q4"] = [P, I32, I64, I64, I64, P, P, P, I64, P, P, I32, I64, I32, I32, P]
 
 _lib: ctypes.CDLL | None = None
 

@@ -521,6 +521,275 @@ def flash_attention_split(
     )  # fmt: skip
 
 
+# ------------------------------------------------------------------ text side
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """Call an entry point on ``device``'s current stream, whichever device is current."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, stream)
+        return
+    with torch.cuda.device(device):
+        _lib.call(name, *args, stream)
+
+
+def _require_same(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """CUDA tensors of one device."""
+    _require(first.is_cuda, "the B200 kernels need CUDA tensors (there is no CPU path)")
+    device = first.device
+    for t in others:
+        _require(t is None or t.device == device, "tensors must be on one CUDA device")
+
+
+def _head_rows(name: str, t: torch.Tensor, batch: int, heads: int, n: int, dim: int) -> tuple[int, int, int]:
+    """Element strides of a ``[batch, heads, n, dim]`` view with contiguous head rows."""
+    _require(t.dim() == 4 and t.shape == (batch, heads, n, dim), f"{name} must be [{batch}, {heads}, {n}, {dim}]")
+    sb, sh, sn, sd = t.stride()
+    _require(sd == 1 or dim == 1, f"{name}: head rows must be contiguous")
+    return (sb if batch > 1 else 0), (sh if heads > 1 else 0), (sn if n > 1 else 0)  # a lone row's stride says nothing
+
+
+def _writable(name: str, t: torch.Tensor) -> None:
+    """No two elements in one place (an expanded output would be a race)."""
+    _require(all(st != 0 or size == 1 for st, size in zip(t.stride(), t.shape)), f"{name} must not be an expanded view")
+
+
+def _int32_rows(name: str, t: torch.Tensor | None, batch: int) -> None:
+    _require(t is None or (t.dtype == torch.int32 and t.shape == (batch,) and t.is_contiguous()),
+             f"{name} must be contiguous int32 [{batch}]")  # fmt: skip
+
+
+def _rope_table(cos: torch.Tensor, sin: torch.Tensor, dim: int, layout: str) -> int:
+    _require(layout in _lib.ROPE_LAYOUTS, f"layout must be one of {sorted(_lib.ROPE_LAYOUTS)}")
+    _require_fp32(cos=cos, sin=sin)
+    _require(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[0] > 0 and 0 < 2 * cos.shape[1] <= dim,
+             "rotary tables must be [positions, rotary / 2] with rotary <= head_dim")  # fmt: skip
+    return 2 * cos.shape[1]
+
+
+def rope(
+    x: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    positions: torch.Tensor | None = None,
+    *,
+    layout: str = "interleaved",
+    inverse: bool = False,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Rotary positions on head rows: ``x`` ``[B, H, N, D]`` (FP32, BF16 or FP16, any
+    strides with contiguous rows, e.g. a view of a packed projection) with its first
+    ``2 * cos.shape[1]`` columns turned by pairs, ``(2i, 2i + 1)`` (``"interleaved"``)
+    or ``(i, i + R / 2)`` (``"half"``), and the others copied.
+
+    ``cos``/``sin``: FP32 ``[P, R / 2]`` (:func:`iris_b200.tables.rope_table`);
+    ``positions``: int32 or int64 ``[N]`` or ``[B, N]`` rows of the tables, default ``0 ..
+    N - 1``. ``inverse`` turns back, which is also the gradient's map. ``out`` may be
+    ``x``; by default it is a new contiguous tensor. A position outside the tables
+    gives a NaN row and sets bit 1 of :func:`device_error`."""
+    _require(x.dim() == 4, "rope needs [B, H, N, D] head rows")
+    batch, heads, n, dim = x.shape
+    code = _dtype(x)
+    rotary = _rope_table(cos, sin, dim, layout)
+    strides = _head_rows("x", x, batch, heads, n, dim)
+    pos_stride = wide = 0
+    if positions is None:
+        _require(n <= cos.shape[0], "rope: the tables do not cover the rows")
+    else:
+        _require(positions.dtype in (torch.int32, torch.int64) and positions.shape in ((n,), (batch, n)),
+                 f"positions must be int32 or int64 [{n}] or [{batch}, {n}]")  # fmt: skip
+        _require(positions.stride(-1) == 1 or n <= 1, "positions must be contiguous along the rows")
+        pos_stride = positions.stride(0) if positions.dim() == 2 else 0
+        wide = int(positions.dtype == torch.int64)
+    _require_same(x, cos, sin, positions, out)
+    if out is None:
+        out = torch.empty((batch, heads, n, dim), device=x.device, dtype=x.dtype)
+    else:
+        _require(out.dtype == x.dtype, "rope: out must have the input's type")
+        _writable("out", out)
+    out_strides = _head_rows("out", out, batch, heads, n, dim)
+    _call_on(
+        x.device, "iris_rope", x.data_ptr(), code, batch, heads, n, dim, *strides, out.data_ptr(), *out_strides,
+        cos.data_ptr(), sin.data_ptr(), rotary, cos.shape[0], _ptr(positions), wide, pos_stride,
+        _lib.ROPE_LAYOUTS[layout], int(inverse),
+    )  # fmt: skip
+    return out
+
+
+def rope_append(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    starts: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    *,
+    sinks: int | None = None,
+    counts: torch.Tensor | None = None,
+    layout: str = "interleaved",
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Rotate ``q`` (returned) and append rotated ``k`` and ``v`` to a cache, in one launch.
+
+    ``q`` ``[B, H, N, D]``, ``k``/``v`` ``[B, H_kv, N, D]`` in any strides with
+    contiguous rows; ``k_cache``/``v_cache`` ``[B, H_kv, C, D]`` of the same type, updated
+    in place. Row ``t < counts[b]`` (int32 ``[B]``; default: every row) of sample ``b``
+    is at position ``starts[b] + t`` (``starts``: int32 ``[B]``). ``sinks=None``: position
+    ``p`` goes to slot ``p``. With ``sinks`` the cache rolls: it keeps the first ``sinks``
+    positions and the latest ``C - sinks``, so that all of its first
+    ``min(positions, C)`` slots are visible to the next token
+    (``window_attention(q, k_cache, v_cache, lengths=positions, right=None)``). Rows from
+    ``counts[b]`` on are not touched (zeros in a new ``out``). A position outside the
+    tables (NaN row, not appended) or past a plain cache (not appended) sets bit 1 of
+    :func:`device_error`. ``layout`` and the tables as for :func:`rope`."""
+    _require(q.dim() == 4 and k.dim() == 4 and k_cache.dim() == 4, "rope_append needs [B, H, N, D] head rows")
+    batch, heads, n, dim = q.shape
+    kv_heads, capacity = k.shape[1], k_cache.shape[2]
+    code = _dtype(q)
+    rotary = _rope_table(cos, sin, dim, layout)
+    _require(all(t.dtype == q.dtype for t in (k, v, k_cache, v_cache)), "rope_append: one type for rows and cache")
+    rows = [_head_rows("q", q, batch, heads, n, dim), _head_rows("k", k, batch, kv_heads, n, dim),
+            _head_rows("v", v, batch, kv_heads, n, dim)]  # fmt: skip
+    caches = [_head_rows(name, t, batch, kv_heads, capacity, dim) for name, t in (("k_cache", k_cache), ("v_cache", v_cache))]
+    _writable("k_cache", k_cache)
+    _writable("v_cache", v_cache)
+    _require(sinks is None or 0 <= sinks < capacity, "rope_append: a rolling cache needs more slots than sinks")
+    _int32_rows("starts", starts, batch)
+    _int32_rows("counts", counts, batch)
+    _require_same(q, k, v, cos, sin, starts, k_cache, v_cache, counts, out)
+    if out is None:
+        new = torch.empty if counts is None else torch.zeros
+        out = new((batch, heads, n, dim), device=q.device, dtype=q.dtype)
+    else:
+        _require(out.dtype == q.dtype, "rope_append: out must have the input's type")
+        _writable("out", out)
+    out_strides = _head_rows("out", out, batch, heads, n, dim)
+    _call_on(
+        q.device, "iris_rope_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, batch, heads, kv_heads, n, dim,
+        *rows[0], *rows[1], *rows[2], out.data_ptr(), *out_strides, k_cache.data_ptr(), *caches[0], v_cache.data_ptr(),
+        *caches[1], capacity, -1 if sinks is None else sinks, cos.data_ptr(), sin.data_ptr(), rotary, cos.shape[0],
+        starts.data_ptr(), _ptr(counts), _lib.ROPE_LAYOUTS[layout],
+    )  # fmt: skip
+    return out
+
+
+def window_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    left: int | None = None,
+    right: int | None = 0,
+    sinks: int = 0,
+    starts: torch.Tensor | None = None,
+    lengths: torch.Tensor | None = None,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``softmax(q k^T * scale) v`` over a window of the keys, for prompts, chunks and
+    single tokens: ``q`` ``[B, H, N, D]``, ``k``/``v`` ``[B, H_kv, N_kv, D]`` (BF16 or FP16,
+    ``D`` 64 or 128, any strides of multiples of 8 elements with contiguous rows);
+    returns ``[B, N, H * D]`` (``out``, or a new tensor).
+
+    Query ``i`` of sample ``b`` is at position ``p = starts[b] + i`` (int32 ``[B]``;
+    default ``N_kv - N + i``) and sees the keys ``j < lengths[b]`` (int32 ``[B]``, clamped
+    to ``[0, N_kv]``; default ``N_kv``) with ``j <= p + right`` and ``j >= p - left`` or ``j <
+    sinks``; ``None`` is no bound, the default is causal. A query that sees no key
+    gives 0. Other keys' rows may hold anything."""
+    _require(q.dim() == 4 and k.dim() == 4, "window_attention: q [B, H, N, D], k/v [B, H_kv, N_kv, D]")
+    batch, heads, n, dim = q.shape
+    kv_heads, n_kv = k.shape[1], k.shape[2]
+    _require(q.dtype in (torch.bfloat16, torch.float16) and q.dtype == k.dtype == v.dtype,
+             "window_attention: q, k and v in one of bf16, f16")  # fmt: skip
+    _require(dim in (64, 128), "window_attention: head_dim must be 64 or 128")
+    rows = [_head_rows("q", q, batch, heads, n, dim), _head_rows("k", k, batch, kv_heads, n_kv, dim),
+            _head_rows("v", v, batch, kv_heads, n_kv, dim)]  # fmt: skip
+    _require(all(bound is None or bound >= 0 for bound in (left, right)) and sinks >= 0,
+             "window_attention: left, right and sinks must not be negative")  # fmt: skip
+    _int32_rows("starts", starts, batch)
+    _int32_rows("lengths", lengths, batch)
+    _require_same(q, k, v, starts, lengths, out)
+    if out is None:
+        out = torch.empty((batch, n, heads * dim), device=q.device, dtype=q.dtype)
+    else:
+        _require(out.shape == (batch, n, heads * dim) and out.dtype == q.dtype and out.stride(2) == 1,
+                 f"window_attention: out must be [{batch}, {n}, {heads * dim}] rows of the input's type")  # fmt: skip
+        _writable("out", out)
+    _call_on(
+        q.device, "iris_window_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _dtype(q), batch,
+        heads, kv_heads, n, n_kv, dim, *rows[0], *rows[1], *rows[2], out.stride(0) if batch > 1 else 0,
+        out.stride(1) if n > 1 else 0, _ptr(starts), _ptr(lengths), -1 if left is None else left, -1 if right is None else right, sinks,
+        float(scale if scale is not None else dim**-0.5),
+    )  # fmt: skip
+    return out
+
+
+def pack_q4(
+    w: torch.Tensor, group: int = 64, symmetric: bool = True
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """Weights ``[N, K]`` to 4 bits for :func:`gemv_q4`, once: ``(packed, scale, zero)``,
+    uint8 ``[N, K / 2]`` (low nibble first), BF16 ``[N, K / group]`` and uint8 ``[N, K /
+    group]`` (``None`` when ``symmetric``: 8 everywhere). Each value goes to the nearest
+    level of its group, spaced by the BF16 scale that is kept: largest magnitude
+    over 7, or the group's range (0 included) over 15 from a whole zero point."""
+    _require(w.dim() == 2 and group in (32, 64, 128) and w.shape[1] % group == 0 and w.shape[1] > 0,
+             "pack_q4 needs [N, K] weights, K a multiple of the group (32, 64 or 128)")  # fmt: skip
+    g = w.float().reshape(w.shape[0], -1, group)
+    if symmetric:
+        step, zero = g.abs().amax(dim=-1) / 7, None
+    else:
+        lo, hi = g.amin(dim=-1).clamp_max(0), g.amax(dim=-1).clamp_min(0)
+        step = (hi - lo) / 15
+    scale = step.to(torch.bfloat16)
+    s = torch.where(scale == 0, 1.0, scale.float())
+    if not symmetric:
+        zero = (-lo / s).round().clamp(0, 15).to(torch.uint8)
+    q = ((g / s[..., None]).round() + (8.0 if zero is None else zero[..., None].float())).clamp(0, 15).to(torch.uint8)
+    q = q.reshape(w.shape)
+    return (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous(), scale.contiguous(), zero
+
+
+def gemv_q4(
+    x: torch.Tensor,
+    packed: torch.Tensor,
+    scale: torch.Tensor,
+    zero: torch.Tensor | None = None,
+    bias: torch.Tensor | None = None,
+    *,
+    silu_in: bool = False,
+    silu_out: bool = False,
+    out_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """``act(act(x) @ w.T + bias)`` for 1 to 64 rows ``x`` ``[M, K]`` (FP32, BF16 or FP16; the
+    row stride may exceed ``K``) and 4-bit weights from :func:`pack_q4`, with FP32 sums;
+    ``silu_in`` / ``silu_out`` turn the activations on, ``bias``: FP32 ``[N]``. The result
+    is ``[M, N]`` of ``out_dtype`` (default: the input's)."""
+    _require(x.dim() == 2 and packed.dim() == 2, "gemv_q4 needs x [M, K] and packed weights [N, K / 2]")
+    m, inner = x.shape
+    n = packed.shape[0]
+    _require(packed.dtype == torch.uint8 and packed.is_contiguous() and packed.shape[1] * 2 == inner,
+             "gemv_q4: packed must be contiguous uint8 [N, K / 2]")  # fmt: skip
+    _require(scale.dtype == torch.bfloat16 and scale.is_contiguous() and scale.dim() == 2 and scale.shape[0] == n
+             and scale.shape[1] > 0 and inner % scale.shape[1] == 0, "gemv_q4: scale must be contiguous bf16 [N, K / group]")  # fmt: skip
+    _require(zero is None or (zero.dtype == torch.uint8 and zero.is_contiguous() and zero.shape == scale.shape),
+             "gemv_q4: zero must be contiguous uint8 [N, K / group]")  # fmt: skip
+    _require(x.stride(1) == 1, "gemv_q4: x rows must be contiguous")
+    if bias is not None:
+        _require_fp32(bias=bias)
+        _require(bias.shape == (n,), "gemv_q4: bias width")
+    _require_same(x, packed, scale, zero, bias)
+    out_dtype = out_dtype or x.dtype
+    code, out_code = _dtype(x), _dtype(out_dtype)
+    out = torch.empty((m, n), device=x.device, dtype=out_dtype)
+    _call_on(
+        x.device, "iris_gemv_q4", x.data_ptr(), code, m, inner, x.stride(0) if m > 1 else inner, packed.data_ptr(),
+        scale.data_ptr(), _ptr(zero), inner // scale.shape[1], _ptr(bias), out.data_ptr(), out_code, n, int(silu_in),
+        int(silu_out),
+    )  # fmt: skip
+    return out
+
+
 def block_copy(
     dst: torch.Tensor,
     dst_strides: tuple[int, int, int],

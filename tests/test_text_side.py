@@ -1,0 +1,207 @@
+"""The text-side operators without a GPU: refusals (all before any launch), the
+scaled rotary tables and the 4-bit packing."""
+
+import math
+
+import pytest
+import torch
+
+from text_side import unpacked
+from test_library import _einval, lib  # noqa: F401 (lib: the built library)
+
+
+@pytest.fixture(scope="module")
+def K():
+    from iris_b200 import kernels
+
+    return kernels
+
+
+def test_c_entries_refuse_bad_arguments(lib):  # noqa: F811
+    def rope(dtype=1, batch=1, heads=2, n=3, dim=64, rotary=64, rows=9, layout=0, x=16):
+        return ("iris_rope", x, dtype, batch, heads, n, dim, 0, 0, 0, 16, 0, 0, 0, 16, 16, rotary, rows, None, 0, 0, layout,
+                0, None)  # fmt: skip
+
+    for bad, message in [(dict(dtype=3), "dtype"), (dict(dim=63), "even"), (dict(rotary=66), "rotated columns"),
+                         (dict(rotary=0), "rotated columns"), (dict(rows=0), "table"), (dict(layout=2), "layout"),
+                         (dict(x=None), "null"), (dict(n=1 << 31), "row counts"), (dict(heads=0), "row counts")]:  # fmt: skip
+        assert message in _einval(lib, *rope(**bad)), bad
+
+    def append(kv=1, capacity=8, sinks=-1, starts=16):
+        return ("iris_rope_append", 16, 16, 16, 1, 1, 2, kv, 3, 64, *[0] * 9, 16, 0, 0, 0, 16, 0, 0, 0, 16, 0, 0, 0, capacity,
+                sinks, 16, 16, 64, 9, starts, None, 0, None)  # fmt: skip
+
+    for bad, message in [(dict(kv=0), "head counts"), (dict(capacity=0), "slots"), (dict(sinks=8), "slots"),
+                         (dict(sinks=-2), "slots"), (dict(starts=None), "null")]:  # fmt: skip
+        assert message in _einval(lib, *append(**bad)), bad
+
+    def attend(q=16, dtype=1, batch=1, heads=4, kv=2, n=3, m=5, dim=128, qn=128, left=-1, right=0, sinks=0, scale=0.1):
+        return ("iris_window_attn_fwd", q, 16, 16, 16, dtype, batch, heads, kv, n, m, dim, 0, 0, qn, *[0] * 8, None, None,
+                left, right, sinks, scale, None)  # fmt: skip
+
+    for bad, message in [(dict(dtype=0), "bf16 or f16"), (dict(heads=3), "multiple of heads_kv"), (dict(dim=80), "head_dim"),
+                         (dict(qn=12), "16 bytes"), (dict(q=8), "16 bytes"), (dict(left=-2), "bounds"), (dict(right=-2), "bounds"),
+                         (dict(sinks=-1), "bounds"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
+                         (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"), (dict(m=1 << 30), "sizes"),
+                         (dict(batch=65536), "sizes"), (dict(q=None), "null")]:  # fmt: skip
+        assert message in _einval(lib, *attend(**bad)), bad
+
+    def q4(x=16, dtype=1, m=1, k=128, ldx=128, group=32, n=4, out=16, out_dtype=1):
+        return ("iris_gemv_q4", x, dtype, m, k, ldx, 16, 16, None, group, None, out, out_dtype, n, 0, 0, None)
+
+    for bad, message in [(dict(group=16), "groups"), (dict(m=0), "1 to 64"), (dict(m=65), "1 to 64"), (dict(k=96, group=64), "multiple"),
+                         (dict(ldx=120), "size"), (dict(n=0), "1 to 64"), (dict(x=8), "aligned"), (dict(ldx=132), "aligned"),
+                         (dict(dtype=3), "dtype"), (dict(out_dtype=-1), "dtype"), (dict(out=None), "null")]:  # fmt: skip
+        assert message in _einval(lib, *q4(**bad)), bad
+
+
+def test_wrappers_refuse_before_any_launch(K):
+    x = torch.zeros(2, 4, 3, 64)
+    cos = sin = torch.zeros(9, 32)
+    with pytest.raises(ValueError, match="CUDA"):
+        K.rope(x, cos, sin)
+    for args, kw, message in [
+        ((x[0], cos, sin), {}, "head rows"),
+        ((x, cos.half(), sin), {}, "FP32"),
+        ((x, torch.zeros(9, 33), torch.zeros(9, 33)), {}, "tables"),
+        ((x, cos, torch.zeros(9, 31)), {}, "tables"),
+        ((x, torch.zeros(2, 32), torch.zeros(2, 32)), {}, "cover"),
+        ((x, cos, sin, torch.zeros(4, dtype=torch.int64)), {}, "positions"),
+        ((x, cos, sin, torch.zeros(3)), {}, "positions"),
+        ((x, cos, sin, torch.zeros(6, dtype=torch.int32)[::2]), {}, "positions"),
+        ((x.double(), cos, sin), {}, "dtype"),
+        ((torch.zeros(2, 4, 3, 128)[..., ::2], cos, sin), {}, "contiguous"),
+        ((x, cos, sin), {"layout": "both"}, "layout"),
+    ]:
+        with pytest.raises(ValueError, match=message):
+            K.rope(*args, **kw)
+    q, k, cache = torch.zeros(2, 4, 3, 64), torch.zeros(2, 2, 3, 64), torch.zeros(2, 2, 8, 64)
+    starts = torch.zeros(2, dtype=torch.int32)
+    good = dict(q=q, k=k, v=k, cos=cos, sin=sin, starts=starts, k_cache=cache, v_cache=cache.clone())
+    with pytest.raises(ValueError, match="CUDA"):
+        K.rope_append(**good)
+    for bad, message in [
+        (dict(k=k.half()), "one type"), (dict(v=k[:, :1]), "v must be"), (dict(starts=starts.long()), "starts"),
+        (dict(starts=starts[:1]), "starts"), (dict(counts=starts.long()), "counts"), (dict(sinks=8), "rolling"),
+        (dict(sinks=-1), "rolling"), (dict(k_cache=cache[:1].expand(2, 2, 8, 64)), "expanded"),
+        (dict(v_cache=cache[:, :, :7]), "v_cache must be"), (dict(out=q.half()), "CUDA"),
+    ]:  # fmt: skip
+        with pytest.raises(ValueError, match=message):
+            K.rope_append(**{**good, **bad})
+    q, k = q.bfloat16(), k.bfloat16()
+    with pytest.raises(ValueError, match="CUDA"):
+        K.window_attention(q, k, k)
+    for args, kw, message in [
+        ((q.float(), k.float(), k.float()), {}, "bf16, f16"),
+        ((q, k, k.half()), {}, "bf16, f16"),
+        ((q[..., :48], k[..., :48], k[..., :48]), {}, "head_dim"),
+        ((q, k, k[:, :, :2]), {}, "v must be"),
+        ((q, k, k), {"left": -1}, "negative"),
+        ((q, k, k), {"right": -3}, "negative"),
+        ((q, k, k), {"sinks": -1}, "negative"),
+        ((q, k, k), {"lengths": torch.zeros(3, dtype=torch.int32)}, "lengths"),
+        ((q, k, k), {"starts": torch.zeros(2)}, "starts"),
+    ]:
+        with pytest.raises(ValueError, match=message):
+            K.window_attention(*args, **kw)
+    packed, scale, zero = K.pack_q4(torch.randn(6, 128), 32, symmetric=False)
+    x = torch.zeros(2, 128)
+    with pytest.raises(ValueError, match="CUDA"):
+        K.gemv_q4(x, packed, scale, zero)
+    for args, message in [
+        ((x[:, :64], packed, scale, zero), "packed"), ((x, packed.int(), scale, zero), "packed"),
+        ((x, packed, scale.float(), zero), "scale"), ((x, packed, scale[:5], None), "scale"),
+        ((x, packed, scale, zero[:, :2]), "zero"), ((x, packed, scale, zero, torch.zeros(5)), "bias"),
+        ((x, packed, scale, zero, torch.zeros(6).half()), "FP32"), ((x.t(), packed, scale, zero), "packed"),
+    ]:  # fmt: skip
+        with pytest.raises(ValueError, match=message):
+            K.gemv_q4(*args)
+    for w, group in [(torch.zeros(4, 100), 32), (torch.zeros(4, 128), 16), (torch.zeros(128), 32)]:
+        with pytest.raises(ValueError, match="pack_q4"):
+            K.pack_q4(w, group)
+
+
+def test_calls_go_to_the_tensors_device(K, monkeypatch):
+    """On another device than the current one: that device's stream, with it made current for the call."""
+    from iris_b200 import _lib
+
+    seen = []
+
+    class Stream:
+        def __init__(self, device):
+            self.cuda_stream = 100 + device.index
+
+    class Device:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            seen.append(("enter", self.device.index))
+
+        def __exit__(self, *a):
+            seen.append(("exit", self.device.index))
+
+    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: seen.append((name, args)))
+    K._call_on(torch.device("cuda", 0), "entry", 7)
+    K._call_on(torch.device("cuda", 1), "entry", 8)
+    assert seen == [("entry", (7, 100)), ("enter", 1), ("entry", (8, 101)), ("exit", 1)]
+
+
+def test_rope_table_matches_its_formulas():
+    from iris_b200.tables import rope_table
+
+    r, length, theta = 64, 5000, 10000.0
+    p = torch.arange(length, dtype=torch.float64)[:, None]
+    plain = theta ** (-torch.arange(0, r, 2, dtype=torch.float64) / r)
+
+    def same(got, angles, magnitude=1.0):
+        # one rounding to fp32 of a value of at most `magnitude`, and 64-bit angles of up to 5000 (2^-40 at most)
+        for table, exact in zip(got, (angles.cos(), angles.sin())):
+            assert table.dtype == torch.float32 and table.is_contiguous() and table.shape == (length, r // 2)
+            assert torch.all((table.double() - magnitude * exact).abs() <= magnitude * (2.0**-24 + 2.0**-38))
+
+    same(rope_table(r, length, theta), p * plain)
+    same(rope_table(r, length, theta, scaling="linear", factor=8.0), p * plain / 8)
+    ntk = rope_table(r, length, theta, scaling="ntk", factor=8.0)
+    same(ntk, p * (theta * 8.0 ** (r / (r - 2))) ** (-torch.arange(0, r, 2, dtype=torch.float64) / r))
+    stretched = (theta * 8.0 ** (r / (r - 2))) ** (-torch.arange(0, r, 2, dtype=torch.float64) / r)
+    assert stretched[0] == plain[0] and math.isclose(stretched[-1], plain[-1] / 8, rel_tol=1e-12)
+    got = rope_table(r, length, theta, scaling="ramp", factor=4.0, trained_length=1024)
+    magnitude = 0.1 * math.log(4.0) + 1
+    turns = 1024 * plain / (2 * math.pi)
+    # the pairs beyond either end of the ramp: kept, or divided
+    kept, divided = turns > 33 * 1.4, turns < 1 / 1.4
+    assert kept.any() and divided.any()
+    for where, freqs in ((kept, plain), (divided, plain / 4)):
+        angles = p * freqs
+        for table, exact in zip(got, (angles.cos(), angles.sin())):
+            assert torch.all((table.double() - magnitude * exact)[:, where].abs() <= magnitude * (2.0**-24 + 2.0**-38))
+    # between the ends the angle of position 1 falls from one to the other, pair by pair
+    first = (torch.atan2(got[1], got[0])[1]).double() / plain
+    assert torch.all(first[1:] <= first[:-1] + 2e-6) and torch.all((first > 0.25 - 1e-6) & (first < 1 + 1e-6))
+    for bad in (dict(rotary=63), dict(rotary=0), dict(length=0), dict(theta=1.0), dict(factor=0.5, scaling="linear"),
+                dict(factor=2.0), dict(scaling="other"), dict(scaling="ramp", factor=2.0), dict(rotary=2, scaling="ntk")):  # fmt: skip
+        with pytest.raises(ValueError):
+            rope_table(**{"rotary": r, "length": length, **bad})
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_pack_q4_takes_the_nearest_level(K, group, symmetric):
+    gen = torch.Generator().manual_seed(group)
+    w = torch.randn(5, 3 * group, generator=gen)
+    w[1, :group] = 0  # an empty group
+    w[2] = w[2].abs() + 0.5  # one sign
+    w[3, 0] = 40.0  # an outlier
+    packed, scale, zero = K.pack_q4(w, group, symmetric)
+    assert packed.dtype == torch.uint8 and packed.shape == (5, 3 * group // 2) and scale.dtype == torch.bfloat16
+    assert (zero is None) == symmetric
+    back = unpacked(packed, scale, zero).float()
+    step = scale.float().repeat_interleave(group, dim=1)
+    # half a level; at the range's ends the bf16 scale may fall short by 2^-8 of up to 15 levels, and a whole zero point
+    # is up to half a level off
+    assert torch.all((back - w).abs() <= step * (0.5 + 15 * 2.0**-8 + (0 if symmetric else 0.5)) + 1e-6)
+    assert torch.all(back[1, :group] == 0)
