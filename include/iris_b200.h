@@ -297,7 +297,8 @@ int iris_flash_attn_fwd_peers(const void* q, const void* k, const void* v, int64
  * visible keys, 0 where there is none; what lies in other keys' rows, NaN
  * included, does not reach a row. q [batch, heads_q, n, head_dim], k / v [batch,
  * heads_kv, n_kv, head_dim], bf16 or f16, element strides of the first three
- * dimensions (multiples of 8; 0 repeats), head_dim 64 or 128 contiguous. */
+ * dimensions (multiples of 8; 0 repeats a head or a sample), head_dim 64 or 128
+ * contiguous. */
 int iris_window_attn_fwd(const void* q, const void* k, const void* v, void* out, int dtype, int64_t batch,
                          int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv, int64_t head_dim,
                          int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,

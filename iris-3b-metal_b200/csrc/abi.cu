@@ -78,6 +78,25 @@ int make_tmap_3d_bf16(CUtensorMap* map, const void* base, int64_t d0, int64_t d1
   return IRIS_OK;
 }
 
+int make_tmap_heads(CUtensorMap* map, const void* base, int dtype, int64_t head_dim, int64_t tokens, int64_t heads,
+                    int64_t batch, int64_t stride_n, int64_t stride_h, int64_t stride_b, int box_rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return set_error(IRIS_ECUDA, "cuTensorMapEncodeTiled is unavailable (driver too old?)");
+  const int64_t sizes[3] = {tokens, heads, batch}, steps[3] = {stride_n, stride_h, stride_b};
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), 1, 1, 1}, strides[3];
+  for (int i = 0; i < 3; ++i) {
+    if (steps[i] != 0) dims[i + 1] = static_cast<cuuint64_t>(sizes[i]);
+    strides[i] = static_cast<cuuint64_t>((steps[i] != 0 ? steps[i] : head_dim) * 2);  // a single entry's is not used
+  }
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
+  cuuint32_t elem[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, dtype == IRIS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                  const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(IRIS_ECUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return IRIS_OK;
+}
+
 }  // namespace iris
 
 extern "C" const char* iris_last_error(void) { return iris::g_message; }

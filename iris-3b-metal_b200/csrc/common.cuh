@@ -162,6 +162,15 @@ IRIS_DEVICE void tma_load_3d(const CUtensorMap* map, uint64_t* bar, void* dst, i
       : "memory");
 }
 
+IRIS_DEVICE void tma_load_4d(const CUtensorMap* map, uint64_t* bar, void* dst, int32_t c0, int32_t c1, int32_t c2,
+                             int32_t c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_addr(bar))
+      : "memory");
+}
+
 IRIS_DEVICE void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }

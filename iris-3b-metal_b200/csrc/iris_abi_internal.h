@@ -26,6 +26,13 @@ int make_tmap_2d_bf16(CUtensorMap* map, const void* base, int64_t inner, int64_t
 int make_tmap_3d_bf16(CUtensorMap* map, const void* base, int64_t d0, int64_t d1, int64_t d2, int64_t stride1_elems,
                       int64_t stride2_elems, int box0, int box1, int box2);
 
+// 4-D map (head columns, tokens, heads, batch) of 2-byte elements (dtype
+// IRIS_BF16 or IRIS_F16) with 128-byte swizzle and boxes of 64 columns x box_rows
+// tokens; element strides. A stride of 0 (heads, batch) maps one entry: its
+// coordinate must be 0.
+int make_tmap_heads(CUtensorMap* map, const void* base, int dtype, int64_t head_dim, int64_t tokens, int64_t heads,
+                    int64_t batch, int64_t stride_n, int64_t stride_h, int64_t stride_b, int box_rows);
+
 }  // namespace iris
 
 #define IRIS_REQUIRE(cond, msg)                           \

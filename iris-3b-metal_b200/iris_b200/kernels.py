@@ -696,7 +696,8 @@ def window_attention(
     default ``N_kv - N + i``) and sees the keys ``j < lengths[b]`` (int32 ``[B]``, clamped
     to ``[0, N_kv]``; default ``N_kv``) with ``j <= p + right`` and ``j >= p - left`` or ``j <
     sinks``; ``None`` is no bound, the default is causal. A query that sees no key
-    gives 0. Other keys' rows may hold anything."""
+    gives 0. Other keys' rows may hold anything. Heads and samples may be expanded,
+    tokens not."""
     _require(q.dim() == 4 and k.dim() == 4, "window_attention: q [B, H, N, D], k/v [B, H_kv, N_kv, D]")
     batch, heads, n, dim = q.shape
     kv_heads, n_kv = k.shape[1], k.shape[2]

@@ -36,14 +36,14 @@ def test_c_entries_refuse_bad_arguments(lib):  # noqa: F811
         assert message in _einval(lib, *append(**bad)), bad
 
     def attend(q=16, dtype=1, batch=1, heads=4, kv=2, n=3, m=5, dim=128, qn=128, left=-1, right=0, sinks=0, scale=0.1):
-        return ("iris_window_attn_fwd", q, 16, 16, 16, dtype, batch, heads, kv, n, m, dim, 0, 0, qn, *[0] * 8, None, None,
+        return ("iris_window_attn_fwd", q, 16, 16, 16, dtype, batch, heads, kv, n, m, dim, 0, 0, qn, 0, 0, 128, 0, 0, 128, 0, 0, None, None,
                 left, right, sinks, scale, None)  # fmt: skip
 
     for bad, message in [(dict(dtype=0), "bf16 or f16"), (dict(heads=3), "multiple of heads_kv"), (dict(dim=80), "head_dim"),
                          (dict(qn=12), "16 bytes"), (dict(q=8), "16 bytes"), (dict(left=-2), "bounds"), (dict(right=-2), "bounds"),
                          (dict(sinks=-1), "bounds"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
                          (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"), (dict(m=1 << 30), "sizes"),
-                         (dict(batch=65536), "sizes"), (dict(q=None), "null")]:  # fmt: skip
+                         (dict(batch=65536), "sizes"), (dict(qn=0), "repeat"), (dict(q=None), "null")]:  # fmt: skip
         assert message in _einval(lib, *attend(**bad)), bad
 
     def q4(x=16, dtype=1, m=1, k=128, ldx=128, group=32, n=4, out=16, out_dtype=1):

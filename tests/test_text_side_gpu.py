@@ -319,9 +319,8 @@ def test_window_attention_strides(K, n):
     kk, vv = k.expand(2, 2, 300, dim), v.transpose(0, 1)[None].expand(2, 2, 300, dim)
     got = K.window_attention(q, kk, vv, right=None)
     assert torch.equal(got, K.window_attention(q, kk.contiguous(), vv.contiguous(), right=None))
-    one = v[:1].transpose(0, 1)[None].expand(2, 2, 300, dim)  # one row repeated along the keys
-    got = K.window_attention(q, kk, one, right=None)
-    assert torch.equal(got, K.window_attention(q, kk.contiguous(), one.contiguous(), right=None))
+    with pytest.raises(ValueError, match="repeat"):
+        K.window_attention(q, kk, v[:1].transpose(0, 1)[None].expand(2, 2, 300, dim), right=None)
     wide = normal(4, 2, n, 4 * dim + 24, dtype=dtype)
     before = wide.clone()
     K.window_attention(q, kk, vv, right=None, out=wide[..., 8 : 8 + 4 * dim])
