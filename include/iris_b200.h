@@ -304,7 +304,14 @@ int iris_window_attn_fwd(const void* q, const void* k, const void* v, void* out,
                          int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
                          int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
                          int64_t v_stride_n, int64_t out_stride_b, int64_t out_stride_n, const int* starts,
-                         const int* lengths, int64_t left, int64_t right, int64_t sinks, float scale, void* stream);
+                         const int* lengths, int64_t left, int64_t right, int64_t sinks, float scale, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace (16-byte aligned; null for 0) that iris_window_attn_fwd needs for
+ * these sizes: a few rows' keys are split over CTAs and the parts joined there. Two
+ * calls that may run at the same time need one each. */
+int iris_window_attn_workspace(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv,
+                               int64_t head_dim, int64_t left, int64_t right, int64_t sinks, int64_t* bytes);
 
 /* ---- peer memory (sequence parallelism across processes) ---------------- */
 /* No reference counterpart. iris_ipc_export: the IPC handle (IRIS_IPC_HANDLE_BYTES)

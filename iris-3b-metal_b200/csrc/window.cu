@@ -127,23 +127,6 @@ __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, fl
     acc[c] = count == 0 ? make_float2(0.f, 0.f) : l == 0.f ? make_float2(NAN, NAN) : make_float2(acc[c].x * inv, acc[c].y * inv);
 }
 
-constexpr int ROW_WARPS = 8;
-
-template <typename T, int D>
-__global__ void __launch_bounds__(ROW_WARPS * 32) rows_kernel(const __grid_constant__ Params p) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROW_WARPS + (threadIdx.x >> 5);
-  const int64_t per_sample = static_cast<int64_t>(p.heads_q) * p.n;
-  if (row >= p.batch * per_sample) return;
-  const int b = static_cast<int>(row / per_sample);
-  const int64_t rest = row - b * per_sample;
-  const int i = static_cast<int>(rest / p.heads_q), h = static_cast<int>(rest - static_cast<int64_t>(i) * p.heads_q);
-  float2 acc[D / 64];
-  attend_row<T, D>(p, b, h, i, acc);
-  T* o = reinterpret_cast<T*>(p.out) + b * p.ob + i * p.on + static_cast<int64_t>(h) * D + 2 * (threadIdx.x & 31);
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c) *reinterpret_cast<uint32_t*>(o + 64 * c) = pack2<T>(acc[c].x, acc[c].y);
-}
-
 // ------------------------------------------------------------- tensor cores
 // Prompts and chunks: the pipeline of attention.cu (TMA warp, MMA warp, eight
 // softmax warps per 128-row query tile, two tiles per CTA sharing the K / V blocks
@@ -618,14 +601,399 @@ int launch_tiles(Params p, int dtype, cudaStream_t st) {
   return IRIS_OK;
 }
 
+// ------------------------------------------------- few rows over many keys
+// Single tokens and short chunks: the keys are split over CTAs and the parts joined.
+// A CTA takes 16 query rows (the tokens' query heads of one key head, so K and V are
+// read once for all of them) and a chunk of the keys that some of them sees; its
+// warps walk 16-key tiles of their own, each with its own softmax state and its own
+// ring of cp.async copies (no barrier until the end), scores and P V on mma.sync
+// m16n8k16: HBM-bound, one K and V byte is used for 16 rows at most, which leaves the
+// 5th-generation tensor cores' 128-row tiles seven eighths empty. Chunks are the same
+// length for every sample, so samples of different lengths give equal work; a second
+// kernel joins the chunks of a row (programmatic launch: its start overlaps).
+constexpr int STEP_WARPS = 4, STEP_STAGES = 3, STEP_KEYS = 16, STEP_ROWS = 16;
+
+struct Split {
+  int row_tiles;  // 16-row tiles of a key head's query rows
+  int chunk;      // keys per CTA
+  int splits;     // chunks of the longest list
+  float* parts;   // [batch, heads_kv, row_tiles, splits, 16, D] sums, then [.., 16] maxima and totals; null: one chunk
+};
+
+template <typename T>
+IRIS_DEVICE void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (IsHalf<T>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+IRIS_DEVICE void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+IRIS_DEVICE void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 bytes global -> shared, or 16 zero bytes
+IRIS_DEVICE void copy16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+
+template <int D>
+constexpr int step_smem() {
+  return STEP_WARPS * STEP_STAGES * 2 * STEP_KEYS * D * 2;
+}
+
+// Writes row (b, h, i), columns [64 c + 2 lane, + 2); rows that are not finite again
+// from visible keys alone (a masked key's V may be NaN or infinite: 0 times it is NaN).
 template <typename T, int D>
-int launch(const Params& p, int dtype, cudaStream_t st) {
-  if (p.n > 16 && p.n_kv > 0) return launch_tiles<T, D>(p, dtype, st);
+IRIS_DEVICE void finish_row(const Params& p, int b, int h, int i, float2 (&acc)[D / 64], float total) {
+  const float inv = 1.f / total;
+  bool finite = true;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    acc[c] = make_float2(acc[c].x * inv, acc[c].y * inv);
+    finite = finite && isfinite(acc[c].x) && isfinite(acc[c].y);
+  }
+  if (!__all_sync(0xffffffffu, finite)) attend_row<T, D>(p, b, h, i, acc);
+  T* o = reinterpret_cast<T*>(p.out) + b * p.ob + i * p.on + static_cast<int64_t>(h) * D + 2 * (threadIdx.x & 31);
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) *reinterpret_cast<uint32_t*>(o + 64 * c) = pack2<T>(acc[c].x, acc[c].y);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_constant__ Params p,
+                                                               const __grid_constant__ Split sp) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  constexpr int TILE = STEP_KEYS * D * 2;  // bytes of one K or V tile
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (sp.parts) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int split = static_cast<int>(blockIdx.x % sp.splits);
+  const int unit = static_cast<int>(blockIdx.x / sp.splits);  // (b, hk, row tile)
+  const int rt = unit % sp.row_tiles, hk = unit / sp.row_tiles % p.heads_kv, b = unit / sp.row_tiles / p.heads_kv;
+  const int group = p.heads_q / p.heads_kv;
+  const int rows = p.n * group;  // of this key head: row r is token r / group, head hk * group + r % group
+  const int r0 = rt * STEP_ROWS, r_last = min(r0 + STEP_ROWS, rows) - 1;
+  const int length = sample_length(p, b);
+  const int64_t start = sample_start(p, b);
+  // keys that some row of the tile sees: [0, early) and [lo, hi)
+  const Span first = visible(p, start + r0 / group, length), last = visible(p, start + r_last / group, length);
+  Span all = last;
+  all.lo = first.lo;
+  all.early = min(last.early, first.lo);
+  const bool same = r0 / group == r_last / group;  // one token: every row sees all of them
+  const int count = all.early + max(0, all.hi - all.lo);
+  const int c_begin = min(split * sp.chunk, count), c_end = min(c_begin + sp.chunk, count);
+
+  const T* k = reinterpret_cast<const T*>(p.k) + b * p.kb + hk * p.kh;
+  const T* v = reinterpret_cast<const T*>(p.v) + b * p.vb + hk * p.vh;
+  const uint32_t ring = smem_addr(smem_raw) + warp * (STEP_STAGES * 2 * TILE);
+  const int tiles = (c_end - c_begin + STEP_KEYS - 1) / STEP_KEYS;
+  const int mine = tiles > warp ? (tiles - warp + STEP_WARPS - 1) / STEP_WARPS : 0;
+  // tile t of the warp into its slot: rows of D / 8 16-byte pieces, piece x of row r at x ^ (r & 7)
+  constexpr int PIECES = D / 8;
+  auto load = [&](int t) {
+    if (t < mine) {
+      const int c0 = c_begin + (warp + t * STEP_WARPS) * STEP_KEYS;
+      const uint32_t slot = ring + (t % STEP_STAGES) * 2 * TILE;
+#pragma unroll
+      for (int e = 0; e < STEP_KEYS * PIECES / 32; ++e) {
+        const int at = e * 32 + lane, r = at / PIECES, x = at % PIECES;
+        const bool real = c0 + r < c_end;
+        const int64_t key = real ? all.key(c0 + r) : 0;
+        const uint32_t dst = slot + r * (D * 2) + ((x ^ (r & 7)) * 16);
+        copy16(dst, k + (real ? key * p.kn + x * 8 : 0), real);
+        copy16(dst + TILE, v + (real ? key * p.vn + x * 8 : 0), real);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int t = 0; t < STEP_STAGES - 1; ++t) load(t);
+
+  // Q rows as the A operand: this lane's rows g and g + 8, columns 2 (lane % 4) + {0, 1} of each 8
+  const int g = lane >> 2, quad = lane & 3;
+  uint32_t qa[D / 16][4];
+  Span seen[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int r = r0 + g + 8 * u;
+    const int i = min(r, rows - 1) / group, h = hk * group + min(r, rows - 1) % group;
+    seen[u] = visible(p, start + i, length);
+    const T* q = reinterpret_cast<const T*>(p.q) + b * p.qb + h * p.qh + static_cast<int64_t>(i) * p.qn + 2 * quad;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      qa[d][u] = *reinterpret_cast<const uint32_t*>(q + 16 * d);
+      qa[d][u + 2] = *reinterpret_cast<const uint32_t*>(q + 16 * d + 8);
+    }
+  }
+  float o[D / 8][4];
+#pragma unroll
+  for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+
+  for (int t = 0; t < mine; ++t) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STEP_STAGES - 2) : "memory");
+    __syncwarp();  // every lane's copies of the tile have landed; the slot refilled next was read by all
+    load(t + STEP_STAGES - 1);
+    const uint32_t slot = ring + (t % STEP_STAGES) * 2 * TILE;
+    const int c0 = c_begin + (warp + t * STEP_WARPS) * STEP_KEYS;
+    // S: keys [8 j, 8 j + 8) in s[j]
+    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) {  // two k steps per load: pieces 4 d .. 4 d + 3 of the 8 key rows
+        uint32_t kb[4];
+        const int r = 8 * j + (lane & 7), x = 4 * d + (lane >> 3);
+        ldmatrix4(kb, slot + r * (D * 2) + ((x ^ (r & 7)) * 16));
+        mma_16816<T>(s[j], qa[2 * d], kb[0], kb[1]);
+        mma_16816<T>(s[j], qa[2 * d + 1], kb[2], kb[3]);
+      }
+    }
+    if (!same || c0 + STEP_KEYS > c_end) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = c0 + 8 * j + 2 * quad + (e & 1);
+          const Span& w = seen[e >> 1];
+          const int key = all.key(c);
+          if (c >= c_end || key >= w.hi || (key < w.lo && key >= p.sinks)) s[j][e] = -INFINITY;
+        }
+    }
+    bool rescale = false;
+    float corr[2], shift[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float mx = fmaxf(fmaxf(s[0][2 * u], s[0][2 * u + 1]), fmaxf(s[1][2 * u], s[1][2 * u + 1])) * p.scale_log2;
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const bool grow = mx > m_run[u] + RESCALE;
+      const float m_new = grow ? mx : m_run[u];
+      corr[u] = grow && m_run[u] != -INFINITY ? ex2(m_run[u] - m_new) : 1.f;
+      rescale = rescale || corr[u] != 1.f;
+      m_run[u] = m_new;
+      shift[u] = m_new == -INFINITY ? 0.f : -m_new;
+    }
+    if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] *= corr[e >> 1];
+      l_run[0] *= corr[0];
+      l_run[1] *= corr[1];
+    }
+    // weights, rounded once to the operand type (the fp32 values go into the totals)
+    uint32_t pa[4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float w0 = ex2(fmaf(s[j][2 * u], p.scale_log2, shift[u]));
+        const float w1 = ex2(fmaf(s[j][2 * u + 1], p.scale_log2, shift[u]));
+        l_run[u] += w0 + w1;
+        pa[2 * j + u] = pack2<T>(w0, w1);
+      }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {  // 16 columns per load: key rows 0-7 and 8-15, pieces 2 d and 2 d + 1
+      uint32_t vb[4];
+      const int r = lane & 15, x = 2 * d + (lane >> 4);
+      ldmatrix4_trans(vb, slot + TILE + r * (D * 2) + ((x ^ (r & 7)) * 16));
+      mma_16816<T>(o[2 * d], pa, vb[0], vb[1]);
+      mma_16816<T>(o[2 * d + 1], pa, vb[2], vb[3]);
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    l_run[u] += __shfl_xor_sync(0xffffffffu, l_run[u], 1);
+    l_run[u] += __shfl_xor_sync(0xffffffffu, l_run[u], 2);
+  }
+  // the warps' states, joined per row: warp w finishes rows w, w + 4, ...
+  __syncthreads();  // the rings are done with
+  float* sums = reinterpret_cast<float*>(smem_raw);  // [warp][16][D]
+  __shared__ float tops[STEP_WARPS][STEP_ROWS], totals[STEP_WARPS][STEP_ROWS];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    float* dst = sums + (warp * STEP_ROWS + g + 8 * u) * D + 2 * quad;
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(dst + 8 * d) = make_float2(o[d][2 * u], o[d][2 * u + 1]);
+    if (quad == 0) {
+      tops[warp][g + 8 * u] = m_run[u];
+      totals[warp][g + 8 * u] = l_run[u];
+    }
+  }
+  __syncthreads();
+  for (int r = warp; r <= r_last - r0; r += STEP_WARPS) {
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < STEP_WARPS; ++w) top = fmaxf(top, tops[w][r]);
+    float2 acc[D / 64];
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < STEP_WARPS; ++w) {
+      // a warp that saw nothing has sums of 0 (or NaN, from a masked V: kept, it marks the row)
+      const float f = tops[w][r] == -INFINITY ? 1.f : ex2(tops[w][r] - top);
+      total += f * totals[w][r];
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        const float2 x = *reinterpret_cast<const float2*>(sums + (w * STEP_ROWS + r) * D + 64 * c + 2 * lane);
+        acc[c] = make_float2(fmaf(f, x.x, acc[c].x), fmaf(f, x.y, acc[c].y));
+      }
+    }
+    if (sp.parts == nullptr) {
+      finish_row<T, D>(p, b, hk * group + (r0 + r) % group, (r0 + r) / group, acc, total);
+    } else {
+      const int64_t part = (static_cast<int64_t>(unit) * sp.splits + split) * STEP_ROWS + r;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) *reinterpret_cast<float2*>(sp.parts + part * D + 64 * c + 2 * lane) = acc[c];
+      if (lane == 0) {
+        const int64_t all_rows = static_cast<int64_t>(p.batch) * p.heads_kv * sp.row_tiles * sp.splits * STEP_ROWS;
+        float2* state = reinterpret_cast<float2*>(sp.parts + all_rows * D);
+        state[part] = make_float2(top, total);
+      }
+    }
+  }
+}
+
+// One row's chunks joined by a block: its warps take every fourth chunk.
+template <typename T, int D>
+__global__ void __launch_bounds__(STEP_WARPS * 32) join_kernel(const __grid_constant__ Params p,
+                                                               const __grid_constant__ Split sp) {
+  __shared__ float2 sums[STEP_WARPS][D / 2];
+  __shared__ float totals[STEP_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = p.heads_q / p.heads_kv, rows = p.n * group;
+  const int unit_rows = static_cast<int>(blockIdx.x) / rows;  // (b, hk)
+  const int row = static_cast<int>(blockIdx.x) - unit_rows * rows;
+  const int64_t unit = static_cast<int64_t>(unit_rows) * sp.row_tiles + row / STEP_ROWS;
+  const int64_t part0 = unit * sp.splits * STEP_ROWS + row % STEP_ROWS;
+  const int64_t all_rows = static_cast<int64_t>(p.batch) * p.heads_kv * sp.row_tiles * sp.splits * STEP_ROWS;
+  const float2* state = reinterpret_cast<const float2*>(sp.parts + all_rows * D);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float top = -INFINITY;
+  for (int c = lane; c < sp.splits; c += 32) top = fmaxf(top, state[part0 + c * STEP_ROWS].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float total = 0.f;
+  float2 acc[D / 64];
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int c = warp; c < sp.splits; c += STEP_WARPS) {
+    const int64_t part = part0 + static_cast<int64_t>(c) * STEP_ROWS;
+    const float2 st = state[part];
+    const float f = st.x == -INFINITY ? 1.f : ex2(st.x - top);
+    total = fmaf(f, st.y, total);
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d) {
+      const float2 x = *reinterpret_cast<const float2*>(sp.parts + part * D + 64 * d + 2 * lane);
+      acc[d] = make_float2(fmaf(f, x.x, acc[d].x), fmaf(f, x.y, acc[d].y));
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < D / 64; ++d) sums[warp][32 * d + lane] = acc[d];
+  if (lane == 0) totals[warp] = total;
+  __syncthreads();
+  if (warp != 0) return;
+#pragma unroll
+  for (int w = 1; w < STEP_WARPS; ++w) {
+    total += totals[w];
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d) {
+      const float2 x = sums[w][32 * d + lane];
+      acc[d] = make_float2(acc[d].x + x.x, acc[d].y + x.y);
+    }
+  }
+  const int b = unit_rows / p.heads_kv, hk = unit_rows % p.heads_kv;
+  finish_row<T, D>(p, b, hk * group + row % group, row / group, acc, total);
+}
+
+// Few rows per key head leave a 128-row tile mostly empty, and few CTAs: split the keys instead.
+bool few_rows(int64_t n, int64_t group) { return n * group <= 64; }
+
+// Chunks of a call: a bound on the keys that a row tile sees, and pieces of at least
+// one tile per warp, about STEP_WAVES rounds of two CTAs per SM in all.
+constexpr int64_t STEP_WAVES = 6;
+
+void split_keys(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv, int64_t left, int64_t right,
+                int64_t sinks, Split* sp) {
+  int64_t span = n_kv;
+  if (left < kNoBound && right < kNoBound && left + right + n + sinks < n_kv) span = left + right + n + sinks;
+  const int64_t row_tiles = (n * (heads_q / heads_kv) + STEP_ROWS - 1) / STEP_ROWS;
+  const int64_t units = batch * heads_kv * row_tiles;
+  constexpr int64_t unit = STEP_WARPS * STEP_KEYS;
+  int64_t chunk = span * units / (num_sms() * 2 * STEP_WAVES);
+  chunk = (chunk + unit - 1) / unit * unit;
+  if (chunk < unit) chunk = unit;
+  sp->row_tiles = static_cast<int>(row_tiles);
+  sp->chunk = static_cast<int>(chunk);
+  sp->splits = static_cast<int>(span > chunk ? (span + chunk - 1) / chunk : 1);
+}
+
+template <typename T, int D>
+int launch_step(const Params& p, float* parts, int64_t parts_bytes, cudaStream_t st) {
+  Split sp = {};
+  split_keys(p.batch, p.heads_q, p.heads_kv, p.n, p.n_kv, p.left, p.right, p.sinks, &sp);
+  const int64_t units = static_cast<int64_t>(p.batch) * p.heads_kv * sp.row_tiles;
   const int64_t rows = static_cast<int64_t>(p.batch) * p.heads_q * p.n;
-  const int64_t blocks = (rows + ROW_WARPS - 1) / ROW_WARPS;
-  IRIS_REQUIRE(blocks < (1ll << 31), "window_attn_fwd: too many rows");
-  rows_kernel<T, D><<<static_cast<unsigned>(blocks), ROW_WARPS * 32, 0, st>>>(p);
+  IRIS_REQUIRE(units * sp.splits < (1ll << 31) && rows < (1ll << 31), "window_attn_fwd: too many rows");
+  if (sp.splits > 1) {
+    IRIS_REQUIRE(parts != nullptr && aligned16(parts) && parts_bytes >= units * sp.splits * STEP_ROWS * (D + 2) * 4,
+                 "window_attn_fwd: workspace too small");
+    sp.parts = parts;
+  }
+  auto kernel = step_kernel<T, D>;
+  static bool configured[64] = {false};
+  int dev = 0;
+  IRIS_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !configured[dev]) {
+    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, step_smem<D>()));
+    if (dev < 64) configured[dev] = true;
+  }
+  kernel<<<static_cast<unsigned>(units * sp.splits), STEP_WARPS * 32, step_smem<D>(), st>>>(p, sp);
   IRIS_CUDA(cudaGetLastError());
+  if (sp.parts == nullptr) return IRIS_OK;
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(rows));
+  config.blockDim = dim3(STEP_WARPS * 32);
+  config.stream = st;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  IRIS_CUDA(cudaLaunchKernelEx(&config, join_kernel<T, D>, p, sp));
+  return IRIS_OK;
+}
+
+template <typename T, int D>
+int launch(const Params& p, int dtype, void* workspace, int64_t workspace_bytes, cudaStream_t st) {
+  if (few_rows(p.n, p.heads_q / p.heads_kv) || p.n_kv == 0)
+    return launch_step<T, D>(p, static_cast<float*>(workspace), workspace_bytes, st);
+  return launch_tiles<T, D>(p, dtype, st);
+}
+
+inline int64_t bound(int64_t v) { return v < 0 || v > kNoBound ? kNoBound : v; }
+
+inline int check_sizes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv, int64_t head_dim,
+                       int64_t left, int64_t right, int64_t sinks) {
+  IRIS_REQUIRE(head_dim == 64 || head_dim == 128, "window_attn_fwd: head_dim must be 64 or 128");
+  IRIS_REQUIRE(heads_q > 0 && heads_kv > 0 && heads_q % heads_kv == 0,
+               "window_attn_fwd: heads_q must be a positive multiple of heads_kv");
+  IRIS_REQUIRE(batch >= 0 && n >= 0 && n_kv >= 0 && batch <= 65535 && heads_q <= 65535 && n < (1ll << 30) &&
+                   n_kv < (1ll << 30),
+               "window_attn_fwd: sizes");
+  IRIS_REQUIRE(left >= -1 && right >= -1 && sinks >= 0, "window_attn_fwd: window bounds are -1 (none) or more");
   return IRIS_OK;
 }
 
@@ -634,22 +1002,29 @@ int launch(const Params& p, int dtype, cudaStream_t st) {
 
 using namespace iris;
 
+extern "C" int iris_window_attn_workspace(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv,
+                                          int64_t head_dim, int64_t left, int64_t right, int64_t sinks, int64_t* bytes) {
+  using namespace iris::window;
+  IRIS_REQUIRE(bytes != nullptr, "window_attn_workspace: null output");
+  IRIS_CHECK_STATUS(check_sizes(batch, heads_q, heads_kv, n, n_kv, head_dim, left, right, sinks));
+  *bytes = 0;
+  if (batch * n == 0 || n_kv == 0 || !few_rows(n, heads_q / heads_kv)) return IRIS_OK;
+  Split sp = {};
+  split_keys(batch, heads_q, heads_kv, n, n_kv, bound(left), bound(right), sinks < n_kv ? sinks : n_kv, &sp);
+  if (sp.splits > 1) *bytes = batch * heads_kv * sp.row_tiles * sp.splits * STEP_ROWS * (head_dim + 2) * 4;
+  return IRIS_OK;
+}
+
 extern "C" int iris_window_attn_fwd(const void* q, const void* k, const void* v, void* out, int dtype, int64_t batch,
                                     int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv, int64_t head_dim,
                                     int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
                                     int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
                                     int64_t v_stride_n, int64_t out_stride_b, int64_t out_stride_n, const int* starts,
                                     const int* lengths, int64_t left, int64_t right, int64_t sinks, float scale,
-                                    void* stream) {
+                                    void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace iris::window;
   IRIS_REQUIRE(dtype == IRIS_BF16 || dtype == IRIS_F16, "window_attn_fwd: bf16 or f16");
-  IRIS_REQUIRE(head_dim == 64 || head_dim == 128, "window_attn_fwd: head_dim must be 64 or 128");
-  IRIS_REQUIRE(heads_q > 0 && heads_kv > 0 && heads_q % heads_kv == 0,
-               "window_attn_fwd: heads_q must be a positive multiple of heads_kv");
-  IRIS_REQUIRE(batch >= 0 && n >= 0 && n_kv >= 0 && batch <= 65535 && heads_q <= 65535 && n < (1ll << 30) &&
-                   n_kv < (1ll << 30),
-               "window_attn_fwd: sizes");
-  IRIS_REQUIRE(left >= -1 && right >= -1 && sinks >= 0, "window_attn_fwd: window bounds are -1 (none) or more");
+  IRIS_CHECK_STATUS(check_sizes(batch, heads_q, heads_kv, n, n_kv, head_dim, left, right, sinks));
   IRIS_REQUIRE(scale > 0.f && scale < INFINITY, "window_attn_fwd: scale must be positive and finite");
   IRIS_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && q_stride_b % 8 == 0 &&
                    q_stride_h % 8 == 0 && q_stride_n % 8 == 0 && k_stride_b % 8 == 0 && k_stride_h % 8 == 0 &&
@@ -670,12 +1045,11 @@ extern "C" int iris_window_attn_fwd(const void* q, const void* k, const void* v,
   p.batch = static_cast<int>(batch), p.heads_q = static_cast<int>(heads_q), p.heads_kv = static_cast<int>(heads_kv);
   p.n = static_cast<int>(n), p.n_kv = static_cast<int>(n_kv);
   p.starts = starts, p.lengths = lengths;
-  p.left = left < 0 || left > kNoBound ? kNoBound : left;
-  p.right = right < 0 || right > kNoBound ? kNoBound : right;
+  p.left = bound(left), p.right = bound(right);
   p.sinks = static_cast<int>(sinks < n_kv ? sinks : n_kv);
   p.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == IRIS_BF16)
-    return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, dtype, st) : launch<__nv_bfloat16, 64>(p, dtype, st);
-  return head_dim == 128 ? launch<__half, 128>(p, dtype, st) : launch<__half, 64>(p, dtype, st);
+    return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, dtype, workspace, workspace_bytes, st) : launch<__nv_bfloat16, 64>(p, dtype, workspace, workspace_bytes, st);
+  return head_dim == 128 ? launch<__half, 128>(p, dtype, workspace, workspace_bytes, st) : launch<__half, 64>(p, dtype, workspace, workspace_bytes, st);
 }

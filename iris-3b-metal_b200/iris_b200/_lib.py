@@ -103,7 +103,8 @@ SIGNATURES["iris_flash_attn_fwd_split"] = [P, P, P, I64, I64, I64, I64, I64, I64
 SIGNATURES["iris_rope"] = [P, I32, *[I64] * 7, P, *[I64] * 3, P, P, I64, I64, P, I32, I64, I32, I32, P]
 SIGNATURES["iris_rope_append"] = [P, P, P, I32, *[I64] * 14, P, *[I64] * 3, P, *[I64] * 3, P, *[I64] * 5, P, P, I64, I64,
                                   P, P, I32, P]  # fmt: skip
-SIGNATURES["iris_window_attn_fwd"] = [P, P, P, P, I32, *[I64] * 17, P, P, I64, I64, I64, F, P]
+SIGNATURES["iris_window_attn_fwd"] = [P, P, P, P, I32, *[I64] * 17, P, P, I64, I64, I64, F, P, I64, P]
+SIGNATURES["iris_window_attn_workspace"] = [*[I64] * 9, ctypes.POINTER(I64)]
 SIGNATURES["iris_gemv_q4"] = [P, I32, I64, I64, I64, P, P, P, I64, P, P, I32, I64, I32, I32, P]
 
 _lib: ctypes.CDLL | None = None
@@ -133,7 +134,7 @@ def load() -> ctypes.CDLL:
 _launches = 0
 # kernels each entry point enqueues (1 unless listed)
 _KERNELS_PER_CALL = {"iris_device_error": 0, "iris_all_finite": 2, "iris_ipc_export": 0, "iris_ipc_import": 0,
-                     "iris_ipc_close": 0}
+                     "iris_ipc_close": 0, "iris_window_attn_workspace": 0}
 
 
 def launch_count() -> int:

@@ -20,6 +20,7 @@ engine (``gemm``, ``flash_attention``, ...) follow the same rules.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -674,6 +675,14 @@ def rope_append(
     return out
 
 
+@functools.lru_cache(maxsize=4096)
+def _window_workspace(device: int, *sizes: int) -> int:
+    """Bytes that ``iris_window_attn_fwd`` needs for these sizes on the current device (``device``)."""
+    need = ctypes.c_int64(0)
+    _lib.call("iris_window_attn_workspace", *sizes, ctypes.byref(need))
+    return int(need.value)
+
+
 def window_attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -717,12 +726,17 @@ def window_attention(
         _require(out.shape == (batch, n, heads * dim) and out.dtype == q.dtype and out.stride(2) == 1,
                  f"window_attention: out must be [{batch}, {n}, {heads * dim}] rows of the input's type")  # fmt: skip
         _writable("out", out)
+    left, right = -1 if left is None else left, -1 if right is None else right
+    sizes = (batch, heads, kv_heads, n, n_kv, dim, left, right, sinks)
+    need = _window_workspace(q.device.index, *sizes)
+    workspace = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
     _call_on(
         q.device, "iris_window_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _dtype(q), batch,
         heads, kv_heads, n, n_kv, dim, *rows[0], *rows[1], *rows[2], out.stride(0) if batch > 1 else 0,
-        out.stride(1) if n > 1 else 0, _ptr(starts), _ptr(lengths), -1 if left is None else left, -1 if right is None else right, sinks,
-        float(scale if scale is not None else dim**-0.5),
+        out.stride(1) if n > 1 else 0, _ptr(starts), _ptr(lengths), left, right, sinks, float(scale if scale is not None else dim**-0.5), _ptr(workspace), need,
     )  # fmt: skip
+    if need:
+        _lib.count_launches(1)  # the join of the parts
     return out
 
 

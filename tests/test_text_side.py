@@ -37,7 +37,7 @@ def test_c_entries_refuse_bad_arguments(lib):  # noqa: F811
 
     def attend(q=16, dtype=1, batch=1, heads=4, kv=2, n=3, m=5, dim=128, qn=128, left=-1, right=0, sinks=0, scale=0.1):
         return ("iris_window_attn_fwd", q, 16, 16, 16, dtype, batch, heads, kv, n, m, dim, 0, 0, qn, 0, 0, 128, 0, 0, 128, 0, 0, None, None,
-                left, right, sinks, scale, None)  # fmt: skip
+                left, right, sinks, scale, None, 0, None)  # fmt: skip
 
     for bad, message in [(dict(dtype=0), "bf16 or f16"), (dict(heads=3), "multiple of heads_kv"), (dict(dim=80), "head_dim"),
                          (dict(qn=12), "16 bytes"), (dict(q=8), "16 bytes"), (dict(left=-2), "bounds"), (dict(right=-2), "bounds"),
