@@ -78,6 +78,21 @@ int make_tmap_3d_bf16(CUtensorMap* map, const void* base, int64_t d0, int64_t d1
   return IRIS_OK;
 }
 
+int make_tmap_2d_bytes(CUtensorMap* map, const void* base, int64_t inner, int64_t outer, int64_t row_bytes,
+                       int box_inner, int box_outer) {
+  auto fn = encode_fn();
+  if (fn == nullptr) return set_error(IRIS_ECUDA, "cuTensorMapEncodeTiled is unavailable (driver too old?)");
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer)};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(IRIS_ECUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return IRIS_OK;
+}
+
 int make_tmap_heads(CUtensorMap* map, const void* base, int dtype, int64_t head_dim, int64_t tokens, int64_t heads,
                     int64_t batch, int64_t stride_n, int64_t stride_h, int64_t stride_b, int box_rows) {
   auto fn = encode_fn();

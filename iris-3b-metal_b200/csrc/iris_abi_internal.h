@@ -26,6 +26,10 @@ int make_tmap_2d_bf16(CUtensorMap* map, const void* base, int64_t inner, int64_t
 int make_tmap_3d_bf16(CUtensorMap* map, const void* base, int64_t d0, int64_t d1, int64_t d2, int64_t stride1_elems,
                       int64_t stride2_elems, int box0, int box1, int box2);
 
+// 2-D map of bytes with 128-byte swizzle (row_bytes a multiple of 16).
+int make_tmap_2d_bytes(CUtensorMap* map, const void* base, int64_t inner, int64_t outer, int64_t row_bytes,
+                       int box_inner, int box_outer);
+
 // 4-D map (head columns, tokens, heads, batch) of 2-byte elements (dtype
 // IRIS_BF16 or IRIS_F16) with 128-byte swizzle and boxes of 64 columns x box_rows
 // tokens; element strides. A stride of 0 (heads, batch) maps one entry: its

@@ -16,10 +16,10 @@
 //  - x in 16 bits goes in as it is. FP32 (and act_in's results) go in as three bf16
 //    columns, 8 bits each of the 24, cut off rather than rounded: their sum is x, and
 //    the columns are free up to 8 of them.
-// A CTA owns 32 weight rows and, in a cluster, one part of K; its warps take 128-wide
-// pieces of K in turn, each through its own ring of cp.async copies, which is filled
-// before x is laid out. Sums are joined in shared memory (over the cluster's CTAs
-// through distributed shared memory) in a fixed order.
+// A CTA owns 32 weight rows and, in a cluster, one part of K; its warps take 256-wide
+// pieces of K in turn, each through its own ring of TMA copies (one instruction for 32
+// rows; filled before x is laid out). Sums are joined in shared memory (over the
+// cluster's CTAs through distributed shared memory) in a fixed order.
 #include "common.cuh"
 #include "iris_abi_internal.h"
 
@@ -27,11 +27,12 @@ namespace iris {
 namespace q4 {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int STAGES = 4;
+constexpr int STAGES = 2;                    // ring slots of a warp; two to four CTAs share an SM
 constexpr int TILES = 2, ROWS = 16 * TILES;  // weight rows of a CTA
-constexpr int STEP = 128;                    // k of one ring slot: 64 bytes of each row
+constexpr int STEP = 256;                    // k of one ring slot: 128 bytes of each row
 constexpr int SLOT = ROWS * STEP / 2;        // bytes
 constexpr int ROUND = STEP * WARPS;          // k of one round of the warps
+constexpr int MOST_PARTS = 8;                // CTAs of a cluster
 
 struct Params {
   const void* x;
@@ -54,55 +55,86 @@ struct Params {
 
 IRIS_DEVICE float silu(float v) { return v / (1.f + __expf(-v)); }
 
+// (v & mask) | bits in one instruction
+IRIS_DEVICE uint32_t put(uint32_t v, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(v), "r"(mask), "r"(bits));
+  return d;
+}
+
+// Weights of two nibbles as the operand type, and the products. unpack<I>: nibbles I
+// and I + 4 of word w, less their zero, as a pair; less(z): what a group's zero is kept as.
 template <typename T>
-struct Magic;
+struct Operand;
 template <>
-struct Magic<__nv_bfloat16> {
-  static constexpr uint32_t kOne = 0x43004300u;  // 128, 128
-  IRIS_DEVICE static uint32_t sub(uint32_t a, uint32_t b) {
-    __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+struct Operand<__nv_bfloat16> {
+  static constexpr uint32_t kOne = 0x43004300u;  // 128: the mantissa's last bit is 1
+  using Less = uint32_t;
+  IRIS_DEVICE static Less less(uint32_t z) { return z * 0x00010001u | kOne; }
+  template <int I>
+  IRIS_DEVICE static uint32_t unpack(uint32_t w, Less z) {
+    uint32_t a = put(w >> (4 * I), 0x000f000fu, kOne);
+    __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&z));
     return *reinterpret_cast<uint32_t*>(&r);
   }
   IRIS_DEVICE static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 template <>
-struct Magic<__half> {
-  static constexpr uint32_t kOne = 0x64006400u;  // 1024, 1024
-  IRIS_DEVICE static uint32_t sub(uint32_t a, uint32_t b) {
-    __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+struct Operand<__half> {
+  static constexpr uint32_t kOne = 0x64006400u;  // 1024
+  struct Less {
+    uint32_t low, high;  // 1024 + z; -(64 + z)
+  };
+  IRIS_DEVICE static Less less(uint32_t z) { return Less{z * 0x00010001u | kOne, z * 0x00100010u | 0xd400d400u}; }
+  template <int I>
+  IRIS_DEVICE static uint32_t unpack(uint32_t w, Less z) {
+    __half2 r;
+    if constexpr (I % 2 == 0) {
+      uint32_t a = put(w >> (4 * I), 0x000f000fu, kOne);
+      r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&z.low));
+    } else {  // four bits up: 1024 + 16 q, a sixteenth of it less 64 + z (both exact), without a shift of its own
+      uint32_t a = put(w >> (4 * (I - 1)), 0x00f000f0u, kOne);
+      const uint32_t sixteenth = 0x2c002c00u;
+      r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<const __half2*>(&sixteenth), *reinterpret_cast<__half2*>(&z.high));
+    }
     return *reinterpret_cast<uint32_t*>(&r);
   }
   IRIS_DEVICE static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 
 // x as three bf16 values whose sum it is: the top 8 bits of its mantissa, the next 8,
 // the rest. Infinities and NaN go into the first alone.
-IRIS_DEVICE void split3(float v, uint16_t (&t)[3]) {
+IRIS_DEVICE void split3(float v, uint32_t (&t)[3]) {
   const bool finite = isfinite(v);
   const uint32_t top = __float_as_uint(v) & 0xffff0000u;
-  t[0] = isnan(v) ? 0x7fc0u : static_cast<uint16_t>(top >> 16);
+  t[0] = isnan(v) ? 0x7fc0u : top >> 16;
   const float rest = finite ? v - __uint_as_float(top) : 0.f;
   const uint32_t mid = __float_as_uint(rest) & 0xffff0000u;
-  t[1] = static_cast<uint16_t>(mid >> 16);
-  t[2] = static_cast<uint16_t>(__float_as_uint(rest - __uint_as_float(mid)) >> 16);
+  t[1] = mid >> 16;
+  t[2] = __float_as_uint(rest - __uint_as_float(mid)) >> 16;
 }
 
-// Where 16-byte piece `piece` of row `row` lies in a slot's 64-byte row: rows two apart
-// take turned pieces, so that 4-, 8- and 16-byte reads of 8 rows meet no bank twice.
-IRIS_DEVICE int swizzle(int row, int piece) { return piece ^ ((row >> 2 & 1) | (row & 2)); }
+// The weight row that a lane's row index g of the mma stands for: with the copy's
+// 128-byte swizzle (16-byte piece x of row r at x ^ (r % 8)) the 4-, 8- or 16-byte reads
+// of lanes that read together then meet no bank twice.
+IRIS_DEVICE int weight_row(int g) { return (g & 1) << 2 | (g & 2) | g >> 2; }
 
 // COLS8: groups of 8 columns of the mma (rows of x times TERMS); G: weights per scale.
 template <typename T, int TERMS, int COLS8, int G>
-__global__ void __launch_bounds__(THREADS) gemv_q4_kernel(const __grid_constant__ Params p) {
-  extern __shared__ __align__(128) uint8_t smem_raw[];
+__global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(const __grid_constant__ CUtensorMap tw,
+                                                          const __grid_constant__ Params p) {
+  extern __shared__ __align__(1024) uint8_t smem_unaligned[];
+  __shared__ uint64_t full[WARPS][STAGES];
+  __shared__ int abort_flag;
+  uint8_t* smem_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, quad = lane & 3;
   const int n0 = static_cast<int>(blockIdx.x / p.parts) * ROWS;
@@ -112,95 +144,125 @@ __global__ void __launch_bounds__(THREADS) gemv_q4_kernel(const __grid_constant_
   const int k0 = part * p.part_k, k1 = min(k0 + p.part_k, p.K);
   const int groups = p.K / G;
   const int rounds = k1 > k0 ? (k1 - k0 + ROUND - 1) / ROUND : 0;
-  constexpr int PER = STEP / G;  // groups per step
-  constexpr int WORDS = G / 32;  // words of a group per lane of a row
+  constexpr int PER = STEP / G;   // groups per step
+  constexpr int WORDS = G / 32;   // words of a group per lane of a row
+  constexpr int HELD = (PER + 3) / 4;  // a step's scales and zeros that a lane holds for each of its rows
 
-  const uint32_t ring = smem_addr(smem_raw) + warp * (STAGES * SLOT);
-  uint8_t* ring_ptr = smem_raw + warp * (STAGES * SLOT);
+  uint8_t* ring = smem_raw + warp * (STAGES * SLOT);
   uint8_t* xs = smem_raw + WARPS * STAGES * SLOT;  // [chunk_k / 32][cols][32] in the order of use
+  volatile int* abort = &abort_flag;
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < WARPS; ++w)
+      for (int u = 0; u < STAGES; ++u) mbar_init(&full[w][u], 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
 
-  // this lane's share of a step's scales and zeros: group `quad` of rows g, g + 8, g + 16, g + 24
-  uint32_t sz[STAGES][2 * TILES];
-  auto load = [&](int t, int u) {  // round t into slot u
+  auto load = [&](int t) {  // round t into its slot
     const int k = k0 + t * ROUND + warp * STEP;
-    if (t < rounds && k < k1) {
+    if (lane == 0 && t < rounds && k < k1) {
+      uint64_t* bar = &full[warp][t % STAGES];
+      mbar_arrive_expect_tx(bar, SLOT);
+      tma_load_2d(&tw, bar, ring + t % STAGES * SLOT, k / 2, n0);  // rows from N on and k from K on: zeros
+    }
+  };
+  for (int t = 0; t < STAGES; ++t) load(t);
+
+  // lane (g, quad) holds groups quad, quad + 4 of a step, of rows weight_row(g) + 0, 8, 16, 24: scale above zero;
+  // fetched a round ahead
+  const int row_g = weight_row(g);
+  const int64_t meta0 = static_cast<int64_t>(n0 + row_g) * groups + quad;
+  uint32_t sz[2 * TILES][HELD];
+  auto fetch = [&](int t) {
+    const int k = k0 + t * ROUND + warp * STEP;
 #pragma unroll
-      for (int e = 0; e < ROWS * 4 / 32; ++e) {
-        const int row = e * 8 + g, n = n0 + row;
-        const bool real = n < p.N && k + quad * 32 < p.K;
-        const uint8_t* src = p.packed + (real ? (static_cast<int64_t>(n) * p.K + k) / 2 + quad * 16 : 0);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ring + u * SLOT + row * 64 +
-                                                                           swizzle(row, quad) * 16),
-                     "l"(src), "r"(real ? 16 : 0)
-                     : "memory");
-      }
+    for (int h = 0; h < HELD; ++h) {
+      const int grp = k / G + 4 * h;  // + quad
+      const bool real = t < rounds && k < k1 && quad + 4 * h < PER && grp + quad < groups;
 #pragma unroll
       for (int r = 0; r < 2 * TILES; ++r) {
-        const int n = n0 + g + 8 * r, grp = k / G + quad;
         uint32_t v = 0;
-        if (quad < PER && n < p.N && grp < groups) {
-          const int64_t at = static_cast<int64_t>(n) * groups + grp;
-          v = static_cast<uint32_t>(__bfloat16_as_ushort(__ldg(p.scale + at))) << 16;
+        if (real && n0 + row_g + 8 * r < p.N) {
+          const int64_t at = meta0 + static_cast<int64_t>(8 * r) * groups + grp;
+          v = static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(p.scale) + at)) << 16;
           v |= p.zero ? __ldg(p.zero + at) : 8u;
         }
-        sz[u][r] = v;
+        sz[r][h] = v;
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-#pragma unroll
-  for (int u = 0; u < STAGES; ++u) load(u, u);
+  fetch(0);
 
-  // x for k in [from, from + chunk_k) of this part: zeros behind K
+  // x for k in [from, from + chunk_k) of this part: zeros behind K. Word w (8 k) of a
+  // row is word j of lane q's share of its group; BATCH words a thread at once, so that
+  // their loads overlap.
+  auto place = [&](int w, int col) {
+    const int grp = w / (G / 8), in = w % (G / 8), q = in / WORDS, j = in % WORDS;
+    return reinterpret_cast<uint4*>(xs + ((grp * WORDS + j) * cols + col) * 64 + q * 16);
+  };
   auto lay_out = [&](int from) {
-    const int words = min(p.chunk_k, (k1 - from + ROUND - 1) / ROUND * ROUND) / 8;  // 8 k each
-    for (int e = threadIdx.x; e < words * rows; e += THREADS) {
-      const int m = e / words, w = e - m * words;
-      const int k = from + w * 8;
-      float v[8];
-      if (k < p.K) {
-        const int64_t at = static_cast<int64_t>(m0 + m) * p.ldx + k;
-        if (p.x_dtype == IRIS_F32) {
-          const float4 a = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at));
-          const float4 b = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at) + 1);
-          v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        } else {
-          const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at));
-          const uint32_t h[4] = {a.x, a.y, a.z, a.w};
+    constexpr int BATCH = TERMS == 1 ? 8 : 4;
+    const int words = min(p.chunk_k, (k1 - from + ROUND - 1) / ROUND * ROUND) / 8;
+    for (int m = 0; m < rows; ++m) {
+      const int64_t row_at = static_cast<int64_t>(m0 + m) * p.ldx + from;
+      for (int w0 = threadIdx.x; w0 < words; w0 += BATCH * THREADS) {
+        if constexpr (TERMS == 1) {  // in 16 bits as it is: only the order changes
+          uint4 v[BATCH];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = p.x_dtype == IRIS_BF16 ? unpack_bf16x2(h[i])
-                                                    : __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-            v[2 * i] = f.x, v[2 * i + 1] = f.y;
+          for (int i = 0; i < BATCH; ++i) {
+            const int w = w0 + i * THREADS;
+            v[i] = w < words && from + w * 8 < p.K
+                       ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + row_at + w * 8))
+                       : make_uint4(0u, 0u, 0u, 0u);
+          }
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            const int w = w0 + i * THREADS;
+            if (w < words)
+              *place(w, m) = make_uint4(__byte_perm(v[i].x, v[i].z, 0x5410), __byte_perm(v[i].x, v[i].z, 0x7632),
+                                        __byte_perm(v[i].y, v[i].w, 0x5410), __byte_perm(v[i].y, v[i].w, 0x7632));
+          }
+        } else {
+          float v[BATCH][8];
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            const int w = w0 + i * THREADS;
+            if (w < words && from + w * 8 < p.K) {
+              if (p.x_dtype == IRIS_F32) {
+                const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + row_at + w * 8);
+                const float4 a = __ldg(src), b = __ldg(src + 1);
+                v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w;
+                v[i][4] = b.x, v[i][5] = b.y, v[i][6] = b.z, v[i][7] = b.w;
+              } else {
+                const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + row_at + w * 8));
+                const uint32_t h[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 f = p.x_dtype == IRIS_BF16 ? unpack_bf16x2(h[e])
+                                                          : __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
+                  v[i][2 * e] = f.x, v[i][2 * e + 1] = f.y;
+                }
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            const int w = w0 + i * THREADS;
+            if (w < words) {
+              uint32_t t[8][3];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) split3(p.silu_in ? silu(v[i][e]) : v[i][e], t[e]);
+#pragma unroll
+              for (int c = 0; c < 3; ++c)
+                *place(w, 3 * m + c) = make_uint4(t[0][c] | t[4][c] << 16, t[1][c] | t[5][c] << 16,
+                                                  t[2][c] | t[6][c] << 16, t[3][c] | t[7][c] << 16);
+            }
           }
         }
-        if (p.silu_in) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = silu(v[i]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      }
-      // word w is word j of lane q's share of its group
-      const int grp = w / (G / 8), in = w % (G / 8), q = in / WORDS, j = in % WORDS;
-      uint16_t h[TERMS][8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (TERMS == 3) {
-          uint16_t t[3];
-          split3(v[i], t);
-          h[0][i] = t[0], h[1][i] = t[1], h[2][i] = t[2];
-        } else {
-          h[0][i] = sizeof(T) == 2 && Magic<T>::kOne == Magic<__half>::kOne ? __half_as_ushort(__float2half_rn(v[i]))
-                                                                            : __bfloat16_as_ushort(__float2bfloat16_rn(v[i]));
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < TERMS; ++t) {
-        uint32_t* dst = reinterpret_cast<uint32_t*>(xs + ((grp * WORDS + j) * cols + m * TERMS + t) * 64 + q * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dst[i] = h[t][i] | static_cast<uint32_t>(h[t][i + 4]) << 16;
       }
     }
   };
@@ -213,97 +275,108 @@ __global__ void __launch_bounds__(THREADS) gemv_q4_kernel(const __grid_constant_
 #pragma unroll
       for (int e = 0; e < 4; ++e) total[r][c][e] = 0.f;
 
+  bool ok = true;
   const int chunk_rounds = p.chunk_k / ROUND;
   int chunk_t = 0;  // round within the chunk
-  for (int t0 = 0; t0 < rounds; t0 += STAGES) {
+#pragma unroll 1
+  for (int t = 0; t < rounds; ++t) {
+    if (chunk_t == 0) {  // uniform over the CTA
+      if (t > 0) __syncthreads();  // the chunk before is read
+      lay_out(k0 + t * ROUND);
+      __syncthreads();
+    }
+    uint32_t now[2 * TILES][HELD];
 #pragma unroll
-    for (int u = 0; u < STAGES; ++u) {
-      const int t = t0 + u;
-      if (t < rounds) {  // uniform over the CTA
-        if (chunk_t == 0) {
-          if (t > 0) __syncthreads();  // the chunk before is read
-          lay_out(k0 + t * ROUND);
-          __syncthreads();
+    for (int r = 0; r < 2 * TILES; ++r)
+#pragma unroll
+      for (int h = 0; h < HELD; ++h) now[r][h] = sz[r][h];
+    fetch(t + 1);
+    if (k0 + t * ROUND + warp * STEP < k1 && ok) {
+      ok = mbar_wait(&full[warp][t % STAGES], static_cast<uint32_t>((t / STAGES) & 1), abort);
+      const uint8_t* slot = ring + t % STAGES * SLOT + row_g * 128;
+      const uint8_t* xk = xs + (chunk_t * WARPS + warp) * (STEP / 32) * cols * 64 + g * 64 + quad * 16;
+      const int xstep = cols * 64;
+#pragma unroll
+      for (int grp = 0; grp < PER; ++grp) {
+        float acc[TILES][COLS8][4];
+#pragma unroll
+        for (int r = 0; r < TILES; ++r)
+#pragma unroll
+          for (int c = 0; c < COLS8; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[r][c][e] = 0.f;
+        uint32_t meta[2 * TILES], w[2 * TILES][WORDS];
+        typename Operand<T>::Less less[2 * TILES];
+#pragma unroll
+        for (int r = 0; r < 2 * TILES; ++r) {
+          meta[r] = __shfl_sync(0xffffffffu, now[r][grp / 4], (lane & ~3) + grp % 4);
+          less[r] = Operand<T>::less(meta[r] & 0xffu);
+          const int byte = grp * (G / 2) + quad * (G / 8);  // of the row's 128
+          const uint8_t* src = slot + r * 1024 + (((byte >> 4) ^ row_g) * 16 | (byte & 15));
+          if constexpr (WORDS == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            w[r][0] = v.x, w[r][1] = v.y, w[r][2] = v.z, w[r][3] = v.w;
+          } else if constexpr (WORDS == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(src);
+            w[r][0] = v.x, w[r][1] = v.y;
+          } else {
+            w[r][0] = *reinterpret_cast<const uint32_t*>(src);
+          }
         }
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-        __syncwarp();
-        const int k = k0 + t * ROUND + warp * STEP;
-        if (k < k1) {
-          const uint8_t* slot = ring_ptr + u * SLOT;
-          const uint8_t* xk = xs + (chunk_t * WARPS + warp) * 4 * cols * 64 + g * 64 + quad * 16;
 #pragma unroll
-          for (int grp = 0; grp < PER; ++grp) {
-            float acc[TILES][COLS8][4];
+        for (int j = 0; j < WORDS; ++j) {
+          uint4 xb[COLS8];
 #pragma unroll
-            for (int r = 0; r < TILES; ++r)
+          for (int c = 0; c < COLS8; ++c)
+            xb[c] = c * 8 + g < cols ? *reinterpret_cast<const uint4*>(xk + c * 512) : make_uint4(0u, 0u, 0u, 0u);
+          xk += xstep;
 #pragma unroll
-              for (int c = 0; c < COLS8; ++c)
+          for (int r = 0; r < TILES; ++r) {
+            const uint32_t u0 = w[2 * r][j], u1 = w[2 * r + 1][j];
+            const auto z0 = less[2 * r], z1 = less[2 * r + 1];
+            const uint32_t a[4] = {Operand<T>::template unpack<0>(u0, z0), Operand<T>::template unpack<0>(u1, z1),
+                                   Operand<T>::template unpack<1>(u0, z0), Operand<T>::template unpack<1>(u1, z1)};
+            const uint32_t b[4] = {Operand<T>::template unpack<2>(u0, z0), Operand<T>::template unpack<2>(u1, z1),
+                                   Operand<T>::template unpack<3>(u0, z0), Operand<T>::template unpack<3>(u1, z1)};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[r][c][e] = 0.f;
-            uint32_t meta[2 * TILES], less[2 * TILES], w[2 * TILES][WORDS];
-#pragma unroll
-            for (int r = 0; r < 2 * TILES; ++r) {
-              meta[r] = __shfl_sync(0xffffffffu, sz[u][r], (lane & ~3) + grp);
-              less[r] = (meta[r] & 0xffu) * 0x00010001u | Magic<T>::kOne;
-              const int row = g + 8 * r;
-              const int byte = grp * (G / 2) + quad * (G / 8);  // of the row's 64
-              const uint8_t* src = slot + row * 64 + swizzle(row, byte >> 4) * 16 + (byte & 15);
-              if constexpr (WORDS == 4) {
-                const uint4 v = *reinterpret_cast<const uint4*>(src);
-                w[r][0] = v.x, w[r][1] = v.y, w[r][2] = v.z, w[r][3] = v.w;
-              } else if constexpr (WORDS == 2) {
-                const uint2 v = *reinterpret_cast<const uint2*>(src);
-                w[r][0] = v.x, w[r][1] = v.y;
-              } else {
-                w[r][0] = *reinterpret_cast<const uint32_t*>(src);
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < WORDS; ++j) {
-              uint4 xb[COLS8];
-#pragma unroll
-              for (int c = 0; c < COLS8; ++c)
-                xb[c] = c * 8 + g < cols ? *reinterpret_cast<const uint4*>(xk + (grp * WORDS + j) * cols * 64 + c * 512)
-                                         : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-              for (int s = 0; s < 2; ++s) {  // nibbles 0, 4 and 1, 5, then 2, 6 and 3, 7
-#pragma unroll
-                for (int r = 0; r < TILES; ++r) {
-                  uint32_t a[4];
-#pragma unroll
-                  for (int h = 0; h < 4; ++h) {  // rows g, g + 8; then the second pair of nibbles
-                    const int row = 2 * r + (h & 1);
-                    const uint32_t v = w[row][j] >> (8 * s + 4 * (h >> 1));
-                    a[h] = Magic<T>::sub((v & 0x000f000fu) | Magic<T>::kOne, less[row]);
-                  }
-#pragma unroll
-                  for (int c = 0; c < COLS8; ++c)
-                    Magic<T>::mma(acc[r][c], a, s == 0 ? xb[c].x : xb[c].z, s == 0 ? xb[c].y : xb[c].w);
-                }
-              }
-            }
-#pragma unroll
-            for (int r = 0; r < TILES; ++r) {
-              const float s0 = __uint_as_float(meta[2 * r] & 0xffff0000u), s1 = __uint_as_float(meta[2 * r + 1] & 0xffff0000u);
-#pragma unroll
-              for (int c = 0; c < COLS8; ++c) {
-                total[r][c][0] = fmaf(s0, acc[r][c][0], total[r][c][0]);
-                total[r][c][1] = fmaf(s0, acc[r][c][1], total[r][c][1]);
-                total[r][c][2] = fmaf(s1, acc[r][c][2], total[r][c][2]);
-                total[r][c][3] = fmaf(s1, acc[r][c][3], total[r][c][3]);
-              }
+            for (int c = 0; c < COLS8; ++c) {
+              Operand<T>::mma(acc[r][c], a, xb[c].x, xb[c].y);
+              Operand<T>::mma(acc[r][c], b, xb[c].z, xb[c].w);
             }
           }
         }
-        __syncwarp();  // the slot is read
-        load(t + STAGES, u);
-        if (++chunk_t == chunk_rounds) chunk_t = 0;
+#pragma unroll
+        for (int r = 0; r < TILES; ++r) {
+          const float s0 = __uint_as_float(meta[2 * r] & 0xffff0000u), s1 = __uint_as_float(meta[2 * r + 1] & 0xffff0000u);
+#pragma unroll
+          for (int c = 0; c < COLS8; ++c) {
+            total[r][c][0] = fmaf(s0, acc[r][c][0], total[r][c][0]);
+            total[r][c][1] = fmaf(s0, acc[r][c][1], total[r][c][1]);
+            total[r][c][2] = fmaf(s1, acc[r][c][2], total[r][c][2]);
+            total[r][c][3] = fmaf(s1, acc[r][c][3], total[r][c][3]);
+          }
+        }
       }
     }
+    ok = __all_sync(0xffffffffu, ok);  // and the slot is read by every lane
+    if (ok) load(t + STAGES);
+    if (++chunk_t == chunk_rounds) chunk_t = 0;
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (!ok) {  // a wait gave up (device error word): no copy may land after the CTA is gone; NaN rather than wrong sums
+    int dummy = 0;
+    for (int u = 0; u < STAGES; ++u)
+      for (int t = u; t < rounds && k0 + t * ROUND + warp * STEP < k1; t += STAGES)
+        mbar_wait(&full[warp][u], static_cast<uint32_t>((t / STAGES) & 1), &dummy);
+#pragma unroll
+    for (int r = 0; r < TILES; ++r)
+#pragma unroll
+      for (int c = 0; c < COLS8; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) total[r][c][e] = __int_as_float(0x7fc00000);
+  }
   __syncthreads();  // rings and x are done with
-  // [warp][row][COLS8 * 8] sums; then one thread per (row of x, weight row)
+  // the warps' sums, [warp][row][COLS8 * 8], joined in the first one's place; then over the cluster, its CTAs
+  // taking the outputs in turn
   float* sums = reinterpret_cast<float*>(smem_raw);
   constexpr int WIDTH = COLS8 * 8;
 #pragma unroll
@@ -312,40 +385,43 @@ __global__ void __launch_bounds__(THREADS) gemv_q4_kernel(const __grid_constant_
     for (int c = 0; c < COLS8; ++c)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<float2*>(sums + (warp * ROWS + 16 * r + 8 * h + g) * WIDTH + c * 8 + 2 * quad) =
+        *reinterpret_cast<float2*>(sums + (warp * ROWS + 16 * r + 8 * h + row_g) * WIDTH + c * 8 + 2 * quad) =
             make_float2(total[r][c][2 * h], total[r][c][2 * h + 1]);
+  __syncthreads();
+  for (int e = threadIdx.x; e < ROWS * rows; e += THREADS) {
+    const int row = e % ROWS, m = e / ROWS;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w)
+#pragma unroll
+      for (int c = TERMS - 1; c >= 0; --c) v += sums[(w * ROWS + row) * WIDTH + m * TERMS + c];
+    sums[row * WIDTH + m * TERMS] = v;
+  }
   if (p.parts > 1) cluster_sync();
-  else __syncthreads();
-  if (part == 0) {
-    for (int e = threadIdx.x; e < rows * ROWS; e += THREADS) {
-      const int m = e / ROWS, row = e % ROWS;
-      float v = 0.f;
-      for (int q = 0; q < p.parts; ++q) {
-        const uint32_t base = p.parts > 1 ? map_to_cta(sums, static_cast<uint32_t>(q)) : smem_addr(sums);
+  for (int e = part * THREADS + threadIdx.x; e < ROWS * rows; e += THREADS * p.parts) {
+    const int row = e % ROWS, m = e / ROWS, at = row * WIDTH + m * TERMS;
+    float v = sums[at];
+    if (p.parts > 1) {
+      float x[MOST_PARTS];
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-          float x[TERMS];
+      for (int q = 0; q < MOST_PARTS; ++q)
+        if (q < p.parts)
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[q]) : "r"(map_to_cta(sums + at, static_cast<uint32_t>(q))));
+      v = 0.f;
 #pragma unroll
-          for (int t = 0; t < TERMS; ++t)
-            asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                         : "=f"(x[t])
-                         : "r"(base + 4 * ((w * ROWS + row) * WIDTH + m * TERMS + t))
-                         : "memory");
-#pragma unroll
-          for (int t = TERMS - 1; t >= 0; --t) v += x[t];
-        }
-      }
-      const int n = n0 + row;
-      if (n < p.N) {
-        if (p.bias) v += __ldg(p.bias + n);
-        store_elem(p.out, static_cast<int64_t>(m0 + m) * p.N + n, p.out_dtype, p.silu_out ? silu(v) : v);
-      }
+      for (int q = 0; q < MOST_PARTS; ++q)
+        if (q < p.parts) v += x[q];
+    }
+    const int n = n0 + row;
+    if (n < p.N) {
+      if (p.bias) v += __ldg(p.bias + n);
+      store_elem(p.out, static_cast<int64_t>(m0 + m) * p.N + n, p.out_dtype, p.silu_out ? silu(v) : v);
     }
   }
   if (p.parts > 1) cluster_sync();  // no CTA leaves while its sums are read
 }
 
-constexpr int X_BYTES = 64 * 1024;  // x in shared memory at a time, at most
+constexpr int X_BYTES = 96 * 1024;  // x in shared memory at a time, at most: one ROUND of 48 columns
 
 template <typename T, int TERMS, int COLS8, int G>
 int launch_g(Params& p, int passes, cudaStream_t st) {
@@ -355,7 +431,7 @@ int launch_g(Params& p, int passes, cudaStream_t st) {
   // parts of K over a cluster's CTAs: as many as give every SM two CTAs, or as keep a part of x in shared memory
   int parts = 1;
   const int64_t wanted = 2 * num_sms();
-  while (parts < 8 && p.K > 2 * parts * ROUND &&
+  while (parts < MOST_PARTS && p.K > 2 * parts * ROUND &&
          (tiles * passes * parts < wanted || static_cast<int64_t>(p.K) * cols * 2 / parts > X_BYTES))
     parts *= 2;
   p.parts = parts;
@@ -364,14 +440,16 @@ int launch_g(Params& p, int passes, cudaStream_t st) {
   p.chunk_k = p.part_k < most ? p.part_k : most;
   const int used = WARPS * STAGES * SLOT + p.chunk_k * cols * 2;
   const int sums = WARPS * ROWS * COLS8 * 8 * 4;
-  const int smem = used > sums ? used : sums;
+  const int smem = 1024 + (used > sums ? used : sums);
   static int configured[64] = {0};
   int dev = 0;
   IRIS_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || configured[dev] == 0) {
-    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, WARPS * STAGES * SLOT + X_BYTES));
+    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + WARPS * STAGES * SLOT + X_BYTES));
     if (dev < 64) configured[dev] = 1;
   }
+  CUtensorMap tw;
+  IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tw, p.packed, p.K / 2, p.N, p.K / 2, STEP / 2, ROWS));
   cudaLaunchAttribute cluster = {};
   cluster.id = cudaLaunchAttributeClusterDimension;
   cluster.val.clusterDim.x = static_cast<unsigned>(parts);
@@ -383,7 +461,7 @@ int launch_g(Params& p, int passes, cudaStream_t st) {
   config.stream = st;
   config.attrs = &cluster;
   config.numAttrs = 1;
-  IRIS_CUDA(cudaLaunchKernelEx(&config, kernel, p));
+  IRIS_CUDA(cudaLaunchKernelEx(&config, kernel, tw, p));
   return IRIS_OK;
 }
 
