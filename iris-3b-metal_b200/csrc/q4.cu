@@ -48,7 +48,7 @@ struct Params {
   int N;
   int silu_in, silu_out;
   int parts;     // CTAs of a cluster: parts of K
-  int part_k;    // k of a part, a multiple of ROUND
+  int part_k;    // k of a part, a multiple of STEP
   int chunk_k;   // k of x in shared memory at a time, a multiple of ROUND
   int pass_rows;  // rows of x per blockIdx.y
 };
@@ -70,7 +70,7 @@ template <>
 struct Operand<__nv_bfloat16> {
   static constexpr uint32_t kOne = 0x43004300u;  // 128: the mantissa's last bit is 1
   using Less = uint32_t;
-  IRIS_DEVICE static Less less(uint32_t z) { return z * 0x00010001u | kOne; }
+  IRIS_DEVICE static Less less(uint32_t z) { return __byte_perm(z, 0x43u, 0x4040); }  // z in byte 0
   template <int I>
   IRIS_DEVICE static uint32_t unpack(uint32_t w, Less z) {
     uint32_t a = put(w >> (4 * I), 0x000f000fu, kOne);
@@ -89,7 +89,9 @@ struct Operand<__half> {
   struct Less {
     uint32_t low, high;  // 1024 + z; -(64 + z)
   };
-  IRIS_DEVICE static Less less(uint32_t z) { return Less{z * 0x00010001u | kOne, z * 0x00100010u | 0xd400d400u}; }
+  IRIS_DEVICE static Less less(uint32_t z) {  // z in byte 0, 16 z in byte 1
+    return Less{__byte_perm(z, 0x64u, 0x4040), __byte_perm(z, 0xd4u, 0x4141)};
+  }
   template <int I>
   IRIS_DEVICE static uint32_t unpack(uint32_t w, Less z) {
     __half2 r;
@@ -151,6 +153,8 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   uint8_t* ring = smem_raw + warp * (STAGES * SLOT);
   uint8_t* xs = smem_raw + WARPS * STAGES * SLOT;  // [chunk_k / 32][cols][32] in the order of use
   volatile int* abort = &abort_flag;
+  __shared__ __align__(16) uint8_t zeros[16];
+  if (threadIdx.x < 4) reinterpret_cast<uint32_t*>(zeros)[threadIdx.x] = 0u;
   if (threadIdx.x == 0) {
     for (int w = 0; w < WARPS; ++w)
       for (int u = 0; u < STAGES; ++u) mbar_init(&full[w][u], 1);
@@ -172,27 +176,35 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   // lane (g, quad) holds groups quad, quad + 4 of a step, of rows weight_row(g) + 0, 8, 16, 24: scale above zero;
   // fetched a round ahead
   const int row_g = weight_row(g);
-  const int64_t meta0 = static_cast<int64_t>(n0 + row_g) * groups + quad;
-  uint32_t sz[2 * TILES][HELD];
-  auto fetch = [&](int t) {
-    const int k = k0 + t * ROUND + warp * STEP;
+  uint16_t sz_scale[2 * TILES][HELD];
+  uint32_t sz_zero[2 * TILES][HELD];
+  const int64_t meta0 = static_cast<int64_t>(n0 + row_g) * groups + (k0 + warp * STEP) / G + quad;
+  const uint16_t* scale_at = reinterpret_cast<const uint16_t*>(p.scale) + meta0;
+  const uint8_t* zero_at = p.zero ? p.zero + meta0 : nullptr;
+  const int real_rows = min(2 * TILES, max(0, (p.N - n0 - row_g + 7) / 8));  // of this lane's that exist
+  int grps_left = min(k1, p.K) / G - (k0 + warp * STEP) / G - quad;          // groups of this lane's from here on
+  auto fetch = [&]() {
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-      const int grp = k / G + 4 * h;  // + quad
-      const bool real = t < rounds && k < k1 && quad + 4 * h < PER && grp + quad < groups;
+    for (int r = 0; r < 2 * TILES; ++r) {
 #pragma unroll
-      for (int r = 0; r < 2 * TILES; ++r) {
-        uint32_t v = 0;
-        if (real && n0 + row_g + 8 * r < p.N) {
-          const int64_t at = meta0 + static_cast<int64_t>(8 * r) * groups + grp;
-          v = static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(p.scale) + at)) << 16;
-          v |= p.zero ? __ldg(p.zero + at) : 8u;
+      for (int h = 0; h < HELD; ++h) {
+        uint16_t scale = 0;
+        uint32_t zero = 8;
+        if (r < real_rows && 4 * h < grps_left && quad + 4 * h < PER) {
+          // volatile: where they stand, a round ahead of their use
+          const int64_t at = static_cast<int64_t>(8 * r) * groups + 4 * h;
+          asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(scale) : "l"(scale_at + at));
+          if (zero_at) asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(zero) : "l"(zero_at + at));
         }
-        sz[r][h] = v;
+        sz_scale[r][h] = scale;
+        sz_zero[r][h] = zero;
       }
     }
+    scale_at += ROUND / G;
+    if (zero_at) zero_at += ROUND / G;
+    grps_left -= ROUND / G;
   };
-  fetch(0);
+  fetch();
 
   // x for k in [from, from + chunk_k) of this part: zeros behind K. Word w (8 k) of a
   // row is word j of lane q's share of its group; BATCH words a thread at once, so that
@@ -203,65 +215,62 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   };
   auto lay_out = [&](int from) {
     constexpr int BATCH = TERMS == 1 ? 8 : 4;
-    const int words = min(p.chunk_k, (k1 - from + ROUND - 1) / ROUND * ROUND) / 8;
-    for (int m = 0; m < rows; ++m) {
-      const int64_t row_at = static_cast<int64_t>(m0 + m) * p.ldx + from;
-      for (int w0 = threadIdx.x; w0 < words; w0 += BATCH * THREADS) {
-        if constexpr (TERMS == 1) {  // in 16 bits as it is: only the order changes
-          uint4 v[BATCH];
+    static_assert(ROUND / 8 == THREADS, "a round's words are one per thread");
+    const int turns = min(p.chunk_k, k1 - from + ROUND - 1) / ROUND;  // of a row
+    const int all = turns * rows;
+    for (int i0 = 0; i0 < all; i0 += BATCH) {
+      int word[BATCH], col[BATCH];
+      int64_t at[BATCH];  // in x, or -1: behind K
 #pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            const int w = w0 + i * THREADS;
-            v[i] = w < words && from + w * 8 < p.K
-                       ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + row_at + w * 8))
-                       : make_uint4(0u, 0u, 0u, 0u);
-          }
+      for (int i = 0; i < BATCH; ++i) {
+        const int m = (i0 + i) / turns, w = (i0 + i - m * turns) * THREADS + threadIdx.x;
+        word[i] = w, col[i] = m * TERMS;
+        at[i] = i0 + i < all && from + w * 8 < p.K ? static_cast<int64_t>(m0 + m) * p.ldx + from + w * 8 : -1;
+      }
+      if constexpr (TERMS == 1) {  // in 16 bits as it is: only the order changes
+        uint4 v[BATCH];
 #pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            const int w = w0 + i * THREADS;
-            if (w < words)
-              *place(w, m) = make_uint4(__byte_perm(v[i].x, v[i].z, 0x5410), __byte_perm(v[i].x, v[i].z, 0x7632),
-                                        __byte_perm(v[i].y, v[i].w, 0x5410), __byte_perm(v[i].y, v[i].w, 0x7632));
-          }
-        } else {
-          float v[BATCH][8];
+        for (int i = 0; i < BATCH; ++i)
+          v[i] = at[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at[i]))
+                            : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            const int w = w0 + i * THREADS;
-            if (w < words && from + w * 8 < p.K) {
-              if (p.x_dtype == IRIS_F32) {
-                const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + row_at + w * 8);
-                const float4 a = __ldg(src), b = __ldg(src + 1);
-                v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w;
-                v[i][4] = b.x, v[i][5] = b.y, v[i][6] = b.z, v[i][7] = b.w;
-              } else {
-                const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + row_at + w * 8));
-                const uint32_t h[4] = {a.x, a.y, a.z, a.w};
+        for (int i = 0; i < BATCH; ++i)
+          if (i0 + i < all)
+            *place(word[i], col[i]) = make_uint4(__byte_perm(v[i].x, v[i].z, 0x5410), __byte_perm(v[i].x, v[i].z, 0x7632),
+                                                 __byte_perm(v[i].y, v[i].w, 0x5410), __byte_perm(v[i].y, v[i].w, 0x7632));
+      } else {
+        float v[BATCH][8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float2 f = p.x_dtype == IRIS_BF16 ? unpack_bf16x2(h[e])
-                                                          : __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
-                  v[i][2 * e] = f.x, v[i][2 * e + 1] = f.y;
-                }
-              }
-            } else {
+        for (int i = 0; i < BATCH; ++i) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+          for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+          if (at[i] < 0) continue;
+          if (p.x_dtype == IRIS_F32) {
+            const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at[i]);
+            const float4 a = __ldg(src), b = __ldg(src + 1);
+            v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w;
+            v[i][4] = b.x, v[i][5] = b.y, v[i][6] = b.z, v[i][7] = b.w;
+          } else {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at[i]));
+            const uint32_t h[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = p.x_dtype == IRIS_BF16 ? unpack_bf16x2(h[e])
+                                                      : __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
+              v[i][2 * e] = f.x, v[i][2 * e + 1] = f.y;
             }
           }
+        }
 #pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            const int w = w0 + i * THREADS;
-            if (w < words) {
-              uint32_t t[8][3];
+        for (int i = 0; i < BATCH; ++i) {
+          if (i0 + i >= all) continue;
+          uint32_t t[8][3];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) split3(p.silu_in ? silu(v[i][e]) : v[i][e], t[e]);
+          for (int e = 0; e < 8; ++e) split3(p.silu_in ? silu(v[i][e]) : v[i][e], t[e]);
 #pragma unroll
-              for (int c = 0; c < 3; ++c)
-                *place(w, 3 * m + c) = make_uint4(t[0][c] | t[4][c] << 16, t[1][c] | t[5][c] << 16,
-                                                  t[2][c] | t[6][c] << 16, t[3][c] | t[7][c] << 16);
-            }
-          }
+          for (int c = 0; c < 3; ++c)
+            *place(word[i], col[i] + c) = make_uint4(t[0][c] | t[4][c] << 16, t[1][c] | t[5][c] << 16,
+                                                     t[2][c] | t[6][c] << 16, t[3][c] | t[7][c] << 16);
         }
       }
     }
@@ -289,13 +298,21 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
 #pragma unroll
     for (int r = 0; r < 2 * TILES; ++r)
 #pragma unroll
-      for (int h = 0; h < HELD; ++h) now[r][h] = sz[r][h];
-    fetch(t + 1);
+      for (int h = 0; h < HELD; ++h)  // scale, 16 zero, zero
+        now[r][h] = static_cast<uint32_t>(sz_scale[r][h]) << 16 | sz_zero[r][h] * 0x1001u;
+    fetch();
     if (k0 + t * ROUND + warp * STEP < k1 && ok) {
       ok = mbar_wait(&full[warp][t % STAGES], static_cast<uint32_t>((t / STAGES) & 1), abort);
       const uint8_t* slot = ring + t % STAGES * SLOT + row_g * 128;
-      const uint8_t* xk = xs + (chunk_t * WARPS + warp) * (STEP / 32) * cols * 64 + g * 64 + quad * 16;
-      const int xstep = cols * 64;
+      // this lane's column of each 8, or the zeros behind x
+      const uint8_t* xk[COLS8];
+      int xstep[COLS8];
+#pragma unroll
+      for (int c = 0; c < COLS8; ++c) {
+        const bool real = c * 8 + g < cols;
+        xk[c] = real ? xs + ((chunk_t * WARPS + warp) * (STEP / 32) * cols + c * 8 + g) * 64 + quad * 16 : zeros;
+        xstep[c] = real ? cols * 64 : 0;
+      }
 #pragma unroll
       for (int grp = 0; grp < PER; ++grp) {
         float acc[TILES][COLS8][4];
@@ -310,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
 #pragma unroll
         for (int r = 0; r < 2 * TILES; ++r) {
           meta[r] = __shfl_sync(0xffffffffu, now[r][grp / 4], (lane & ~3) + grp % 4);
-          less[r] = Operand<T>::less(meta[r] & 0xffu);
+          less[r] = Operand<T>::less(meta[r]);
           const int byte = grp * (G / 2) + quad * (G / 8);  // of the row's 128
           const uint8_t* src = slot + r * 1024 + (((byte >> 4) ^ row_g) * 16 | (byte & 15));
           if constexpr (WORDS == 4) {
@@ -327,9 +344,10 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
         for (int j = 0; j < WORDS; ++j) {
           uint4 xb[COLS8];
 #pragma unroll
-          for (int c = 0; c < COLS8; ++c)
-            xb[c] = c * 8 + g < cols ? *reinterpret_cast<const uint4*>(xk + c * 512) : make_uint4(0u, 0u, 0u, 0u);
-          xk += xstep;
+          for (int c = 0; c < COLS8; ++c) {
+            xb[c] = *reinterpret_cast<const uint4*>(xk[c]);
+            xk[c] += xstep[c];
+          }
 #pragma unroll
           for (int r = 0; r < TILES; ++r) {
             const uint32_t u0 = w[2 * r][j], u1 = w[2 * r + 1][j];
@@ -421,6 +439,7 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   if (p.parts > 1) cluster_sync();  // no CTA leaves while its sums are read
 }
 
+constexpr int WANTED = 4;
 constexpr int X_BYTES = 96 * 1024;  // x in shared memory at a time, at most: one ROUND of 48 columns
 
 template <typename T, int TERMS, int COLS8, int G>
@@ -430,14 +449,15 @@ int launch_g(Params& p, int passes, cudaStream_t st) {
   const int64_t tiles = (p.N + ROWS - 1) / ROWS;
   // parts of K over a cluster's CTAs: as many as give every SM two CTAs, or as keep a part of x in shared memory
   int parts = 1;
-  const int64_t wanted = 2 * num_sms();
-  while (parts < MOST_PARTS && p.K > 2 * parts * ROUND &&
+  const int64_t wanted = WANTED * num_sms();
+  while (parts < MOST_PARTS && p.K > parts * ROUND &&
          (tiles * passes * parts < wanted || static_cast<int64_t>(p.K) * cols * 2 / parts > X_BYTES))
     parts *= 2;
   p.parts = parts;
-  p.part_k = ((p.K + parts - 1) / parts + ROUND - 1) / ROUND * ROUND;
+  p.part_k = ((p.K + parts - 1) / parts + STEP - 1) / STEP * STEP;
   const int most = X_BYTES / (cols * 2) / ROUND * ROUND;
-  p.chunk_k = p.part_k < most ? p.part_k : most;
+  const int whole = (p.part_k + ROUND - 1) / ROUND * ROUND;
+  p.chunk_k = whole < most ? whole : most;
   const int used = WARPS * STAGES * SLOT + p.chunk_k * cols * 2;
   const int sums = WARPS * ROWS * COLS8 * 8 * 4;
   const int smem = 1024 + (used > sums ? used : sums);

@@ -669,7 +669,7 @@ IRIS_DEVICE void finish_row(const Params& p, int b, int h, int i, float2 (&acc)[
 template <typename T, int D>
 __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_constant__ Params p,
                                                                const __grid_constant__ Split sp) {
-  extern __shared__ __align__(128) uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   constexpr int TILE = STEP_KEYS * D * 2;  // bytes of one K or V tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (sp.parts) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
