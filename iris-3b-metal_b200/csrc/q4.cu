@@ -16,10 +16,10 @@
 //  - x in 16 bits goes in as it is. FP32 (and act_in's results) go in as three bf16
 //    columns, 8 bits each of the 24, cut off rather than rounded: their sum is x, and
 //    the columns are free up to 8 of them.
-// A CTA owns 32 weight rows and, in a cluster, one part of K; its warps take 256-wide
-// pieces of K in turn, each through its own ring of TMA copies (one instruction for 32
-// rows; filled before x is laid out). Sums are joined in shared memory (over the
-// cluster's CTAs through distributed shared memory) in a fixed order.
+// A CTA owns 128 weight rows, 32 a warp, and, in a cluster, one part of K, whose x it
+// lays out once for all of them; a warp streams 256-wide pieces of its rows through
+// its own ring of TMA copies (one instruction for 32 rows; filled before x is laid
+// out). The parts' sums are joined through distributed shared memory in a fixed order.
 #include "common.cuh"
 #include "iris_abi_internal.h"
 
@@ -28,10 +28,9 @@ namespace q4 {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int STAGES = 2;                    // ring slots of a warp; two to four CTAs share an SM
-constexpr int TILES = 2, ROWS = 16 * TILES;  // weight rows of a CTA
+constexpr int TILES = 2, ROWS = 16 * TILES;  // weight rows of a warp
 constexpr int STEP = 256;                    // k of one ring slot: 128 bytes of each row
 constexpr int SLOT = ROWS * STEP / 2;        // bytes
-constexpr int ROUND = STEP * WARPS;          // k of one round of the warps
 constexpr int MOST_PARTS = 8;                // CTAs of a cluster
 
 struct Params {
@@ -49,7 +48,7 @@ struct Params {
   int silu_in, silu_out;
   int parts;     // CTAs of a cluster: parts of K
   int part_k;    // k of a part, a multiple of STEP
-  int chunk_k;   // k of x in shared memory at a time, a multiple of ROUND
+  int chunk_k;   // k of x in shared memory at a time, a multiple of STEP
   int pass_rows;  // rows of x per blockIdx.y
 };
 
@@ -82,6 +81,11 @@ struct Operand<__nv_bfloat16> {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
+  IRIS_DEVICE static void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  }
 };
 template <>
 struct Operand<__half> {
@@ -109,6 +113,11 @@ struct Operand<__half> {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  IRIS_DEVICE static void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
   }
 };
 
@@ -139,16 +148,17 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   uint8_t* smem_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, quad = lane & 3;
-  const int n0 = static_cast<int>(blockIdx.x / p.parts) * ROWS;
+  const int n0 = (static_cast<int>(blockIdx.x / p.parts) * WARPS + warp) * ROWS;  // this warp's first weight row
   const int part = static_cast<int>(blockIdx.x % p.parts);
   const int m0 = static_cast<int>(blockIdx.y) * p.pass_rows;
   const int rows = min(p.pass_rows, p.M - m0), cols = rows * TERMS;
   const int k0 = part * p.part_k, k1 = min(k0 + p.part_k, p.K);
   const int groups = p.K / G;
-  const int rounds = k1 > k0 ? (k1 - k0 + ROUND - 1) / ROUND : 0;
-  constexpr int PER = STEP / G;   // groups per step
-  constexpr int WORDS = G / 32;   // words of a group per lane of a row
-  constexpr int HELD = (PER + 3) / 4;  // a step's scales and zeros that a lane holds for each of its rows
+  const int steps = k1 > k0 ? (k1 - k0 + STEP - 1) / STEP : 0;
+  constexpr int PER = STEP / G;                // groups per step
+  constexpr int WORDS = G / 32;                // words of a group per lane of a row
+  constexpr int HELD = (PER + 3) / 4;          // scales and zeros that a lane holds for each of its rows:
+  constexpr int SPAN = PER < 4 ? 4 / PER : 1;  // of so many steps
 
   uint8_t* ring = smem_raw + warp * (STAGES * SLOT);
   uint8_t* xs = smem_raw + WARPS * STAGES * SLOT;  // [chunk_k / 32][cols][32] in the order of use
@@ -163,26 +173,25 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   }
   __syncthreads();
 
-  auto load = [&](int t) {  // round t into its slot
-    const int k = k0 + t * ROUND + warp * STEP;
-    if (lane == 0 && t < rounds && k < k1) {
+  auto load = [&](int t) {  // step t into its slot
+    if (lane == 0 && t < steps && n0 < p.N) {
       uint64_t* bar = &full[warp][t % STAGES];
       mbar_arrive_expect_tx(bar, SLOT);
-      tma_load_2d(&tw, bar, ring + t % STAGES * SLOT, k / 2, n0);  // rows from N on and k from K on: zeros
+      // rows from N on and k from K on: zeros
+      tma_load_2d(&tw, bar, ring + t % STAGES * SLOT, (k0 + t * STEP) / 2, n0);
     }
   };
   for (int t = 0; t < STAGES; ++t) load(t);
 
-  // lane (g, quad) holds groups quad, quad + 4 of a step, of rows weight_row(g) + 0, 8, 16, 24: scale above zero;
-  // fetched a round ahead
+  // lane (g, quad) holds groups quad, quad + 4 of SPAN steps, of rows weight_row(g) + 0, 8, 16, 24, fetched ahead
   const int row_g = weight_row(g);
   uint16_t sz_scale[2 * TILES][HELD];
   uint32_t sz_zero[2 * TILES][HELD];
-  const int64_t meta0 = static_cast<int64_t>(n0 + row_g) * groups + (k0 + warp * STEP) / G + quad;
+  const int64_t meta0 = static_cast<int64_t>(n0 + row_g) * groups + k0 / G + quad;
   const uint16_t* scale_at = reinterpret_cast<const uint16_t*>(p.scale) + meta0;
   const uint8_t* zero_at = p.zero ? p.zero + meta0 : nullptr;
   const int real_rows = min(2 * TILES, max(0, (p.N - n0 - row_g + 7) / 8));  // of this lane's that exist
-  int grps_left = min(k1, p.K) / G - (k0 + warp * STEP) / G - quad;          // groups of this lane's from here on
+  int grps_left = k1 / G - k0 / G - quad;                                    // groups of this lane's from here on
   auto fetch = [&]() {
 #pragma unroll
     for (int r = 0; r < 2 * TILES; ++r) {
@@ -190,8 +199,8 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
       for (int h = 0; h < HELD; ++h) {
         uint16_t scale = 0;
         uint32_t zero = 8;
-        if (r < real_rows && 4 * h < grps_left && quad + 4 * h < PER) {
-          // volatile: where they stand, a round ahead of their use
+        if (r < real_rows && 4 * h < grps_left && quad + 4 * h < PER * SPAN) {
+          // volatile: where they stand, a span ahead of their use
           const int64_t at = static_cast<int64_t>(8 * r) * groups + 4 * h;
           asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(scale) : "l"(scale_at + at));
           if (zero_at) asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(zero) : "l"(zero_at + at));
@@ -200,9 +209,9 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
         sz_zero[r][h] = zero;
       }
     }
-    scale_at += ROUND / G;
-    if (zero_at) zero_at += ROUND / G;
-    grps_left -= ROUND / G;
+    scale_at += SPAN * STEP / G;
+    if (zero_at) zero_at += SPAN * STEP / G;
+    grps_left -= SPAN * STEP / G;
   };
   fetch();
 
@@ -215,17 +224,17 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   };
   auto lay_out = [&](int from) {
     constexpr int BATCH = TERMS == 1 ? 8 : 4;
-    static_assert(ROUND / 8 == THREADS, "a round's words are one per thread");
-    const int turns = min(p.chunk_k, k1 - from + ROUND - 1) / ROUND;  // of a row
-    const int all = turns * rows;
-    for (int i0 = 0; i0 < all; i0 += BATCH) {
+    const int words = min(p.chunk_k, (k1 - from + STEP - 1) / STEP * STEP) / 8;  // of a row
+    const int all = words * rows;
+    for (int e0 = threadIdx.x; e0 < all; e0 += BATCH * THREADS) {
       int word[BATCH], col[BATCH];
       int64_t at[BATCH];  // in x, or -1: behind K
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
-        const int m = (i0 + i) / turns, w = (i0 + i - m * turns) * THREADS + threadIdx.x;
+        const int e = e0 + i * THREADS;
+        const int m = e / words, w = e - m * words;
         word[i] = w, col[i] = m * TERMS;
-        at[i] = i0 + i < all && from + w * 8 < p.K ? static_cast<int64_t>(m0 + m) * p.ldx + from + w * 8 : -1;
+        at[i] = e < all && from + w * 8 < p.K ? static_cast<int64_t>(m0 + m) * p.ldx + from + w * 8 : -1;
       }
       if constexpr (TERMS == 1) {  // in 16 bits as it is: only the order changes
         uint4 v[BATCH];
@@ -235,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
                             : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int i = 0; i < BATCH; ++i)
-          if (i0 + i < all)
+          if (e0 + i * THREADS < all)
             *place(word[i], col[i]) = make_uint4(__byte_perm(v[i].x, v[i].z, 0x5410), __byte_perm(v[i].x, v[i].z, 0x7632),
                                                  __byte_perm(v[i].y, v[i].w, 0x5410), __byte_perm(v[i].y, v[i].w, 0x7632));
       } else {
@@ -263,7 +272,7 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
         }
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
-          if (i0 + i >= all) continue;
+          if (e0 + i * THREADS >= all) continue;
           uint32_t t[8][3];
 #pragma unroll
           for (int e = 0; e < 8; ++e) split3(p.silu_in ? silu(v[i][e]) : v[i][e], t[e]);
@@ -285,48 +294,45 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
       for (int e = 0; e < 4; ++e) total[r][c][e] = 0.f;
 
   bool ok = true;
-  const int chunk_rounds = p.chunk_k / ROUND;
-  int chunk_t = 0;  // round within the chunk
+  const int chunk_steps = p.chunk_k / STEP;
+  int chunk_t = 0;  // step within the chunk
+  uint32_t now[2 * TILES][HELD];
 #pragma unroll 1
-  for (int t = 0; t < rounds; ++t) {
+  for (int t = 0; t < steps; ++t) {
     if (chunk_t == 0) {  // uniform over the CTA
       if (t > 0) __syncthreads();  // the chunk before is read
-      lay_out(k0 + t * ROUND);
+      lay_out(k0 + t * STEP);
       __syncthreads();
     }
-    uint32_t now[2 * TILES][HELD];
+    if (t % SPAN == 0) {
 #pragma unroll
-    for (int r = 0; r < 2 * TILES; ++r)
+      for (int r = 0; r < 2 * TILES; ++r)
 #pragma unroll
-      for (int h = 0; h < HELD; ++h)  // scale, 16 zero, zero
-        now[r][h] = static_cast<uint32_t>(sz_scale[r][h]) << 16 | sz_zero[r][h] * 0x1001u;
-    fetch();
-    if (k0 + t * ROUND + warp * STEP < k1 && ok) {
+        for (int h = 0; h < HELD; ++h)  // scale, 16 zero, zero
+          now[r][h] = static_cast<uint32_t>(sz_scale[r][h]) << 16 | sz_zero[r][h] * 0x1001u;
+      fetch();
+    }
+    if (n0 < p.N && ok) {
       ok = mbar_wait(&full[warp][t % STAGES], static_cast<uint32_t>((t / STAGES) & 1), abort);
       const uint8_t* slot = ring + t % STAGES * SLOT + row_g * 128;
-      // this lane's column of each 8, or the zeros behind x
+      const int held_by = (lane & ~3) + t % SPAN * PER;  // the lane with the step's first group
+      // this lane's column of each 8, or zeros
       const uint8_t* xk[COLS8];
       int xstep[COLS8];
 #pragma unroll
       for (int c = 0; c < COLS8; ++c) {
         const bool real = c * 8 + g < cols;
-        xk[c] = real ? xs + ((chunk_t * WARPS + warp) * (STEP / 32) * cols + c * 8 + g) * 64 + quad * 16 : zeros;
+        xk[c] = real ? xs + (chunk_t * (STEP / 32) * cols + c * 8 + g) * 64 + quad * 16 : zeros;
         xstep[c] = real ? cols * 64 : 0;
       }
 #pragma unroll
       for (int grp = 0; grp < PER; ++grp) {
         float acc[TILES][COLS8][4];
-#pragma unroll
-        for (int r = 0; r < TILES; ++r)
-#pragma unroll
-          for (int c = 0; c < COLS8; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[r][c][e] = 0.f;
         uint32_t meta[2 * TILES], w[2 * TILES][WORDS];
         typename Operand<T>::Less less[2 * TILES];
 #pragma unroll
         for (int r = 0; r < 2 * TILES; ++r) {
-          meta[r] = __shfl_sync(0xffffffffu, now[r][grp / 4], (lane & ~3) + grp % 4);
+          meta[r] = __shfl_sync(0xffffffffu, now[r][grp / 4], held_by + grp % 4);
           less[r] = Operand<T>::less(meta[r]);
           const int byte = grp * (G / 2) + quad * (G / 8);  // of the row's 128
           const uint8_t* src = slot + r * 1024 + (((byte >> 4) ^ row_g) * 16 | (byte & 15));
@@ -358,7 +364,8 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
                                    Operand<T>::template unpack<3>(u0, z0), Operand<T>::template unpack<3>(u1, z1)};
 #pragma unroll
             for (int c = 0; c < COLS8; ++c) {
-              Operand<T>::mma(acc[r][c], a, xb[c].x, xb[c].y);
+              if (j == 0) Operand<T>::mma_first(acc[r][c], a, xb[c].x, xb[c].y);
+              else Operand<T>::mma(acc[r][c], a, xb[c].x, xb[c].y);
               Operand<T>::mma(acc[r][c], b, xb[c].z, xb[c].w);
             }
           }
@@ -378,13 +385,12 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
     }
     ok = __all_sync(0xffffffffu, ok);  // and the slot is read by every lane
     if (ok) load(t + STAGES);
-    if (++chunk_t == chunk_rounds) chunk_t = 0;
+    if (++chunk_t == chunk_steps) chunk_t = 0;
   }
   if (!ok) {  // a wait gave up (device error word): no copy may land after the CTA is gone; NaN rather than wrong sums
     int dummy = 0;
-    for (int u = 0; u < STAGES; ++u)
-      for (int t = u; t < rounds && k0 + t * ROUND + warp * STEP < k1; t += STAGES)
-        mbar_wait(&full[warp][u], static_cast<uint32_t>((t / STAGES) & 1), &dummy);
+    for (int t = 0; t < steps && n0 < p.N; ++t)
+      mbar_wait(&full[warp][t % STAGES], static_cast<uint32_t>((t / STAGES) & 1), &dummy);
 #pragma unroll
     for (int r = 0; r < TILES; ++r)
 #pragma unroll
@@ -393,8 +399,7 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
         for (int e = 0; e < 4; ++e) total[r][c][e] = __int_as_float(0x7fc00000);
   }
   __syncthreads();  // rings and x are done with
-  // the warps' sums, [warp][row][COLS8 * 8], joined in the first one's place; then over the cluster, its CTAs
-  // taking the outputs in turn
+  // sums [row][COLS8 * 8] of the CTA's rows, joined over the cluster, whose CTAs take the outputs in turn
   float* sums = reinterpret_cast<float*>(smem_raw);
   constexpr int WIDTH = COLS8 * 8;
 #pragma unroll
@@ -405,32 +410,30 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
       for (int h = 0; h < 2; ++h)
         *reinterpret_cast<float2*>(sums + (warp * ROWS + 16 * r + 8 * h + row_g) * WIDTH + c * 8 + 2 * quad) =
             make_float2(total[r][c][2 * h], total[r][c][2 * h + 1]);
-  __syncthreads();
-  for (int e = threadIdx.x; e < ROWS * rows; e += THREADS) {
-    const int row = e % ROWS, m = e / ROWS;
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w)
-#pragma unroll
-      for (int c = TERMS - 1; c >= 0; --c) v += sums[(w * ROWS + row) * WIDTH + m * TERMS + c];
-    sums[row * WIDTH + m * TERMS] = v;
-  }
   if (p.parts > 1) cluster_sync();
-  for (int e = part * THREADS + threadIdx.x; e < ROWS * rows; e += THREADS * p.parts) {
-    const int row = e % ROWS, m = e / ROWS, at = row * WIDTH + m * TERMS;
-    float v = sums[at];
-    if (p.parts > 1) {
-      float x[MOST_PARTS];
+  else __syncthreads();
+  const int n_cta = static_cast<int>(blockIdx.x / p.parts) * WARPS * ROWS;
+  for (int e = part * THREADS + threadIdx.x; e < WARPS * ROWS * rows; e += THREADS * p.parts) {
+    const int row = e % (WARPS * ROWS), m = e / (WARPS * ROWS), n = n_cta + row;
+    const float* at = sums + row * WIDTH + m * TERMS;
+    float v = 0.f;
+    if (p.parts == 1) {
+#pragma unroll
+      for (int c = TERMS - 1; c >= 0; --c) v += at[c];
+    } else {
+      float x[MOST_PARTS][TERMS];
 #pragma unroll
       for (int q = 0; q < MOST_PARTS; ++q)
         if (q < p.parts)
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[q]) : "r"(map_to_cta(sums + at, static_cast<uint32_t>(q))));
-      v = 0.f;
+#pragma unroll
+          for (int c = 0; c < TERMS; ++c)
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[q][c]) : "r"(map_to_cta(at + c, static_cast<uint32_t>(q))));
 #pragma unroll
       for (int q = 0; q < MOST_PARTS; ++q)
-        if (q < p.parts) v += x[q];
+        if (q < p.parts)
+#pragma unroll
+          for (int c = TERMS - 1; c >= 0; --c) v += x[q][c];
     }
-    const int n = n0 + row;
     if (n < p.N) {
       if (p.bias) v += __ldg(p.bias + n);
       store_elem(p.out, static_cast<int64_t>(m0 + m) * p.N + n, p.out_dtype, p.silu_out ? silu(v) : v);
@@ -440,24 +443,20 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
 }
 
 constexpr int WANTED = 4;
-constexpr int X_BYTES = 96 * 1024;  // x in shared memory at a time, at most: one ROUND of 48 columns
+constexpr int X_BYTES = 48 * 1024;  // x in shared memory at a time, at most
 
 template <typename T, int TERMS, int COLS8, int G>
 int launch_g(Params& p, int passes, cudaStream_t st) {
   auto kernel = gemv_q4_kernel<T, TERMS, COLS8, G>;
   const int cols = p.pass_rows * TERMS;
-  const int64_t tiles = (p.N + ROWS - 1) / ROWS;
-  // parts of K over a cluster's CTAs: as many as give every SM two CTAs, or as keep a part of x in shared memory
+  const int64_t tiles = (p.N + WARPS * ROWS - 1) / (WARPS * ROWS);
+  // parts of K over a cluster's CTAs: as many as still run at once
   int parts = 1;
-  const int64_t wanted = WANTED * num_sms();
-  while (parts < MOST_PARTS && p.K > parts * ROUND &&
-         (tiles * passes * parts < wanted || static_cast<int64_t>(p.K) * cols * 2 / parts > X_BYTES))
-    parts *= 2;
+  while (parts < MOST_PARTS && p.K > parts * STEP && tiles * passes * parts * 2 <= WANTED * num_sms()) parts *= 2;
   p.parts = parts;
   p.part_k = ((p.K + parts - 1) / parts + STEP - 1) / STEP * STEP;
-  const int most = X_BYTES / (cols * 2) / ROUND * ROUND;
-  const int whole = (p.part_k + ROUND - 1) / ROUND * ROUND;
-  p.chunk_k = whole < most ? whole : most;
+  const int most = X_BYTES / (cols * 2) / STEP * STEP;
+  p.chunk_k = p.part_k < most ? p.part_k : most;
   const int used = WARPS * STAGES * SLOT + p.chunk_k * cols * 2;
   const int sums = WARPS * ROWS * COLS8 * 8 * 4;
   const int smem = 1024 + (used > sums ? used : sums);
