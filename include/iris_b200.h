@@ -146,20 +146,30 @@ int iris_qkv_heads(const void* qkv, int64_t batch, int64_t tokens, int64_t row_s
                    float eps, void* q_out, void* k_out, void* v_out, int64_t n_out, int64_t n_out_kv, int64_t offset,
                    int head_major, void* stream);
 
-/* Rotary positions on their own (the text side's heads; no QK norm), in any
- * strides: x and out hold rows [batch, heads, n, head_dim] (element strides of the
- * first three, head_dim contiguous; out may be x). The first `rotary` columns
- * turn by pairs (IRIS_ROPE_*) through row p of the fp32 tables [table_rows,
- * rotary / 2], the others are copied; p = positions[b * positions_stride + t]
- * (int32, or int64 with positions_64 != 0), or t where positions is null.
- * inverse != 0 turns back. A position outside the table gives a NaN row and sets
- * bit 1 of the device error word. The reference's counterpart is apply_rope,
- * src/iris3b/nn/rope.py:92-101 (interleaved, whole head, positions in order). */
-int iris_rope(const void* x, int dtype, int64_t batch, int64_t heads, int64_t n, int64_t head_dim, int64_t x_stride_b,
-              int64_t x_stride_h, int64_t x_stride_n, void* out, int64_t out_stride_b, int64_t out_stride_h,
-              int64_t out_stride_n, const float* cos, const float* sin, int64_t rotary, int64_t table_rows,
-              const void* positions, int positions_64, int64_t positions_stride, int layout, int inverse,
-              void* stream);
+/* Head rows [batch, heads, n, head_dim]: element strides of the first three
+ * dimensions, head_dim contiguous. */
+typedef struct iris_head_rows {
+  void* data;
+  int64_t stride_b, stride_h, stride_n;
+} iris_head_rows;
+
+/* Rotary positions on their own (the text side's heads; no QK norm): the first
+ * `rotary` columns of each row turn by pairs (IRIS_ROPE_*) through row p of the fp32
+ * tables [table_rows, rotary / 2], the others are copied; p = positions[b *
+ * positions_stride + t] (int32, or int64 with positions_64 != 0), or t where positions
+ * is null. out may be x. inverse != 0 turns back. A position outside the table gives
+ * a NaN row and sets bit 1 of the device error word. The reference's counterpart is
+ * apply_rope, src/iris3b/nn/rope.py:92-101 (interleaved, whole head, positions in
+ * order). */
+typedef struct iris_rope_problem {
+  iris_head_rows x, out;
+  const float* cos;
+  const float* sin;
+  const void* positions;
+  int64_t positions_stride, positions_64;
+  int64_t dtype, batch, heads, n, head_dim, rotary, table_rows, layout, inverse;
+} iris_rope_problem;
+int iris_rope(const iris_rope_problem* problem, void* stream);
 
 /* The same rotation of q and k with the append of k and v to a cache
  * [batch, heads_kv, capacity, head_dim] of the same type, in one launch (no
@@ -171,14 +181,15 @@ int iris_rope(const void* x, int dtype, int64_t batch, int64_t heads, int64_t n,
  * for one slot the later is kept. Rows from counts[b] on are left as they are. A
  * position outside the table (NaN row, nothing appended) or past the end of a
  * plain cache (nothing appended) sets bit 1 of the device error word. */
-int iris_rope_append(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads_q,
-                     int64_t heads_kv, int64_t n, int64_t head_dim, int64_t q_stride_b, int64_t q_stride_h,
-                     int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b,
-                     int64_t v_stride_h, int64_t v_stride_n, void* out, int64_t out_stride_b, int64_t out_stride_h,
-                     int64_t out_stride_n, void* k_cache, int64_t kc_stride_b, int64_t kc_stride_h, int64_t kc_stride_n,
-                     void* v_cache, int64_t vc_stride_b, int64_t vc_stride_h, int64_t vc_stride_n, int64_t capacity,
-                     int64_t sinks, const float* cos, const float* sin, int64_t rotary, int64_t table_rows,
-                     const int* starts, const int* counts, int layout, void* stream);
+typedef struct iris_append_problem {
+  iris_head_rows q, k, v, out, k_cache, v_cache;
+  const float* cos;
+  const float* sin;
+  const int* starts;
+  const int* counts;
+  int64_t dtype, batch, heads_q, heads_kv, n, head_dim, rotary, table_rows, capacity, sinks, layout;
+} iris_append_problem;
+int iris_rope_append(const iris_append_problem* problem, void* stream);
 
 /* ---- tensor-core kernels ------------------------------------------------ */
 /* F.linear in the step (src/iris_metal/model.py:46-52): C = epi(A W^T).
@@ -296,22 +307,26 @@ int iris_flash_attn_fwd_peers(const void* q, const void* k, const void* v, int64
  * no bound. out[b, i, h * head_dim + d] = sum_j softmax_j(scale q . k_j) v_j over the
  * visible keys, 0 where there is none; what lies in other keys' rows, NaN
  * included, does not reach a row. q [batch, heads_q, n, head_dim], k / v [batch,
- * heads_kv, n_kv, head_dim], bf16 or f16, element strides of the first three
- * dimensions (multiples of 8; 0 repeats a head or a sample), head_dim 64 or 128
- * contiguous. */
-int iris_window_attn_fwd(const void* q, const void* k, const void* v, void* out, int dtype, int64_t batch,
-                         int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv, int64_t head_dim,
-                         int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
-                         int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
-                         int64_t v_stride_n, int64_t out_stride_b, int64_t out_stride_n, const int* starts,
-                         const int* lengths, int64_t left, int64_t right, int64_t sinks, float scale, void* workspace,
-                         int64_t workspace_bytes, void* stream);
+ * heads_kv, n_kv, head_dim], bf16 or f16, strides multiples of 8 (0 repeats a head or
+ * a sample), head_dim 64 or 128. workspace: iris_window_attn_workspace bytes. */
+typedef struct iris_window_problem {
+  iris_head_rows q, k, v;
+  void* out;
+  int64_t out_stride_b, out_stride_n;
+  const int* starts;
+  const int* lengths;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t dtype, batch, heads_q, heads_kv, n, n_kv, head_dim, left, right, sinks;
+  double scale;
+} iris_window_problem;
+int iris_window_attn_fwd(const iris_window_problem* problem, void* stream);
 
 /* Bytes of workspace (16-byte aligned; null for 0) that iris_window_attn_fwd needs for
- * these sizes: a few rows' keys are split over CTAs and the parts joined there. Two
- * calls that may run at the same time need one each. */
-int iris_window_attn_workspace(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv,
-                               int64_t head_dim, int64_t left, int64_t right, int64_t sinks, int64_t* bytes);
+ * a problem's sizes, window and type (its pointers and strides are not read): a few
+ * rows' keys are split over CTAs and the parts joined there. Two calls that may run
+ * at the same time need one each. */
+int iris_window_attn_workspace(const iris_window_problem* problem, int64_t* bytes);
 
 /* ---- peer memory (sequence parallelism across processes) ---------------- */
 /* No reference counterpart. iris_ipc_export: the IPC handle (IRIS_IPC_HANDLE_BYTES)
@@ -408,13 +423,20 @@ int iris_gemv(const float* x, int64_t M, int64_t K, const void* w, int w_dtype, 
 /* The small-M linear over 4-bit weights (iris_gemv with a quarter of the BF16
  * weights' bytes): w[n, k] = scale[n, k / group] (q[n, k] - zero[n, k / group]), q the
  * low (k even) or high nibble of packed[n, k / 2], scale bf16 [N, K / group], zero
- * uint8 [N, K / group] or null (8 everywhere), group 32, 64 or 128;
+ * uint8 [N, K / group] of 0 to 15 or null (8 everywhere), group 32, 64 or 128;
  * out[m, n] = act_out(sum_k act_in(x[m, k]) w[n, k] + bias[n]), the activations silu
  * where asked for, bias fp32 or null. x [M, K] with row stride ldx, M <= 64; fp32
  * sums; out [M, N] contiguous. */
-int iris_gemv_q4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const void* packed, const void* scale,
-                 const void* zero, int64_t group, const float* bias, void* out, int out_dtype, int64_t N, int silu_in,
-                 int silu_out, void* stream);
+typedef struct iris_q4_problem {
+  const void* x;
+  const void* packed;
+  const void* scale;
+  const void* zero;
+  const float* bias;
+  void* out;
+  int64_t M, K, N, ldx, group, x_dtype, out_dtype, silu_in, silu_out;
+} iris_q4_problem;
+int iris_gemv_q4(const iris_q4_problem* problem, void* stream);
 
 /* Per-block modulation rows, SharedCoreBias.forward (src/iris3b/nn/modulation.py:284-285):
  * out[j, b, :] = core[b, :] + bias[j, :] for j < n_blocks. */

@@ -508,29 +508,30 @@ int launch_rows(Params& p, int64_t group, cudaStream_t st) {
 
 using namespace iris;
 
-extern "C" int iris_gemv_q4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, const void* packed,
-                            const void* scale, const void* zero, int64_t group, const float* bias, void* out,
-                            int out_dtype, int64_t N, int silu_in, int silu_out, void* stream) {
+extern "C" int iris_gemv_q4(const iris_q4_problem* q, void* stream) {
   using namespace iris::q4;
-  IRIS_REQUIRE(x && packed && scale && out, "gemv_q4: null pointer");
-  IRIS_REQUIRE(group == 32 || group == 64 || group == 128, "gemv_q4: groups of 32, 64 or 128 weights");
-  IRIS_REQUIRE(M > 0 && M <= 64 && N > 0 && K > 0 && K % group == 0, "gemv_q4: 1 to 64 rows; K must be a multiple of the group");
-  IRIS_REQUIRE(N < (1ll << 28) && K < (1ll << 28) && ldx >= K, "gemv_q4: size");
-  IRIS_REQUIRE(x_dtype >= IRIS_F32 && x_dtype <= IRIS_F16 && out_dtype >= IRIS_F32 && out_dtype <= IRIS_F16, "gemv_q4: bad dtype");
-  IRIS_REQUIRE(aligned16(x) && aligned16(packed) && aligned_n(scale, 2) && ldx % 8 == 0,
+  IRIS_REQUIRE(q != nullptr && q->x && q->packed && q->scale && q->out, "gemv_q4: null pointer");
+  IRIS_REQUIRE(q->group == 32 || q->group == 64 || q->group == 128, "gemv_q4: groups of 32, 64 or 128 weights");
+  IRIS_REQUIRE(q->M > 0 && q->M <= 64 && q->N > 0 && q->K > 0 && q->K % q->group == 0,
+               "gemv_q4: 1 to 64 rows; K must be a multiple of the group");
+  IRIS_REQUIRE(q->N < (1ll << 28) && q->K < (1ll << 28) && q->ldx >= q->K, "gemv_q4: size");
+  IRIS_REQUIRE(q->x_dtype >= IRIS_F32 && q->x_dtype <= IRIS_F16 && q->out_dtype >= IRIS_F32 && q->out_dtype <= IRIS_F16,
+               "gemv_q4: bad dtype");
+  IRIS_REQUIRE(aligned16(q->x) && aligned16(q->packed) && aligned_n(q->scale, 2) && q->ldx % 8 == 0,
                "gemv_q4: x rows and weights must be 16-byte aligned");
   Params p = {};
-  p.x = x, p.x_dtype = x_dtype, p.M = static_cast<int>(M), p.K = static_cast<int>(K), p.ldx = ldx;
-  p.packed = static_cast<const uint8_t*>(packed), p.scale = static_cast<const __nv_bfloat16*>(scale);
-  p.zero = static_cast<const uint8_t*>(zero), p.bias = bias, p.out = out, p.out_dtype = out_dtype;
-  p.N = static_cast<int>(N), p.silu_in = silu_in, p.silu_out = silu_out;
+  p.x = q->x, p.x_dtype = static_cast<int>(q->x_dtype), p.M = static_cast<int>(q->M), p.K = static_cast<int>(q->K);
+  p.ldx = q->ldx, p.packed = static_cast<const uint8_t*>(q->packed);
+  p.scale = static_cast<const __nv_bfloat16*>(q->scale), p.zero = static_cast<const uint8_t*>(q->zero);
+  p.bias = q->bias, p.out = q->out, p.out_dtype = static_cast<int>(q->out_dtype), p.N = static_cast<int>(q->N);
+  p.silu_in = q->silu_in != 0, p.silu_out = q->silu_out != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (x_dtype == IRIS_F32 || silu_in) {  // fp32 values: three columns a row
-    if (M <= 2) return launch<__nv_bfloat16, 3, 1>(p, group, st);
-    if (M <= 5) return launch<__nv_bfloat16, 3, 2>(p, group, st);
-    if (M <= 8) return launch<__nv_bfloat16, 3, 3>(p, group, st);
-    return launch<__nv_bfloat16, 3, 6>(p, group, st);
+  if (p.x_dtype == IRIS_F32 || p.silu_in) {  // fp32 values: three columns a row
+    if (p.M <= 2) return launch<__nv_bfloat16, 3, 1>(p, q->group, st);
+    if (p.M <= 5) return launch<__nv_bfloat16, 3, 2>(p, q->group, st);
+    if (p.M <= 8) return launch<__nv_bfloat16, 3, 3>(p, q->group, st);
+    return launch<__nv_bfloat16, 3, 6>(p, q->group, st);
   }
-  if (x_dtype == IRIS_F16) return launch_rows<__half>(p, group, st);
-  return launch_rows<__nv_bfloat16>(p, group, st);
+  if (p.x_dtype == IRIS_F16) return launch_rows<__half>(p, q->group, st);
+  return launch_rows<__nv_bfloat16>(p, q->group, st);
 }

@@ -198,15 +198,15 @@ int launch(Params& a, bool half, cudaStream_t st) {
 }
 
 template <bool APPEND>
-int dispatch(Params& a, int dtype, bool half, void* stream) {
+int dispatch(Params& a, int64_t dtype, bool half, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == IRIS_F32) return launch<float, APPEND>(a, half, st);
   if (dtype == IRIS_BF16) return launch<__nv_bfloat16, APPEND>(a, half, st);
   return launch<__half, APPEND>(a, half, st);
 }
 
-inline int check(int dtype, int64_t batch, int64_t heads, int64_t n, int64_t head_dim, int64_t rotary, int64_t table_rows,
-                 int layout) {
+inline int check(int64_t dtype, int64_t batch, int64_t heads, int64_t n, int64_t head_dim, int64_t rotary,
+                 int64_t table_rows, int64_t layout) {
   IRIS_REQUIRE(dtype >= IRIS_F32 && dtype <= IRIS_F16, "rope: bad dtype");
   IRIS_REQUIRE(batch >= 0 && n >= 0 && heads > 0 && batch < (1ll << 31) && n < (1ll << 31) && batch * n < (1ll << 31),
                "rope: bad row counts");
@@ -222,64 +222,63 @@ inline int check(int dtype, int64_t batch, int64_t heads, int64_t n, int64_t hea
 
 using namespace iris;
 
-extern "C" int iris_rope(const void* x, int dtype, int64_t batch, int64_t heads, int64_t n, int64_t head_dim,
-                         int64_t x_stride_b, int64_t x_stride_h, int64_t x_stride_n, void* out, int64_t out_stride_b,
-                         int64_t out_stride_h, int64_t out_stride_n, const float* cos, const float* sin, int64_t rotary,
-                         int64_t table_rows, const void* positions, int positions_64, int64_t positions_stride,
-                         int layout, int inverse, void* stream) {
+namespace {
+iris::rope::View view(const iris_head_rows& from, const iris_head_rows& to) {
+  return iris::rope::View{from.data, from.stride_b, from.stride_h, from.stride_n, to.data, to.stride_b, to.stride_h, to.stride_n};
+}
+}  // namespace
+
+extern "C" int iris_rope(const iris_rope_problem* q, void* stream) {
   using namespace iris::rope;
-  IRIS_CHECK_STATUS(check(dtype, batch, heads, n, head_dim, rotary, table_rows, layout));
-  if (batch * n == 0) return IRIS_OK;
-  IRIS_REQUIRE(x && out && cos && sin, "rope: null pointer");
+  IRIS_REQUIRE(q != nullptr, "rope: null pointer");
+  IRIS_CHECK_STATUS(check(q->dtype, q->batch, q->heads, q->n, q->head_dim, q->rotary, q->table_rows, q->layout));
+  if (q->batch * q->n == 0) return IRIS_OK;
+  IRIS_REQUIRE(q->x.data && q->out.data && q->cos && q->sin, "rope: null pointer");
   Params a = {};
-  a.q = View{x, x_stride_b, x_stride_h, x_stride_n, out, out_stride_b, out_stride_h, out_stride_n};
-  a.heads_q = static_cast<int>(heads);
-  a.n = static_cast<int>(n);
-  a.head_dim = static_cast<int>(head_dim);
-  a.rotary = static_cast<int>(rotary);
-  a.tokens = batch * n;
-  a.cos = cos;
-  a.sin = sin;
-  a.table_rows = table_rows;
-  a.positions = positions;
-  a.pos_stride = positions_stride;
-  a.pos64 = positions_64;
-  a.sign = inverse ? -1.f : 1.f;
-  return dispatch<false>(a, dtype, layout == IRIS_ROPE_HALF, stream);
+  a.q = view(q->x, q->out);
+  a.heads_q = static_cast<int>(q->heads);
+  a.n = static_cast<int>(q->n);
+  a.head_dim = static_cast<int>(q->head_dim);
+  a.rotary = static_cast<int>(q->rotary);
+  a.tokens = q->batch * q->n;
+  a.cos = q->cos;
+  a.sin = q->sin;
+  a.table_rows = q->table_rows;
+  a.positions = q->positions;
+  a.pos_stride = q->positions_stride;
+  a.pos64 = q->positions_64 != 0;
+  a.sign = q->inverse ? -1.f : 1.f;
+  return dispatch<false>(a, q->dtype, q->layout == IRIS_ROPE_HALF, stream);
 }
 
-extern "C" int iris_rope_append(const void* q, const void* k, const void* v, int dtype, int64_t batch, int64_t heads_q,
-                                int64_t heads_kv, int64_t n, int64_t head_dim, int64_t q_stride_b, int64_t q_stride_h,
-                                int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_n,
-                                int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_n, void* out,
-                                int64_t out_stride_b, int64_t out_stride_h, int64_t out_stride_n, void* k_cache,
-                                int64_t kc_stride_b, int64_t kc_stride_h, int64_t kc_stride_n, void* v_cache,
-                                int64_t vc_stride_b, int64_t vc_stride_h, int64_t vc_stride_n, int64_t capacity,
-                                int64_t sinks, const float* cos, const float* sin, int64_t rotary, int64_t table_rows,
-                                const int* starts, const int* counts, int layout, void* stream) {
+extern "C" int iris_rope_append(const iris_append_problem* q, void* stream) {
   using namespace iris::rope;
-  IRIS_CHECK_STATUS(check(dtype, batch, heads_q, n, head_dim, rotary, table_rows, layout));
-  IRIS_REQUIRE(heads_kv > 0 && heads_kv <= 65536, "rope_append: bad head counts");
-  IRIS_REQUIRE(capacity > 0 && sinks >= -1 && sinks < capacity, "rope_append: a rolling cache needs more slots than sinks");
-  if (batch * n == 0) return IRIS_OK;
-  IRIS_REQUIRE(q && k && v && out && k_cache && v_cache && cos && sin && starts, "rope_append: null pointer");
+  IRIS_REQUIRE(q != nullptr, "rope_append: null pointer");
+  IRIS_CHECK_STATUS(check(q->dtype, q->batch, q->heads_q, q->n, q->head_dim, q->rotary, q->table_rows, q->layout));
+  IRIS_REQUIRE(q->heads_kv > 0 && q->heads_kv <= 65536, "rope_append: bad head counts");
+  IRIS_REQUIRE(q->capacity > 0 && q->sinks >= -1 && q->sinks < q->capacity,
+               "rope_append: a rolling cache needs more slots than sinks");
+  if (q->batch * q->n == 0) return IRIS_OK;
+  IRIS_REQUIRE(q->q.data && q->k.data && q->v.data && q->out.data && q->k_cache.data && q->v_cache.data && q->cos &&
+                   q->sin && q->starts,
+               "rope_append: null pointer");
   Params a = {};
-  a.q = View{q, q_stride_b, q_stride_h, q_stride_n, out, out_stride_b, out_stride_h, out_stride_n};
-  a.k = View{k, k_stride_b, k_stride_h, k_stride_n, k_cache, kc_stride_b, kc_stride_h, kc_stride_n};
-  a.v = View{v, v_stride_b, v_stride_h, v_stride_n, v_cache, vc_stride_b, vc_stride_h, vc_stride_n};
-  a.heads_q = static_cast<int>(heads_q);
-  a.heads_kv = static_cast<int>(heads_kv);
-  a.n = static_cast<int>(n);
-  a.head_dim = static_cast<int>(head_dim);
-  a.rotary = static_cast<int>(rotary);
-  a.tokens = batch * n;
-  a.cos = cos;
-  a.sin = sin;
-  a.table_rows = table_rows;
+  a.q = view(q->q, q->out);
+  a.k = view(q->k, q->k_cache);
+  a.v = view(q->v, q->v_cache);
+  a.heads_q = static_cast<int>(q->heads_q);
+  a.heads_kv = static_cast<int>(q->heads_kv);
+  a.n = static_cast<int>(q->n);
+  a.head_dim = static_cast<int>(q->head_dim);
+  a.rotary = static_cast<int>(q->rotary);
+  a.tokens = q->batch * q->n;
+  a.cos = q->cos;
+  a.sin = q->sin;
+  a.table_rows = q->table_rows;
   a.sign = 1.f;
-  a.starts = starts;
-  a.counts = counts;
-  a.capacity = capacity;
-  a.sinks = sinks;
-  return dispatch<true>(a, dtype, layout == IRIS_ROPE_HALF, stream);
+  a.starts = q->starts;
+  a.counts = q->counts;
+  a.capacity = q->capacity;
+  a.sinks = q->sinks;
+  return dispatch<true>(a, q->dtype, q->layout == IRIS_ROPE_HALF, stream);
 }

@@ -985,16 +985,23 @@ int launch(const Params& p, int dtype, void* workspace, int64_t workspace_bytes,
 
 inline int64_t bound(int64_t v) { return v < 0 || v > kNoBound ? kNoBound : v; }
 
-inline int check_sizes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv, int64_t head_dim,
-                       int64_t left, int64_t right, int64_t sinks) {
-  IRIS_REQUIRE(head_dim == 64 || head_dim == 128, "window_attn_fwd: head_dim must be 64 or 128");
-  IRIS_REQUIRE(heads_q > 0 && heads_kv > 0 && heads_q % heads_kv == 0,
+inline int check_sizes(const iris_window_problem& q) {
+  IRIS_REQUIRE(q.dtype == IRIS_BF16 || q.dtype == IRIS_F16, "window_attn_fwd: bf16 or f16");
+  IRIS_REQUIRE(q.head_dim == 64 || q.head_dim == 128, "window_attn_fwd: head_dim must be 64 or 128");
+  IRIS_REQUIRE(q.heads_q > 0 && q.heads_kv > 0 && q.heads_q % q.heads_kv == 0,
                "window_attn_fwd: heads_q must be a positive multiple of heads_kv");
-  IRIS_REQUIRE(batch >= 0 && n >= 0 && n_kv >= 0 && batch <= 65535 && heads_q <= 65535 && n < (1ll << 30) &&
-                   n_kv < (1ll << 30),
+  IRIS_REQUIRE(q.batch >= 0 && q.n >= 0 && q.n_kv >= 0 && q.batch <= 65535 && q.heads_q <= 65535 &&
+                   q.n < (1ll << 30) && q.n_kv < (1ll << 30),
                "window_attn_fwd: sizes");
-  IRIS_REQUIRE(left >= -1 && right >= -1 && sinks >= 0, "window_attn_fwd: window bounds are -1 (none) or more");
+  IRIS_REQUIRE(q.left >= -1 && q.right >= -1 && q.sinks >= 0, "window_attn_fwd: window bounds are -1 (none) or more");
   return IRIS_OK;
+}
+
+inline bool rows_aligned(const iris_head_rows& r) {
+  return aligned16(r.data) && r.stride_b % 8 == 0 && r.stride_h % 8 == 0 && r.stride_n % 8 == 0;
+}
+inline bool rows_apart(const iris_head_rows& r, int64_t n) {
+  return r.stride_b >= 0 && r.stride_h >= 0 && (n <= 1 || r.stride_n > 0);
 }
 
 }  // namespace window
@@ -1002,54 +1009,49 @@ inline int check_sizes(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t
 
 using namespace iris;
 
-extern "C" int iris_window_attn_workspace(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv,
-                                          int64_t head_dim, int64_t left, int64_t right, int64_t sinks, int64_t* bytes) {
+extern "C" int iris_window_attn_workspace(const iris_window_problem* q, int64_t* bytes) {
   using namespace iris::window;
-  IRIS_REQUIRE(bytes != nullptr, "window_attn_workspace: null output");
-  IRIS_CHECK_STATUS(check_sizes(batch, heads_q, heads_kv, n, n_kv, head_dim, left, right, sinks));
+  IRIS_REQUIRE(q != nullptr && bytes != nullptr, "window_attn_workspace: null pointer");
+  IRIS_CHECK_STATUS(check_sizes(*q));
   *bytes = 0;
-  if (batch * n == 0 || n_kv == 0 || !few_rows(n, heads_q / heads_kv)) return IRIS_OK;
+  if (q->batch * q->n == 0 || q->n_kv == 0 || !few_rows(q->n, q->heads_q / q->heads_kv)) return IRIS_OK;
   Split sp = {};
-  split_keys(batch, heads_q, heads_kv, n, n_kv, bound(left), bound(right), sinks < n_kv ? sinks : n_kv, &sp);
-  if (sp.splits > 1) *bytes = batch * heads_kv * sp.row_tiles * sp.splits * STEP_ROWS * (head_dim + 2) * 4;
+  split_keys(q->batch, q->heads_q, q->heads_kv, q->n, q->n_kv, bound(q->left), bound(q->right),
+             q->sinks < q->n_kv ? q->sinks : q->n_kv, &sp);
+  if (sp.splits > 1) *bytes = q->batch * q->heads_kv * sp.row_tiles * sp.splits * STEP_ROWS * (q->head_dim + 2) * 4;
   return IRIS_OK;
 }
 
-extern "C" int iris_window_attn_fwd(const void* q, const void* k, const void* v, void* out, int dtype, int64_t batch,
-                                    int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv, int64_t head_dim,
-                                    int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_n, int64_t k_stride_b,
-                                    int64_t k_stride_h, int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_h,
-                                    int64_t v_stride_n, int64_t out_stride_b, int64_t out_stride_n, const int* starts,
-                                    const int* lengths, int64_t left, int64_t right, int64_t sinks, float scale,
-                                    void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int iris_window_attn_fwd(const iris_window_problem* q, void* stream) {
   using namespace iris::window;
-  IRIS_REQUIRE(dtype == IRIS_BF16 || dtype == IRIS_F16, "window_attn_fwd: bf16 or f16");
-  IRIS_CHECK_STATUS(check_sizes(batch, heads_q, heads_kv, n, n_kv, head_dim, left, right, sinks));
+  IRIS_REQUIRE(q != nullptr, "window_attn_fwd: null pointer");
+  IRIS_CHECK_STATUS(check_sizes(*q));
+  const float scale = static_cast<float>(q->scale);
   IRIS_REQUIRE(scale > 0.f && scale < INFINITY, "window_attn_fwd: scale must be positive and finite");
-  IRIS_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && q_stride_b % 8 == 0 &&
-                   q_stride_h % 8 == 0 && q_stride_n % 8 == 0 && k_stride_b % 8 == 0 && k_stride_h % 8 == 0 &&
-                   k_stride_n % 8 == 0 && v_stride_b % 8 == 0 && v_stride_h % 8 == 0 && v_stride_n % 8 == 0 &&
-                   out_stride_b % 8 == 0 && out_stride_n % 8 == 0,
+  IRIS_REQUIRE(rows_aligned(q->q) && rows_aligned(q->k) && rows_aligned(q->v) && aligned16(q->out) &&
+                   q->out_stride_b % 8 == 0 && q->out_stride_n % 8 == 0,
                "window_attn_fwd: pointers and strides must be multiples of 16 bytes");
-  IRIS_REQUIRE((n <= 1 || q_stride_n > 0) && (n_kv <= 1 || (k_stride_n > 0 && v_stride_n > 0)) && q_stride_b >= 0 &&
-                   q_stride_h >= 0 && k_stride_b >= 0 && k_stride_h >= 0 && v_stride_b >= 0 && v_stride_h >= 0,
+  IRIS_REQUIRE(rows_apart(q->q, q->n) && rows_apart(q->k, q->n_kv) && rows_apart(q->v, q->n_kv),
                "window_attn_fwd: rows must not repeat along the tokens");
-  if (batch * n == 0) return IRIS_OK;
-  IRIS_REQUIRE(q && out && ((k && v) || n_kv == 0), "window_attn_fwd: null pointer");
+  if (q->batch * q->n == 0) return IRIS_OK;
+  IRIS_REQUIRE(q->q.data && q->out && ((q->k.data && q->v.data) || q->n_kv == 0), "window_attn_fwd: null pointer");
   Params p = {};
-  p.q = q, p.k = k, p.v = v, p.out = out;
-  p.qb = q_stride_b, p.qh = q_stride_h, p.qn = q_stride_n;
-  p.kb = k_stride_b, p.kh = k_stride_h, p.kn = k_stride_n;
-  p.vb = v_stride_b, p.vh = v_stride_h, p.vn = v_stride_n;
-  p.ob = out_stride_b, p.on = out_stride_n;
-  p.batch = static_cast<int>(batch), p.heads_q = static_cast<int>(heads_q), p.heads_kv = static_cast<int>(heads_kv);
-  p.n = static_cast<int>(n), p.n_kv = static_cast<int>(n_kv);
-  p.starts = starts, p.lengths = lengths;
-  p.left = bound(left), p.right = bound(right);
-  p.sinks = static_cast<int>(sinks < n_kv ? sinks : n_kv);
+  p.q = q->q.data, p.k = q->k.data, p.v = q->v.data, p.out = q->out;
+  p.qb = q->q.stride_b, p.qh = q->q.stride_h, p.qn = q->q.stride_n;
+  p.kb = q->k.stride_b, p.kh = q->k.stride_h, p.kn = q->k.stride_n;
+  p.vb = q->v.stride_b, p.vh = q->v.stride_h, p.vn = q->v.stride_n;
+  p.ob = q->out_stride_b, p.on = q->out_stride_n;
+  p.batch = static_cast<int>(q->batch), p.heads_q = static_cast<int>(q->heads_q);
+  p.heads_kv = static_cast<int>(q->heads_kv), p.n = static_cast<int>(q->n), p.n_kv = static_cast<int>(q->n_kv);
+  p.starts = q->starts, p.lengths = q->lengths;
+  p.left = bound(q->left), p.right = bound(q->right);
+  p.sinks = static_cast<int>(q->sinks < q->n_kv ? q->sinks : q->n_kv);
   p.scale_log2 = scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int dtype = static_cast<int>(q->dtype);
   if (dtype == IRIS_BF16)
-    return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, dtype, workspace, workspace_bytes, st) : launch<__nv_bfloat16, 64>(p, dtype, workspace, workspace_bytes, st);
-  return head_dim == 128 ? launch<__half, 128>(p, dtype, workspace, workspace_bytes, st) : launch<__half, 64>(p, dtype, workspace, workspace_bytes, st);
+    return q->head_dim == 128 ? launch<__nv_bfloat16, 128>(p, dtype, q->workspace, q->workspace_bytes, st)
+                              : launch<__nv_bfloat16, 64>(p, dtype, q->workspace, q->workspace_bytes, st);
+  return q->head_dim == 128 ? launch<__half, 128>(p, dtype, q->workspace, q->workspace_bytes, st)
+                            : launch<__half, 64>(p, dtype, q->workspace, q->workspace_bytes, st);
 }

@@ -8,6 +8,7 @@ symbols. ``call`` raises ``ValueError`` for a rejected argument
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().parent / "libiris_b200.so"
@@ -100,12 +101,15 @@ SIGNATURES["iris_ipc_close"] = [P]
 SIGNATURES["iris_peer_barrier"] = [P, P, I32, I32, ctypes.c_uint, I64, P]
 SIGNATURES["iris_flash_attn_fwd_split"] = [P, P, P, I64, I64, I64, I64, I64, I64, F, F, I64, P, P, P, P, I64, P]
 
-SIGNATURES["iris_rope"] = [P, I32, *[I64] * 7, P, *[I64] * 3, P, P, I64, I64, P, I32, I64, I32, I32, P]
-SIGNATURES["iris_rope_append"] = [P, P, P, I32, *[I64] * 14, P, *[I64] * 3, P, *[I64] * 3, P, *[I64] * 5, P, P, I64, I64,
-                                  P, P, I32, P]  # fmt: skip
-SIGNATURES["iris_window_attn_fwd"] = [P, P, P, P, I32, *[I64] * 17, P, P, I64, I64, I64, F, P, I64, P]
-SIGNATURES["iris_window_attn_workspace"] = [*[I64] * 9, ctypes.POINTER(I64)]
-SIGNATURES["iris_gemv_q4"] = [P, I32, I64, I64, I64, P, P, P, I64, P, P, I32, I64, I32, I32, P]
+# Problems of one struct of 8-byte members, packed from plain integers (pointers as
+# addresses, 0 for none): a call then takes two arguments, not forty.
+ROPE_PROBLEM = struct.Struct("@22q")  # iris_rope_problem
+APPEND_PROBLEM = struct.Struct("@39q")  # iris_append_problem
+WINDOW_PROBLEM = struct.Struct("@29qd")  # iris_window_problem
+Q4_PROBLEM = struct.Struct("@15q")  # iris_q4_problem
+for _name in ("iris_rope", "iris_rope_append", "iris_window_attn_fwd", "iris_gemv_q4"):
+    SIGNATURES[_name] = [P, P]
+SIGNATURES["iris_window_attn_workspace"] = [P, ctypes.POINTER(I64)]
 
 _lib: ctypes.CDLL | None = None
 

@@ -2,10 +2,12 @@
 scaled rotary tables and the 4-bit packing."""
 
 import math
+import re
 
 import pytest
 import torch
 
+from conftest import REPO
 from text_side import unpacked
 from test_library import _einval, lib  # noqa: F401 (lib: the built library)
 
@@ -17,42 +19,65 @@ def K():
     return kernels
 
 
+def test_problem_structs_match_the_header():
+    """Every struct is 8-byte members in the order that the binding packs them."""
+    from iris_b200 import _lib
+
+    text = re.sub(r"/\*.*?\*/", "", (REPO / "include" / "iris_b200.h").read_text(), flags=re.S)
+    for name, packing in [("rope", _lib.ROPE_PROBLEM), ("append", _lib.APPEND_PROBLEM), ("window", _lib.WINDOW_PROBLEM),
+                          ("q4", _lib.Q4_PROBLEM)]:  # fmt: skip
+        body = re.search(rf"typedef struct iris_{name}_problem {{(.*?)}}", text, flags=re.S).group(1)
+        fields = 0
+        for line in filter(str.strip, body.split(";")):
+            kind = re.match(r"\s*(const )?(iris_head_rows|void\*|float\*|int\*|int64_t|double)", line).group(2)
+            fields += (4 if kind == "iris_head_rows" else 1) * (line.count(",") + 1)
+        assert packing.size == 8 * fields, name
+
+
 def test_c_entries_refuse_bad_arguments(lib):  # noqa: F811
-    def rope(dtype=1, batch=1, heads=2, n=3, dim=64, rotary=64, rows=9, layout=0, x=16):
-        return ("iris_rope", x, dtype, batch, heads, n, dim, 0, 0, 0, 16, 0, 0, 0, 16, 16, rotary, rows, None, 0, 0, layout,
-                0, None)  # fmt: skip
+    from iris_b200 import _lib
+
+    def rows(data=16, b=0, h=0, n=0):
+        return data, b, h, n
+
+    def rope(dtype=1, batch=1, heads=2, n=3, dim=64, rotary=64, table=9, layout=0, x=16):
+        return "iris_rope", _lib.ROPE_PROBLEM.pack(*rows(x), *rows(), 16, 16, 0, 0, 0, dtype, batch, heads, n, dim, rotary,
+                                                   table, layout, 0), None  # fmt: skip
 
     for bad, message in [(dict(dtype=3), "dtype"), (dict(dim=63), "even"), (dict(rotary=66), "rotated columns"),
-                         (dict(rotary=0), "rotated columns"), (dict(rows=0), "table"), (dict(layout=2), "layout"),
-                         (dict(x=None), "null"), (dict(n=1 << 31), "row counts"), (dict(heads=0), "row counts")]:  # fmt: skip
+                         (dict(rotary=0), "rotated columns"), (dict(table=0), "table"), (dict(layout=2), "layout"),
+                         (dict(x=0), "null"), (dict(n=1 << 31), "row counts"), (dict(heads=0), "row counts")]:  # fmt: skip
         assert message in _einval(lib, *rope(**bad)), bad
 
     def append(kv=1, capacity=8, sinks=-1, starts=16):
-        return ("iris_rope_append", 16, 16, 16, 1, 1, 2, kv, 3, 64, *[0] * 9, 16, 0, 0, 0, 16, 0, 0, 0, 16, 0, 0, 0, capacity,
-                sinks, 16, 16, 64, 9, starts, None, 0, None)  # fmt: skip
+        return "iris_rope_append", _lib.APPEND_PROBLEM.pack(*rows() * 6, 16, 16, starts, 0, 1, 1, 2, kv, 3, 64, 64, 9, capacity,
+                                                            sinks, 0), None  # fmt: skip
 
     for bad, message in [(dict(kv=0), "head counts"), (dict(capacity=0), "slots"), (dict(sinks=8), "slots"),
-                         (dict(sinks=-2), "slots"), (dict(starts=None), "null")]:  # fmt: skip
+                         (dict(sinks=-2), "slots"), (dict(starts=0), "null")]:  # fmt: skip
         assert message in _einval(lib, *append(**bad)), bad
 
-    def attend(q=16, dtype=1, batch=1, heads=4, kv=2, n=3, m=5, dim=128, qn=128, left=-1, right=0, sinks=0, scale=0.1):
-        return ("iris_window_attn_fwd", q, 16, 16, 16, dtype, batch, heads, kv, n, m, dim, 0, 0, qn, 0, 0, 128, 0, 0, 128, 0, 0, None, None,
-                left, right, sinks, scale, None, 0, None)  # fmt: skip
+    def attend(q=16, dtype=1, batch=1, heads=4, kv=2, n=3, m=5, dim=128, qn=128, kn=128, left=-1, right=0, sinks=0, scale=0.1):
+        return "iris_window_attn_fwd", _lib.WINDOW_PROBLEM.pack(
+            *rows(q, n=qn), *rows(n=kn), *rows(n=128), 16, 0, 0, 0, 0, 0, 0, dtype, batch, heads, kv, n, m, dim, left, right,
+            sinks, scale), None  # fmt: skip
 
     for bad, message in [(dict(dtype=0), "bf16 or f16"), (dict(heads=3), "multiple of heads_kv"), (dict(dim=80), "head_dim"),
                          (dict(qn=12), "16 bytes"), (dict(q=8), "16 bytes"), (dict(left=-2), "bounds"), (dict(right=-2), "bounds"),
                          (dict(sinks=-1), "bounds"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
                          (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"), (dict(m=1 << 30), "sizes"),
-                         (dict(batch=65536), "sizes"), (dict(qn=0), "repeat"), (dict(q=None), "null")]:  # fmt: skip
+                         (dict(batch=65536), "sizes"), (dict(qn=0), "repeat"), (dict(kn=0), "repeat"), (dict(q=0), "null")]:  # fmt: skip
         assert message in _einval(lib, *attend(**bad)), bad
 
     def q4(x=16, dtype=1, m=1, k=128, ldx=128, group=32, n=4, out=16, out_dtype=1):
-        return ("iris_gemv_q4", x, dtype, m, k, ldx, 16, 16, None, group, None, out, out_dtype, n, 0, 0, None)
+        return "iris_gemv_q4", _lib.Q4_PROBLEM.pack(x, 16, 16, 0, 0, out, m, k, n, ldx, group, dtype, out_dtype, 0, 0), None
 
     for bad, message in [(dict(group=16), "groups"), (dict(m=0), "1 to 64"), (dict(m=65), "1 to 64"), (dict(k=96, group=64), "multiple"),
                          (dict(ldx=120), "size"), (dict(n=0), "1 to 64"), (dict(x=8), "aligned"), (dict(ldx=132), "aligned"),
-                         (dict(dtype=3), "dtype"), (dict(out_dtype=-1), "dtype"), (dict(out=None), "null")]:  # fmt: skip
+                         (dict(dtype=3), "dtype"), (dict(out_dtype=-1), "dtype"), (dict(out=0), "null")]:  # fmt: skip
         assert message in _einval(lib, *q4(**bad)), bad
+    for name in ("iris_rope", "iris_rope_append", "iris_window_attn_fwd", "iris_gemv_q4"):
+        assert "null" in _einval(lib, name, None, None)
 
 
 def test_wrappers_refuse_before_any_launch(K):
@@ -68,7 +93,7 @@ def test_wrappers_refuse_before_any_launch(K):
         ((x, torch.zeros(2, 32), torch.zeros(2, 32)), {}, "cover"),
         ((x, cos, sin, torch.zeros(4, dtype=torch.int64)), {}, "positions"),
         ((x, cos, sin, torch.zeros(3)), {}, "positions"),
-        ((x, cos, sin, torch.zeros(6, dtype=torch.int32)[::2]), {}, "positions"),
+        ((x, cos, sin, torch.zeros(6, dtype=torch.int32)[::2]), {}, "positions must be contiguous"),
         ((x.double(), cos, sin), {}, "dtype"),
         ((torch.zeros(2, 4, 3, 128)[..., ::2], cos, sin), {}, "contiguous"),
         ((x, cos, sin), {"layout": "both"}, "layout"),
@@ -127,10 +152,6 @@ def test_calls_go_to_the_tensors_device(K, monkeypatch):
 
     seen = []
 
-    class Stream:
-        def __init__(self, device):
-            self.cuda_stream = 100 + device.index
-
     class Device:
         def __init__(self, device):
             self.device = device
@@ -141,13 +162,13 @@ def test_calls_go_to_the_tensors_device(K, monkeypatch):
         def __exit__(self, *a):
             seen.append(("exit", self.device.index))
 
-    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index, raising=False)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     monkeypatch.setattr(torch.cuda, "device", Device)
     monkeypatch.setattr(_lib, "call", lambda name, *args: seen.append((name, args)))
-    K._call_on(torch.device("cuda", 0), "entry", 7)
-    K._call_on(torch.device("cuda", 1), "entry", 8)
-    assert seen == [("entry", (7, 100)), ("enter", 1), ("entry", (8, 101)), ("exit", 1)]
+    K._call_on(torch.device("cuda", 0), "entry", b"7")
+    K._call_on(torch.device("cuda", 1), "entry", b"8")
+    assert seen == [("entry", (b"7", 100)), ("enter", 1), ("entry", (b"8", 101)), ("exit", 1)]
 
 
 def test_rope_table_matches_its_formulas():
