@@ -24,7 +24,6 @@ struct Params {
   int64_t left, right;  // kNoBound: none
   int sinks;
   float scale_log2;
-  int pair_heads;  // tiles_kernel: a CTA's tiles are two heads of one key head
 };
 
 template <typename T>
@@ -128,53 +127,51 @@ __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, fl
 }
 
 // ------------------------------------------------------------- tensor cores
-// Prompts and chunks: the pipeline of attention.cu (TMA warp, MMA warp, eight
-// softmax warps per 128-row query tile, two tiles per CTA sharing the K / V blocks
-// of 128 keys; S, P and O in TMEM) over the key blocks that some row of the CTA sees:
-// the blocks of the first `sinks` keys, then the window's. The two tiles are the same
-// rows of two query heads of one key head where the heads per key head are even (both
-// see the same keys: no tile waits on a block it does not need), else two neighbouring
-// row tiles of one head, which skip the blocks that only the other one sees.
+// Prompts and chunks on the 5th-generation tensor cores: a CTA takes 128 query rows of
+// one head, S, P and O in TMEM, over the blocks of 64 keys that some row sees (the blocks
+// of the first `sinks` keys, then the window's), two CTAs to an SM. Warp 0 brings Q once
+// and K and V through two-slot rings by TMA; warp 1 issues the MMAs; warps 2 to 5 do
+// the softmax, a thread per row (TMEM lane), its 64 scores in registers: no exchange
+// between threads. Exponentials (4096 a quarter and block at 4 a clock) take as long as
+// the MMAs, so what costs is waiting: S alternates between two buffers and runs a block
+// ahead of P V, so that a block's scores are there when the softmax of the one before
+// ends, and the other CTA fills what waits are left (its start and its epilogue too).
 //
 // A block that every row of a warp sees in full takes no mask; others get one bit per
-// (row, key) from the row's span. Keys behind the sample's length are zeroed in shared
+// key from the row's span. Keys behind the sample's length are zeroed in shared
 // memory (their K only reaches masked scores), so cache rows never written cost
 // nothing. A masked key's weight is exactly 0, and 0 times a NaN or infinity of
 // its V row is NaN: a row that comes out not finite is computed again by attend_row,
 // which reads visible keys alone (also rows that see no key: 0 / 0 here).
-constexpr int BQ = 128, BKV = 128, TILES = 2;
-constexpr int SOFTMAX_WARPS = 8;  // per tile: two per TMEM lane quarter, one per 64 keys
-constexpr int TILE_THREADS = 64 + TILES * SOFTMAX_WARPS * 32;
-constexpr int HALF_BYTES = 128 * 64 * 2;  // 128 rows x 64 columns
-constexpr uint32_t COL_S = 0, COL_O = 256;
+constexpr int BQ = 128, BKV = 64, KV = 2;  // rows, keys of a block, slots of the K and V rings
+constexpr int TILE_THREADS = 192;
+constexpr int Q_HALF = BQ * 128, KV_HALF = BKV * 128;  // bytes of 64 columns of a tile
+constexpr uint32_t COL_S = 0, COL_O = 2 * BKV, TILE_COLS = 256;
 constexpr float RESCALE = 8.0f;  // the running maximum is kept until a row exceeds it by 2^8
 
 struct TileSmem {
-  uint64_t q_full, k_full[2], k_free[2], v_full[2], v_free[2], v_tail;
-  uint64_t s_full[TILES], p_full[TILES], o_final[TILES], teardown;
+  uint64_t q_full, k_full[KV], k_free[KV], v_full[KV], v_free[KV], v_tail;
+  uint64_t s_full[2], p_full[2], pv_done, o_final, teardown;
   uint32_t tmem_base;
   int abort;
-  float row_max[2][TILES][2][BQ];  // [parity][tile][column half][row]
-  float row_sum[TILES][2][BQ];
 };
 
 template <int D>
-constexpr size_t tile_smem() {
-  return 1024 + (TILES + 4) * (D / 64) * HALF_BYTES + sizeof(TileSmem);
+constexpr int tile_smem() {
+  return 1024 + (D / 64) * (Q_HALF + 2 * KV * KV_HALF) + static_cast<int>(sizeof(TileSmem));
 }
 
-// Key blocks of one query tile: [0, early) and [lo, hi).
+// Key blocks that rows at positions [pos, pos + rows) see: [0, early) and [lo, hi).
 struct Blocks {
   int early, lo, hi;
-  IRIS_DEVICE bool has(int j) const { return j < early || (j >= lo && j < hi); }
+  IRIS_DEVICE int count() const { return early + hi - lo; }
+  IRIS_DEVICE int at(int it) const { return it < early ? it : lo + it - early; }
 };
 
-// Rows at positions [pos, pos + rows).
 IRIS_DEVICE Blocks key_blocks(const Params& p, int64_t pos, int rows, int length) {
-  Blocks x = {0, 0, 0};
-  if (rows <= 0) return x;
-  const Span first = visible(p, pos, length), last = visible(p, pos + rows - 1, length);
   // lo, hi and early grow with the row
+  const Span first = visible(p, pos, length), last = visible(p, pos + rows - 1, length);
+  Blocks x;
   x.early = (last.early + BKV - 1) / BKV;
   x.lo = first.lo / BKV;
   x.hi = (last.hi + BKV - 1) / BKV;
@@ -193,71 +190,52 @@ IRIS_DEVICE float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-IRIS_DEVICE void pair_barrier(uint32_t id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 // Bits [0, n) of a 32-bit word, n of any value.
 IRIS_DEVICE uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(TILE_THREADS, 1)
+__global__ void __launch_bounds__(TILE_THREADS, 2)
     tiles_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                  const __grid_constant__ CUtensorMap tv, const __grid_constant__ Params p) {
-  constexpr int HALVES = D / 64, TILE_BYTES = HALVES * HALF_BYTES;
+  constexpr int HALVES = D / 64, KV_BYTES = HALVES * KV_HALF;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* q_tile = base;
-  uint8_t* k_tile = base + TILES * TILE_BYTES;
-  uint8_t* v_tile = base + (TILES + 2) * TILE_BYTES;
-  TileSmem* s = reinterpret_cast<TileSmem*>(base + (TILES + 4) * TILE_BYTES);
+  uint8_t* q_tile = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* k_tile = q_tile + HALVES * Q_HALF;
+  uint8_t* v_tile = k_tile + KV * KV_BYTES;
+  TileSmem* s = reinterpret_cast<TileSmem*>(v_tile + KV * KV_BYTES);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   // later rows first: under a causal mask they see the most keys
-  const int slots = p.pair_heads ? p.heads_q / 2 : p.heads_q;
-  const int per_row = slots * p.batch;
-  const int row_block = static_cast<int>(gridDim.x / per_row) - 1 - static_cast<int>(blockIdx.x / per_row);
-  const int rest = blockIdx.x % per_row;
-  const int b = rest / slots, slot = rest % slots;
-  const int h0 = p.pair_heads ? 2 * slot : slot;  // head of tile 0; tile 1: h0 + 1 or the same
-  const int hk = h0 / (p.heads_q / p.heads_kv);
+  const int per_row = p.heads_q * p.batch;
+  const int row0 = (static_cast<int>(gridDim.x / per_row) - 1 - static_cast<int>(blockIdx.x / per_row)) * BQ;
+  const int b = blockIdx.x % per_row / p.heads_q, h = blockIdx.x % p.heads_q;
+  const int hk = h / (p.heads_q / p.heads_kv);
   const int length = sample_length(p, b);
   const int64_t start = sample_start(p, b);
-  const int row0[TILES] = {p.pair_heads ? row_block * BQ : row_block * 2 * BQ,
-                           p.pair_heads ? row_block * BQ : row_block * 2 * BQ + BQ};
-  Blocks blocks[TILES];
-#pragma unroll
-  for (int t = 0; t < TILES; ++t)
-    blocks[t] = key_blocks(p, start + row0[t], min(BQ, p.n - row0[t]), length);
-  // the union of the tiles' blocks, in order: [0, early) and [lo, hi)
-  Blocks all = blocks[0];
-  if (all.hi <= all.lo && all.early == 0) {
-    all = blocks[1];
-  } else if (blocks[1].hi > blocks[1].lo || blocks[1].early > 0) {
-    all.lo = min(all.lo, blocks[1].lo);
-    all.hi = max(all.hi, blocks[1].hi);
-    all.early = min(max(all.early, blocks[1].early), all.lo);
-  }
-  const int iters = all.early + all.hi - all.lo;
-  auto block_of = [&](int it) { return it < all.early ? it : all.lo + it - all.early; };
+  const Blocks blocks = key_blocks(p, start + row0, min(BQ, p.n - row0), length);
+  const int iters = blocks.count();
 
   if (threadIdx.x == 0) {
     mbar_init(&s->q_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < KV; ++i) {
       mbar_init(&s->k_full[i], 1);
       mbar_init(&s->k_free[i], 1);
       mbar_init(&s->v_full[i], 1);
       mbar_init(&s->v_free[i], 1);
     }
-    for (int t = 0; t < TILES; ++t) {
-      mbar_init(&s->s_full[t], 1);
-      mbar_init(&s->p_full[t], SOFTMAX_WARPS);
-      mbar_init(&s->o_final[t], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s->s_full[i], 1);
+      mbar_init(&s->p_full[i], 4);
     }
+    mbar_init(&s->pv_done, 1);
+    mbar_init(&s->o_final, 1);
     mbar_init(&s->v_tail, 1);
     mbar_init(&s->teardown, 1);
     s->abort = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(&s->tmem_base, 512);
+  if (warp == 1) tmem_alloc(&s->tmem_base, TILE_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -268,51 +246,53 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     // ----------------------------------------------------------------- TMA
     const int kb = p.kb != 0 ? b : 0, kh = p.kh != 0 ? hk : 0;
     const int vb = p.vb != 0 ? b : 0, vh = p.vh != 0 ? hk : 0;
-    int issued_k[2] = {-1, -1}, issued_v[2] = {-1, -1};
+    int issued_k[KV], issued_v[KV];
+    for (int i = 0; i < KV; ++i) issued_k[i] = issued_v[i] = -1;
     bool tail_issued = false;
     bool ok = true;
     if (lane == 0 && iters > 0) {
       tma_prefetch_desc(&tk);
       tma_prefetch_desc(&tv);
-      mbar_arrive_expect_tx(&s->q_full, TILES * TILE_BYTES);
-#pragma unroll
-      for (int t = 0; t < TILES; ++t)
-        for (int c = 0; c < HALVES; ++c)
-          tma_load_4d(&tq, &s->q_full, q_tile + t * TILE_BYTES + c * HALF_BYTES, c * 64, row0[t],
-                      p.qh != 0 ? (p.pair_heads ? h0 + t : h0) : 0, p.qb != 0 ? b : 0);
+      mbar_arrive_expect_tx(&s->q_full, HALVES * Q_HALF);
+      for (int c = 0; c < HALVES; ++c)
+        tma_load_4d(&tq, &s->q_full, q_tile + c * Q_HALF, c * 64, row0, p.qh != 0 ? h : 0, p.qb != 0 ? b : 0);
     }
+    auto load_k = [&](int it) {
+      const int st = it % KV;
+      const uint32_t ph = static_cast<uint32_t>((it / KV) & 1);
+      ok = mbar_wait(&s->k_free[st], ph ^ 1u, abort);
+      if (!ok) return;
+      mbar_arrive_expect_tx(&s->k_full[st], KV_BYTES);
+      for (int c = 0; c < HALVES; ++c)
+        tma_load_4d(&tk, &s->k_full[st], k_tile + st * KV_BYTES + c * KV_HALF, c * 64, blocks.at(it) * BKV, kh, kb);
+      issued_k[st] = static_cast<int>(ph);
+    };
+    if (lane == 0 && iters > 0) load_k(0);
     for (int it = 0; it < iters; ++it) {
-      const int st = it & 1;
-      const uint32_t ph = static_cast<uint32_t>((it >> 1) & 1);
-      const int key = block_of(it) * BKV;
+      const int st = it % KV;
+      const uint32_t ph = static_cast<uint32_t>((it / KV) & 1);
+      const int key = blocks.at(it) * BKV;
       // keys behind the length that the tensor map does not end before
       const bool tail = key + BKV > length && length < p.n_kv;
-      if (lane == 0) {
-        ok = mbar_wait(&s->k_free[st], ph ^ 1u, abort);
-        if (ok) {
-          mbar_arrive_expect_tx(&s->k_full[st], TILE_BYTES);
-          for (int c = 0; c < HALVES; ++c)
-            tma_load_4d(&tk, &s->k_full[st], k_tile + st * TILE_BYTES + c * HALF_BYTES, c * 64, key, kh, kb);
-          issued_k[st] = static_cast<int>(ph);
-          ok = mbar_wait(&s->v_free[st], ph ^ 1u, abort);
-        }
+      if (lane == 0 && ok) {
+        if (it + 1 < iters) load_k(it + 1);  // scores run a block ahead
+        ok = ok && mbar_wait(&s->v_free[st], ph ^ 1u, abort);
         if (ok) {
           uint64_t* bar = tail ? &s->v_tail : &s->v_full[st];
-          mbar_arrive_expect_tx(bar, TILE_BYTES);
+          mbar_arrive_expect_tx(bar, KV_BYTES);
           for (int c = 0; c < HALVES; ++c)
-            tma_load_4d(&tv, bar, v_tile + st * TILE_BYTES + c * HALF_BYTES, c * 64, key, vh, vb);
+            tma_load_4d(&tv, bar, v_tile + st * KV_BYTES + c * KV_HALF, c * 64, key, vh, vb);
           if (tail) tail_issued = true;
           else issued_v[st] = static_cast<int>(ph);
         }
       }
       if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-      if (tail) {  // one block of the CTA at most
+      if (tail) {  // one block of the CTA at most: the one that the length ends in
         ok = __all_sync(0xffffffffu, mbar_wait(&s->v_tail, 0, abort));
         if (!ok) break;
-        const int first = max(0, length - key);
-        for (int e = first * 8 + lane; e < BKV * 8; e += 32)
+        for (int e = (length - key) * 8 + lane; e < BKV * 8; e += 32)
           for (int c = 0; c < HALVES; ++c)
-            *reinterpret_cast<uint4*>(v_tile + st * TILE_BYTES + c * HALF_BYTES + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(v_tile + st * KV_BYTES + c * KV_HALF + e * 16) = make_uint4(0u, 0u, 0u, 0u);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s->v_full[st]);
@@ -321,7 +301,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
     if (lane == 0 && !ok) {  // given up: no copy may land after the CTA is gone
       int dummy = 0;
       mbar_wait(&s->q_full, 0, &dummy);
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < KV; ++i) {
         if (issued_k[i] >= 0) mbar_wait(&s->k_full[i], static_cast<uint32_t>(issued_k[i]), &dummy);
         if (issued_v[i] >= 0) mbar_wait(&s->v_full[i], static_cast<uint32_t>(issued_v[i]), &dummy);
       }
@@ -334,239 +314,166 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
       constexpr uint32_t clear = IsHalf<T>::value ? f16 : 0u;
       const uint32_t idesc_s = idesc_bf16_f32(BQ, BKV) & ~clear;
       const uint32_t idesc_o = idesc_bf16_f32(BQ, D, false, true) & ~clear;  // V is MN-major (columns contiguous)
-      auto issue_s = [&](int t, int it) {
-        const uint32_t q_addr = smem_addr(q_tile + t * TILE_BYTES);
-        const uint32_t k_addr = smem_addr(k_tile + (it & 1) * TILE_BYTES);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * HALF_BYTES + (kk & 3) * 32;
-          umma_ss(tmem + COL_S + t * BKV, umma_desc(q_addr + off, 16, 1024, kLayoutSw128),
-                  umma_desc(k_addr + off, 16, 1024, kLayoutSw128), idesc_s, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&s->s_full[t]);
-      };
-      // P of keys [0, 64) lies packed in S_t columns [0, 32), of keys [64, 128) in [64, 96)
-      auto issue_pv = [&](int t, int it, bool first) {
-        const uint32_t v_addr = smem_addr(v_tile + (it & 1) * TILE_BYTES);
-#pragma unroll
-        for (int kk = 0; kk < BKV / 16; ++kk) {
-          const uint64_t bd = umma_desc(v_addr + kk * 16 * 128, HALF_BYTES, 1024, kLayoutSw128);
-          umma_ts(tmem + COL_O + t * D, tmem + COL_S + t * BKV + (kk >> 2) * 64 + (kk & 3) * 8, bd, idesc_o,
-                  (!first || kk > 0) ? 1u : 0u);
-        }
-      };
-      int done[TILES] = {0, 0}, total[TILES];
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) total[t] = blocks[t].early + blocks[t].hi - blocks[t].lo;
-      bool ok = mbar_wait(&s->q_full, 0, abort) && mbar_wait(&s->k_full[0], 0, abort);
-      if (ok) {
+      bool ok = mbar_wait(&s->q_full, 0, abort);
+      // scores of block `it` into buffer it % 2
+      auto issue_s = [&](int it) {
+        ok = ok && mbar_wait(&s->k_full[it % KV], static_cast<uint32_t>((it / KV) & 1), abort);
+        if (!ok) return;
         tc_fence_after();
+        const uint32_t q_addr = smem_addr(q_tile), k_addr = smem_addr(k_tile + (it % KV) * KV_BYTES);
 #pragma unroll
-        for (int t = 0; t < TILES; ++t)
-          if (blocks[t].has(block_of(0))) issue_s(t, 0);
-        umma_commit(&s->k_free[0]);
-      }
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_ss(tmem + COL_S + (it & 1) * BKV, umma_desc(q_addr + (kk >> 2) * Q_HALF + (kk & 3) * 32, 16, 1024, kLayoutSw128),
+                  umma_desc(k_addr + (kk >> 2) * KV_HALF + (kk & 3) * 32, 16, 1024, kLayoutSw128), idesc_s, kk > 0 ? 1u : 0u);
+        umma_commit(&s->s_full[it & 1]);
+        umma_commit(&s->k_free[it % KV]);
+      };
+      issue_s(0);
+      if (iters > 1) issue_s(1);
       for (int it = 0; it < iters && ok; ++it) {
-        const int st = it & 1;
-        const uint32_t ph = static_cast<uint32_t>((it >> 1) & 1);
-        const bool more = it + 1 < iters;
-        const int j = block_of(it), jn = block_of(it + 1);
-        if (!mbar_wait(&s->v_full[st], ph, abort)) { ok = false; break; }
-        if (more && !mbar_wait(&s->k_full[(it + 1) & 1], static_cast<uint32_t>(((it + 1) >> 1) & 1), abort)) {
-          ok = false;
-          break;
-        }
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-          if (ok && blocks[t].has(j)) {
-            ok = mbar_wait(&s->p_full[t], static_cast<uint32_t>(done[t] & 1), abort);
-            if (ok) {
-              tc_fence_after();
-              issue_pv(t, it, done[t] == 0);
-              if (++done[t] == total[t]) umma_commit(&s->o_final[t]);
-            }
-          }
-          if (ok && more && blocks[t].has(jn)) issue_s(t, it + 1);
-        }
+        const int st = it % KV;
+        ok = mbar_wait(&s->v_full[st], static_cast<uint32_t>((it / KV) & 1), abort) &&
+             mbar_wait(&s->p_full[it & 1], static_cast<uint32_t>((it >> 1) & 1), abort);
         if (!ok) break;
+        tc_fence_after();
+        const uint32_t v_addr = smem_addr(v_tile + st * KV_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < BKV / 16; ++kk)  // P lies packed over the first half of its scores
+          umma_ts(tmem + COL_O, tmem + COL_S + (it & 1) * BKV + kk * 8,
+                  umma_desc(v_addr + kk * 16 * 128, KV_HALF, 1024, kLayoutSw128), idesc_o, (it > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&s->pv_done);
         umma_commit(&s->v_free[st]);
-        if (more) umma_commit(&s->k_free[(it + 1) & 1]);
+        // into the buffer of the P just read: one thread's MMAs run in order
+        if (it + 2 < iters) issue_s(it + 2);
       }
+      if (ok) umma_commit(&s->o_final);
       umma_commit(&s->teardown);
       int dummy = 0;
       mbar_wait(&s->teardown, 0, &dummy);
     }
   } else {
     // ------------------------------------------------------------- softmax
-    // The two warps of a (tile, lane quarter) hold the same 32 query rows, keys
-    // [0, 64) and [64, 128) of a block; they combine maxima and sums in shared memory.
-    const int sw = warp - 2;
-    const int tile = sw / SOFTMAX_WARPS;
-    const int half = (sw / 4) & 1;
     const int quarter = warp & 3;
-    const int row = quarter * 32 + lane;
-    const uint32_t bar_id = 1 + tile * 4 + quarter;
-    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_col = COL_S + tile * BKV + half * 64;
-    const uint32_t o_col = COL_O + tile * D + half * (D / 2);
-    const Blocks mine = tile == 0 ? blocks[0] : blocks[1];
-    const int first_row = tile == 0 ? row0[0] : row0[1];
-    const int i = first_row + row;  // query row
+    const int i = row0 + quarter * 32 + lane;  // query row
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const Span span = visible(p, start + i, length);
     // what every row of the warp sees: keys below hi_all that are sinks or from lo_all on
     const int hi_all = __shfl_sync(0xffffffffu, span.hi, 0), lo_all = __shfl_sync(0xffffffffu, span.lo, 31);
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
-    int done = 0;
-    const int total = mine.early + mine.hi - mine.lo;
-    for (; done < total; ++done) {
-      const int key0 = (done < mine.early ? done : mine.lo + done - mine.early) * BKV + half * 64;
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(&s->s_full[tile], static_cast<uint32_t>(done & 1), abort));
-      if (!ok) {  // given up: the barriers with the other warp of the rows go on, so that it ends too
-        pair_barrier(bar_id);
-        continue;
-      }
+    for (int it = 0; it < iters; ++it) {
+      const int key0 = blocks.at(it) * BKV;
+      const bool full = key0 + BKV <= hi_all && (key0 >= lo_all || key0 + BKV <= p.sinks);
+      const uint32_t s_at = lanes + COL_S + (it & 1) * BKV;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s->s_full[it & 1], static_cast<uint32_t>((it >> 1) & 1), abort));
+      if (!ok) break;
       tc_fence_after();
-      const bool full = key0 + 64 <= hi_all && (key0 >= lo_all || key0 + 64 <= p.sinks);
-      uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+      uint32_t r[2][32];
+      tmem_ld32(s_at, r[0]);
+      tmem_ld32(s_at + 32, r[1]);
+      tmem_wait_ld();
       if (!full) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int k0 = key0 + c * 32;
-          see[c] = low_bits(span.hi - k0) & (~low_bits(span.lo - k0) | low_bits(p.sinks - k0));
+          const uint32_t see = low_bits(span.hi - k0) & (~low_bits(span.lo - k0) | low_bits(p.sinks - k0));
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!(see >> e & 1u)) r[c][e] = __float_as_uint(-INFINITY);
         }
       }
-      float mx;
-      {
-        uint32_t r[2][32];
-        tmem_ld32(tmem + lane_addr + s_col, r[0]);
-        tmem_ld32(tmem + lane_addr + s_col + 32, r[1]);
-        tmem_wait_ld();
-        float ma = -INFINITY, mb = -INFINITY, mc = -INFINITY, md = -INFINITY;
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (!full) {
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(see[c] >> e & 1u)) r[c][e] = __float_as_uint(-INFINITY);
-          }
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            ma = max3(ma, __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
-            mb = max3(mb, __uint_as_float(r[c][e + 2]), __uint_as_float(r[c][e + 3]));
-            mc = max3(mc, __uint_as_float(r[c][e + 4]), __uint_as_float(r[c][e + 5]));
-            md = max3(md, __uint_as_float(r[c][e + 6]), __uint_as_float(r[c][e + 7]));
-          }
-        }
-        const float part = fmaxf(max3(ma, mb, mc), md);
-        s->row_max[done & 1][tile][half][row] = part;
-        pair_barrier(bar_id);
-        mx = fmaxf(part, s->row_max[done & 1][tile][half ^ 1][row]) * p.scale_log2;
-      }
+        for (int e = 0; e < 32; e += 2)
+          top[e / 2 % 4] = max3(top[e / 2 % 4], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+      const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.scale_log2;
       // the maximum is kept until a row exceeds it by 2^8 (O and l share it: exact); a row
       // that has seen nothing yet (-inf) has weights and sums of 0
       const bool grow = mx > m_run + RESCALE;
       const float m_new = grow ? mx : m_run;
       const bool rescale = grow && m_run != -INFINITY;
-      const float corr = rescale ? ex2(m_run - m_new) : 1.f;
       if (__any_sync(0xffffffffu, rescale)) {
-        // O_t holds the P V of earlier blocks: S_t of this one complete implies them complete
+        const float corr = rescale ? ex2(m_run - m_new) : 1.f;
+        l_run *= corr;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s->pv_done, static_cast<uint32_t>((it - 1) & 1), abort));
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t r[32];
-          tmem_ld32(tmem + lane_addr + o_col + c * 32, r);
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld16(lanes + COL_O + c * 16, o);
           tmem_wait_ld();
-          uint32_t lo[16], hi[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            lo[e] = __float_as_uint(__uint_as_float(r[e]) * corr);
-            hi[e] = __float_as_uint(__uint_as_float(r[16 + e]) * corr);
-          }
-          tmem_st16(tmem + lane_addr + o_col + c * 32, lo);
-          tmem_st16(tmem + lane_addr + o_col + c * 32 + 16, hi);
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+          tmem_st16(lanes + COL_O + c * 16, o);
         }
       }
+      m_run = m_new;
       // weights 2^(s * scale - m), rounded once to the operand type of the P V product
       // (their fp32 values go into the sum); masked keys give exact zeros
       const float shift = m_new == -INFINITY ? 0.f : -m_new;
       const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(shift, shift);
       float2 sum2 = make_float2(0.f, 0.f);
-      uint32_t buf[2][32];
-      tmem_ld32(tmem + lane_addr + s_col, buf[0]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        tmem_wait_ld();
-        if (c == 0) tmem_ld32(tmem + lane_addr + s_col + 32, buf[1]);
-        uint32_t(&r)[32] = buf[c];
-        if (!full) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!(see[c] >> e & 1u)) r[e] = __float_as_uint(-INFINITY);
-        }
         uint32_t pk[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), scale2, shift2);
+          const float2 x =
+              __ffma2_rn(make_float2(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), scale2, shift2);
           const float2 w = make_float2(ex2(x.x), ex2(x.y));
           sum2 = __fadd2_rn(sum2, w);
           pk[e] = pack2<T>(w.x, w.y);
         }
-        tmem_st16(tmem + lane_addr + s_col + c * 16, pk);
+        tmem_st16(s_at + c * 16, pk);
       }
-      l_run = l_run * corr + (sum2.x + sum2.y);
-      m_run = m_new;
+      l_run += sum2.x + sum2.y;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s->p_full[tile]);
+      if (lane == 0) mbar_arrive(&s->p_full[it & 1]);
     }
-    s->row_sum[tile][half][row] = l_run;
-    pair_barrier(bar_id);
-    const float inv = 1.f / (l_run + s->row_sum[tile][half ^ 1][row]);
-    const int h = p.pair_heads ? h0 + tile : h0;
-    if (total > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&s->o_final[tile], 0, abort));
+    if (iters > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&s->o_final, 0, abort));
     ok = ok && *abort == 0;
-    constexpr int COLS = D / 2;  // output columns of this half
     T* out = reinterpret_cast<T*>(p.out) + b * p.ob + static_cast<int64_t>(h) * D;
     if (!ok) {  // a wait gave up (device error word): NaN rather than a wrong row
       if (i < p.n)
-        for (int c = 0; c < COLS; c += 2) *reinterpret_cast<uint32_t*>(out + i * p.on + half * COLS + c) = pack2<T>(NAN, NAN);
+        for (int c = 0; c < D; c += 2) *reinterpret_cast<uint32_t*>(out + i * p.on + c) = pack2<T>(NAN, NAN);
     } else {
       tc_fence_after();
+      const float inv = 1.f / l_run;
       bool finite = true;
 #pragma unroll
-      for (int c = 0; c < COLS / 32; ++c) {
+      for (int c = 0; c < D / 32; ++c) {
         uint32_t r[32];
-        if (total > 0) {
-          tmem_ld32(tmem + lane_addr + o_col + c * 32, r);
+        if (iters > 0) {
+          tmem_ld32(lanes + COL_O + c * 32, r);
           tmem_wait_ld();
         }
         uint32_t pk[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float a = total > 0 ? __uint_as_float(r[2 * e]) * inv : 0.f;
-          const float z = total > 0 ? __uint_as_float(r[2 * e + 1]) * inv : 0.f;
+          const float a = iters > 0 ? __uint_as_float(r[2 * e]) * inv : 0.f;
+          const float z = iters > 0 ? __uint_as_float(r[2 * e + 1]) * inv : 0.f;
           finite = finite && isfinite(a) && isfinite(z);
           pk[e] = pack2<T>(a, z);
         }
         if (i < p.n) {
-          uint4* dst = reinterpret_cast<uint4*>(out + i * p.on + half * COLS + c * 32);
+          uint4* dst = reinterpret_cast<uint4*>(out + i * p.on + c * 32);
 #pragma unroll
           for (int e = 0; e < 4; ++e) dst[e] = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
         }
       }
+      __syncwarp();  // a row that is computed again comes after what was written of it
       for (uint32_t again = __ballot_sync(0xffffffffu, !finite && i < p.n); again != 0; again &= again - 1) {
-        const int r = first_row + quarter * 32 + __ffs(again) - 1;
+        const int r = row0 + quarter * 32 + __ffs(again) - 1;
         float2 acc[D / 64];
         attend_row<T, D>(p, b, h, r, acc);
-        // this warp's columns of the row
         T* o = out + static_cast<int64_t>(r) * p.on + 2 * lane;
-        if constexpr (D == 128) {
-          const float2 a = half == 0 ? acc[0] : acc[D / 64 - 1];
-          *reinterpret_cast<uint32_t*>(o + 64 * half) = pack2<T>(a.x, a.y);
-        } else if (lane / 16 == half) {
-          *reinterpret_cast<uint32_t*>(o) = pack2<T>(acc[0].x, acc[0].y);
-        }
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) *reinterpret_cast<uint32_t*>(o + 64 * c) = pack2<T>(acc[c].x, acc[c].y);
       }
     }
   }
@@ -574,15 +481,12 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (warp == 1) tmem_dealloc(tmem, TILE_COLS);
 }
 
 template <typename T, int D>
-int launch_tiles(Params p, int dtype, cudaStream_t st) {
-  const int group = p.heads_q / p.heads_kv;
-  p.pair_heads = group % 2 == 0;
-  const int64_t rows = p.pair_heads ? BQ : 2 * BQ;
-  const int64_t ctas = (p.n + rows - 1) / rows * (p.pair_heads ? p.heads_q / 2 : p.heads_q) * p.batch;
+int launch_tiles(const Params& p, int dtype, cudaStream_t st) {
+  const int64_t ctas = static_cast<int64_t>((p.n + BQ - 1) / BQ) * p.heads_q * p.batch;
   IRIS_REQUIRE(ctas < (1ll << 31), "window_attn_fwd: too many rows");
   CUtensorMap tq, tk, tv;
   IRIS_CHECK_STATUS(make_tmap_heads(&tq, p.q, dtype, D, p.n, p.heads_q, p.batch, p.qn, p.qh, p.qb, BQ));
@@ -593,7 +497,7 @@ int launch_tiles(Params p, int dtype, cudaStream_t st) {
   int dev = 0;
   IRIS_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !configured[dev]) {
-    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(tile_smem<D>())));
+    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem<D>()));
     if (dev < 64) configured[dev] = true;
   }
   kernel<<<static_cast<unsigned>(ctas), TILE_THREADS, tile_smem<D>(), st>>>(tq, tk, tv, p);
