@@ -178,7 +178,8 @@ int iris_rope(const iris_rope_problem* problem, void* stream);
  * (rotated) and v to slot p, or with sinks >= 0 (a rolling cache: the first
  * `sinks` positions and the latest capacity - sinks) to slot
  * p < sinks ? p : sinks + (p - sinks) % (capacity - sinks); of two rows of the call
- * for one slot the later is kept. Rows from counts[b] on are left as they are. A
+ * for one slot the later is kept. Rows from counts[b] on are left as they are, or
+ * with zero_rest != 0 zeroed in out. A
  * position outside the table (NaN row, nothing appended) or past the end of a
  * plain cache (nothing appended) sets bit 1 of the device error word. */
 typedef struct iris_append_problem {
@@ -188,6 +189,7 @@ typedef struct iris_append_problem {
   const int* starts;
   const int* counts;
   int64_t dtype, batch, heads_q, heads_kv, n, head_dim, rotary, table_rows, capacity, sinks, layout;
+  int64_t zero_rest;
 } iris_append_problem;
 int iris_rope_append(const iris_append_problem* problem, void* stream);
 

@@ -41,6 +41,7 @@ struct Params {
   const int* counts;   // append: rows of each sample, or null (all n)
   int64_t capacity;    // append: slots of the cache
   int64_t sinks;       // append: -1 plain cache, else slots that a rolling cache never overwrites
+  bool zero_rest;      // append: zeros in out's rows from counts[b] on
   int units, hslots, tokens_per_block;
 };
 
@@ -100,7 +101,16 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const __grid_constant__ P
     if constexpr (APPEND) {
       const int64_t first = a.starts[b];
       const int64_t count = a.counts ? min(a.counts[b], a.n) : a.n;
-      if (t >= count) continue;
+      if (t >= count) {
+        if (!a.zero_rest) continue;
+        const Vec<T, V> none = {};
+        for (int h = slot; h < a.heads_q; h += a.hslots) {
+          T* dst = reinterpret_cast<T*>(a.q.dst) + b * a.q.db + h * a.q.dh + t * a.q.dn + u * 2 * V;
+          *reinterpret_cast<Vec<T, V>*>(dst) = none;
+          *reinterpret_cast<Vec<T, V>*>(dst + V) = none;
+        }
+        continue;
+      }
       p = first + t;
       bad = p < 0 || p >= a.table_rows;
       bool full = false;
@@ -280,5 +290,6 @@ extern "C" int iris_rope_append(const iris_append_problem* q, void* stream) {
   a.counts = q->counts;
   a.capacity = q->capacity;
   a.sinks = q->sinks;
+  a.zero_rest = q->zero_rest != 0;
   return dispatch<true>(a, q->dtype, q->layout == IRIS_ROPE_HALF, stream);
 }

@@ -8,10 +8,11 @@ symbols. ``call`` raises ``ValueError`` for a rejected argument
 from __future__ import annotations
 
 import ctypes
-import struct
+import importlib.util
 from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().parent / "libiris_b200.so"
+TEXT_SIDE = LIBRARY.with_name("_text_side.so")
 
 IRIS_OK, IRIS_EINVAL, IRIS_ECUDA = 0, 1, 2
 F32, BF16, F16 = 0, 1, 2
@@ -19,7 +20,6 @@ EPI_STORE, EPI_SWIGLU, EPI_GATE, EPI_HEADS, EPI_ADD, EPI_SILU = 0, 1, 2, 3, 4, 5
 HEADS_LOCAL, HEADS_PEER_SCATTER, HEADS_PEER_BROADCAST_KV = 0, 1, 2
 MAX_PEERS = 8  # IRIS_MAX_PEERS
 IPC_HANDLE_BYTES = 64
-ROPE_LAYOUTS = {"interleaved": 0, "half": 1}  # IRIS_ROPE_*
 NEXT_NONE, NEXT_NORM_MODULATE, NEXT_SILU_ADD = 0, 1, 2
 
 P, I64, I32, F = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
@@ -101,14 +101,8 @@ SIGNATURES["iris_ipc_close"] = [P]
 SIGNATURES["iris_peer_barrier"] = [P, P, I32, I32, ctypes.c_uint, I64, P]
 SIGNATURES["iris_flash_attn_fwd_split"] = [P, P, P, I64, I64, I64, I64, I64, I64, F, F, I64, P, P, P, P, I64, P]
 
-# Problems of one struct of 8-byte members, packed from plain integers (pointers as
-# addresses, 0 for none): a call then takes two arguments, not forty.
-ROPE_PROBLEM = struct.Struct("@22q")  # iris_rope_problem
-APPEND_PROBLEM = struct.Struct("@39q")  # iris_append_problem
-WINDOW_PROBLEM = struct.Struct("@29qd")  # iris_window_problem
-Q4_PROBLEM = struct.Struct("@15q")  # iris_q4_problem
 for _name in ("iris_rope", "iris_rope_append", "iris_window_attn_fwd", "iris_gemv_q4"):
-    SIGNATURES[_name] = [P, P]
+    SIGNATURES[_name] = [P, P]  # a problem struct and the stream
 SIGNATURES["iris_window_attn_workspace"] = [P, ctypes.POINTER(I64)]
 
 _lib: ctypes.CDLL | None = None
@@ -135,6 +129,28 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+# the text side's entry points, in the order of the module's bind()
+_TEXT_ENTRIES = ("iris_rope", "iris_rope_append", "iris_window_attn_fwd", "iris_window_attn_workspace", "iris_gemv_q4",
+                 "iris_last_error")  # fmt: skip
+_text_side = None
+
+
+def text_side():
+    """The CPython module of the text side's calls, bound to the loaded library;
+    raises if either was not built."""
+    global _text_side
+    if _text_side is None:
+        lib = load()
+        if not TEXT_SIDE.exists():
+            raise RuntimeError(f"{TEXT_SIDE.name} is not built; run `python -m iris_b200.build`")
+        spec = importlib.util.spec_from_file_location("_text_side", TEXT_SIDE)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib, name), P).value for name in _TEXT_ENTRIES))
+        _text_side = module
+    return _text_side
+
+
 _launches = 0
 # kernels each entry point enqueues (1 unless listed)
 _KERNELS_PER_CALL = {"iris_device_error": 0, "iris_all_finite": 2, "iris_ipc_export": 0, "iris_ipc_import": 0,
@@ -144,7 +160,7 @@ _KERNELS_PER_CALL = {"iris_device_error": 0, "iris_all_finite": 2, "iris_ipc_exp
 def launch_count() -> int:
     """Kernels of this library enqueued so far by this process (replays of a
     captured CUDA graph count the library kernels the graph holds)."""
-    return _launches
+    return _launches + (_text_side.launched() if _text_side is not None else 0)
 
 
 def count_launches(n: int) -> None:

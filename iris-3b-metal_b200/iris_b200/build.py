@@ -3,7 +3,9 @@
     python -m iris_b200.build            # from the iris-3b-metal_b200 directory
 
 The library is one translation unit (``csrc/iris_b200.cu``); the output lands
-next to this file so it travels with the source tree.
+next to this file so it travels with the source tree. So does ``_text_side.so``
+(``csrc/text_side.cpp``), the CPython module through which the text side's per-token
+calls reach the library, built by the host compiler against torch's headers.
 """
 
 from __future__ import annotations
@@ -12,12 +14,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE.parent / "csrc"
 INCLUDE = PACKAGE.parent.parent / "include"
 LIBRARY = PACKAGE / "libiris_b200.so"
+MODULE = PACKAGE / "_text_side.so"
+MODULE_SOURCE = CSRC / "text_side.cpp"
 
 NVCC_FLAGS = [
     "-gencode",
@@ -49,19 +54,47 @@ def up_to_date() -> bool:
     return all(src.stat().st_mtime <= built for src in sources())
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and up_to_date():
-        return LIBRARY
-    tmp = LIBRARY.with_suffix(f".so.tmp{os.getpid()}")
-    cmd = [nvcc(), *NVCC_FLAGS, f"-I{INCLUDE}", "-o", str(tmp), str(CSRC / "iris_b200.cu")]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    result = subprocess.run(cmd, capture_output=True, text=True)
+def module_up_to_date() -> bool:
+    if not MODULE.exists():
+        return False
+    built = MODULE.stat().st_mtime
+    return all(src.stat().st_mtime <= built for src in (MODULE_SOURCE, INCLUDE / "iris_b200.h"))
+
+
+def _run(cmd: list[str], target: Path, verbose: bool) -> None:
+    """Run a compiler that writes ``target`` (renamed into place when it is whole)."""
+    tmp = target.with_suffix(f".so.tmp{os.getpid()}")
+    result = subprocess.run([*cmd, "-o", str(tmp)], capture_output=True, text=True)
     if result.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({result.returncode}):\n{result.stderr[-4000:]}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed ({result.returncode}):\n{result.stderr[-4000:]}")
     if verbose:
         sys.stderr.write(result.stderr)
-    os.replace(tmp, LIBRARY)
+    os.replace(tmp, target)
+
+
+def build_module(force: bool = False, verbose: bool = False) -> Path:
+    if not force and module_up_to_date():
+        return MODULE
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    includes = [root / "include", root / "include/torch/csrc/api/include", cuda / "include", sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in includes),
+           str(MODULE_SOURCE), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]  # fmt: skip
+    _run(cmd, MODULE, verbose)
+    return MODULE
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    build_module(force, verbose)
+    if not force and up_to_date():
+        return LIBRARY
+    cmd = [nvcc(), *NVCC_FLAGS, f"-I{INCLUDE}", str(CSRC / "iris_b200.cu")]
+    if verbose:
+        cmd.insert(1, "-Xptxas=-v")
+    _run(cmd, LIBRARY, verbose)
     return LIBRARY
 
 

@@ -20,7 +20,6 @@ engine (``gemm``, ``flash_attention``, ...) follow the same rules.
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 
 import torch
@@ -523,71 +522,8 @@ def flash_attention_split(
 
 
 # ------------------------------------------------------------------ text side
-# These run once per token: checks are plain comparisons with fixed messages, and a
-# call packs its arguments into one struct.
-def _call_on(device: torch.device, name: str, problem: bytes) -> None:
-    """Call an entry point on ``device``'s current stream, whichever device is current."""
-    index = device.index
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if index == torch.cuda.current_device():
-        _lib.call(name, problem, stream)
-        return
-    with torch.cuda.device(device):
-        _lib.call(name, problem, stream)
-
-
-def _same_device(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    """The CUDA device of all of them."""
-    device = first.device
-    _require(device.type == "cuda", "the B200 kernels need CUDA tensors (there is no CPU path)")
-    for t in others:
-        if t is not None and t.device != device:
-            raise ValueError("tensors must be on one CUDA device")
-    return device
-
-
-def _head_rows(t: torch.Tensor, shape: tuple[int, int, int, int], message: str) -> tuple[int, int, int, int]:
-    """Address and element strides (0 for a lone row: its stride says nothing) of head
-    rows of ``shape`` ``[B, H, N, D]``, contiguous along ``D``."""
-    if t.shape != shape:
-        raise ValueError(message)
-    sb, sh, sn, sd = t.stride()
-    if sd != 1 and shape[3] != 1:
-        raise ValueError("head rows must be contiguous")
-    return t.data_ptr(), sb if shape[0] > 1 else 0, sh if shape[1] > 1 else 0, sn if shape[2] > 1 else 0
-
-
-def _writable(t: torch.Tensor) -> None:
-    """No two elements in one place (an expanded output would be a race)."""
-    if 0 in t.stride():
-        _require(all(st != 0 or size <= 1 for st, size in zip(t.stride(), t.shape)), "an output must not be an expanded view")
-
-
-def _int32_rows(t: torch.Tensor | None, batch: int, message: str) -> int:
-    if t is None:
-        return 0
-    if t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous():
-        raise ValueError(message)
-    return t.data_ptr()
-
-
-def _rope_table(cos: torch.Tensor, sin: torch.Tensor, dim: int) -> tuple[int, int]:
-    """(rows, rotated columns) of the tables."""
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
-        raise ValueError("rotary tables must be contiguous FP32")
-    shape = cos.shape
-    if len(shape) != 2 or shape != sin.shape or shape[0] == 0 or not 0 < 2 * shape[1] <= dim:
-        raise ValueError("rotary tables must be [positions, rotary / 2] with rotary <= head_dim")
-    return shape[0], 2 * shape[1]
-
-
-def _layout(layout: str) -> int:
-    code = _lib.ROPE_LAYOUTS.get(layout)
-    if code is None:
-        raise ValueError(f"layout must be one of {sorted(_lib.ROPE_LAYOUTS)}")
-    return code
-
-
+# One call per token and layer: checked and launched by a CPython module
+# (csrc/text_side.cpp), on the tensors' device, whichever is current.
 def rope(
     x: torch.Tensor,
     cos: torch.Tensor,
@@ -608,34 +544,7 @@ def rope(
     N - 1``. ``inverse`` turns back, which is also the gradient's map. ``out`` may be
     ``x``; by default it is a new contiguous tensor. A position outside the tables
     gives a NaN row and sets bit 1 of :func:`device_error`."""
-    _require(x.dim() == 4, "rope needs [B, H, N, D] head rows")
-    shape = x.shape
-    batch, heads, n, dim = shape
-    code = _dtype(x)
-    table_rows, rotary = _rope_table(cos, sin, dim)
-    rows = _head_rows(x, shape, "rope needs [B, H, N, D] head rows")
-    at = pos_stride = wide = 0
-    if positions is None:
-        _require(n <= table_rows, "rope: the tables do not cover the rows")
-    else:
-        wide = positions.dtype == torch.int64
-        if not (wide or positions.dtype == torch.int32) or positions.shape not in ((n,), (batch, n)):
-            raise ValueError("positions must be int32 or int64 [N] or [B, N]")
-        _require(n <= 1 or positions.stride(-1) == 1, "positions must be contiguous along the rows")
-        pos_stride = positions.stride(0) if positions.dim() == 2 else 0
-        at = positions.data_ptr()
-    turn = _layout(layout)
-    device = _same_device(x, cos, sin, positions, out)
-    if out is None:
-        out = x.new_empty(shape)
-    else:
-        _require(out.dtype == x.dtype, "rope: out must have the input's type")
-        _writable(out)
-    target = _head_rows(out, shape, "rope: out must have the input's shape")
-    _call_on(device, "iris_rope", _lib.ROPE_PROBLEM.pack(
-        *rows, *target, cos.data_ptr(), sin.data_ptr(), at, pos_stride, wide, code, batch, heads, n, dim, rotary,
-        table_rows, turn, inverse))  # fmt: skip
-    return out
+    return (_lib._text_side or _lib.text_side()).rope(x, cos, sin, positions, layout, inverse, out)
 
 
 def rope_append(
@@ -666,53 +575,7 @@ def rope_append(
     ``counts[b]`` on are not touched (zeros in a new ``out``). A position outside the
     tables (NaN row, not appended) or past a plain cache (not appended) sets bit 1 of
     :func:`device_error`. ``layout`` and the tables as for :func:`rope`."""
-    _require(q.dim() == k.dim() == k_cache.dim() == 4, "rope_append needs [B, H, N, D] head rows")
-    shape = q.shape
-    batch, heads, n, dim = shape
-    kv_heads, capacity = k.shape[1], k_cache.shape[2]
-    dtype = q.dtype
-    code = _dtype(dtype)
-    table_rows, rotary = _rope_table(cos, sin, dim)
-    if not dtype == k.dtype == v.dtype == k_cache.dtype == v_cache.dtype:
-        raise ValueError("rope_append: one type for rows and cache")
-    q_rows = _head_rows(q, shape, "rope_append needs [B, H, N, D] head rows")
-    new = (batch, kv_heads, n, dim)
-    k_rows = _head_rows(k, new, "rope_append: k must be [B, H_kv, N, D]")
-    v_rows = _head_rows(v, new, "rope_append: v must be [B, H_kv, N, D]")
-    kept = (batch, kv_heads, capacity, dim)
-    k_slots = _head_rows(k_cache, kept, "rope_append: k_cache must be [B, H_kv, C, D]")
-    v_slots = _head_rows(v_cache, kept, "rope_append: v_cache must be [B, H_kv, C, D]")
-    _writable(k_cache)
-    _writable(v_cache)
-    if sinks is None:
-        sinks = -1
-    else:
-        _require(0 <= sinks < capacity, "rope_append: a rolling cache needs more slots than sinks")
-    _require(starts is not None, "rope_append needs starts")
-    first = _int32_rows(starts, batch, "starts must be contiguous int32 [B]")
-    real = _int32_rows(counts, batch, "counts must be contiguous int32 [B]")
-    turn = _layout(layout)
-    device = _same_device(q, k, v, cos, sin, starts, k_cache, v_cache, counts, out)
-    if out is None:
-        out = q.new_empty(shape) if counts is None else q.new_zeros(shape)
-    else:
-        _require(out.dtype == dtype, "rope_append: out must have the input's type")
-        _writable(out)
-    target = _head_rows(out, shape, "rope_append: out must have q's shape")
-    _call_on(device, "iris_rope_append", _lib.APPEND_PROBLEM.pack(
-        *q_rows, *k_rows, *v_rows, *target, *k_slots, *v_slots, cos.data_ptr(), sin.data_ptr(), first, real, code, batch,
-        heads, kv_heads, n, dim, rotary, table_rows, capacity, sinks, turn))  # fmt: skip
-    return out
-
-
-@functools.lru_cache(maxsize=4096)
-def _window_workspace(device: int, *sizes: int) -> int:
-    """Bytes that ``iris_window_attn_fwd`` needs for these sizes (dtype, batch .. sinks)
-    on a device: the split follows its SM count."""
-    need = ctypes.c_int64(0)
-    with torch.cuda.device(device):
-        _lib.call("iris_window_attn_workspace", _lib.WINDOW_PROBLEM.pack(*[0] * 19, *sizes, 1.0), ctypes.byref(need))
-    return need.value
+    return (_lib._text_side or _lib.text_side()).rope_append(q, k, v, cos, sin, starts, k_cache, v_cache, sinks, counts, layout, out)
 
 
 def window_attention(
@@ -739,39 +602,7 @@ def window_attention(
     sinks``; ``None`` is no bound, the default is causal. A query that sees no key
     gives 0. Other keys' rows may hold anything. Heads and samples may be expanded,
     tokens not."""
-    _require(q.dim() == k.dim() == 4, "window_attention: q [B, H, N, D], k/v [B, H_kv, N_kv, D]")
-    shape = q.shape
-    batch, heads, n, dim = shape
-    kv_heads, n_kv = k.shape[1], k.shape[2]
-    dtype = q.dtype
-    if not (dtype == torch.bfloat16 or dtype == torch.float16) or not dtype == k.dtype == v.dtype:
-        raise ValueError("window_attention: q, k and v in one of bf16, f16")
-    _require(dim == 128 or dim == 64, "window_attention: head_dim must be 64 or 128")
-    q_rows = _head_rows(q, shape, "window_attention: q must be [B, H, N, D]")
-    keys = (batch, kv_heads, n_kv, dim)
-    k_rows = _head_rows(k, keys, "window_attention: k must be [B, H_kv, N_kv, D]")
-    v_rows = _head_rows(v, keys, "window_attention: v must be [B, H_kv, N_kv, D]")
-    if (left is not None and left < 0) or (right is not None and right < 0) or sinks < 0:
-        raise ValueError("window_attention: left, right and sinks must not be negative")
-    first = _int32_rows(starts, batch, "starts must be contiguous int32 [B]")
-    end = _int32_rows(lengths, batch, "lengths must be contiguous int32 [B]")
-    device = _same_device(q, k, v, starts, lengths, out)
-    if out is None:
-        out = q.new_empty((batch, n, heads * dim))
-    else:
-        if out.shape != (batch, n, heads * dim) or out.dtype != dtype or out.stride(2) != 1:
-            raise ValueError("window_attention: out must be [B, N, H * D] rows of the input's type")
-        _writable(out)
-    sizes = (_DTYPES[dtype], batch, heads, kv_heads, n, n_kv, dim, -1 if left is None else left,
-             -1 if right is None else right, sinks)  # fmt: skip
-    need = _window_workspace(device.index, *sizes)
-    workspace = q.new_empty(need, dtype=torch.uint8) if need else None
-    _call_on(device, "iris_window_attn_fwd", _lib.WINDOW_PROBLEM.pack(
-        *q_rows, *k_rows, *v_rows, out.data_ptr(), out.stride(0) if batch > 1 else 0, out.stride(1) if n > 1 else 0, first,
-        end, workspace.data_ptr() if need else 0, need, *sizes, scale if scale is not None else dim**-0.5))  # fmt: skip
-    if need:
-        _lib.count_launches(1)  # the join of the parts
-    return out
+    return (_lib._text_side or _lib.text_side()).window_attention(q, k, v, left, right, sinks, starts, lengths, scale, out)
 
 
 def pack_q4(
@@ -814,29 +645,7 @@ def gemv_q4(
     row stride may exceed ``K``) and 4-bit weights from :func:`pack_q4`, with FP32 sums;
     ``silu_in`` / ``silu_out`` turn the activations on, ``bias``: FP32 ``[N]``. The result
     is ``[M, N]`` of ``out_dtype`` (default: the input's)."""
-    _require(x.dim() == packed.dim() == scale.dim() == 2, "gemv_q4 needs x [M, K], packed [N, K / 2], scale [N, K / group]")
-    m, inner = x.shape
-    n = packed.shape[0]
-    if packed.dtype != torch.uint8 or not packed.is_contiguous() or packed.shape[1] * 2 != inner:
-        raise ValueError("gemv_q4: packed must be contiguous uint8 [N, K / 2]")
-    groups = scale.shape[1]
-    if scale.dtype != torch.bfloat16 or not scale.is_contiguous() or scale.shape[0] != n or not groups or inner % groups:
-        raise ValueError("gemv_q4: scale must be contiguous bf16 [N, K / group]")
-    if zero is not None and (zero.dtype != torch.uint8 or not zero.is_contiguous() or zero.shape != scale.shape):
-        raise ValueError("gemv_q4: zero must be contiguous uint8 [N, K / group]")
-    _require(x.stride(1) == 1, "gemv_q4: x rows must be contiguous")
-    if bias is not None:
-        _require_fp32(bias=bias)
-        _require(bias.shape == (n,), "gemv_q4: bias width")
-    device = _same_device(x, packed, scale, zero, bias)
-    code = _dtype(x)
-    out_code = code if out_dtype is None else _dtype(out_dtype)
-    out = x.new_empty((m, n), dtype=out_dtype)
-    _call_on(device, "iris_gemv_q4", _lib.Q4_PROBLEM.pack(
-        x.data_ptr(), packed.data_ptr(), scale.data_ptr(), 0 if zero is None else zero.data_ptr(),
-        0 if bias is None else bias.data_ptr(), out.data_ptr(), m, inner, n, x.stride(0) if m > 1 else inner,
-        inner // groups, code, out_code, silu_in, silu_out))  # fmt: skip
-    return out
+    return (_lib._text_side or _lib.text_side()).gemv_q4(x, packed, scale, zero, bias, silu_in, silu_out, out_dtype)
 
 
 def block_copy(

@@ -3,6 +3,7 @@ scaled rotary tables and the 4-bit packing."""
 
 import math
 import re
+import struct
 
 import pytest
 import torch
@@ -13,19 +14,19 @@ from test_library import _einval, lib  # noqa: F401 (lib: the built library)
 
 
 @pytest.fixture(scope="module")
-def K():
+def K(lib):  # noqa: F811
     from iris_b200 import kernels
 
     return kernels
 
 
-def test_problem_structs_match_the_header():
-    """Every struct is 8-byte members in the order that the binding packs them."""
-    from iris_b200 import _lib
+# the problem structs of include/iris_b200.h: 8-byte members, pointers as addresses
+ROPE, APPEND, WINDOW, Q4 = (struct.Struct(f) for f in ("@22q", "@40q", "@29qd", "@15q"))
 
+
+def test_problem_structs_are_as_packed_here():
     text = re.sub(r"/\*.*?\*/", "", (REPO / "include" / "iris_b200.h").read_text(), flags=re.S)
-    for name, packing in [("rope", _lib.ROPE_PROBLEM), ("append", _lib.APPEND_PROBLEM), ("window", _lib.WINDOW_PROBLEM),
-                          ("q4", _lib.Q4_PROBLEM)]:  # fmt: skip
+    for name, packing in [("rope", ROPE), ("append", APPEND), ("window", WINDOW), ("q4", Q4)]:
         body = re.search(rf"typedef struct iris_{name}_problem {{(.*?)}}", text, flags=re.S).group(1)
         fields = 0
         for line in filter(str.strip, body.split(";")):
@@ -35,13 +36,11 @@ def test_problem_structs_match_the_header():
 
 
 def test_c_entries_refuse_bad_arguments(lib):  # noqa: F811
-    from iris_b200 import _lib
-
     def rows(data=16, b=0, h=0, n=0):
         return data, b, h, n
 
     def rope(dtype=1, batch=1, heads=2, n=3, dim=64, rotary=64, table=9, layout=0, x=16):
-        return "iris_rope", _lib.ROPE_PROBLEM.pack(*rows(x), *rows(), 16, 16, 0, 0, 0, dtype, batch, heads, n, dim, rotary,
+        return "iris_rope", ROPE.pack(*rows(x), *rows(), 16, 16, 0, 0, 0, dtype, batch, heads, n, dim, rotary,
                                                    table, layout, 0), None  # fmt: skip
 
     for bad, message in [(dict(dtype=3), "dtype"), (dict(dim=63), "even"), (dict(rotary=66), "rotated columns"),
@@ -50,15 +49,14 @@ def test_c_entries_refuse_bad_arguments(lib):  # noqa: F811
         assert message in _einval(lib, *rope(**bad)), bad
 
     def append(kv=1, capacity=8, sinks=-1, starts=16):
-        return "iris_rope_append", _lib.APPEND_PROBLEM.pack(*rows() * 6, 16, 16, starts, 0, 1, 1, 2, kv, 3, 64, 64, 9, capacity,
-                                                            sinks, 0), None  # fmt: skip
+        return "iris_rope_append", APPEND.pack(*rows() * 6, 16, 16, starts, 0, 1, 1, 2, kv, 3, 64, 64, 9, capacity, sinks, 0, 0), None  # fmt: skip
 
     for bad, message in [(dict(kv=0), "head counts"), (dict(capacity=0), "slots"), (dict(sinks=8), "slots"),
                          (dict(sinks=-2), "slots"), (dict(starts=0), "null")]:  # fmt: skip
         assert message in _einval(lib, *append(**bad)), bad
 
     def attend(q=16, dtype=1, batch=1, heads=4, kv=2, n=3, m=5, dim=128, qn=128, kn=128, left=-1, right=0, sinks=0, scale=0.1):
-        return "iris_window_attn_fwd", _lib.WINDOW_PROBLEM.pack(
+        return "iris_window_attn_fwd", WINDOW.pack(
             *rows(q, n=qn), *rows(n=kn), *rows(n=128), 16, 0, 0, 0, 0, 0, 0, dtype, batch, heads, kv, n, m, dim, left, right,
             sinks, scale), None  # fmt: skip
 
@@ -70,7 +68,7 @@ def test_c_entries_refuse_bad_arguments(lib):  # noqa: F811
         assert message in _einval(lib, *attend(**bad)), bad
 
     def q4(x=16, dtype=1, m=1, k=128, ldx=128, group=32, n=4, out=16, out_dtype=1):
-        return "iris_gemv_q4", _lib.Q4_PROBLEM.pack(x, 16, 16, 0, 0, out, m, k, n, ldx, group, dtype, out_dtype, 0, 0), None
+        return "iris_gemv_q4", Q4.pack(x, 16, 16, 0, 0, out, m, k, n, ldx, group, dtype, out_dtype, 0, 0), None
 
     for bad, message in [(dict(group=16), "groups"), (dict(m=0), "1 to 64"), (dict(m=65), "1 to 64"), (dict(k=96, group=64), "multiple"),
                          (dict(ldx=120), "size"), (dict(n=0), "1 to 64"), (dict(x=8), "aligned"), (dict(ldx=132), "aligned"),
@@ -146,29 +144,27 @@ def test_wrappers_refuse_before_any_launch(K):
             K.pack_q4(w, group)
 
 
-def test_calls_go_to_the_tensors_device(K, monkeypatch):
-    """On another device than the current one: that device's stream, with it made current for the call."""
+def test_wrappers_refuse_what_is_no_tensor_or_number(K):
+    x, cos = torch.zeros(2, 4, 3, 64), torch.zeros(9, 32)
+    for call in (lambda: K.rope(None, cos, cos), lambda: K.rope(x, [1.0], cos), lambda: K.rope(x, cos, cos, 3),
+                 lambda: K.rope(x, cos, cos, out=x.numpy()), lambda: K.rope(x, cos, cos, layout=1),
+                 lambda: K.rope_append(x, x, x, cos, cos, None, x, x), lambda: K.gemv_q4(x, None, x),
+                 lambda: K.gemv_q4(x[0, 0], x[0, 0].byte(), x[0, 0].bfloat16(), out_dtype="f32")):  # fmt: skip
+        with pytest.raises(ValueError):
+            call()
+    q = x.bfloat16()
+    for bad in (dict(left="1"), dict(sinks=1.5), dict(scale="a"), dict(right=2**70)):
+        with pytest.raises((TypeError, OverflowError)):
+            K.window_attention(q, q, q, **bad)
+
+
+def test_missing_module_fails_loudly(lib, monkeypatch, tmp_path):  # noqa: F811
     from iris_b200 import _lib
 
-    seen = []
-
-    class Device:
-        def __init__(self, device):
-            self.device = device
-
-        def __enter__(self):
-            seen.append(("enter", self.device.index))
-
-        def __exit__(self, *a):
-            seen.append(("exit", self.device.index))
-
-    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index, raising=False)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
-    monkeypatch.setattr(torch.cuda, "device", Device)
-    monkeypatch.setattr(_lib, "call", lambda name, *args: seen.append((name, args)))
-    K._call_on(torch.device("cuda", 0), "entry", b"7")
-    K._call_on(torch.device("cuda", 1), "entry", b"8")
-    assert seen == [("entry", (b"7", 100)), ("enter", 1), ("entry", (b"8", 101)), ("exit", 1)]
+    monkeypatch.setattr(_lib, "_text_side", None)
+    monkeypatch.setattr(_lib, "TEXT_SIDE", tmp_path / "_text_side.so")
+    with pytest.raises(RuntimeError, match="not built"):
+        _lib.text_side()
 
 
 def test_rope_table_matches_its_formulas():
