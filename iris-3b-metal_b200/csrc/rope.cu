@@ -5,11 +5,13 @@
 // (2 i, 2 i + 1) or (i, i + R / 2), the columns from R on are copied.
 // Arithmetic in fp32, one rounding to the row's type.
 //
-// HBM-bound (3 flops per element read and written once). A thread owns one unit
-// of a token's rows, two vectors of V elements: V neighbouring pairs (interleaved)
-// or V columns and their partners R / 2 further (half), so both layouts read and
-// write whole vectors. It takes that unit in several heads, so the token's table
-// entries are read once for all of them.
+// HBM-bound (3 flops per element read and written once), as long as few instructions
+// are spent on finding the element. A thread owns one unit of a token's rows, two
+// vectors of V elements: V neighbouring pairs (interleaved) or V columns and their
+// partners R / 2 further (half), so both layouts read and write whole vectors. Where
+// there are threads to spare it takes that unit in EACH = 4 heads of one tensor, their
+// loads in flight together and the token's table entries read once for them. Slots
+// are the heads of a tensor that its threads begin at: `step` of them.
 #include "common.cuh"
 #include "iris_abi_internal.h"
 
@@ -17,6 +19,7 @@ namespace iris {
 namespace rope {
 
 constexpr int THREADS = 256;
+constexpr int64_t SPARE_THREADS = 4096;  // per SM, from which a thread takes four heads
 
 struct View {  // [batch, heads, n, D] rows, element strides
   const void* src;
@@ -42,7 +45,11 @@ struct Params {
   int64_t capacity;    // append: slots of the cache
   int64_t sinks;       // append: -1 plain cache, else slots that a rolling cache never overwrites
   bool zero_rest;      // append: zeros in out's rows from counts[b] on
-  int units, hslots, tokens_per_block;
+  int units;           // of a row
+  int step_q, step_kv;  // slots of q; of k and of v
+  int items;           // units * slots of a token
+  int tokens_per_block;
+  unsigned by_units, by_items;  // ceil(2^20 / d): exact quotients of numbers below 1024
 };
 
 template <typename T>
@@ -64,8 +71,12 @@ IRIS_DEVICE __half from_f32(float v) { return __float2half_rn(v); }
 
 // The turned pair, contracted the same way in every variant: a row's bits do not
 // depend on its alignment.
-IRIS_DEVICE float turn_a(float a, float b, float c, float s) { return fmaf(a, c, -__fmul_rn(b, s)); }
-IRIS_DEVICE float turn_b(float a, float b, float c, float s) { return fmaf(a, s, __fmul_rn(b, c)); }
+template <typename T>
+IRIS_DEVICE void turn(T& a, T& b, float c, float s) {
+  const float f = to_f32(a), g = to_f32(b);
+  a = from_f32<T>(fmaf(f, c, -__fmul_rn(g, s)));
+  b = from_f32<T>(fmaf(f, s, __fmul_rn(g, c)));
+}
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
@@ -85,89 +96,112 @@ IRIS_DEVICE int64_t cache_slot(const Params& a, int64_t p, int64_t last, bool* b
   return a.sinks + (p - a.sinks) % turn;
 }
 
-template <typename T, int V, bool HALF, bool APPEND>
+template <int V>
+IRIS_DEVICE void load_floats(const float* p, float (&v)[V]) {
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(p + i));
+      v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = __ldg(p + i);
+  }
+}
+
+template <typename T, int V, bool HALF, bool APPEND, int EACH>
 __global__ void __launch_bounds__(THREADS) rope_kernel(const __grid_constant__ Params a) {
-  const int items = a.tokens_per_block * a.hslots * a.units;
-  const int heads = a.heads_q + 2 * a.heads_kv;
-  for (int item = threadIdx.x; item < items; item += THREADS) {
-    const int u = item % a.units;
-    const int rest = item / a.units;
-    const int slot = rest % a.hslots;
-    const int64_t token = static_cast<int64_t>(blockIdx.x) * a.tokens_per_block + rest / a.hslots;
+  // rows wider than the block's threads take several turns
+  for (unsigned item = threadIdx.x; item < static_cast<unsigned>(a.tokens_per_block * a.items); item += THREADS) {
+    const unsigned local = a.items <= THREADS ? (item * a.by_items) >> 20 : 0u;
+    const unsigned rest = item - local * a.items;
+    const int slot0 = a.items <= THREADS ? static_cast<int>((rest * a.by_units) >> 20) : static_cast<int>(rest / a.units);
+    const int u = static_cast<int>(rest) - slot0 * a.units;
+    const unsigned token = blockIdx.x * static_cast<unsigned>(a.tokens_per_block) + local;
     if (token >= a.tokens) return;
-    const int b = static_cast<int>(token / a.n), t = static_cast<int>(token - static_cast<int64_t>(b) * a.n);
-    int64_t p = t, row = t;  // position; row of the cache
+    const int b = static_cast<int>(token / static_cast<unsigned>(a.n)), t = static_cast<int>(token) - b * a.n;
+    // the tensor of this slot, and its first head
+    const bool isq = !APPEND || slot0 < a.step_q, isv = APPEND && slot0 >= a.step_q + a.step_kv;
+    const View& w = isq ? a.q : isv ? a.v : a.k;
+    const int heads = isq ? a.heads_q : a.heads_kv, step = isq ? a.step_q : a.step_kv;
+    const int head = isq ? slot0 : isv ? slot0 - a.step_q - a.step_kv : slot0 - a.step_q;
+    int64_t p = t, row = t;  // position; row of the target
     bool bad = false;
     if constexpr (APPEND) {
       const int64_t first = a.starts[b];
       const int64_t count = a.counts ? min(a.counts[b], a.n) : a.n;
       if (t >= count) {
-        if (!a.zero_rest) continue;
-        const Vec<T, V> none = {};
-        for (int h = slot; h < a.heads_q; h += a.hslots) {
-          T* dst = reinterpret_cast<T*>(a.q.dst) + b * a.q.db + h * a.q.dh + t * a.q.dn + u * 2 * V;
-          *reinterpret_cast<Vec<T, V>*>(dst) = none;
-          *reinterpret_cast<Vec<T, V>*>(dst + V) = none;
+        if (isq && a.zero_rest) {
+          const Vec<T, V> none = {};
+          T* dst = reinterpret_cast<T*>(w.dst) + b * w.db + t * w.dn + u * 2 * V;
+          for (int h = head; h < heads; h += step) {
+            *reinterpret_cast<Vec<T, V>*>(dst + h * w.dh) = none;
+            *reinterpret_cast<Vec<T, V>*>(dst + h * w.dh + V) = none;
+          }
         }
         continue;
       }
       p = first + t;
       bad = p < 0 || p >= a.table_rows;
       bool full = false;
-      row = bad ? -1 : cache_slot(a, p, first + count - 1, &full);
-      if ((bad || full) && u == 0 && slot == 0) atomicOr(&g_device_error, kErrBadArgument);
+      const int64_t kept = bad ? -1 : cache_slot(a, p, first + count - 1, &full);
+      if ((bad || full) && u == 0 && slot0 == 0) atomicOr(&g_device_error, kErrBadArgument);
+      if (!isq) {
+        if (kept < 0) continue;
+        row = kept;
+      }
     } else {
       if (a.positions) {
         const int64_t at = b * a.pos_stride + t;
         p = a.pos64 ? reinterpret_cast<const int64_t*>(a.positions)[at] : reinterpret_cast<const int*>(a.positions)[at];
       }
       bad = p < 0 || p >= a.table_rows;
-      if (bad && u == 0 && slot == 0) atomicOr(&g_device_error, kErrBadArgument);
+      if (bad && u == 0 && slot0 == 0) atomicOr(&g_device_error, kErrBadArgument);
     }
-    const bool turns = u * 2 * V < a.rotary;  // a unit past the rotated columns is copied
+    const bool turns = u * 2 * V < a.rotary && !isv;  // a unit past the rotated columns is copied, and so is v
     // the unit's two vectors: first and second elements of its pairs (half layout), or one run of pairs
-    const int c0 = !turns ? u * 2 * V : HALF ? u * V : u * 2 * V;
+    const int c0 = turns && HALF ? u * V : u * 2 * V;
     const int c1 = turns && HALF ? a.rotary / 2 + u * V : c0 + V;
+    const T* src = reinterpret_cast<const T*>(w.src) + b * w.sb + t * w.sn + head * w.sh;
+    T* dst = reinterpret_cast<T*>(w.dst) + b * w.db + row * w.dn + head * w.dh;
+    Vec<T, V> x[EACH], y[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      if (j > 0 && head + j * step >= heads) break;
+      const T* from = src + j * step * w.sh;
+      x[j] = *reinterpret_cast<const Vec<T, V>*>(from + c0);
+      y[j] = *reinterpret_cast<const Vec<T, V>*>(from + c1);
+    }
     float cs[V], sn[V];
     if (turns) {
       const int64_t at = (bad ? 0 : p) * (a.rotary / 2) + u * V;
+      load_floats<V>(a.cos + at, cs);
+      load_floats<V>(a.sin + at, sn);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        cs[i] = bad ? __int_as_float(0x7fc00000) : __ldg(a.cos + at + i);  // a position outside the table: NaN
-        sn[i] = a.sign * __ldg(a.sin + at + i);
+        sn[i] *= a.sign;
+        if (bad) cs[i] = __int_as_float(0x7fc00000);  // a position outside the table: NaN
       }
     }
-    for (int h = slot; h < heads; h += a.hslots) {
-      const bool isq = !APPEND || h < a.heads_q;
-      const bool isv = APPEND && h >= a.heads_q + a.heads_kv;
-      const View& w = isq ? a.q : isv ? a.v : a.k;
-      const int hh = isq ? h : isv ? h - a.heads_q - a.heads_kv : h - a.heads_q;
-      if (!isq && row < 0) continue;
-      const T* src = reinterpret_cast<const T*>(w.src) + b * w.sb + hh * w.sh + t * w.sn;
-      T* dst = reinterpret_cast<T*>(w.dst) + b * w.db + hh * w.dh + (isq ? t : row) * w.dn;
-      Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(src + c0), y = *reinterpret_cast<const Vec<T, V>*>(src + c1);
-      if (turns && !isv) {
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      if (j > 0 && head + j * step >= heads) break;
+      if (turns) {
         if constexpr (HALF || V == 1) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float f = to_f32(x.e[i]), g = to_f32(y.e[i]);
-            x.e[i] = from_f32<T>(turn_a(f, g, cs[i], sn[i]));
-            y.e[i] = from_f32<T>(turn_b(f, g, cs[i], sn[i]));
-          }
+          for (int i = 0; i < V; ++i) turn(x[j].e[i], y[j].e[i], cs[i], sn[i]);
         } else {
 #pragma unroll
           for (int i = 0; i < V / 2; ++i) {
-            float f = to_f32(x.e[2 * i]), g = to_f32(x.e[2 * i + 1]);
-            x.e[2 * i] = from_f32<T>(turn_a(f, g, cs[i], sn[i]));
-            x.e[2 * i + 1] = from_f32<T>(turn_b(f, g, cs[i], sn[i]));
-            f = to_f32(y.e[2 * i]), g = to_f32(y.e[2 * i + 1]);
-            y.e[2 * i] = from_f32<T>(turn_a(f, g, cs[V / 2 + i], sn[V / 2 + i]));
-            y.e[2 * i + 1] = from_f32<T>(turn_b(f, g, cs[V / 2 + i], sn[V / 2 + i]));
+            turn(x[j].e[2 * i], x[j].e[2 * i + 1], cs[i], sn[i]);
+            turn(y[j].e[2 * i], y[j].e[2 * i + 1], cs[V / 2 + i], sn[V / 2 + i]);
           }
         }
       }
-      *reinterpret_cast<Vec<T, V>*>(dst + c0) = x;
-      *reinterpret_cast<Vec<T, V>*>(dst + c1) = y;
+      T* to = dst + j * step * w.dh;
+      *reinterpret_cast<Vec<T, V>*>(to + c0) = x[j];
+      *reinterpret_cast<Vec<T, V>*>(to + c1) = y[j];
     }
   }
 }
@@ -180,27 +214,37 @@ inline bool fits(const View& w, int64_t elems, int64_t size) {
                               w.dn % elems == 0);
 }
 
-template <typename T, int V, bool APPEND>
-int launch_v(Params& a, bool half, cudaStream_t st) {
+template <typename T, int V, bool APPEND, int EACH>
+int launch_each(Params& a, bool half, cudaStream_t st) {
   a.units = a.head_dim / (2 * V);
-  const int heads = a.heads_q + 2 * a.heads_kv;
-  a.hslots = heads;
-  a.tokens_per_block = THREADS / (a.units * a.hslots);
-  if (a.tokens_per_block < 1) a.tokens_per_block = 1;
+  a.step_q = (a.heads_q + EACH - 1) / EACH;
+  a.step_kv = (a.heads_kv + EACH - 1) / EACH;
+  a.items = a.units * (a.step_q + 2 * a.step_kv);
+  a.tokens_per_block = a.items <= THREADS ? THREADS / a.items : 1;
+  a.by_units = ((1u << 20) + a.units - 1) / a.units;
+  a.by_items = ((1u << 20) + a.items - 1) / a.items;
   const int64_t blocks = (a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
   if (half)
-    rope_kernel<T, V, true, APPEND><<<static_cast<unsigned>(blocks), THREADS, 0, st>>>(a);
+    rope_kernel<T, V, true, APPEND, EACH><<<static_cast<unsigned>(blocks), THREADS, 0, st>>>(a);
   else
-    rope_kernel<T, V, false, APPEND><<<static_cast<unsigned>(blocks), THREADS, 0, st>>>(a);
+    rope_kernel<T, V, false, APPEND, EACH><<<static_cast<unsigned>(blocks), THREADS, 0, st>>>(a);
   IRIS_CUDA(cudaGetLastError());
   return IRIS_OK;
+}
+
+template <typename T, int V, bool APPEND>
+int launch_v(Params& a, bool half, cudaStream_t st) {
+  const int64_t threads = a.tokens * (a.head_dim / (2 * V)) * (a.heads_q + 2 * a.heads_kv);
+  if (threads >= static_cast<int64_t>(num_sms()) * SPARE_THREADS) return launch_each<T, V, APPEND, 4>(a, half, st);
+  return launch_each<T, V, APPEND, 1>(a, half, st);
 }
 
 template <typename T, bool APPEND>
 int launch(Params& a, bool half, cudaStream_t st) {
   constexpr int S = sizeof(T), W = 16 / S;
   auto ok = [&](int v) {
-    return a.rotary % (2 * v) == 0 && a.head_dim % (2 * v) == 0 && fits(a.q, v, S) && fits(a.k, v, S) && fits(a.v, v, S);
+    return a.rotary % (2 * v) == 0 && a.head_dim % (2 * v) == 0 && fits(a.q, v, S) && fits(a.k, v, S) && fits(a.v, v, S) &&
+           aligned16(a.cos) && aligned16(a.sin);
   };
   if (ok(W)) return launch_v<T, W, APPEND>(a, half, st);
   if (ok(W / 2)) return launch_v<T, W / 2, APPEND>(a, half, st);
