@@ -75,6 +75,14 @@ IRIS_DEVICE uint64_t global_timer_ns() {
   return t;
 }
 
+// ------------------------------------------------------- programmatic launch
+// A kernel launched with launch_early (iris_abi_internal.h) may start while the one
+// before it in the stream ends: it touches global memory only after grid_wait
+// (that kernel complete and its writes visible; no wait where it was launched
+// otherwise), and lets its own successor start with grid_trigger, after its wait.
+IRIS_DEVICE void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+IRIS_DEVICE void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ----------------------------------------------------------------- mbarrier
 IRIS_DEVICE uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -37,6 +37,27 @@ int make_tmap_2d_bytes(CUtensorMap* map, const void* base, int64_t inner, int64_
 int make_tmap_heads(CUtensorMap* map, const void* base, int dtype, int64_t head_dim, int64_t tokens, int64_t heads,
                     int64_t batch, int64_t stride_n, int64_t stride_h, int64_t stride_b, int box_rows);
 
+// Launch a kernel that may start before its predecessor in the stream has ended (it
+// begins with grid_wait, common.cuh); cluster: CTAs per cluster along x.
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+                         unsigned cluster, const Args&... args) {
+  cudaLaunchAttribute attrs[2] = {};
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = attrs;
+  config.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 }  // namespace iris
 
 #define IRIS_REQUIRE(cond, msg)                           \

@@ -172,6 +172,8 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
     fence_barrier_init();
   }
   __syncthreads();
+  grid_wait();
+  grid_trigger();
 
   auto load = [&](int t) {  // step t into its slot
     if (lane == 0 && t < steps && n0 < p.N) {
@@ -469,18 +471,8 @@ int launch_g(Params& p, int passes, cudaStream_t st) {
   }
   CUtensorMap tw;
   IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tw, p.packed, p.K / 2, p.N, p.K / 2, STEP / 2, ROWS));
-  cudaLaunchAttribute cluster = {};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = static_cast<unsigned>(parts);
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(tiles * parts), static_cast<unsigned>(passes));
-  config.blockDim = dim3(THREADS);
-  config.dynamicSmemBytes = static_cast<size_t>(smem);
-  config.stream = st;
-  config.attrs = &cluster;
-  config.numAttrs = 1;
-  IRIS_CUDA(cudaLaunchKernelEx(&config, kernel, tw, p));
+  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(tiles * parts), static_cast<unsigned>(passes)), THREADS, smem, st,
+                         static_cast<unsigned>(parts), tw, p));
   return IRIS_OK;
 }
 

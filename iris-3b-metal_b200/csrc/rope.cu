@@ -112,6 +112,8 @@ IRIS_DEVICE void load_floats(const float* p, float (&v)[V]) {
 
 template <typename T, int V, bool HALF, bool APPEND, int EACH>
 __global__ void __launch_bounds__(THREADS) rope_kernel(const __grid_constant__ Params a) {
+  grid_wait();
+  grid_trigger();
   // rows wider than the block's threads take several turns
   for (unsigned item = threadIdx.x; item < static_cast<unsigned>(a.tokens_per_block * a.items); item += THREADS) {
     const unsigned local = a.items <= THREADS ? (item * a.by_items) >> 20 : 0u;
@@ -224,11 +226,8 @@ int launch_each(Params& a, bool half, cudaStream_t st) {
   a.by_units = ((1u << 20) + a.units - 1) / a.units;
   a.by_items = ((1u << 20) + a.items - 1) / a.items;
   const int64_t blocks = (a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
-  if (half)
-    rope_kernel<T, V, true, APPEND, EACH><<<static_cast<unsigned>(blocks), THREADS, 0, st>>>(a);
-  else
-    rope_kernel<T, V, false, APPEND, EACH><<<static_cast<unsigned>(blocks), THREADS, 0, st>>>(a);
-  IRIS_CUDA(cudaGetLastError());
+  auto kernel = half ? rope_kernel<T, V, true, APPEND, EACH> : rope_kernel<T, V, false, APPEND, EACH>;
+  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(blocks)), THREADS, 0, st, 1, a));
   return IRIS_OK;
 }
 

@@ -211,6 +211,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 2)
   const int row0 = (static_cast<int>(gridDim.x / per_row) - 1 - static_cast<int>(blockIdx.x / per_row)) * BQ;
   const int b = blockIdx.x % per_row / p.heads_q, h = blockIdx.x % p.heads_q;
   const int hk = h / (p.heads_q / p.heads_kv);
+  grid_wait();
+  grid_trigger();
   const int length = sample_length(p, b);
   const int64_t start = sample_start(p, b);
   const Blocks blocks = key_blocks(p, start + row0, min(BQ, p.n - row0), length);
@@ -500,8 +502,7 @@ int launch_tiles(const Params& p, int dtype, cudaStream_t st) {
     IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem<D>()));
     if (dev < 64) configured[dev] = true;
   }
-  kernel<<<static_cast<unsigned>(ctas), TILE_THREADS, tile_smem<D>(), st>>>(tq, tk, tv, p);
-  IRIS_CUDA(cudaGetLastError());
+  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(ctas)), TILE_THREADS, tile_smem<D>(), st, 1, tq, tk, tv, p));
   return IRIS_OK;
 }
 
@@ -576,7 +577,8 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   constexpr int TILE = STEP_KEYS * D * 2;  // bytes of one K or V tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (sp.parts) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  grid_wait();
+  grid_trigger();
   const int split = static_cast<int>(blockIdx.x % sp.splits);
   const int unit = static_cast<int>(blockIdx.x / sp.splits);  // (b, hk, row tile)
   const int rt = unit % sp.row_tiles, hk = unit / sp.row_tiles % p.heads_kv, b = unit / sp.row_tiles / p.heads_kv;
@@ -783,7 +785,8 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) join_kernel(const __grid_cons
   const int64_t part0 = unit * sp.splits * STEP_ROWS + row % STEP_ROWS;
   const int64_t all_rows = static_cast<int64_t>(p.batch) * p.heads_kv * sp.row_tiles * sp.splits * STEP_ROWS;
   const float2* state = reinterpret_cast<const float2*>(sp.parts + all_rows * D);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  grid_wait();
+  grid_trigger();
   float top = -INFINITY;
   for (int c = lane; c < sp.splits; c += 32) top = fmaxf(top, state[part0 + c * STEP_ROWS].x);
 #pragma unroll
@@ -864,19 +867,9 @@ int launch_step(const Params& p, float* parts, int64_t parts_bytes, cudaStream_t
     IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, step_smem<D>()));
     if (dev < 64) configured[dev] = true;
   }
-  kernel<<<static_cast<unsigned>(units * sp.splits), STEP_WARPS * 32, step_smem<D>(), st>>>(p, sp);
-  IRIS_CUDA(cudaGetLastError());
+  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(units * sp.splits)), STEP_WARPS * 32, step_smem<D>(), st, 1, p, sp));
   if (sp.parts == nullptr) return IRIS_OK;
-  cudaLaunchAttribute early = {};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(rows));
-  config.blockDim = dim3(STEP_WARPS * 32);
-  config.stream = st;
-  config.attrs = &early;
-  config.numAttrs = 1;
-  IRIS_CUDA(cudaLaunchKernelEx(&config, join_kernel<T, D>, p, sp));
+  IRIS_CUDA(launch_early(join_kernel<T, D>, dim3(static_cast<unsigned>(rows)), STEP_WARPS * 32, 0, st, 1, p, sp));
   return IRIS_OK;
 }
 
