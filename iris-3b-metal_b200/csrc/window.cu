@@ -6,6 +6,8 @@
 // A row's visible keys are two runs, [0, early) and [lo, hi) (struct Span).
 #include <math.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "iris_abi_internal.h"
 
@@ -514,15 +516,17 @@ int launch_tiles(const Params& p, int dtype, cudaStream_t st) {
 // ring of cp.async copies (no barrier until the end), scores and P V on mma.sync
 // m16n8k16: HBM-bound, one K and V byte is used for 16 rows at most, which leaves the
 // 5th-generation tensor cores' 128-row tiles seven eighths empty. Chunks are the same
-// length for every sample, so samples of different lengths give equal work; a second
-// kernel joins the chunks of a row (programmatic launch: its start overlaps).
+// length for every sample, so samples of different lengths give equal work. Up to
+// eight chunks are a cluster's CTAs, joined through distributed shared memory: one
+// launch, nothing in global memory. More of them are joined by a second kernel.
 constexpr int STEP_WARPS = 4, STEP_STAGES = 3, STEP_KEYS = 16, STEP_ROWS = 16;
 
 struct Split {
   int row_tiles;  // 16-row tiles of a key head's query rows
   int chunk;      // keys per CTA
   int splits;     // chunks of the longest list
-  float* parts;   // [batch, heads_kv, row_tiles, splits, 16, D] sums, then [.., 16] maxima and totals; null: one chunk
+  bool cluster;   // the chunks of a row tile are a cluster
+  float* parts;   // else [batch, heads_kv, row_tiles, splits, 16, D] sums, then [.., 16] maxima and totals; null: one chunk
 };
 
 template <typename T>
@@ -547,6 +551,13 @@ IRIS_DEVICE void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
 // 16 bytes global -> shared, or 16 zero bytes
 IRIS_DEVICE void copy16(uint32_t dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+
+constexpr int MOST_CLUSTER = 8;
+IRIS_DEVICE float remote(uint32_t at) {  // another CTA's shared memory (map_to_cta)
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
 }
 
 template <int D>
@@ -756,7 +767,12 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
         acc[c] = make_float2(fmaf(f, x.x, acc[c].x), fmaf(f, x.y, acc[c].y));
       }
     }
-    if (sp.parts == nullptr) {
+    if (sp.cluster) {  // in the first warp's place: these lanes alone have read it
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) *reinterpret_cast<float2*>(sums + r * D + 64 * c + 2 * lane) = acc[c];
+      __syncwarp();
+      if (lane == 0) tops[0][r] = top, totals[0][r] = total;
+    } else if (sp.parts == nullptr) {
       finish_row<T, D>(p, b, hk * group + (r0 + r) % group, (r0 + r) / group, acc, total);
     } else {
       const int64_t part = (static_cast<int64_t>(unit) * sp.splits + split) * STEP_ROWS + r;
@@ -768,6 +784,38 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
         state[part] = make_float2(top, total);
       }
     }
+  }
+  if (sp.cluster) {
+    cluster_sync();
+    for (int r = split * STEP_WARPS + warp; r <= r_last - r0; r += sp.splits * STEP_WARPS) {
+      float top[MOST_CLUSTER], part[MOST_CLUSTER], all_top = -INFINITY, total = 0.f;
+#pragma unroll
+      for (int q = 0; q < MOST_CLUSTER; ++q) {
+        top[q] = -INFINITY, part[q] = 0.f;
+        if (q < sp.splits) {
+          top[q] = remote(map_to_cta(&tops[0][r], q));
+          part[q] = remote(map_to_cta(&totals[0][r], q));
+        }
+        all_top = fmaxf(all_top, top[q]);
+      }
+      float2 acc[D / 64];
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int q = 0; q < MOST_CLUSTER; ++q) {
+        if (q < sp.splits) {
+          const float f = top[q] == -INFINITY ? 1.f : ex2(top[q] - all_top);
+          total = fmaf(f, part[q], total);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            const uint32_t at = map_to_cta(sums + r * D + 64 * c + 2 * lane, q);
+            acc[c] = make_float2(fmaf(f, remote(at), acc[c].x), fmaf(f, remote(at + 4), acc[c].y));
+          }
+        }
+      }
+      finish_row<T, D>(p, b, hk * group + (r0 + r) % group, (r0 + r) / group, acc, total);
+    }
+    cluster_sync();  // no CTA leaves while its sums are read
   }
 }
 
@@ -828,23 +876,38 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) join_kernel(const __grid_cons
 // Few rows per key head leave a 128-row tile mostly empty, and few CTAs: split the keys instead.
 bool few_rows(int64_t n, int64_t group) { return n * group <= 64; }
 
-// Chunks of a call: a bound on the keys that a row tile sees, and pieces of at least
-// one tile per warp, about STEP_WAVES rounds of two CTAs per SM in all.
-constexpr int64_t STEP_WAVES = 6;
+// Chunks of a call, from a bound on the keys that a row tile sees. The CTAs that the SMs
+// hold at once are a wave; w waves take about w times a chunk and a CTA's own time
+// (CTA_KEYS), so the number of waves whose chunks waste least is taken, and more of
+// them for several samples, whose lengths may differ, where that costs little and
+// leaves long chunks. One token, 128 wide, us (chunks of one wave against six or against
+// LONG_CHUNK alone): one sample, 5 key heads, 65536 keys 35 against 60 and 48; 4
+// samples, 8 key heads, 4096 keys 18.6 against 27 and 21.
+constexpr int64_t STEP_WAVES = 6, STEP_CTAS = 2, LONG_CHUNK = 1024, SHORT_CHUNK = 192, CTA_KEYS = 96;
 
 void split_keys(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv, int64_t left, int64_t right,
                 int64_t sinks, Split* sp) {
   int64_t span = n_kv;
   if (left < kNoBound && right < kNoBound && left + right + n + sinks < n_kv) span = left + right + n + sinks;
   const int64_t row_tiles = (n * (heads_q / heads_kv) + STEP_ROWS - 1) / STEP_ROWS;
-  const int64_t units = batch * heads_kv * row_tiles;
+  const int64_t units = batch * heads_kv * row_tiles, slots = num_sms() * STEP_CTAS;
   constexpr int64_t unit = STEP_WARPS * STEP_KEYS;
-  int64_t chunk = span * units / (num_sms() * 2 * STEP_WAVES);
-  chunk = (chunk + unit - 1) / unit * unit;
-  if (chunk < unit) chunk = unit;
+  auto pieces = [&](int64_t splits) { return std::max(unit, ((span + splits - 1) / splits + unit - 1) / unit * unit); };
+  const int64_t first = (units + slots - 1) / slots;  // fewer waves do not hold every unit
+  int64_t chunk = pieces(1), least = first * (chunk + CTA_KEYS);
+  for (int64_t w = first; w < first + STEP_WAVES; ++w) {
+    const int64_t c = pieces(w * slots / units), cost = w * (c + CTA_KEYS);
+    if (cost < least || (batch > 1 && c >= LONG_CHUNK && cost < least + least / 12)) {
+      chunk = c;
+      least = std::min(least, cost);
+    }
+  }
+  // eight short chunks rather than more of them and a second launch
+  if (span > MOST_CLUSTER * chunk && pieces(MOST_CLUSTER) <= SHORT_CHUNK) chunk = pieces(MOST_CLUSTER);
   sp->row_tiles = static_cast<int>(row_tiles);
   sp->chunk = static_cast<int>(chunk);
   sp->splits = static_cast<int>(span > chunk ? (span + chunk - 1) / chunk : 1);
+  sp->cluster = sp->splits > 1 && sp->splits <= MOST_CLUSTER;
 }
 
 template <typename T, int D>
@@ -854,7 +917,7 @@ int launch_step(const Params& p, float* parts, int64_t parts_bytes, cudaStream_t
   const int64_t units = static_cast<int64_t>(p.batch) * p.heads_kv * sp.row_tiles;
   const int64_t rows = static_cast<int64_t>(p.batch) * p.heads_q * p.n;
   IRIS_REQUIRE(units * sp.splits < (1ll << 31) && rows < (1ll << 31), "window_attn_fwd: too many rows");
-  if (sp.splits > 1) {
+  if (sp.splits > 1 && !sp.cluster) {
     IRIS_REQUIRE(parts != nullptr && aligned16(parts) && parts_bytes >= units * sp.splits * STEP_ROWS * (D + 2) * 4,
                  "window_attn_fwd: workspace too small");
     sp.parts = parts;
@@ -867,7 +930,8 @@ int launch_step(const Params& p, float* parts, int64_t parts_bytes, cudaStream_t
     IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, step_smem<D>()));
     if (dev < 64) configured[dev] = true;
   }
-  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(units * sp.splits)), STEP_WARPS * 32, step_smem<D>(), st, 1, p, sp));
+  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(units * sp.splits)), STEP_WARPS * 32, step_smem<D>(), st,
+                         sp.cluster ? static_cast<unsigned>(sp.splits) : 1u, p, sp));
   if (sp.parts == nullptr) return IRIS_OK;
   IRIS_CUDA(launch_early(join_kernel<T, D>, dim3(static_cast<unsigned>(rows)), STEP_WARPS * 32, 0, st, 1, p, sp));
   return IRIS_OK;
@@ -915,7 +979,7 @@ extern "C" int iris_window_attn_workspace(const iris_window_problem* q, int64_t*
   Split sp = {};
   split_keys(q->batch, q->heads_q, q->heads_kv, q->n, q->n_kv, bound(q->left), bound(q->right),
              q->sinks < q->n_kv ? q->sinks : q->n_kv, &sp);
-  if (sp.splits > 1) *bytes = q->batch * q->heads_kv * sp.row_tiles * sp.splits * STEP_ROWS * (q->head_dim + 2) * 4;
+  if (sp.splits > 1 && !sp.cluster) *bytes = q->batch * q->heads_kv * sp.row_tiles * sp.splits * STEP_ROWS * (q->head_dim + 2) * 4;
   return IRIS_OK;
 }
 
