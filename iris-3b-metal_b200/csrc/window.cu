@@ -873,47 +873,94 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) join_kernel(const __grid_cons
   finish_row<T, D>(p, b, hk * group + row % group, row / group, acc, total);
 }
 
-// Few rows per key head leave a 128-row tile mostly empty, and few CTAs: split the keys instead.
-bool few_rows(int64_t n, int64_t group) { return n * group <= 64; }
+// Clusters of `size` step_kernel CTAs that run at once: GPCs hold whole clusters, so
+// fewer CTAs than the SMs hold alone.
+int64_t clusters_at_once(int size) {
+  static int cache[64][MOST_CLUSTER + 1] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return num_sms() * 2 / size;
+  if (cache[dev][size] == 0) {
+    auto kernel = step_kernel<__nv_bfloat16, 128>;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(size);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(size));
+    config.blockDim = dim3(STEP_WARPS * 32);
+    config.dynamicSmemBytes = step_smem<128>();
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, step_smem<128>()) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = num_sms() * 2 / size;
+    }
+    cache[dev][size] = n;
+  }
+  return cache[dev][size];
+}
 
-// Chunks of a call, from a bound on the keys that a row tile sees. The CTAs that the SMs
-// hold at once are a wave; w waves take about w times a chunk and a CTA's own time
-// (CTA_KEYS), so the number of waves whose chunks waste least is taken, and more of
-// them for several samples, whose lengths may differ, where that costs little and
-// leaves long chunks. One token, 128 wide, us (chunks of one wave against six or against
-// LONG_CHUNK alone): one sample, 5 key heads, 65536 keys 35 against 60 and 48; 4
-// samples, 8 key heads, 4096 keys 18.6 against 27 and 21.
-constexpr int64_t STEP_WAVES = 6, STEP_CTAS = 2, LONG_CHUNK = 1024, SHORT_CHUNK = 192, CTA_KEYS = 96;
+// How a call's keys are split, or that whole 128-row tiles are the better form.
+//
+// Split: from a bound on the keys that a row tile sees. The CTAs that the SMs hold at
+// once are a wave; w waves take about w times a chunk and a CTA's own time (CTA_KEYS),
+// so the number of waves whose chunks waste least is taken, and more of them for
+// several samples, whose lengths may differ, where that costs little and leaves long
+// chunks. One token, 128 wide, us (chunks of one wave against six or against LONG_CHUNK
+// alone): one sample, 5 key heads, 65536 keys 34 against 60 and 48; 4 samples, 8 key
+// heads, 4096 keys 18.6 against 27 and 21.
+// Tiles: a CTA walks its keys at TILE_NS each whatever rows it has; a split CTA at
+// STEP_NS. One sample, 20 over 5 heads, 2048 keys, us split / tiles: 8 tokens 9.7 / 30,
+// 128 tokens 43 / 32; 16384 keys: 64 tokens 110 / 216, 128 tokens 214 / 217.
+constexpr int64_t STEP_WAVES = 6, STEP_CTAS = 2, LONG_CHUNK = 1024, SHORT_CHUNK = 192, CTA_KEYS = 96, JOIN_KEYS = 64;
+constexpr int64_t STEP_NS = 25, TILE_NS = 13;
 
-void split_keys(int64_t batch, int64_t heads_q, int64_t heads_kv, int64_t n, int64_t n_kv, int64_t left, int64_t right,
-                int64_t sinks, Split* sp) {
-  int64_t span = n_kv;
-  if (left < kNoBound && right < kNoBound && left + right + n + sinks < n_kv) span = left + right + n + sinks;
-  const int64_t row_tiles = (n * (heads_q / heads_kv) + STEP_ROWS - 1) / STEP_ROWS;
-  const int64_t units = batch * heads_kv * row_tiles, slots = num_sms() * STEP_CTAS;
+struct Sizes {
+  int64_t batch, heads_q, heads_kv, n, n_kv, left, right, sinks;
+};
+
+bool split_keys(const Sizes& z, Split* sp) {
+  const int64_t group = z.heads_q / z.heads_kv, slots = num_sms() * STEP_CTAS;
+  auto span_of = [&](int64_t tokens) {  // keys that so many neighbouring rows see at most
+    return z.left < kNoBound && z.right < kNoBound ? std::min(z.n_kv, z.left + z.right + tokens + z.sinks) : z.n_kv;
+  };
+  const int64_t row_tiles = (z.n * group + STEP_ROWS - 1) / STEP_ROWS, units = z.batch * z.heads_kv * row_tiles;
+  const int64_t span = span_of(std::min(z.n, (STEP_ROWS - 1) / group + 2));
   constexpr int64_t unit = STEP_WARPS * STEP_KEYS;
   auto pieces = [&](int64_t splits) { return std::max(unit, ((span + splits - 1) / splits + unit - 1) / unit * unit); };
+  auto cost_of = [&](int64_t chunk, int64_t waves) {
+    const int64_t splits = (span + chunk - 1) / chunk;
+    if (splits > MOST_CLUSTER) return waves * (chunk + CTA_KEYS) + JOIN_KEYS;
+    if (splits > 1) waves = (units + clusters_at_once(static_cast<int>(splits)) - 1) / clusters_at_once(static_cast<int>(splits));
+    return waves * (chunk + CTA_KEYS);
+  };
   const int64_t first = (units + slots - 1) / slots;  // fewer waves do not hold every unit
-  int64_t chunk = pieces(1), least = first * (chunk + CTA_KEYS);
-  for (int64_t w = first; w < first + STEP_WAVES; ++w) {
-    const int64_t c = pieces(w * slots / units), cost = w * (c + CTA_KEYS);
-    if (cost < least || (batch > 1 && c >= LONG_CHUNK && cost < least + least / 12)) {
+  int64_t chunk = pieces(1), least = cost_of(chunk, first);
+  auto consider = [&](int64_t c, int64_t waves) {
+    const int64_t cost = cost_of(c, waves);
+    if (cost < least || (z.batch > 1 && c < chunk && c >= LONG_CHUNK && cost < least + least / 12)) {
       chunk = c;
       least = std::min(least, cost);
     }
-  }
+  };
+  for (int64_t splits = 2; splits <= MOST_CLUSTER; ++splits) consider(pieces(splits), (units * splits + slots - 1) / slots);
+  for (int64_t w = first; w < first + STEP_WAVES; ++w)
+    if (w * slots / units > MOST_CLUSTER) consider(pieces(w * slots / units), w);
   // eight short chunks rather than more of them and a second launch
   if (span > MOST_CLUSTER * chunk && pieces(MOST_CLUSTER) <= SHORT_CHUNK) chunk = pieces(MOST_CLUSTER);
-  sp->row_tiles = static_cast<int>(row_tiles);
+  sp->row_tiles = static_cast<int>(std::min<int64_t>(row_tiles, 1 << 30));
   sp->chunk = static_cast<int>(chunk);
   sp->splits = static_cast<int>(span > chunk ? (span + chunk - 1) / chunk : 1);
   sp->cluster = sp->splits > 1 && sp->splits <= MOST_CLUSTER;
+  const int64_t tiles = z.batch * z.heads_q * ((z.n + BQ - 1) / BQ);
+  const int64_t tile_cost = (tiles + slots - 1) / slots * (span_of(std::min<int64_t>(z.n, BQ)) + 2 * BKV);
+  return z.n_kv == 0 || least * STEP_NS < tile_cost * TILE_NS;
 }
 
 template <typename T, int D>
-int launch_step(const Params& p, float* parts, int64_t parts_bytes, cudaStream_t st) {
-  Split sp = {};
-  split_keys(p.batch, p.heads_q, p.heads_kv, p.n, p.n_kv, p.left, p.right, p.sinks, &sp);
+int launch_step(const Params& p, Split sp, float* parts, int64_t parts_bytes, cudaStream_t st) {
   const int64_t units = static_cast<int64_t>(p.batch) * p.heads_kv * sp.row_tiles;
   const int64_t rows = static_cast<int64_t>(p.batch) * p.heads_q * p.n;
   IRIS_REQUIRE(units * sp.splits < (1ll << 31) && rows < (1ll << 31), "window_attn_fwd: too many rows");
@@ -939,8 +986,9 @@ int launch_step(const Params& p, float* parts, int64_t parts_bytes, cudaStream_t
 
 template <typename T, int D>
 int launch(const Params& p, int dtype, void* workspace, int64_t workspace_bytes, cudaStream_t st) {
-  if (few_rows(p.n, p.heads_q / p.heads_kv) || p.n_kv == 0)
-    return launch_step<T, D>(p, static_cast<float*>(workspace), workspace_bytes, st);
+  Split sp = {};
+  if (split_keys(Sizes{p.batch, p.heads_q, p.heads_kv, p.n, p.n_kv, p.left, p.right, p.sinks}, &sp))
+    return launch_step<T, D>(p, sp, static_cast<float*>(workspace), workspace_bytes, st);
   return launch_tiles<T, D>(p, dtype, st);
 }
 
@@ -975,11 +1023,12 @@ extern "C" int iris_window_attn_workspace(const iris_window_problem* q, int64_t*
   IRIS_REQUIRE(q != nullptr && bytes != nullptr, "window_attn_workspace: null pointer");
   IRIS_CHECK_STATUS(check_sizes(*q));
   *bytes = 0;
-  if (q->batch * q->n == 0 || q->n_kv == 0 || !few_rows(q->n, q->heads_q / q->heads_kv)) return IRIS_OK;
+  if (q->batch * q->n == 0) return IRIS_OK;
   Split sp = {};
-  split_keys(q->batch, q->heads_q, q->heads_kv, q->n, q->n_kv, bound(q->left), bound(q->right),
-             q->sinks < q->n_kv ? q->sinks : q->n_kv, &sp);
-  if (sp.splits > 1 && !sp.cluster) *bytes = q->batch * q->heads_kv * sp.row_tiles * sp.splits * STEP_ROWS * (q->head_dim + 2) * 4;
+  if (split_keys(Sizes{q->batch, q->heads_q, q->heads_kv, q->n, q->n_kv, bound(q->left), bound(q->right),
+                       std::min(q->sinks, q->n_kv)}, &sp) &&
+      sp.splits > 1 && !sp.cluster)
+    *bytes = q->batch * q->heads_kv * sp.row_tiles * sp.splits * STEP_ROWS * (q->head_dim + 2) * 4;
   return IRIS_OK;
 }
 
