@@ -19,7 +19,11 @@
 // A CTA owns 128 weight rows, 32 a warp, and, in a cluster, one part of K, whose x it
 // lays out once for all of them; a warp streams 256-wide pieces of its rows through
 // its own ring of TMA copies (one instruction for 32 rows; filled before x is laid
-// out). The parts' sums are joined through distributed shared memory in a fixed order.
+// out). Each part's sums are stored into the shared memory of the CTA that owns the
+// row (no CTA waits on another's memory: reading the sums from there instead took 2 to
+// 4 us of a call's 12 to 21), which adds them in a fixed order.
+#include <algorithm>
+
 #include "common.cuh"
 #include "iris_abi_internal.h"
 
@@ -27,7 +31,7 @@ namespace iris {
 namespace q4 {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
-constexpr int STAGES = 2;                    // ring slots of a warp; two to four CTAs share an SM
+constexpr int MOST_STAGES = 4;               // ring slots of a warp: two to four (see launch_g)
 constexpr int TILES = 2, ROWS = 16 * TILES;  // weight rows of a warp
 constexpr int STEP = 256;                    // k of one ring slot: 128 bytes of each row
 constexpr int SLOT = ROWS * STEP / 2;        // bytes
@@ -50,6 +54,7 @@ struct Params {
   int part_k;    // k of a part, a multiple of STEP
   int chunk_k;   // k of x in shared memory at a time, a multiple of STEP
   int pass_rows;  // rows of x per blockIdx.y
+  int stages;     // ring slots of a warp
 };
 
 IRIS_DEVICE float silu(float v) { return v / (1.f + __expf(-v)); }
@@ -143,7 +148,7 @@ template <typename T, int TERMS, int COLS8, int G>
 __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(const __grid_constant__ CUtensorMap tw,
                                                           const __grid_constant__ Params p) {
   extern __shared__ __align__(1024) uint8_t smem_unaligned[];
-  __shared__ uint64_t full[WARPS][STAGES];
+  __shared__ uint64_t full[WARPS][MOST_STAGES];
   __shared__ int abort_flag;
   uint8_t* smem_raw = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -160,30 +165,31 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   constexpr int HELD = (PER + 3) / 4;          // scales and zeros that a lane holds for each of its rows:
   constexpr int SPAN = PER < 4 ? 4 / PER : 1;  // of so many steps
 
-  uint8_t* ring = smem_raw + warp * (STAGES * SLOT);
-  uint8_t* xs = smem_raw + WARPS * STAGES * SLOT;  // [chunk_k / 32][cols][32] in the order of use
+  uint8_t* ring = smem_raw + warp * (p.stages * SLOT);
+  float* sums = reinterpret_cast<float*>(smem_raw + WARPS * p.stages * SLOT);  // other CTAs store here: a place of its own
+  uint8_t* xs = smem_raw + WARPS * p.stages * SLOT + WARPS * ROWS * COLS8 * 8 * 4;  // [chunk_k / 32][cols][32] in the order of use
   volatile int* abort = &abort_flag;
   __shared__ __align__(16) uint8_t zeros[16];
   if (threadIdx.x < 4) reinterpret_cast<uint32_t*>(zeros)[threadIdx.x] = 0u;
   if (threadIdx.x == 0) {
     for (int w = 0; w < WARPS; ++w)
-      for (int u = 0; u < STAGES; ++u) mbar_init(&full[w][u], 1);
+      for (int u = 0; u < p.stages; ++u) mbar_init(&full[w][u], 1);
     abort_flag = 0;
     fence_barrier_init();
   }
   __syncthreads();
+  if (p.parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   grid_wait();
   grid_trigger();
 
-  auto load = [&](int t) {  // step t into its slot
+  auto load = [&](int t, int slot) {  // step t into its slot
     if (lane == 0 && t < steps && n0 < p.N) {
-      uint64_t* bar = &full[warp][t % STAGES];
-      mbar_arrive_expect_tx(bar, SLOT);
+      mbar_arrive_expect_tx(&full[warp][slot], SLOT);
       // rows from N on and k from K on: zeros
-      tma_load_2d(&tw, bar, ring + t % STAGES * SLOT, (k0 + t * STEP) / 2, n0);
+      tma_load_2d(&tw, &full[warp][slot], ring + slot * SLOT, (k0 + t * STEP) / 2, n0);
     }
   };
-  for (int t = 0; t < STAGES; ++t) load(t);
+  for (int t = 0; t < p.stages; ++t) load(t, t);
 
   // lane (g, quad) holds groups quad, quad + 4 of SPAN steps, of rows weight_row(g) + 0, 8, 16, 24, fetched ahead
   const int row_g = weight_row(g);
@@ -298,6 +304,8 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   bool ok = true;
   const int chunk_steps = p.chunk_k / STEP;
   int chunk_t = 0;  // step within the chunk
+  int at_slot = 0;  // the step's slot and its phase
+  uint32_t phase = 0;
   uint32_t now[2 * TILES][HELD];
 #pragma unroll 1
   for (int t = 0; t < steps; ++t) {
@@ -315,8 +323,8 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
       fetch();
     }
     if (n0 < p.N && ok) {
-      ok = mbar_wait(&full[warp][t % STAGES], static_cast<uint32_t>((t / STAGES) & 1), abort);
-      const uint8_t* slot = ring + t % STAGES * SLOT + row_g * 128;
+      ok = mbar_wait(&full[warp][at_slot], phase, abort);
+      const uint8_t* slot = ring + at_slot * SLOT + row_g * 128;
       const int held_by = (lane & ~3) + t % SPAN * PER;  // the lane with the step's first group
       // this lane's column of each 8, or zeros
       const uint8_t* xk[COLS8];
@@ -386,13 +394,14 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
       }
     }
     ok = __all_sync(0xffffffffu, ok);  // and the slot is read by every lane
-    if (ok) load(t + STAGES);
+    if (ok) load(t + p.stages, at_slot);
+    if (++at_slot == p.stages) at_slot = 0, phase ^= 1u;
     if (++chunk_t == chunk_steps) chunk_t = 0;
   }
   if (!ok) {  // a wait gave up (device error word): no copy may land after the CTA is gone; NaN rather than wrong sums
     int dummy = 0;
     for (int t = 0; t < steps && n0 < p.N; ++t)
-      mbar_wait(&full[warp][t % STAGES], static_cast<uint32_t>((t / STAGES) & 1), &dummy);
+      mbar_wait(&full[warp][t % p.stages], static_cast<uint32_t>((t / p.stages) & 1), &dummy);
 #pragma unroll
     for (int r = 0; r < TILES; ++r)
 #pragma unroll
@@ -400,52 +409,47 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
 #pragma unroll
         for (int e = 0; e < 4; ++e) total[r][c][e] = __int_as_float(0x7fc00000);
   }
-  __syncthreads();  // rings and x are done with
-  // sums [row][COLS8 * 8] of the CTA's rows, joined over the cluster, whose CTAs take the outputs in turn
-  float* sums = reinterpret_cast<float*>(smem_raw);
-  constexpr int WIDTH = COLS8 * 8;
+  if (p.parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the cluster's CTAs have begun
+  // sums [part][row][COLS8 * 8] of the rows that a CTA owns, 128 / parts of them
+  constexpr int WIDTH = COLS8 * 8, CTA_ROWS = WARPS * ROWS;
+  const int owned = CTA_ROWS / p.parts;
 #pragma unroll
   for (int r = 0; r < TILES; ++r)
 #pragma unroll
-    for (int c = 0; c < COLS8; ++c)
+    for (int h = 0; h < 2; ++h) {
+      const int row = warp * ROWS + 16 * r + 8 * h + row_g, owner = row / owned;
+      float* at = sums + (part * owned + row - owner * owned) * WIDTH + 2 * quad;
+      const uint32_t to = p.parts > 1 ? map_to_cta(at, static_cast<uint32_t>(owner)) : 0u;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<float2*>(sums + (warp * ROWS + 16 * r + 8 * h + row_g) * WIDTH + c * 8 + 2 * quad) =
-            make_float2(total[r][c][2 * h], total[r][c][2 * h + 1]);
+      for (int c = 0; c < COLS8; ++c) {
+        const float x = total[r][c][2 * h], y = total[r][c][2 * h + 1];
+        if (p.parts > 1)
+          asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to + c * 32), "f"(x), "f"(y) : "memory");
+        else
+          *reinterpret_cast<float2*>(at + c * 8) = make_float2(x, y);
+      }
+    }
   if (p.parts > 1) cluster_sync();
   else __syncthreads();
-  const int n_cta = static_cast<int>(blockIdx.x / p.parts) * WARPS * ROWS;
-  for (int e = part * THREADS + threadIdx.x; e < WARPS * ROWS * rows; e += THREADS * p.parts) {
-    const int row = e % (WARPS * ROWS), m = e / (WARPS * ROWS), n = n_cta + row;
-    const float* at = sums + row * WIDTH + m * TERMS;
+  const int first_row = static_cast<int>(blockIdx.x / p.parts) * CTA_ROWS + part * owned;
+  for (int e = threadIdx.x; e < owned * rows; e += THREADS) {
+    const int m = e / owned, row = e - m * owned, n = first_row + row;
+    if (n >= p.N) continue;
     float v = 0.f;
-    if (p.parts == 1) {
 #pragma unroll
-      for (int c = TERMS - 1; c >= 0; --c) v += at[c];
-    } else {
-      float x[MOST_PARTS][TERMS];
+    for (int q = 0; q < MOST_PARTS; ++q)
+      if (q < p.parts)
 #pragma unroll
-      for (int q = 0; q < MOST_PARTS; ++q)
-        if (q < p.parts)
-#pragma unroll
-          for (int c = 0; c < TERMS; ++c)
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[q][c]) : "r"(map_to_cta(at + c, static_cast<uint32_t>(q))));
-#pragma unroll
-      for (int q = 0; q < MOST_PARTS; ++q)
-        if (q < p.parts)
-#pragma unroll
-          for (int c = TERMS - 1; c >= 0; --c) v += x[q][c];
-    }
-    if (n < p.N) {
-      if (p.bias) v += __ldg(p.bias + n);
-      store_elem(p.out, static_cast<int64_t>(m0 + m) * p.N + n, p.out_dtype, p.silu_out ? silu(v) : v);
-    }
+        for (int c = TERMS - 1; c >= 0; --c) v += sums[(q * owned + row) * WIDTH + m * TERMS + c];
+    if (p.bias) v += __ldg(p.bias + n);
+    store_elem(p.out, static_cast<int64_t>(m0 + m) * p.N + n, p.out_dtype, p.silu_out ? silu(v) : v);
   }
-  if (p.parts > 1) cluster_sync();  // no CTA leaves while its sums are read
 }
 
 constexpr int WANTED = 4;
+constexpr int SM_BYTES = 228 * 1024, CTA_BYTES = 2048 + 512;  // shared memory of an SM; of a CTA beside its rings and x
 constexpr int X_BYTES = 48 * 1024;  // x in shared memory at a time, at most
+static_assert(X_BYTES / (48 * 2) >= STEP, "a step of x in 48 columns, the most that a pass has");
 
 template <typename T, int TERMS, int COLS8, int G>
 int launch_g(Params& p, int passes, cudaStream_t st) {
@@ -459,14 +463,18 @@ int launch_g(Params& p, int passes, cudaStream_t st) {
   p.part_k = ((p.K + parts - 1) / parts + STEP - 1) / STEP * STEP;
   const int most = X_BYTES / (cols * 2) / STEP * STEP;
   p.chunk_k = p.part_k < most ? p.part_k : most;
-  const int used = WARPS * STAGES * SLOT + p.chunk_k * cols * 2;
-  const int sums = WARPS * ROWS * COLS8 * 8 * 4;
-  const int smem = 1024 + (used > sums ? used : sums);
+  // ring slots: what shared memory leaves once the CTAs that each SM gets (up to four) and their x have a place
+  const int64_t per_sm = std::min<int64_t>(4, (tiles * passes * parts + num_sms() - 1) / num_sms());
+  const int beside = WARPS * ROWS * COLS8 * 8 * 4 + p.chunk_k * cols * 2;  // the sums and x
+  const int64_t left = SM_BYTES / per_sm - CTA_BYTES - beside;
+  const int64_t fit = std::min<int64_t>(left / (WARPS * SLOT), (p.part_k + STEP - 1) / STEP);
+  p.stages = static_cast<int>(std::max<int64_t>(2, std::min<int64_t>(MOST_STAGES, fit)));
+  const int smem = 1024 + WARPS * p.stages * SLOT + beside;
   static int configured[64] = {0};
   int dev = 0;
   IRIS_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || configured[dev] == 0) {
-    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + WARPS * STAGES * SLOT + X_BYTES));
+    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 1024 + WARPS * MOST_STAGES * SLOT + WARPS * ROWS * COLS8 * 8 * 4 + X_BYTES));
     if (dev < 64) configured[dev] = 1;
   }
   CUtensorMap tw;
