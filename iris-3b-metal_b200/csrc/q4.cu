@@ -182,6 +182,69 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   grid_wait();
   grid_trigger();
 
+  // x for k in [from, from + chunk_k) of this part: zeros behind K. Word w (8 k) of a
+  // row is word j of lane q's share of its group. A thread takes BATCH words at once,
+  // grabbed (their loads overlap) and then put in place.
+  constexpr int BATCH = TERMS == 1 ? 8 : 4;
+  uint4 raw[BATCH][TERMS == 1 ? 1 : 2];  // fp32: two pieces a word
+  auto grab = [&](int from, int words, int e0) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int e = e0 + i * THREADS, m = e / words, k = from + (e - m * words) * 8;
+      const bool real = m < rows && k < p.K;
+      const int64_t at = static_cast<int64_t>(m0 + m) * p.ldx + k;
+#pragma unroll
+      for (int h = 0; h < (TERMS == 1 ? 1 : 2); ++h) raw[i][h] = make_uint4(0u, 0u, 0u, 0u);
+      if (!real) continue;
+      if (TERMS == 1 || p.x_dtype != IRIS_F32) {
+        raw[i][0] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at));
+      } else {
+#pragma unroll
+        for (int h = 0; h < (TERMS == 1 ? 1 : 2); ++h)
+          raw[i][h] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.x) + at) + h);
+      }
+    }
+  };
+  auto put = [&](int words, int e0) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int e = e0 + i * THREADS, m = e / words, w = e - m * words;
+      if (m >= rows) continue;
+      const int grp = w / (G / 8), in = w % (G / 8), q = in / WORDS, j = in % WORDS;
+      uint8_t* to = xs + ((grp * WORDS + j) * cols + m * TERMS) * 64 + q * 16;
+      const uint4 a = raw[i][0];
+      if constexpr (TERMS == 1) {  // in 16 bits as it is: only the order changes
+        *reinterpret_cast<uint4*>(to) = make_uint4(__byte_perm(a.x, a.z, 0x5410), __byte_perm(a.x, a.z, 0x7632),
+                                                   __byte_perm(a.y, a.w, 0x5410), __byte_perm(a.y, a.w, 0x7632));
+      } else {
+        float v[8];
+        if (p.x_dtype == IRIS_F32) {
+          const uint4 b = raw[i][TERMS == 1 ? 0 : 1];
+          const uint32_t f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int h = 0; h < 8; ++h) v[h] = __uint_as_float(f[h]);
+        } else {
+          const uint32_t f[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const float2 d = p.x_dtype == IRIS_BF16 ? unpack_bf16x2(f[h])
+                                                    : __half22float2(*reinterpret_cast<const __half2*>(&f[h]));
+            v[2 * h] = d.x, v[2 * h + 1] = d.y;
+          }
+        }
+        uint32_t t[8][3];
+#pragma unroll
+        for (int h = 0; h < 8; ++h) split3(p.silu_in ? silu(v[h]) : v[h], t[h]);
+#pragma unroll
+        for (int c = 0; c < 3; ++c)
+          *reinterpret_cast<uint4*>(to + c * 64) = make_uint4(t[0][c] | t[4][c] << 16, t[1][c] | t[5][c] << 16,
+                                                              t[2][c] | t[6][c] << 16, t[3][c] | t[7][c] << 16);
+      }
+    }
+  };
+  auto words_of = [&](int from) { return min(p.chunk_k, (k1 - from + STEP - 1) / STEP * STEP) / 8; };  // of a row
+  if (steps > 0) grab(k0, words_of(k0), threadIdx.x);  // ahead of the weights, not behind them in the queue
+
   auto load = [&](int t, int slot) {  // step t into its slot
     if (lane == 0 && t < steps && n0 < p.N) {
       mbar_arrive_expect_tx(&full[warp][slot], SLOT);
@@ -223,76 +286,6 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   };
   fetch();
 
-  // x for k in [from, from + chunk_k) of this part: zeros behind K. Word w (8 k) of a
-  // row is word j of lane q's share of its group; BATCH words a thread at once, so that
-  // their loads overlap.
-  auto place = [&](int w, int col) {
-    const int grp = w / (G / 8), in = w % (G / 8), q = in / WORDS, j = in % WORDS;
-    return reinterpret_cast<uint4*>(xs + ((grp * WORDS + j) * cols + col) * 64 + q * 16);
-  };
-  auto lay_out = [&](int from) {
-    constexpr int BATCH = TERMS == 1 ? 8 : 4;
-    const int words = min(p.chunk_k, (k1 - from + STEP - 1) / STEP * STEP) / 8;  // of a row
-    const int all = words * rows;
-    for (int e0 = threadIdx.x; e0 < all; e0 += BATCH * THREADS) {
-      int word[BATCH], col[BATCH];
-      int64_t at[BATCH];  // in x, or -1: behind K
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const int e = e0 + i * THREADS;
-        const int m = e / words, w = e - m * words;
-        word[i] = w, col[i] = m * TERMS;
-        at[i] = e < all && from + w * 8 < p.K ? static_cast<int64_t>(m0 + m) * p.ldx + from + w * 8 : -1;
-      }
-      if constexpr (TERMS == 1) {  // in 16 bits as it is: only the order changes
-        uint4 v[BATCH];
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i)
-          v[i] = at[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at[i]))
-                            : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i)
-          if (e0 + i * THREADS < all)
-            *place(word[i], col[i]) = make_uint4(__byte_perm(v[i].x, v[i].z, 0x5410), __byte_perm(v[i].x, v[i].z, 0x7632),
-                                                 __byte_perm(v[i].y, v[i].w, 0x5410), __byte_perm(v[i].y, v[i].w, 0x7632));
-      } else {
-        float v[BATCH][8];
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-          if (at[i] < 0) continue;
-          if (p.x_dtype == IRIS_F32) {
-            const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.x) + at[i]);
-            const float4 a = __ldg(src), b = __ldg(src + 1);
-            v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w;
-            v[i][4] = b.x, v[i][5] = b.y, v[i][6] = b.z, v[i][7] = b.w;
-          } else {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at[i]));
-            const uint32_t h[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 f = p.x_dtype == IRIS_BF16 ? unpack_bf16x2(h[e])
-                                                      : __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
-              v[i][2 * e] = f.x, v[i][2 * e + 1] = f.y;
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          if (e0 + i * THREADS >= all) continue;
-          uint32_t t[8][3];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) split3(p.silu_in ? silu(v[i][e]) : v[i][e], t[e]);
-#pragma unroll
-          for (int c = 0; c < 3; ++c)
-            *place(word[i], col[i] + c) = make_uint4(t[0][c] | t[4][c] << 16, t[1][c] | t[5][c] << 16,
-                                                     t[2][c] | t[6][c] << 16, t[3][c] | t[7][c] << 16);
-        }
-      }
-    }
-  };
-
   float total[TILES][COLS8][4];
 #pragma unroll
   for (int r = 0; r < TILES; ++r)
@@ -301,6 +294,18 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
 #pragma unroll
       for (int e = 0; e < 4; ++e) total[r][c][e] = 0.f;
 
+  auto lay_out = [&](int from, int first) {
+    const int words = words_of(from);
+    for (int e0 = first; e0 < words * rows; e0 += BATCH * THREADS) {
+      grab(from, words, e0);
+      put(words, e0);
+    }
+  };
+  if (steps > 0) {
+    put(words_of(k0), threadIdx.x);
+    lay_out(k0, threadIdx.x + BATCH * THREADS);
+    __syncthreads();
+  }
   bool ok = true;
   const int chunk_steps = p.chunk_k / STEP;
   int chunk_t = 0;  // step within the chunk
@@ -309,9 +314,10 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   uint32_t now[2 * TILES][HELD];
 #pragma unroll 1
   for (int t = 0; t < steps; ++t) {
-    if (chunk_t == 0) {  // uniform over the CTA
-      if (t > 0) __syncthreads();  // the chunk before is read
-      lay_out(k0 + t * STEP);
+    if (chunk_t == chunk_steps) {  // uniform over the CTA
+      chunk_t = 0;
+      __syncthreads();  // the chunk before is read
+      lay_out(k0 + t * STEP, threadIdx.x);
       __syncthreads();
     }
     if (t % SPAN == 0) {
@@ -396,7 +402,7 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
     ok = __all_sync(0xffffffffu, ok);  // and the slot is read by every lane
     if (ok) load(t + p.stages, at_slot);
     if (++at_slot == p.stages) at_slot = 0, phase ^= 1u;
-    if (++chunk_t == chunk_steps) chunk_t = 0;
+    ++chunk_t;
   }
   if (!ok) {  // a wait gave up (device error word): no copy may land after the CTA is gone; NaN rather than wrong sums
     int dummy = 0;
