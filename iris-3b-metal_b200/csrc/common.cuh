@@ -179,6 +179,19 @@ IRIS_DEVICE void tma_load_4d(const CUtensorMap* map, uint64_t* bar, void* dst, i
       : "memory");
 }
 
+// Store of a tile from shared memory (rows past the map's extents are left alone), in
+// this thread's bulk group; tma_store_wait: they have been written.
+IRIS_DEVICE void tma_store_4d(const CUtensorMap* map, const void* src, int32_t c0, int32_t c1, int32_t c2, int32_t c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_addr(src))
+      : "memory");
+}
+IRIS_DEVICE void tma_store_wait() {
+  asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+}
+
 IRIS_DEVICE void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }

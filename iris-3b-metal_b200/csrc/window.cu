@@ -199,7 +199,8 @@ IRIS_DEVICE uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffff
 template <typename T, int D>
 __global__ void __launch_bounds__(TILE_THREADS, 2)
     tiles_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                 const __grid_constant__ CUtensorMap tv, const __grid_constant__ Params p) {
+                 const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
+                 const __grid_constant__ Params p) {
   constexpr int HALVES = D / 64, KV_BYTES = HALVES * KV_HALF;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* q_tile = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -449,6 +450,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 2)
       tc_fence_after();
       const float inv = 1.f / l_run;
       bool finite = true;
+      // the rows into Q's place (every score is computed), in the store's swizzle
+      auto place = [&](int row, int piece) { return row * 128 + ((piece ^ (row & 7)) * 16); };
+      const int row = quarter * 32 + lane;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t r[32];
@@ -464,20 +468,26 @@ __global__ void __launch_bounds__(TILE_THREADS, 2)
           finite = finite && isfinite(a) && isfinite(z);
           pk[e] = pack2<T>(a, z);
         }
-        if (i < p.n) {
-          uint4* dst = reinterpret_cast<uint4*>(out + i * p.on + c * 32);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) dst[e] = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
-        }
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<uint4*>(q_tile + (c >> 1) * Q_HALF + place(row, (c & 1) * 4 + e)) =
+              make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
       }
       __syncwarp();  // a row that is computed again comes after what was written of it
       for (uint32_t again = __ballot_sync(0xffffffffu, !finite && i < p.n); again != 0; again &= again - 1) {
-        const int r = row0 + quarter * 32 + __ffs(again) - 1;
+        const int r = quarter * 32 + __ffs(again) - 1;
         float2 acc[D / 64];
-        attend_row<T, D>(p, b, h, r, acc);
-        T* o = out + static_cast<int64_t>(r) * p.on + 2 * lane;
+        attend_row<T, D>(p, b, h, row0 + r, acc);
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) *reinterpret_cast<uint32_t*>(o + 64 * c) = pack2<T>(acc[c].x, acc[c].y);
+        for (int c = 0; c < D / 64; ++c)
+          *reinterpret_cast<uint32_t*>(q_tile + c * Q_HALF + place(r, lane >> 2) + (lane & 3) * 4) = pack2<T>(acc[c].x, acc[c].y);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0 && row0 + quarter * 32 < p.n) {  // rows from n on are not written
+        for (int c = 0; c < HALVES; ++c)
+          tma_store_4d(&to, q_tile + c * Q_HALF + quarter * 32 * 128, c * 64, row0 + quarter * 32, h, p.ob != 0 ? b : 0);
+        tma_store_wait();
       }
     }
   }
@@ -492,10 +502,11 @@ template <typename T, int D>
 int launch_tiles(const Params& p, int dtype, cudaStream_t st) {
   const int64_t ctas = static_cast<int64_t>((p.n + BQ - 1) / BQ) * p.heads_q * p.batch;
   IRIS_REQUIRE(ctas < (1ll << 31), "window_attn_fwd: too many rows");
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   IRIS_CHECK_STATUS(make_tmap_heads(&tq, p.q, dtype, D, p.n, p.heads_q, p.batch, p.qn, p.qh, p.qb, BQ));
   IRIS_CHECK_STATUS(make_tmap_heads(&tk, p.k, dtype, D, p.n_kv, p.heads_kv, p.batch, p.kn, p.kh, p.kb, BKV));
   IRIS_CHECK_STATUS(make_tmap_heads(&tv, p.v, dtype, D, p.n_kv, p.heads_kv, p.batch, p.vn, p.vh, p.vb, BKV));
+  IRIS_CHECK_STATUS(make_tmap_heads(&to, p.out, dtype, D, p.n, p.heads_q, p.batch, p.on, D, p.ob, 32));
   auto kernel = tiles_kernel<T, D>;
   static bool configured[64] = {false};
   int dev = 0;
@@ -504,7 +515,7 @@ int launch_tiles(const Params& p, int dtype, cudaStream_t st) {
     IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem<D>()));
     if (dev < 64) configured[dev] = true;
   }
-  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(ctas)), TILE_THREADS, tile_smem<D>(), st, 1, tq, tk, tv, p));
+  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(ctas)), TILE_THREADS, tile_smem<D>(), st, 1, tq, tk, tv, to, p));
   return IRIS_OK;
 }
 
