@@ -161,7 +161,7 @@ PyObject* rope(PyObject* const* a) {
   at::Tensor out = given ? *given : at::empty(x.sizes(), x.options());
   q.out = head_rows(out, q.batch, q.heads, q.n, q.head_dim, "rope: out must have the input's shape");
   q.cos = static_cast<const float*>(cos.data_ptr()), q.sin = static_cast<const float*>(sin.data_ptr());
-  on.check("iris_rope", entries.rope(&q, on.stream()), 1);
+  on.check("iris_rope", entries.rope(&q, on.stream()), q.batch * q.n > 0);
   return THPVariable_Wrap(std::move(out));
 }
 
@@ -206,7 +206,7 @@ PyObject* rope_append(PyObject* const* a) {
   q.zero_rest = given == nullptr;  // rows from counts[b] on of a new output
   q.out = head_rows(out, q.batch, q.heads_q, q.n, q.head_dim, "rope_append: out must have q's shape");
   q.cos = static_cast<const float*>(cos.data_ptr()), q.sin = static_cast<const float*>(sin.data_ptr());
-  on.check("iris_rope_append", entries.rope_append(&q, on.stream()), 1);
+  on.check("iris_rope_append", entries.rope_append(&q, on.stream()), q.batch * q.n > 0);
   return THPVariable_Wrap(std::move(out));
 }
 

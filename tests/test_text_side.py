@@ -1,6 +1,7 @@
 """The text-side operators without a GPU: refusals (all before any launch), the
 scaled rotary tables and the 4-bit packing."""
 
+import ctypes
 import math
 import re
 import struct
@@ -76,6 +77,21 @@ def test_c_entries_refuse_bad_arguments(lib):  # noqa: F811
         assert message in _einval(lib, *q4(**bad)), bad
     for name in ("iris_rope", "iris_rope_append", "iris_window_attn_fwd", "iris_gemv_q4"):
         assert "null" in _einval(lib, name, None, None)
+
+
+def test_workspace_is_for_split_keys_alone(lib):  # noqa: F811
+    def need(batch=1, heads=4, kv=1, n=1, m=40000, dim=128, left=-1, right=0, sinks=0):
+        out = ctypes.c_int64(-1)
+        problem = WINDOW.pack(*[0] * 19, 1, batch, heads, kv, n, m, dim, left, right, sinks, 1.0)
+        assert lib.iris_window_attn_workspace(problem, ctypes.byref(out)) == 0
+        return out.value
+
+    parts = need() // (16 * (128 + 2) * 4)  # 16 rows of sums, a maximum and a total each
+    assert need() == parts * 16 * (128 + 2) * 4 and 8 < parts <= 40000 // 64
+    assert need(n=4) == need() and need(dim=64) * (128 + 2) == need() * (64 + 2)
+    # whole tiles, no keys or rows, one chunk, a cluster's chunks: none
+    for none in (dict(n=40000), dict(m=0), dict(n=0), dict(batch=0), dict(m=64), dict(m=1028), dict(left=50), dict(batch=64, kv=4)):
+        assert need(**none) == 0, none
 
 
 def test_wrappers_refuse_before_any_launch(K):

@@ -85,6 +85,16 @@ def test_rope_reads_rows_at_any_alignment(K, dtype, shift):
     assert torch.equal(out[..., shift:], K.rope(aligned, cos, sin)) and torch.all(out[..., :shift] == 0)
 
 
+@pytest.mark.parametrize("shift", [1, 2])
+def test_rope_reads_tables_at_any_alignment(K, shift):
+    cos, sin = table(64, 9)
+    x = normal(1, 2, 3, 9, 64, dtype=BF16)
+    moved = [torch.cat([torch.zeros(shift, device="cuda"), t.flatten()])[shift:].view(9, 32) for t in (cos, sin)]
+    assert all(t.data_ptr() % 16 for t in moved)
+    for layout in ("half", "interleaved"):
+        assert torch.equal(K.rope(x, *moved, layout=layout), K.rope(x, cos, sin, layout=layout))
+
+
 def test_rope_sizes(K):
     cos, sin = table(64, 70000)
     for b, h, n in [(1, 1, 1), (1, 300, 1), (2, 1, 70000), (0, 3, 4), (2, 3, 0), (600, 2, 3)]:
@@ -247,6 +257,41 @@ def test_window_attention_lengths_and_starts(K, dtype, dim, n, n_kv):
         assert torch.all(got[4:] == 0)
 
 
+@pytest.mark.parametrize("dtype, dim", [(BF16, 128), (F16, 128), (BF16, 64)])
+@pytest.mark.parametrize("b, n, n_kv, heads, kv_heads", [(1, 1, 20000, 4, 1), (3, 1, 9001, 8, 8), (1, 5, 30000, 8, 2), (40, 1, 700, 8, 4),
+                                                         (2, 1, 4097, 24, 1), (1, 33, 5000, 6, 2), (1, 200, 3001, 3, 3)])  # fmt: skip
+def test_long_caches(K, dtype, dim, b, n, n_kv, heads, kv_heads):
+    """Enough keys that they are split: over a cluster, over more parts and a join, in several waves, for several row
+    tiles of a key head; samples of very different lengths."""
+    q = normal(1, b, heads, n, dim, dtype=dtype)
+    k, v = normal(2, b, kv_heads, n_kv, dim, dtype=dtype), normal(3, b, kv_heads, n_kv, dim, dtype=dtype)
+    lengths = int32([max(1, n_kv - 977 * i) if i % 3 else n_kv for i in range(b)])
+    for left, sinks in [(None, 0), (2000, 5)]:
+        got = K.window_attention(q, k, v, left=left, sinks=sinks, starts=lengths - n, lengths=lengths)
+        assert_attends(got, q, k, v, left=left, sinks=sinks, starts=lengths - n, lengths=lengths)
+    k[:, :, -1], v[:, :, -1] = math.nan, math.nan  # the last slot is not written yet
+    got = K.window_attention(q, k, v, starts=lengths - n - 1, lengths=(lengths - 1).clamp_max(n_kv - 1))
+    assert torch.isfinite(got).all()
+
+
+def test_kernels_are_counted(K):
+    from iris_b200 import _lib
+
+    q, k = normal(1, 1, 4, 1, 128, dtype=BF16), normal(2, 1, 1, 40000, 128, dtype=BF16)
+    cos, sin = table(128, 1)
+
+    def counted(call):
+        before = _lib.launch_count()
+        call()
+        return _lib.launch_count() - before
+
+    assert counted(lambda: K.window_attention(q, k[:, :, :64], k[:, :, :64])) == 1
+    assert counted(lambda: K.window_attention(q, k, k)) == 2
+    assert counted(lambda: K.rope(q, cos, sin)) == 1 and counted(lambda: K.rope(q[:, :, :0], cos, sin)) == 0
+    w = K.pack_q4(normal(3, 64, 128), 64)
+    assert counted(lambda: K.gemv_q4(q[0, :, 0], *w)) == 1
+
+
 @pytest.mark.parametrize("dtype, dim", [(BF16, 128), (F16, 64)])
 @pytest.mark.parametrize("n, n_kv", [(1, 700), (4, 300), (300, 300), (200, 450)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
@@ -376,6 +421,15 @@ def test_gemv_q4(K, dtype, group, m):
             got = K.gemv_q4(x, packed, scale, zero, bias, silu_in=silu_in, silu_out=silu_out)
             assert got.dtype == dtype and got.shape == (m, n)
             assert_q4(got, x, packed, scale, zero, bias, silu_in, silu_out)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m, n, k", [(1, 40, 57344), (16, 70, 20480), (64, 33, 16384), (9, 300, 30720)])
+def test_gemv_q4_long_rows(K, dtype, m, n, k):
+    """Rows of x that shared memory takes in several pieces."""
+    packed, scale, zero = K.pack_q4(normal(n, n, k), 128, False)
+    x = normal(m, m, k, dtype=dtype)
+    assert_q4(K.gemv_q4(x, packed, scale, zero, out_dtype=F32), x, packed, scale, zero, None)
 
 
 @pytest.mark.parametrize("out_dtype", [F32, BF16, F16])
