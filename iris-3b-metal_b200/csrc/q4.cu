@@ -143,9 +143,12 @@ IRIS_DEVICE void split3(float v, uint32_t (&t)[3]) {
 // of lanes that read together then meet no bank twice.
 IRIS_DEVICE int weight_row(int g) { return (g & 1) << 2 | (g & 2) | g >> 2; }
 
+// CTAs of an SM: as many as leave the columns' sums in registers.
+constexpr int ctas_per_sm(int cols8) { return cols8 == 1 ? 4 : cols8 == 2 ? 3 : 2; }
+
 // COLS8: groups of 8 columns of the mma (rows of x times TERMS); G: weights per scale.
 template <typename T, int TERMS, int COLS8, int G>
-__global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(const __grid_constant__ CUtensorMap tw,
+__global__ void __launch_bounds__(THREADS, ctas_per_sm(COLS8)) gemv_q4_kernel(const __grid_constant__ CUtensorMap tw,
                                                           const __grid_constant__ Params p) {
   extern __shared__ __align__(1024) uint8_t smem_unaligned[];
   __shared__ uint64_t full[WARPS][MOST_STAGES];
@@ -452,7 +455,6 @@ __global__ void __launch_bounds__(THREADS, COLS8 <= 2 ? 4 : 2) gemv_q4_kernel(co
   }
 }
 
-constexpr int WANTED = 4;
 constexpr int SM_BYTES = 228 * 1024, CTA_BYTES = 2048 + 512;  // shared memory of an SM; of a CTA beside its rings and x
 constexpr int X_BYTES = 48 * 1024;  // x in shared memory at a time, at most
 static_assert(X_BYTES / (48 * 2) >= STEP, "a step of x in 48 columns, the most that a pass has");
@@ -464,13 +466,13 @@ int launch_g(Params& p, int passes, cudaStream_t st) {
   const int64_t tiles = (p.N + WARPS * ROWS - 1) / (WARPS * ROWS);
   // parts of K over a cluster's CTAs: as many as still run at once
   int parts = 1;
-  while (parts < MOST_PARTS && p.K > parts * STEP && tiles * passes * parts * 2 <= WANTED * num_sms()) parts *= 2;
+  while (parts < MOST_PARTS && p.K > parts * STEP && tiles * passes * parts * 2 <= ctas_per_sm(COLS8) * num_sms()) parts *= 2;
   p.parts = parts;
   p.part_k = ((p.K + parts - 1) / parts + STEP - 1) / STEP * STEP;
   const int most = X_BYTES / (cols * 2) / STEP * STEP;
   p.chunk_k = p.part_k < most ? p.part_k : most;
-  // ring slots: what shared memory leaves once the CTAs that each SM gets (up to four) and their x have a place
-  const int64_t per_sm = std::min<int64_t>(4, (tiles * passes * parts + num_sms() - 1) / num_sms());
+  // ring slots: what shared memory leaves once the CTAs that each SM gets (at most ctas_per_sm) and their x have a place
+  const int64_t per_sm = std::min<int64_t>(ctas_per_sm(COLS8), (tiles * passes * parts + num_sms() - 1) / num_sms());
   const int beside = WARPS * ROWS * COLS8 * 8 * 4 + p.chunk_k * cols * 2;  // the sums and x
   const int64_t left = SM_BYTES / per_sm - CTA_BYTES - beside;
   const int64_t fit = std::min<int64_t>(left / (WARPS * SLOT), (p.part_k + STEP - 1) / STEP);

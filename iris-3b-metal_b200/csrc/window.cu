@@ -922,11 +922,11 @@ int64_t clusters_at_once(int size) {
 // chunks. One token, 128 wide, us (chunks of one wave against six or against LONG_CHUNK
 // alone): one sample, 5 key heads, 65536 keys 34 against 60 and 48; 4 samples, 8 key
 // heads, 4096 keys 18.6 against 27 and 21.
-// Tiles: a CTA walks its keys at TILE_NS each whatever rows it has; a split CTA at
-// STEP_NS. One sample, 20 over 5 heads, 2048 keys, us split / tiles: 8 tokens 9.7 / 30,
+// Tiles: a CTA walks its keys at TILE_NS each whatever rows it has, and starts and ends
+// in the time of TILE_KEYS; a split CTA's keys take STEP_NS. One sample, 20 over 5 heads, 2048 keys, us split / tiles: 8 tokens 9.7 / 30,
 // 128 tokens 43 / 32; 16384 keys: 64 tokens 110 / 216, 128 tokens 214 / 217.
 constexpr int64_t STEP_WAVES = 6, STEP_CTAS = 2, LONG_CHUNK = 1024, SHORT_CHUNK = 192, CTA_KEYS = 96, JOIN_KEYS = 64;
-constexpr int64_t STEP_NS = 25, TILE_NS = 13;
+constexpr int64_t STEP_NS = 25, TILE_NS = 13, TILE_KEYS = 288;
 
 struct Sizes {
   int64_t batch, heads_q, heads_kv, n, n_kv, left, right, sinks;
@@ -966,7 +966,7 @@ bool split_keys(const Sizes& z, Split* sp) {
   sp->splits = static_cast<int>(span > chunk ? (span + chunk - 1) / chunk : 1);
   sp->cluster = sp->splits > 1 && sp->splits <= MOST_CLUSTER;
   const int64_t tiles = z.batch * z.heads_q * ((z.n + BQ - 1) / BQ);
-  const int64_t tile_cost = (tiles + slots - 1) / slots * (span_of(std::min<int64_t>(z.n, BQ)) + 2 * BKV);
+  const int64_t tile_cost = (tiles + slots - 1) / slots * (span_of(std::min<int64_t>(z.n, BQ)) + TILE_KEYS);
   return z.n_kv == 0 || least * STEP_NS < tile_cost * TILE_NS;
 }
 
