@@ -528,8 +528,9 @@ int launch_tiles(const Params& p, int dtype, cudaStream_t st) {
 // m16n8k16: HBM-bound, one K and V byte is used for 16 rows at most, which leaves the
 // 5th-generation tensor cores' 128-row tiles seven eighths empty. Chunks are the same
 // length for every sample, so samples of different lengths give equal work. Up to
-// eight chunks are a cluster's CTAs, joined through distributed shared memory: one
-// launch, nothing in global memory. More of them are joined by a second kernel.
+// eight chunks are a cluster's CTAs: each stores its rows' states into the shared
+// memory of the CTA that owns the row, which joins them: one launch, nothing in global
+// memory. More chunks are joined by a second kernel.
 constexpr int STEP_WARPS = 4, STEP_STAGES = 3, STEP_KEYS = 16, STEP_ROWS = 16;
 
 struct Split {
@@ -565,15 +566,18 @@ IRIS_DEVICE void copy16(uint32_t dst, const void* src, bool real) {
 }
 
 constexpr int MOST_CLUSTER = 8;
-IRIS_DEVICE float remote(uint32_t at) {  // another CTA's shared memory (map_to_cta)
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
+IRIS_DEVICE void store_remote(uint32_t at, float2 v) {  // another CTA's shared memory (map_to_cta)
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(v.x), "f"(v.y) : "memory");
 }
+// Rows that a cluster's CTA owns, and places for the states of all chunks of them.
+IRIS_DEVICE int rows_owned(int splits) { return (STEP_ROWS + splits - 1) / splits; }
+constexpr int STATES = STEP_ROWS + MOST_CLUSTER;  // at least splits * rows_owned(splits)
 
 template <int D>
+constexpr int STEP_RINGS = STEP_WARPS * STEP_STAGES * 2 * STEP_KEYS * D * 2;  // bytes
+template <int D>
 constexpr int step_smem() {
-  return STEP_WARPS * STEP_STAGES * 2 * STEP_KEYS * D * 2;
+  return STEP_RINGS<D> + STATES * (D + 2) * 4;
 }
 
 // Writes row (b, h, i), columns [64 c + 2 lane, + 2); rows that are not finite again
@@ -599,6 +603,7 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   constexpr int TILE = STEP_KEYS * D * 2;  // bytes of one K or V tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (sp.cluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   grid_wait();
   grid_trigger();
   const int split = static_cast<int>(blockIdx.x % sp.splits);
@@ -674,18 +679,22 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
     const uint32_t slot = ring + (t % STEP_STAGES) * 2 * TILE;
     const int c0 = c_begin + (warp + t * STEP_WARPS) * STEP_KEYS;
     // S: keys [8 j, 8 j + 8) in s[j]
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, odd[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int d = 0; d < D / 32; ++d) {  // two k steps per load: pieces 4 d .. 4 d + 3 of the 8 key rows
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) {  // two k steps per load: pieces 4 d .. 4 d + 3 of the 8 key rows
+      for (int j = 0; j < 2; ++j) {
         uint32_t kb[4];
         const int r = 8 * j + (lane & 7), x = 4 * d + (lane >> 3);
         ldmatrix4(kb, slot + r * (D * 2) + ((x ^ (r & 7)) * 16));
         mma_16816<T>(s[j], qa[2 * d], kb[0], kb[1]);
-        mma_16816<T>(s[j], qa[2 * d + 1], kb[2], kb[3]);
+        mma_16816<T>(odd[j], qa[2 * d + 1], kb[2], kb[3]);  // two chains: half the wait for the last
       }
     }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[j][e] += odd[j][e];
     if (!same || c0 + STEP_KEYS > c_end) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
@@ -760,6 +769,10 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
     }
   }
   __syncthreads();
+  // cluster: states [chunk][owned row], sums then {maximum, total}; other CTAs store here once all have begun
+  float* states = reinterpret_cast<float*>(smem_raw + STEP_RINGS<D>);
+  const int owned = rows_owned(sp.splits);
+  if (sp.cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   for (int r = warp; r <= r_last - r0; r += STEP_WARPS) {
     float top = -INFINITY, total = 0.f;
 #pragma unroll
@@ -778,11 +791,12 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
         acc[c] = make_float2(fmaf(f, x.x, acc[c].x), fmaf(f, x.y, acc[c].y));
       }
     }
-    if (sp.cluster) {  // in the first warp's place: these lanes alone have read it
+    if (sp.cluster) {
+      float* at = states + (split * owned + r % owned) * (D + 2);
+      const uint32_t to = map_to_cta(at, static_cast<uint32_t>(r / owned));
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) *reinterpret_cast<float2*>(sums + r * D + 64 * c + 2 * lane) = acc[c];
-      __syncwarp();
-      if (lane == 0) tops[0][r] = top, totals[0][r] = total;
+      for (int c = 0; c < D / 64; ++c) store_remote(to + 4 * (64 * c + 2 * lane), acc[c]);
+      if (lane == 0) store_remote(to + 4 * D, make_float2(top, total));
     } else if (sp.parts == nullptr) {
       finish_row<T, D>(p, b, hk * group + (r0 + r) % group, (r0 + r) / group, acc, total);
     } else {
@@ -798,35 +812,25 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
   }
   if (sp.cluster) {
     cluster_sync();
-    for (int r = split * STEP_WARPS + warp; r <= r_last - r0; r += sp.splits * STEP_WARPS) {
-      float top[MOST_CLUSTER], part[MOST_CLUSTER], all_top = -INFINITY, total = 0.f;
-#pragma unroll
-      for (int q = 0; q < MOST_CLUSTER; ++q) {
-        top[q] = -INFINITY, part[q] = 0.f;
-        if (q < sp.splits) {
-          top[q] = remote(map_to_cta(&tops[0][r], q));
-          part[q] = remote(map_to_cta(&totals[0][r], q));
-        }
-        all_top = fmaxf(all_top, top[q]);
-      }
+    for (int local = warp; local < owned && split * owned + local <= r_last - r0; local += STEP_WARPS) {
+      const int r = r0 + split * owned + local;
+      float top = -INFINITY, total = 0.f;
+      for (int q = 0; q < sp.splits; ++q) top = fmaxf(top, states[(q * owned + local) * (D + 2) + D]);
       float2 acc[D / 64];
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
+      for (int q = 0; q < sp.splits; ++q) {
+        const float* from = states + (q * owned + local) * (D + 2);
+        const float f = from[D] == -INFINITY ? 1.f : ex2(from[D] - top);
+        total = fmaf(f, from[D + 1], total);
 #pragma unroll
-      for (int q = 0; q < MOST_CLUSTER; ++q) {
-        if (q < sp.splits) {
-          const float f = top[q] == -INFINITY ? 1.f : ex2(top[q] - all_top);
-          total = fmaf(f, part[q], total);
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c) {
-            const uint32_t at = map_to_cta(sums + r * D + 64 * c + 2 * lane, q);
-            acc[c] = make_float2(fmaf(f, remote(at), acc[c].x), fmaf(f, remote(at + 4), acc[c].y));
-          }
+        for (int c = 0; c < D / 64; ++c) {
+          const float2 x = *reinterpret_cast<const float2*>(from + 64 * c + 2 * lane);
+          acc[c] = make_float2(fmaf(f, x.x, acc[c].x), fmaf(f, x.y, acc[c].y));
         }
       }
-      finish_row<T, D>(p, b, hk * group + (r0 + r) % group, (r0 + r) / group, acc, total);
+      finish_row<T, D>(p, b, hk * group + r % group, r / group, acc, total);
     }
-    cluster_sync();  // no CTA leaves while its sums are read
   }
 }
 
