@@ -22,6 +22,13 @@
 // out). Each part's sums are stored into the shared memory of the CTA that owns the
 // row (no CTA waits on another's memory: reading the sums from there instead took 2 to
 // 4 us of a call's 12 to 21), which adds them in a fixed order.
+//
+// Measured: 8192 -> 32768, groups of 128, one bf16 row 40 us (3.4 TB/s, 0.53 of a plain
+// copy). The unpacking (7 and / shift operations a word at half rate, 3 more per mma)
+// alone takes about 19 us, the copies alone 25, the start (launch, cluster, first
+// copies, x) 5; they overlap in part. 2560 -> 15360, groups of 64, one fp32 row 12.5 us
+// (1.7 TB/s); 6848 -> 2561, groups of 32 with zeros, 16 f16 rows 16.5 us: latency.
+// Deeper rings change neither; three CTAs an SM for one row instead of four 47.7 us.
 #include <algorithm>
 
 #include "common.cuh"

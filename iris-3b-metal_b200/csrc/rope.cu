@@ -12,6 +12,11 @@
 // there are threads to spare it takes that unit in EACH = 4 heads of one tensor, their
 // loads in flight together and the token's table entries read once for them. Slots
 // are the heads of a tensor that its threads begin at: `step` of them.
+//
+// Measured: 25 fp32 heads of 16384 tokens 67 us (6.3 TB/s, 0.97 of a plain copy); 8 x
+// 300 bf16 tokens, rows in L2, 7.7 us (4.0 TB/s); one token appended 2.3 us on the
+// device. Four heads a thread against one: 67 / 69 us, the append of 8 x 301 f16
+// tokens 5.4 / 6.0 us where there are threads to spare.
 #include "common.cuh"
 #include "iris_abi_internal.h"
 
