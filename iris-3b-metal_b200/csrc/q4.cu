@@ -27,8 +27,11 @@
 // copy). The unpacking (7 and / shift operations a word at half rate, 3 more per mma)
 // alone takes about 19 us, the copies alone 25, the start (launch, cluster, first
 // copies, x) 5; they overlap in part. 2560 -> 15360, groups of 64, one fp32 row 12.5 us
-// (1.7 TB/s); 6848 -> 2561, groups of 32 with zeros, 16 f16 rows 16.5 us: latency.
-// Deeper rings change neither; three CTAs an SM for one row instead of four 47.7 us.
+// (1.7 TB/s); 6848 -> 2561, groups of 32 with zeros, 16 f16 rows 16.0 us: an SM has four
+// warps or eight, each a chain of shared memory -> unpacking -> mma -> scale. Deeper rings,
+// scales prefetched into L2, two accumulators a sum: no gain; eight warps of 16 rows in place
+// of four 15.0 us there, but 7.6 instead of 6.8 for 2560 -> 2560, one row; three CTAs an
+// SM for one row instead of four 47.7 us; twice the parts 43.9 us, 18.5 the 2560 -> 15360.
 #include <algorithm>
 
 #include "common.cuh"
@@ -381,20 +384,26 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(COLS8)) gemv_q4_kernel(co
             xk[c] += xstep[c];
           }
 #pragma unroll
-          for (int r = 0; r < TILES; ++r) {
-            const uint32_t u0 = w[2 * r][j], u1 = w[2 * r + 1][j];
-            const auto z0 = less[2 * r], z1 = less[2 * r + 1];
-            const uint32_t a[4] = {Operand<T>::template unpack<0>(u0, z0), Operand<T>::template unpack<0>(u1, z1),
-                                   Operand<T>::template unpack<1>(u0, z0), Operand<T>::template unpack<1>(u1, z1)};
-            const uint32_t b[4] = {Operand<T>::template unpack<2>(u0, z0), Operand<T>::template unpack<2>(u1, z1),
-                                   Operand<T>::template unpack<3>(u0, z0), Operand<T>::template unpack<3>(u1, z1)};
+          for (int half = 0; half < 2; ++half)  // neighbouring mmas add to different sums: none waits for the one before
 #pragma unroll
-            for (int c = 0; c < COLS8; ++c) {
-              if (j == 0) Operand<T>::mma_first(acc[r][c], a, xb[c].x, xb[c].y);
-              else Operand<T>::mma(acc[r][c], a, xb[c].x, xb[c].y);
-              Operand<T>::mma(acc[r][c], b, xb[c].z, xb[c].w);
+            for (int r = 0; r < TILES; ++r) {
+              const uint32_t u0 = w[2 * r][j], u1 = w[2 * r + 1][j];
+              const auto z0 = less[2 * r], z1 = less[2 * r + 1];
+              uint32_t a[4];
+              if (half == 0) {
+                a[0] = Operand<T>::template unpack<0>(u0, z0), a[1] = Operand<T>::template unpack<0>(u1, z1);
+                a[2] = Operand<T>::template unpack<1>(u0, z0), a[3] = Operand<T>::template unpack<1>(u1, z1);
+              } else {
+                a[0] = Operand<T>::template unpack<2>(u0, z0), a[1] = Operand<T>::template unpack<2>(u1, z1);
+                a[2] = Operand<T>::template unpack<3>(u0, z0), a[3] = Operand<T>::template unpack<3>(u1, z1);
+              }
+#pragma unroll
+              for (int c = 0; c < COLS8; ++c) {
+                if (half == 1) Operand<T>::mma(acc[r][c], a, xb[c].z, xb[c].w);
+                else if (j == 0) Operand<T>::mma_first(acc[r][c], a, xb[c].x, xb[c].y);
+                else Operand<T>::mma(acc[r][c], a, xb[c].x, xb[c].y);
+              }
             }
-          }
         }
 #pragma unroll
         for (int r = 0; r < TILES; ++r) {

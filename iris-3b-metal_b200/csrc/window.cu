@@ -540,8 +540,9 @@ int launch_tiles(const Params& p, int dtype, cudaStream_t st) {
 // memory of the CTA that owns the row, which joins them: one launch, nothing in global
 // memory. More chunks are joined by a second kernel.
 //
-// Measured, one token, 128 wide: 16 samples of up to 32768 keys, 32 over 8 heads 217 us
-// (6.2 TB/s, 0.94 of a plain copy); one sample, 20 over 5 heads: 64 keys 3.7 us, 256 4.6,
+// Measured, one token, 128 wide: 16 samples of 21400 keys on average, 32768 at most, 32
+// over 8 heads 217 us (6.45 TB/s, 0.98 of a plain copy; 1280 keys a chunk instead of
+// 2560: 220, 512: 239); one sample, 20 over 5 heads: 64 keys 3.7 us, 256 4.6,
 // 1028 6.5 (each CTA reading the others' states at the end, scores in one chain of mmas:
 // 8.1 us, and 228 us the long caches), 65536 keys 34 (4.9 TB/s). Six ring slots instead
 // of three 5.6 us at 64 keys and 9.6 at 1028; eight warps a CTA slower on long caches.
