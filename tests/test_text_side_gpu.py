@@ -257,6 +257,19 @@ def test_window_attention_lengths_and_starts(K, dtype, dim, n, n_kv):
         assert torch.all(got[4:] == 0)
 
 
+@pytest.mark.parametrize("dtype, dim", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("n, heads", [(1, 1), (1, 5), (1, 16), (3, 7), (17, 1)])
+def test_every_number_of_chunks(K, dtype, dim, n, heads):
+    """A chunk of 64 keys more each time: clusters of two to eight CTAs, few and many rows of the tile, and chunks that
+    see nothing (a length inside the first one)."""
+    for n_kv in range(50, 640, 64):
+        q = normal(n_kv, 2, heads, n, dim, dtype=dtype)
+        k, v = normal(1, 2, 1, n_kv, dim, dtype=dtype), normal(2, 2, 1, n_kv, dim, dtype=dtype)
+        lengths = int32([n_kv, 30])
+        got = K.window_attention(q, k, v, right=None, lengths=lengths)
+        assert_attends(got, q, k, v, right=None, lengths=lengths)
+
+
 @pytest.mark.parametrize("dtype, dim", [(BF16, 128), (F16, 128), (BF16, 64)])
 @pytest.mark.parametrize("b, n, n_kv, heads, kv_heads", [(1, 1, 20000, 4, 1), (3, 1, 9001, 8, 8), (1, 5, 30000, 8, 2), (40, 1, 700, 8, 4),
                                                          (2, 1, 4097, 24, 1), (1, 33, 5000, 6, 2), (1, 200, 3001, 3, 3)])  # fmt: skip
