@@ -80,6 +80,9 @@ IRIS_DEVICE uint64_t global_timer_ns() {
 // before it in the stream ends: it touches global memory only after grid_wait
 // (that kernel complete and its writes visible; no wait where it was launched
 // otherwise), and lets its own successor start with grid_trigger, after its wait.
+// What it reads may have been written while it already ran: no __ldg or ld.global.nc in
+// such a kernel, whose promise is data that nobody writes as long as the kernel lives
+// (the compiler may move such a load above the wait).
 IRIS_DEVICE void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 IRIS_DEVICE void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -210,11 +210,11 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(COLS8)) gemv_q4_kernel(co
       for (int h = 0; h < (TERMS == 1 ? 1 : 2); ++h) raw[i][h] = make_uint4(0u, 0u, 0u, 0u);
       if (!real) continue;
       if (TERMS == 1 || p.x_dtype != IRIS_F32) {
-        raw[i][0] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at));
+        raw[i][0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.x) + at);
       } else {
 #pragma unroll
         for (int h = 0; h < (TERMS == 1 ? 1 : 2); ++h)
-          raw[i][h] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.x) + at) + h);
+          raw[i][h] = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.x) + at)[h];
       }
     }
   };
@@ -286,8 +286,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(COLS8)) gemv_q4_kernel(co
         if (r < real_rows && 4 * h < grps_left && quad + 4 * h < PER * SPAN) {
           // volatile: where they stand, a span ahead of their use
           const int64_t at = static_cast<int64_t>(8 * r) * groups + 4 * h;
-          asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(scale) : "l"(scale_at + at));
-          if (zero_at) asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(zero) : "l"(zero_at + at));
+          asm volatile("ld.global.u16 %0, [%1];" : "=h"(scale) : "l"(scale_at + at));
+          if (zero_at) asm volatile("ld.global.u8 %0, [%1];" : "=r"(zero) : "l"(zero_at + at));
         }
         sz_scale[r][h] = scale;
         sz_zero[r][h] = zero;
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(COLS8)) gemv_q4_kernel(co
       if (q < p.parts)
 #pragma unroll
         for (int c = TERMS - 1; c >= 0; --c) v += sums[(q * owned + row) * WIDTH + m * TERMS + c];
-    if (p.bias) v += __ldg(p.bias + n);
+    if (p.bias) v += p.bias[n];
     store_elem(p.out, static_cast<int64_t>(m0 + m) * p.N + n, p.out_dtype, p.silu_out ? silu(v) : v);
   }
 }

@@ -106,12 +106,12 @@ IRIS_DEVICE void load_floats(const float* p, float (&v)[V]) {
   if constexpr (V % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < V; i += 4) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(p + i));
+      const float4 f = *reinterpret_cast<const float4*>(p + i);
       v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = __ldg(p + i);
+    for (int i = 0; i < V; ++i) v[i] = p[i];
   }
 }
 

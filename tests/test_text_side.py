@@ -238,3 +238,13 @@ def test_pack_q4_takes_the_nearest_level(K, group, symmetric):
     # is up to half a level off
     assert torch.all((back - w).abs() <= step * (0.5 + 15 * 2.0**-8 + (0 if symmetric else 0.5)) + 1e-6)
     assert torch.all(back[1, :group] == 0)
+
+
+def test_kernels_that_start_early_use_coherent_loads():
+    """A kernel launched with launch_early lives while its predecessor writes what it will read: a non-coherent load
+    (data that nobody writes as long as the kernel lives) may be served from before the wait."""
+    early = [f for f in sorted((REPO / "iris-3b-metal_b200" / "csrc").glob("*.cu")) if "launch_early(" in f.read_text()]
+    assert {"q4.cu", "rope.cu", "window.cu"} <= {f.name for f in early}
+    for f in early:
+        code = re.sub(r"//.*", "", f.read_text())
+        assert not re.search(r"__ldg|__ldcs|ld\.global\.nc|__restrict__", code), f.name
