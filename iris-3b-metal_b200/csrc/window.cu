@@ -295,8 +295,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 2)
           mbar_arrive_expect_tx(bar, KV_BYTES);
           for (int c = 0; c < HALVES; ++c)
             tma_load_4d(&tv, bar, v_tile + st * KV_BYTES + c * KV_HALF, c * 64, key, vh, vb);
-          if (tail) tail_issued = true;
-          else issued_v[st] = static_cast<int>(ph);
+          tail_issued = tail_issued || tail;
+          issued_v[st] = tail ? -1 : static_cast<int>(ph);  // the copy before in this slot has been read
         }
       }
       if (!__shfl_sync(0xffffffffu, ok, 0)) break;
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 2)
         if (lane == 0) mbar_arrive(&s->v_full[st]);
       }
     }
-    if (lane == 0 && !ok) {  // given up: no copy may land after the CTA is gone
+    if (lane == 0 && iters > 0) {  // whichever warp gives up: no copy may land after the CTA is gone
       int dummy = 0;
       mbar_wait(&s->q_full, 0, &dummy);
       for (int i = 0; i < KV; ++i) {

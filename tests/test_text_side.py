@@ -248,3 +248,13 @@ def test_kernels_that_start_early_use_coherent_loads():
     for f in early:
         code = re.sub(r"//.*", "", f.read_text())
         assert not re.search(r"__ldg|__ldcs|ld\.global\.nc|__restrict__", code), f.name
+
+
+def test_prompt_tiles_wait_for_their_copies_whoever_gives_up():
+    """The thread that issued a tile's last copies waits for them on every path: another warp may give up (and the CTA
+    end) after this one has issued everything."""
+    code = (REPO / "iris-3b-metal_b200" / "csrc" / "window.cu").read_text()
+    issue = code[code.index("--- TMA") : code.index("--- MMA")]
+    guard, drain = re.search(r"\n    if \(([^\n]*)\) \{[^\n]*\n      int dummy = 0;(.*?)\n    \}\n", issue, flags=re.S).groups()
+    assert guard == "lane == 0 && iters > 0"
+    assert all(f"mbar_wait(&s->{bar}" in drain for bar in ("q_full", "k_full", "v_full", "v_tail"))
