@@ -157,7 +157,7 @@ typedef struct iris_head_rows {
  * `rotary` columns of each row turn by pairs (IRIS_ROPE_*) through row p of the fp32
  * tables [table_rows, rotary / 2], the others are copied; p = positions[b *
  * positions_stride + t] (int32, or int64 with positions_64 != 0), or t where positions
- * is null. out may be x. inverse != 0 turns back. A position outside the table gives
+ * is null. out may be x, or shares no memory with it. inverse != 0 turns back. A position outside the table gives
  * a NaN row and sets bit 1 of the device error word. The reference's counterpart is
  * apply_rope, src/iris3b/nn/rope.py:92-101 (interleaved, whole head, positions in
  * order). */
@@ -179,8 +179,8 @@ int iris_rope(const iris_rope_problem* problem, void* stream);
  * `sinks` positions and the latest capacity - sinks) to slot
  * p < sinks ? p : sinks + (p - sinks) % (capacity - sinks); of two rows of the call
  * for one slot the later is kept. Rows from counts[b] on are left as they are, or
- * with zero_rest != 0 zeroed in out. A
- * position outside the table (NaN row, nothing appended) or past the end of a
+ * with zero_rest != 0 zeroed in out. out may be q; the rows, caches and out share no
+ * memory otherwise. A position outside the table (NaN row, nothing appended) or past the end of a
  * plain cache (nothing appended) sets bit 1 of the device error word. */
 typedef struct iris_append_problem {
   iris_head_rows q, k, v, out, k_cache, v_cache;
@@ -310,7 +310,8 @@ int iris_flash_attn_fwd_peers(const void* q, const void* k, const void* v, int64
  * visible keys, 0 where there is none; what lies in other keys' rows, NaN
  * included, does not reach a row. q [batch, heads_q, n, head_dim], k / v [batch,
  * heads_kv, n_kv, head_dim], bf16 or f16, strides multiples of 8 (0 repeats a head or
- * a sample), head_dim 64 or 128. workspace: iris_window_attn_workspace bytes. */
+ * a sample), head_dim 64 or 128; out shares no memory with k or v, and with q only
+ * as its own rows in place. workspace: iris_window_attn_workspace bytes. */
 typedef struct iris_window_problem {
   iris_head_rows q, k, v;
   void* out;

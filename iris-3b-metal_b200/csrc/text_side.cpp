@@ -83,9 +83,36 @@ iris_head_rows head_rows(const at::Tensor& t, int64_t batch, int64_t heads, int6
   return iris_head_rows{t.data_ptr(), batch > 1 ? stride[0] : 0, heads > 1 ? stride[1] : 0, n > 1 ? stride[2] : 0};
 }
 
-// No two elements in one place: an expanded output would be a race.
+// Outputs take every element once: two writes to one place would be a race, as would
+// a write to what other threads of the call still read.
 void writable(const at::Tensor& t) {
-  for (int64_t d = 0; d < t.dim(); ++d) require(t.stride(d) != 0 || t.size(d) <= 1, "an output must not be an expanded view");
+  const int64_t dims = t.dim();
+  for (int64_t d = 0; d < dims; ++d) {
+    if (t.size(d) <= 1) continue;
+    require(t.stride(d) != 0, "an output must not be an expanded view");
+    // rows apart: each stride steps over all that the dimensions of smaller strides span
+    int64_t span = 1;
+    for (int64_t e = 0; e < dims; ++e)
+      if (t.stride(e) < t.stride(d)) span += (t.size(e) - 1) * t.stride(e);
+      else require(e == d || t.size(e) <= 1 || t.stride(e) != t.stride(d), "an output's rows must not overlap");
+    require(t.numel() == 0 || t.stride(d) >= span, "an output's rows must not overlap");
+  }
+}
+
+// Whether both hold an element for certain: the same first one, or dense tensors whose
+// ranges meet (views of one buffer that interleave are the caller's to keep apart).
+bool share(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const char *x = static_cast<const char*>(a.data_ptr()), *y = static_cast<const char*>(b.data_ptr());
+  if (x == y) return true;
+  return a.is_non_overlapping_and_dense() && b.is_non_overlapping_and_dense() && x < y + b.nbytes() && y < x + a.nbytes();
+}
+
+bool same_rows(const at::Tensor& a, const at::Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.sizes() != b.sizes()) return false;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
 }
 
 const int* int32_rows(const at::Tensor* t, int64_t batch, const char* message) {
@@ -153,6 +180,7 @@ PyObject* rope(PyObject* const* a) {
   }
   q.layout = rope_layout(a[4]);
   q.inverse = truth(a[5]);
+  require(given == nullptr || !share(*given, x) || same_rows(*given, x), "rope: out must be x itself or share no memory with it");
   const On on(x, {&cos, &sin, positions, given});
   if (given) {
     require(given->scalar_type() == x.scalar_type(), "rope: out must have the input's type");
@@ -189,6 +217,14 @@ PyObject* rope_append(PyObject* const* a) {
   q.v_cache = head_rows(v_cache, q.batch, q.heads_kv, q.capacity, q.head_dim, "rope_append: v_cache must be [B, H_kv, C, D]");
   writable(k_cache);
   writable(v_cache);
+  require(!share(k_cache, v_cache), "rope_append: the caches must not share memory");
+  for (const at::Tensor* rows : {&qt, &k, &v})
+    require(!share(*rows, k_cache) && !share(*rows, v_cache), "rope_append: the rows must not share memory with a cache");
+  if (given) {
+    require(!share(*given, qt) || same_rows(*given, qt), "rope_append: out must be q itself or share no memory with it");
+    for (const at::Tensor* other : {&k, &v, &k_cache, &v_cache})
+      require(!share(*given, *other), "rope_append: out must not share memory with k, v or a cache");
+  }
   q.sinks = -1;
   if (a[8] != Py_None) {
     q.sinks = whole(a[8]);
@@ -240,8 +276,17 @@ PyObject* window_attention(PyObject* const* a) {
     q.scale = PyFloat_AsDouble(a[8]);
     if (q.scale == -1.0 && PyErr_Occurred()) throw Raised{};
   }
-  const On on(qt, {&k, &v, starts, lengths, given});
   const int64_t width = q.heads_q * q.head_dim;
+  if (given) {
+    // onto q's own rows: a row is read by the CTAs that write it, before they do
+    const bool own = given->dim() == 3 && given->data_ptr() == qt.data_ptr() && given->size(0) == q.batch &&
+                     given->size(1) == q.n && given->size(2) == width && given->stride(2) == 1 &&
+                     (q.batch <= 1 || given->stride(0) == qt.stride(0)) && (q.n <= 1 || given->stride(1) == qt.stride(2)) &&
+                     (q.heads_q <= 1 || qt.stride(1) == q.head_dim);
+    require(own || !share(*given, qt), "window_attention: out must be q's own rows or share no memory with q");
+    require(!share(*given, k) && !share(*given, v), "window_attention: out must not share memory with k or v");
+  }
+  const On on(qt, {&k, &v, starts, lengths, given});
   if (given) {
     require(given->dim() == 3 && given->size(0) == q.batch && given->size(1) == q.n && given->size(2) == width &&
                 given->scalar_type() == type && given->stride(2) == 1,

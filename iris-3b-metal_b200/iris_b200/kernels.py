@@ -542,7 +542,7 @@ def rope(
     ``cos``/``sin``: FP32 ``[P, R / 2]`` (:func:`iris_b200.tables.rope_table`);
     ``positions``: int32 or int64 ``[N]`` or ``[B, N]`` rows of the tables, default ``0 ..
     N - 1``. ``inverse`` turns back, which is also the gradient's map. ``out`` may be
-    ``x``; by default it is a new contiguous tensor. A position outside the tables
+    ``x`` but not overlap it otherwise; by default it is a new contiguous tensor. A position outside the tables
     gives a NaN row and sets bit 1 of :func:`device_error`."""
     return (_lib._text_side or _lib.text_side()).rope(x, cos, sin, positions, layout, inverse, out)
 
@@ -574,7 +574,8 @@ def rope_append(
     (``window_attention(q, k_cache, v_cache, lengths=positions, right=None)``). Rows from
     ``counts[b]`` on are not touched (zeros in a new ``out``). A position outside the
     tables (NaN row, not appended) or past a plain cache (not appended) sets bit 1 of
-    :func:`device_error`. ``layout`` and the tables as for :func:`rope`."""
+    :func:`device_error`. ``layout`` and the tables as for :func:`rope`. ``out`` may be ``q``;
+    the rows, the caches and ``out`` share no memory otherwise."""
     return (_lib._text_side or _lib.text_side()).rope_append(q, k, v, cos, sin, starts, k_cache, v_cache, sinks, counts, layout, out)
 
 
@@ -601,7 +602,7 @@ def window_attention(
     to ``[0, N_kv]``; default ``N_kv``) with ``j <= p + right`` and ``j >= p - left`` or ``j <
     sinks``; ``None`` is no bound, the default is causal. A query that sees no key
     gives 0. Other keys' rows may hold anything. Heads and samples may be expanded,
-    tokens not."""
+    tokens not. ``out`` shares no memory with the inputs, or is ``q``'s own rows."""
     return (_lib._text_side or _lib.text_side()).window_attention(q, k, v, left, right, sinks, starts, lengths, scale, out)
 
 

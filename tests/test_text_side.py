@@ -258,3 +258,45 @@ def test_prompt_tiles_wait_for_their_copies_whoever_gives_up():
     guard, drain = re.search(r"\n    if \(([^\n]*)\) \{[^\n]*\n      int dummy = 0;(.*?)\n    \}\n", issue, flags=re.S).groups()
     assert guard == "lane == 0 && iters > 0"
     assert all(f"mbar_wait(&s->{bar}" in drain for bar in ("q_full", "k_full", "v_full", "v_tail"))
+
+
+def test_outputs_that_would_race_are_refused(K):
+    """Two elements in one place, or an output in what other threads of the call still read (before any device check)."""
+    cos = sin = torch.zeros(9, 32)
+    buf = torch.zeros(4096)
+    x = buf[:1536].view(2, 4, 3, 64)
+
+    def refused(message, call, *args, **kw):
+        with pytest.raises(ValueError, match=message):
+            call(*args, **kw)
+
+    refused("CUDA", K.rope, x, cos, sin, out=x)  # in place is allowed: it gets as far as the device
+    refused("CUDA", K.rope, x, cos, sin, out=x.view(2, 4, 3, 64))
+    refused("CUDA", K.rope, x, cos, sin, out=buf[1536:3072].view(2, 4, 3, 64))
+    refused("x itself", K.rope, x, cos, sin, out=buf[64:1600].view(2, 4, 3, 64))
+    refused("x itself", K.rope, x, cos, sin, out=buf[:1536].view(2, 3, 4, 64).transpose(1, 2))
+    refused("CUDA", K.rope, buf[:0].view(2, 4, 0, 64), cos, sin, out=buf[:0].view(2, 4, 0, 64))
+    for strides in [(768, 192, 32, 1), (192, 192, 64, 1), (768, 64, 64, 1)]:  # rows that overlap without a stride of 0
+        refused("overlap|CUDA", K.rope, x, cos, sin, out=torch.zeros(4096).as_strided((2, 4, 3, 64), strides))
+    packed = torch.zeros(2, 3, 12, 64).transpose(1, 2)  # interleaved heads of one buffer are apart
+    refused("CUDA", K.rope, packed[:, :4], cos, sin, out=packed[:, 4:8])
+
+    q, k, v = torch.zeros(2, 4, 3, 64), torch.zeros(2, 2, 3, 64), torch.zeros(2, 2, 3, 64)
+    caches = torch.zeros(2, 2, 2, 8, 64)
+    good = dict(q=q, k=k, v=v, cos=cos, sin=sin, starts=torch.zeros(2, dtype=torch.int32), k_cache=caches[0], v_cache=caches[1])
+    refused("CUDA", K.rope_append, **good)
+    refused("CUDA", K.rope_append, **{**good, "out": q})
+    refused("CUDA", K.rope_append, **{**good, "v": k})
+    for bad in (dict(v_cache=caches[0]), dict(k=caches[0, :, :, :3]), dict(v=caches[1, :, :, :3]), dict(out=caches.view(-1)[:1536].view_as(q)),
+                dict(out=q.view(2, 3, 4, 64).transpose(1, 2)), dict(k_cache=caches.view(-1)[64:2112].view(2, 2, 8, 64)),
+                dict(k=q.view(-1)[:768].view_as(k), out=q)):  # fmt: skip
+        refused("share", K.rope_append, **{**good, **bad})
+
+    rows = torch.zeros(2, 3, 256, dtype=torch.bfloat16)
+    q, k = rows.view(2, 3, 4, 64).transpose(1, 2), torch.zeros(2, 2, 3, 64, dtype=torch.bfloat16)
+    refused("CUDA", K.window_attention, q, k, k, out=rows)  # q's own rows
+    refused("own rows", K.window_attention, rows.view(2, 4, 3, 64), k, k, out=rows)
+    refused("CUDA", K.window_attention, rows[:, :1].view(2, 4, 1, 64), k, k, out=rows[:, :1])
+    refused("k or v", K.window_attention, q[:, :2], k, rows.view(2, 2, 6, 64)[:, :, :3], out=rows[..., :128])
+    refused("k or v", K.window_attention, q[:, :2], q, q, out=rows[..., :128])
+    refused("overlap|CUDA", K.window_attention, q, k, k, out=torch.zeros(2048, dtype=torch.bfloat16).as_strided((2, 3, 256), (768, 64, 1)))

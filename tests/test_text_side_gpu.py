@@ -574,3 +574,30 @@ def test_same_answer_every_time(K, n):
     x = normal(5, n if n < 64 else 16, 4096, dtype=BF16)
     first = K.gemv_q4(x, *w)
     assert all(torch.equal(first, K.gemv_q4(x, *w)) for _ in range(5))
+
+
+@pytest.mark.parametrize("n, n_kv, b, heads, kv", [(1, 40, 2, 8, 2), (1, 700, 1, 20, 5), (1, 20000, 1, 8, 1), (3, 90, 2, 4, 4),
+                                                   (300, 300, 2, 4, 2), (257, 640, 1, 3, 3)])  # fmt: skip
+def test_window_attention_onto_its_queries(K, n, n_kv, b, heads, kv):
+    """In place on q's rows, in every form of the split and in whole tiles, rows that are computed again among them."""
+    q = normal(1, b, n, heads, 128, dtype=BF16).transpose(1, 2)
+    k, v = normal(2, b, kv, n_kv, 128, dtype=BF16), normal(3, b, kv, n_kv, 128, dtype=BF16)
+    v[:, :, 5] = math.nan
+    for left in (None, 20):
+        expected = K.window_attention(q, k, v, left=left)
+        own = q.transpose(1, 2).contiguous().transpose(1, 2)
+        rows = own.transpose(1, 2).view(b, n, heads * 128)
+        assert K.window_attention(own, k, v, left=left, out=rows) is rows
+        assert torch.equal(rows.view(torch.int16), expected.view(torch.int16))
+
+
+def test_outputs_whose_rows_overlap_are_refused(K):
+    cos, sin = table(64, 9)
+    x = normal(1, 2, 4, 3, 64)
+    room = torch.zeros(4096, device="cuda")
+    for strides in [(768, 192, 32, 1), (192, 192, 64, 1), (768, 64, 64, 1)]:
+        with pytest.raises(ValueError, match="overlap"):
+            K.rope(x, cos, sin, out=room.as_strided((2, 4, 3, 64), strides))
+    q, k = x.bfloat16(), normal(2, 2, 2, 3, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="overlap"):
+        K.window_attention(q, k, k, out=room.bfloat16().as_strided((2, 3, 256), (768, 64, 1)))
