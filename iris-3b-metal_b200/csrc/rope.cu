@@ -88,8 +88,9 @@ struct alignas(sizeof(T) * V) Vec {
   T e[V];
 };
 
-// Slot of position p, or -1 where it is not kept. `last`: the sample's last new
-// position; a rolling cache skips tokens whose slot a later one of the call takes.
+// Slot of position p, or -1 where it is not kept. `last`: the sample's last position
+// that the call appends (none behind the tables); a rolling cache skips tokens whose slot
+// a later one of the call takes.
 IRIS_DEVICE int64_t cache_slot(const Params& a, int64_t p, int64_t last, bool* bad) {
   if (a.sinks < 0) {
     *bad = p >= a.capacity;
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const __grid_constant__ P
       p = first + t;
       bad = p < 0 || p >= a.table_rows;
       bool full = false;
-      const int64_t kept = bad ? -1 : cache_slot(a, p, first + count - 1, &full);
+      const int64_t kept = bad ? -1 : cache_slot(a, p, min(first + count, a.table_rows) - 1, &full);
       if ((bad || full) && u == 0 && slot0 == 0) atomicOr(&g_device_error, kErrBadArgument);
       if (!isq) {
         if (kept < 0) continue;

@@ -601,3 +601,20 @@ def test_outputs_whose_rows_overlap_are_refused(K):
     q, k = x.bfloat16(), normal(2, 2, 2, 3, 64, dtype=BF16)
     with pytest.raises(ValueError, match="overlap"):
         K.window_attention(q, k, k, out=room.bfloat16().as_strided((2, 3, 256), (768, 64, 1)))
+
+
+def test_rolling_append_past_the_tables(K):
+    """Tokens whose position has no table row are not appended, and take no slot from those before them."""
+    cos, sin = table(64, 14)
+    q, k, v = packed_heads(4, 2, 8, 2, 1, 64, BF16)
+    k_cache, v_cache = torch.zeros(2, 1, 6, 64, device="cuda", dtype=BF16), torch.zeros(2, 1, 6, 64, device="cuda", dtype=BF16)
+    K.device_error()
+    K.rope_append(q, k, v, cos, sin, int32([10, 3]), k_cache, v_cache, sinks=2)
+    assert K.device_error() & ERR_BAD_ARGUMENT
+    for s, first in ((0, 10), (1, 3)):
+        latest = {2 + (p - 2) % 4: p for p in range(max(first, 2), min(first + 8, 14))}  # positions 10 to 13; 7 to 10
+        assert len(latest) == 4
+        for slot, p in latest.items():
+            assert torch.equal(v_cache[s, :, slot], v[s, :, p - first])
+            assert_turned(k_cache[s, :, slot], k[s, :, p - first], cos[p], sin[p], "interleaved")
+        assert torch.all(v_cache[s, :, :2] == 0)
