@@ -206,6 +206,9 @@ __global__ void __launch_bounds__(THREADS) rope_kernel(const __grid_constant__ P
             turn(y[j].e[2 * i], y[j].e[2 * i + 1], cs[V / 2 + i], sn[V / 2 + i]);
           }
         }
+      } else if (bad) {  // the whole row is NaN, its copied columns too
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[j].e[i] = y[j].e[i] = from_f32<T>(__int_as_float(0x7fc00000));
       }
       T* to = dst + j * step * w.dh;
       *reinterpret_cast<Vec<T, V>*>(to + c0) = x[j];

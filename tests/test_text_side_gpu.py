@@ -618,3 +618,23 @@ def test_rolling_append_past_the_tables(K):
             assert torch.equal(v_cache[s, :, slot], v[s, :, p - first])
             assert_turned(k_cache[s, :, slot], k[s, :, p - first], cos[p], sin[p], "interleaved")
         assert torch.all(v_cache[s, :, :2] == 0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim, rotary", [(64, 64), (128, 32), (80, 40), (10, 2)])
+def test_rows_outside_the_tables_are_nan_in_every_column(K, dtype, layout, dim, rotary):
+    cos, sin = table(rotary, 8)
+    q, k, v = packed_heads(3, 2, 4, 5, 2, dim, dtype)
+    K.device_error()
+    got = K.rope(q, cos, sin, torch.tensor([3, -1, 7, 8], device="cuda"), layout=layout)
+    assert K.device_error() & ERR_BAD_ARGUMENT
+    assert torch.isnan(got[:, :, [1, 3]]).all()
+    at = torch.tensor([3, 7], device="cuda")
+    assert_turned(got[:, :, [0, 2]], q[:, :, [0, 2]], cos[at], sin[at], layout)
+    caches = torch.zeros(2, 2, 2, 8, dim, device="cuda", dtype=dtype)
+    got = K.rope_append(q, k, v, cos, sin, int32([6, -2]), *caches, layout=layout)
+    assert torch.isnan(got[0, :, 2:]).all() and torch.isnan(got[1, :, :2]).all()
+    assert torch.isfinite(got[0, :, :2]).all() and torch.isfinite(got[1, :, 2:]).all() and torch.isfinite(caches).all()
+    assert torch.equal(caches[1, 0, :, 6:], v[0, :, :2]) and torch.all(caches[:, 0, :, :6] == 0)
+    assert torch.equal(caches[1, 1, :, :2], v[1, :, 2:]) and torch.all(caches[:, 1, :, 2:] == 0)
