@@ -64,7 +64,9 @@ def rope_table(
     that the slowest pair is divided by ``factor`` and the fastest is kept; ``"ramp"``
     keeps pairs that turn at least ``fast_turns`` times over ``trained_length``
     positions, divides those that turn at most ``slow_turns`` times, blends linearly
-    in the pair's index between, and multiplies both tables by ``0.1 ln(factor) + 1``."""
+    in the pair's index between (from the whole index at or before the one end, pair 0
+    at the earliest, to the one at or behind the other), and multiplies both tables by
+    ``0.1 ln(factor) + 1``."""
     if rotary < 2 or rotary % 2 or length < 1 or theta <= 1 or factor < 1:
         raise ValueError("rope_table needs an even rotary width, a positive length, theta > 1 and factor >= 1")
     if scaling not in (None, "linear", "ntk", "ramp"):
@@ -87,9 +89,10 @@ def rope_table(
             return rotary * math.log(trained_length / (2 * math.pi * turns)) / (2 * math.log(theta))
 
         first = max(math.floor(pair(fast_turns)), 0)
-        last = min(math.ceil(pair(slow_turns)), rotary // 2 - 1)
+        last = math.ceil(pair(slow_turns))  # may lie behind the last pair: then none is divided in full
         index = torch.arange(rotary // 2, dtype=torch.float64)
-        divided = ((index - first) / max(last - first, 1e-3)).clamp(0, 1)
+        divided = ((index - first) / max(last - first, 1)).clamp(0, 1)
+        divided[trained_length * freqs <= 2 * math.pi * slow_turns] = 1  # every pair, where they start so slowly
         freqs = freqs / factor * divided + freqs * (1 - divided)
         magnitude = 0.1 * math.log(factor) + 1
     angles = torch.outer(torch.arange(length, dtype=torch.float64), freqs)

@@ -300,3 +300,39 @@ def test_outputs_that_would_race_are_refused(K):
     refused("k or v", K.window_attention, q[:, :2], k, rows.view(2, 2, 6, 64)[:, :, :3], out=rows[..., :128])
     refused("k or v", K.window_attention, q[:, :2], q, q, out=rows[..., :128])
     refused("overlap|CUDA", K.window_attention, q, k, k, out=torch.zeros(2048, dtype=torch.bfloat16).as_strided((2, 3, 256), (768, 64, 1)))
+
+
+@pytest.mark.parametrize("rotary, theta, trained, fast, slow", [
+    (128, 1e4, 131072, 32.0, 1.0),  # the slowest pair still turns 2.4 times
+    (128, 1e4, 4096, 32.0, 1.0),
+    (64, 1e4, 1 << 22, 32.0, 1.0),  # even the slowest pair turns more than 32 times
+    (64, 1e6, 8192, 16.0, 2.0),
+    (32, 1e4, 100, 32.0, 1.0),  # the fastest pair turns 16 times
+    (32, 1e4, 5, 32.0, 1.0),  # no pair turns once
+])  # fmt: skip
+def test_rope_table_ramp_at_every_trained_length(rotary, theta, trained, fast, slow):
+    """Pair by pair: kept from `fast` turns on, divided up to `slow`, in between by the pair's index."""
+    from iris_b200.tables import rope_table
+
+    factor, positions = 4.0, 40
+    cos, sin = rope_table(rotary, positions, theta, scaling="ramp", factor=factor, trained_length=trained, fast_turns=fast, slow_turns=slow)
+    magnitude = 0.1 * math.log(factor) + 1
+
+    def index(turns):  # trained theta^(-2 i / rotary) = 2 pi turns
+        return rotary / 2 * math.log(trained / (2 * math.pi * turns), theta)
+
+    first, last = max(0, math.floor(index(fast))), math.ceil(index(slow))
+    shares = []
+    for i in range(rotary // 2):
+        freq = theta ** (-2 * i / rotary)
+        turns = trained * freq / (2 * math.pi)
+        share = 0.0 if turns >= fast else 1.0 if turns <= slow else (i - first) / (last - first)
+        share = min(1.0, max(0.0, share))
+        freq = freq * (1 - share) + freq / factor * share
+        for p in (1, positions - 1):
+            # one rounding to fp32 of a value of at most 1.2, and a 64-bit angle of at most 40
+            assert abs(float(cos[p, i]) - magnitude * math.cos(p * freq)) <= 2.0**-23
+            assert abs(float(sin[p, i]) - magnitude * math.sin(p * freq)) <= 2.0**-23
+        shares.append(share)
+    assert shares == sorted(shares)
+    assert (max(shares) < 1) == (index(slow) > rotary / 2 - 1) and (min(shares) == 1) == (index(slow) <= 0)
