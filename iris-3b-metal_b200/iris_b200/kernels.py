@@ -616,7 +616,7 @@ def pack_q4(
     over 7, or the group's range (0 included) over 15 from a whole zero point."""
     _require(w.dim() == 2 and group in (32, 64, 128) and w.shape[1] % group == 0 and w.shape[1] > 0,
              "pack_q4 needs [N, K] weights, K a multiple of the group (32, 64 or 128)")  # fmt: skip
-    g = w.float().reshape(w.shape[0], -1, group)
+    g = w.detach().float().reshape(w.shape[0], -1, group)
     if symmetric:
         step, zero = g.abs().amax(dim=-1) / 7, None
     else:

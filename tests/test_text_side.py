@@ -336,3 +336,13 @@ def test_rope_table_ramp_at_every_trained_length(rotary, theta, trained, fast, s
         shares.append(share)
     assert shares == sorted(shares)
     assert (max(shares) < 1) == (index(slow) > rotary / 2 - 1) and (min(shares) == 1) == (index(slow) <= 0)
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_pack_q4_of_a_parameter_keeps_no_graph(K, symmetric):
+    """Packed weights stand alone: nothing of them holds the parameter's values or its autograd graph."""
+    w = torch.nn.Linear(64, 6).weight
+    packed = K.pack_q4(w, 32, symmetric)
+    for got, plain in zip(packed, K.pack_q4(w.detach(), 32, symmetric)):
+        if got is not None:
+            assert not got.requires_grad and got.grad_fn is None and torch.equal(got, plain)
