@@ -426,7 +426,8 @@ int iris_gemv(const float* x, int64_t M, int64_t K, const void* w, int w_dtype, 
 /* The small-M linear over 4-bit weights (iris_gemv with a quarter of the BF16
  * weights' bytes): w[n, k] = scale[n, k / group] (q[n, k] - zero[n, k / group]), q the
  * low (k even) or high nibble of packed[n, k / 2], scale bf16 [N, K / group], zero
- * uint8 [N, K / group] of 0 to 15 or null (8 everywhere), group 32, 64 or 128;
+ * uint8 [N, K / group] of 0 to 15 (a larger one makes out's column n NaN and sets bit 1
+ * of the device error word) or null (8 everywhere), group 32, 64 or 128;
  * out[m, n] = act_out(sum_k act_in(x[m, k]) w[n, k] + bias[n]), the activations silu
  * where asked for, bias fp32 or null. x [M, K] with row stride ldx, M <= 64; fp32
  * sums; out [M, N] contiguous. */

@@ -337,8 +337,11 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(COLS8)) gemv_q4_kernel(co
 #pragma unroll
       for (int r = 0; r < 2 * TILES; ++r)
 #pragma unroll
-        for (int h = 0; h < HELD; ++h)  // scale, 16 zero, zero
-          now[r][h] = static_cast<uint32_t>(sz_scale[r][h]) << 16 | sz_zero[r][h] * 0x1001u;
+        for (int h = 0; h < HELD; ++h) {  // scale, 16 zero, zero; a zero point of more than 4 bits makes its row NaN
+          const bool fits = sz_zero[r][h] < 16u;
+          now[r][h] = fits ? static_cast<uint32_t>(sz_scale[r][h]) << 16 | sz_zero[r][h] * 0x1001u : 0x7fc00000u;
+          if (!fits) atomicOr(&g_device_error, kErrBadArgument);
+        }
       fetch();
     }
     if (n0 < p.N && ok) {

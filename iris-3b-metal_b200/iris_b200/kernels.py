@@ -645,7 +645,8 @@ def gemv_q4(
     """``act(act(x) @ w.T + bias)`` for 1 to 64 rows ``x`` ``[M, K]`` (FP32, BF16 or FP16; the
     row stride may exceed ``K``) and 4-bit weights from :func:`pack_q4`, with FP32 sums;
     ``silu_in`` / ``silu_out`` turn the activations on, ``bias``: FP32 ``[N]``. The result
-    is ``[M, N]`` of ``out_dtype`` (default: the input's)."""
+    is ``[M, N]`` of ``out_dtype`` (default: the input's). ``zero`` holds 0 to 15: a larger
+    value makes its weight row's results NaN and sets bit 1 of :func:`device_error`."""
     return (_lib._text_side or _lib.text_side()).gemv_q4(x, packed, scale, zero, bias, silu_in, silu_out, out_dtype)
 
 

@@ -638,3 +638,25 @@ def test_rows_outside_the_tables_are_nan_in_every_column(K, dtype, layout, dim, 
     assert torch.isfinite(got[0, :, :2]).all() and torch.isfinite(got[1, :, 2:]).all() and torch.isfinite(caches).all()
     assert torch.equal(caches[1, 0, :, 6:], v[0, :, :2]) and torch.all(caches[:, 0, :, :6] == 0)
     assert torch.equal(caches[1, 1, :, :2], v[1, :, 2:]) and torch.all(caches[:, 1, :, 2:] == 0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_gemv_q4_zero_points(K, dtype, group):
+    """Every zero point of 4 bits; one beyond them marks its weight row alone and the device error word."""
+    n, k = 200, 6 * group + 128
+    packed, scale, _ = K.pack_q4(normal(1, n, k), group)
+    zero = (torch.arange(n * scale.shape[1], device="cuda") % 16).to(torch.uint8).view_as(scale)
+    x = normal(2, 3, k, dtype=dtype)
+    K.device_error()
+    good = K.gemv_q4(x, packed, scale, zero)
+    assert_q4(good, x, packed, scale, zero, None)
+    assert K.device_error() == 0
+    rows = torch.tensor([0, 37, 130, 199], device="cuda")
+    for row, value in zip(rows.tolist(), (16, 17, 128, 255)):
+        zero[row, row % scale.shape[1]] = value
+    got = K.gemv_q4(x, packed, scale, zero)
+    assert K.device_error() & ERR_BAD_ARGUMENT
+    assert torch.isnan(got[:, rows]).all()
+    rest = torch.ones(n, dtype=torch.bool, device="cuda").index_fill(0, rows, False)
+    assert torch.equal(got[:, rest], good[:, rest])
