@@ -148,6 +148,32 @@ IRIS_DEVICE void split3(float v, uint32_t (&t)[3]) {
   t[2] = __float_as_uint(rest - __uint_as_float(mid)) >> 16;
 }
 
+// One result from the definition, its weights scaled before the sum: for results that are
+// not finite, since a group's unscaled sum of x (q - zero) leaves fp32 where a scaled one
+// need not (|x| from 2e35 on). By one thread; NaN and infinities in x come here too.
+__device__ __noinline__ float sum_scaled(const Params& p, int group, int m, int n) {
+  const int groups = p.K / group;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(p.packed + static_cast<int64_t>(n) * (p.K / 2));
+  float total = 0.f;
+  for (int g = 0; g < groups; ++g) {
+    const int64_t at = static_cast<int64_t>(n) * groups + g;
+    const uint32_t zero = p.zero ? p.zero[at] : 8u;
+    const float s = zero < 16u ? __bfloat162float(p.scale[at]) : __int_as_float(0x7fc00000), z = static_cast<float>(zero);
+    float part[8] = {};
+    for (int w = g * (group / 8); w < (g + 1) * (group / 8); ++w) {
+      const uint32_t q = words[w];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = load_elem(p.x, m * p.ldx + w * 8 + j, p.x_dtype);
+        part[j] = fmaf(p.silu_in ? silu(v) : v, s * (static_cast<float>(q >> (4 * j) & 15u) - z), part[j]);
+      }
+    }
+    total += ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+    if (isnan(total)) break;
+  }
+  return total;
+}
+
 // The weight row that a lane's row index g of the mma stands for: with the copy's
 // 128-byte swizzle (16-byte piece x of row r at x ^ (r % 8)) the 4-, 8- or 16-byte reads
 // of lanes that read together then meet no bank twice.
@@ -469,6 +495,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(COLS8)) gemv_q4_kernel(co
       if (q < p.parts)
 #pragma unroll
         for (int c = TERMS - 1; c >= 0; --c) v += sums[(q * owned + row) * WIDTH + m * TERMS + c];
+    if (!isfinite(v)) v = sum_scaled(p, G, m0 + m, n);
     if (p.bias) v += p.bias[n];
     store_elem(p.out, static_cast<int64_t>(m0 + m) * p.N + n, p.out_dtype, p.silu_out ? silu(v) : v);
   }

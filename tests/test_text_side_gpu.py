@@ -660,3 +660,21 @@ def test_gemv_q4_zero_points(K, dtype, group):
     assert torch.isnan(got[:, rows]).all()
     rest = torch.ones(n, dtype=torch.bool, device="cuda").index_fill(0, rows, False)
     assert torch.equal(got[:, rest], good[:, rest])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("m, n, k", [(1, 130, 2560), (2, 300, 256), (20, 70, 1280)])
+def test_gemv_q4_rows_near_the_end_of_the_range(K, dtype, group, m, n, k):
+    """Unscaled group sums beyond fp32, finite results: weights of one sign and x of 2e36 to 8e36."""
+    w = normal(1, n, k).abs() * 1e-4
+    packed, scale, zero = K.pack_q4(w, group, False)
+    x = ((0.2 + 0.8 * torch.rand(m, k, device="cuda", generator=torch.Generator("cuda").manual_seed(m))) * 8e36).to(dtype)
+    if m > 1:
+        x[m // 2] *= 1e-36  # a row of ordinary size beside them
+    bias = normal(3, n)
+    got = K.gemv_q4(x, packed, scale, zero, bias, out_dtype=F32)
+    assert torch.isfinite(got).all()
+    assert_q4(got, x, packed, scale, zero, bias)
+    x[0, 5] = math.inf
+    assert not torch.isfinite(K.gemv_q4(x, packed, scale, zero, bias)[0]).any()  # inf, or NaN from a weight of 0
