@@ -1067,7 +1067,8 @@ extern "C" int iris_window_attn_fwd(const iris_window_problem* q, void* stream) 
   IRIS_REQUIRE(q != nullptr, "window_attn_fwd: null pointer");
   IRIS_CHECK_STATUS(check_sizes(*q));
   const float scale = static_cast<float>(q->scale);
-  IRIS_REQUIRE(scale > 0.f && scale < INFINITY, "window_attn_fwd: scale must be positive and finite");
+  // and so must its product with log2(e) be: 0 times infinity is NaN
+  IRIS_REQUIRE(scale > 0.f && scale * 1.4426950408889634f < INFINITY, "window_attn_fwd: scale must be positive and finite");
   IRIS_REQUIRE(rows_aligned(q->q) && rows_aligned(q->k) && rows_aligned(q->v) && aligned16(q->out) &&
                    q->out_stride_b % 8 == 0 && q->out_stride_n % 8 == 0,
                "window_attn_fwd: pointers and strides must be multiples of 16 bytes");

@@ -346,3 +346,15 @@ def test_pack_q4_of_a_parameter_keeps_no_graph(K, symmetric):
     for got, plain in zip(packed, K.pack_q4(w.detach(), 32, symmetric)):
         if got is not None:
             assert not got.requires_grad and got.grad_fn is None and torch.equal(got, plain)
+
+
+def test_scale_beyond_the_range_is_refused(lib):  # noqa: F811
+    """Scores are taken times scale log2(e): past fp32 a score of 0 would be NaN."""
+    def attend(scale):
+        heads = (16, 0, 0, 128)
+        return WINDOW.pack(*heads * 3, 16, 0, 0, 0, 0, 0, 0, 1, 1, 4, 2, 0, 5, 128, -1, 0, 0, scale), None  # no rows: nothing runs
+
+    for scale in (2.4e38, 3.4e38, 1e39, 1e-50):
+        assert "scale" in _einval(lib, "iris_window_attn_fwd", *attend(scale)), scale
+    for scale in (2.3e38, 1e-37):
+        assert lib.iris_window_attn_fwd(*attend(scale)) == 0
