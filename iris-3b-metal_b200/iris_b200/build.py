@@ -15,6 +15,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import warnings
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -83,18 +84,27 @@ def build_module(force: bool = False, verbose: bool = False) -> Path:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in includes),
            str(MODULE_SOURCE), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]  # fmt: skip
-    _run(cmd, MODULE, verbose)
+    try:
+        _run(cmd, MODULE, verbose)
+    except (RuntimeError, OSError):
+        MODULE.unlink(missing_ok=True)  # none of an older source is left
+        raise
     return MODULE
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    build_module(force, verbose)
-    if not force and up_to_date():
-        return LIBRARY
-    cmd = [nvcc(), *NVCC_FLAGS, f"-I{INCLUDE}", str(CSRC / "iris_b200.cu")]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    _run(cmd, LIBRARY, verbose)
+    """The library, then the module. The engine needs the library alone, so that a
+    host without Python's or torch's headers still builds it: it is warned, and the text
+    side's calls raise there."""
+    if force or not up_to_date():
+        cmd = [nvcc(), *NVCC_FLAGS, f"-I{INCLUDE}", str(CSRC / "iris_b200.cu")]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+        _run(cmd, LIBRARY, verbose)
+    try:
+        build_module(force, verbose)
+    except (RuntimeError, OSError) as e:
+        warnings.warn(f"{MODULE.name} is not built, the text side's calls will raise: {e}", stacklevel=2)
     return LIBRARY
 
 

@@ -106,3 +106,24 @@ def test_sources_name_no_cluster_multicast_loads():
     csrc = REPO / "iris-3b-metal_b200" / "csrc"
     for path in list(csrc.glob("*.cu")) + list(csrc.glob("*.cuh")) + list(csrc.glob("*.h")):
         assert "multicast" not in path.read_text(), path
+
+
+def test_the_library_is_built_without_the_module(monkeypatch, tmp_path):
+    """The engine's library does not wait for the text side's module, whose headers a host may lack; the module's
+    failure is seen, and none of an older source is left."""
+    from iris_b200 import build
+
+    built = []
+
+    def run(cmd, target, verbose):
+        built.append(target)
+        if target == build.MODULE:
+            raise RuntimeError("Python.h: No such file or directory")
+
+    (tmp_path / "_text_side.so").write_bytes(b"old")
+    monkeypatch.setattr(build, "MODULE", tmp_path / "_text_side.so")
+    monkeypatch.setattr(build, "LIBRARY", tmp_path / "libiris_b200.so")
+    monkeypatch.setattr(build, "_run", run)
+    with pytest.warns(UserWarning, match="Python.h"):
+        assert build.build(force=True) == build.LIBRARY
+    assert built == [build.LIBRARY, build.MODULE] and not build.MODULE.exists()
