@@ -9,10 +9,21 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import sysconfig
 from pathlib import Path
 
+import torch
+
 LIBRARY = Path(__file__).resolve().parent / "libiris_b200.so"
-TEXT_SIDE = LIBRARY.with_name("_text_side.so")
+
+
+def text_side_path() -> Path:
+    """The text side's module for this Python and torch, whose C++ types it is compiled
+    against: under another version it would load and misread them."""
+    return LIBRARY.with_name(f"_text_side.{sysconfig.get_config_var('SOABI')}-torch{torch.__version__}.so")
+
+
+TEXT_SIDE = text_side_path()
 
 IRIS_OK, IRIS_EINVAL, IRIS_ECUDA = 0, 1, 2
 F32, BF16, F16 = 0, 1, 2

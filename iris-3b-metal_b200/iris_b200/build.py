@@ -3,9 +3,10 @@
     python -m iris_b200.build            # from the iris-3b-metal_b200 directory
 
 The library is one translation unit (``csrc/iris_b200.cu``); the output lands
-next to this file so it travels with the source tree. So does ``_text_side.so``
+next to this file so it travels with the source tree. So does ``_text_side.*.so``
 (``csrc/text_side.cpp``), the CPython module through which the text side's per-token
-calls reach the library, built by the host compiler against torch's headers.
+calls reach the library, built by the host compiler against torch's headers; its name
+holds the Python and torch that it is for.
 """
 
 from __future__ import annotations
@@ -18,11 +19,13 @@ import sysconfig
 import warnings
 from pathlib import Path
 
+from iris_b200 import _lib
+
 PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE.parent / "csrc"
 INCLUDE = PACKAGE.parent.parent / "include"
 LIBRARY = PACKAGE / "libiris_b200.so"
-MODULE = PACKAGE / "_text_side.so"
+MODULE = _lib.TEXT_SIDE
 MODULE_SOURCE = CSRC / "text_side.cpp"
 
 NVCC_FLAGS = [

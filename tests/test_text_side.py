@@ -358,3 +358,21 @@ def test_scale_beyond_the_range_is_refused(lib):  # noqa: F811
         assert "scale" in _einval(lib, "iris_window_attn_fwd", *attend(scale)), scale
     for scale in (2.3e38, 1e-37):
         assert lib.iris_window_attn_fwd(*attend(scale)) == 0
+
+
+def test_the_module_is_for_one_python_and_torch(lib, monkeypatch):  # noqa: F811
+    """Compiled against torch's and CPython's own types: another version does not load it, and builds its own."""
+    from iris_b200 import _lib, build
+
+    assert build.MODULE == _lib.TEXT_SIDE == _lib.text_side_path() and _lib.TEXT_SIDE.exists()
+    for target, name, value in [(torch, "__version__", "9.9.0"), (_lib.sysconfig, "get_config_var", lambda name: "cpython-399")]:
+        with monkeypatch.context() as m:
+            m.setattr(target, name, value)
+            other = _lib.text_side_path()
+            assert other != _lib.TEXT_SIDE and not other.exists()
+            m.setattr(build, "MODULE", other)
+            assert not build.module_up_to_date()
+            m.setattr(_lib, "TEXT_SIDE", other)
+            m.setattr(_lib, "_text_side", None)
+            with pytest.raises(RuntimeError, match="not built"):
+                _lib.text_side()
