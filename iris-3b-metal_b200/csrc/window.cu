@@ -70,7 +70,9 @@ IRIS_DEVICE uint32_t pack2<__half>(float a, float b) { return pack_f16x2(a, b); 
 
 // One output row by one warp, keys 32 at a time (a lane scores one), from global
 // memory: columns [64 c + 2 lane, + 2) of chunk c < D / 64. Only visible keys are
-// read, so what lies in masked places cannot reach the row.
+// read, so what lies in masked places cannot reach the row. The row is kept as the
+// mean so far, for sums over values near the end of bf16's range would leave fp32, where
+// the result does not.
 template <typename T, int D>
 __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, float2 (&acc)[D / 64]) {
   const int lane = threadIdx.x & 31;
@@ -79,6 +81,8 @@ __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, fl
   const T* k = reinterpret_cast<const T*>(p.k) + b * p.kb + hk * p.kh;
   const T* v = reinterpret_cast<const T*>(p.v) + b * p.vb + hk * p.vh;
   const Span s = visible(p, sample_start(p, b) + i, sample_length(p, b));
+  // f16 products stay far below fp32's end, bf16's only once they are scaled
+  const float first = IsHalf<T>::value ? 1.f : p.scale_log2, then = IsHalf<T>::value ? p.scale_log2 : 1.f;
   float m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
@@ -94,22 +98,24 @@ __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, fl
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const float2 f = unpack2<T>(x[u]), g = unpack2<T>(y[u]);
-          dot = fmaf(f.x, g.x, fmaf(f.y, g.y, dot));
+          dot = fmaf(f.x * first, g.x, fmaf(f.y * first, g.y, dot));
         }
       }
     }
-    const float score = real ? dot * p.scale_log2 : -INFINITY;
+    const float score = real ? dot * then : -INFINITY;
     float top = score;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float m_new = fmaxf(m, top);
     const float base = m_new == -INFINITY ? 0.f : m_new;  // nothing above -inf so far: every weight 0
-    const float w = real ? exp2f(score - base) : 0.f;
-    const float corr = m == -INFINITY ? 0.f : exp2f(m - base);
-    l = l * corr + warp_sum(w);
+    float w = real ? exp2f(score - base) : 0.f;
+    const float before = m == -INFINITY ? 0.f : l * exp2f(m - base);
+    l = before + warp_sum(w);
     m = m_new;
+    const float inv = l == 0.f ? 0.f : 1.f / l, keep = before * inv;
+    w *= inv;
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(acc[c].x * corr, acc[c].y * corr);
+    for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(acc[c].x * keep, acc[c].y * keep);
     const int keys = min(32, count - c0);
     for (int j = 0; j < keys; ++j) {
       const float wj = __shfl_sync(0xffffffffu, w, j);
@@ -122,10 +128,9 @@ __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, fl
     }
   }
   // every visible score -inf: 0 / 0, as softmax has it
-  const float inv = count == 0 ? 0.f : 1.f / l;
 #pragma unroll
   for (int c = 0; c < D / 64; ++c)
-    acc[c] = count == 0 ? make_float2(0.f, 0.f) : l == 0.f ? make_float2(NAN, NAN) : make_float2(acc[c].x * inv, acc[c].y * inv);
+    acc[c] = count == 0 ? make_float2(0.f, 0.f) : l == 0.f ? make_float2(NAN, NAN) : acc[c];
 }
 
 // ------------------------------------------------------------- tensor cores

@@ -678,3 +678,25 @@ def test_gemv_q4_rows_near_the_end_of_the_range(K, dtype, group, m, n, k):
     assert_q4(got, x, packed, scale, zero, bias)
     x[0, 5] = math.inf
     assert not torch.isfinite(K.gemv_q4(x, packed, scale, zero, bias)[0]).any()  # inf, or NaN from a weight of 0
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("n, n_kv, heads, kv", [(1, 40, 2, 1), (1, 700, 20, 5), (1, 20000, 8, 1), (3, 90, 4, 4), (300, 300, 4, 2)])
+def test_values_near_the_end_of_the_range(K, dim, n, n_kv, heads, kv):
+    """Values of 1e38 to 3e38: their weighted sum leaves fp32, their mean does not; and scores whose unscaled sums do."""
+    gen = torch.Generator("cuda").manual_seed(n_kv)
+    q, k = normal(1, 1, heads, n, dim, dtype=BF16), normal(2, 1, kv, n_kv, dim, dtype=BF16)
+    v = ((1 + 2 * torch.rand(1, kv, n_kv, dim, device="cuda", generator=gen)) * 1e38).to(BF16)
+    v[..., ::3] *= -1e-38  # ordinary values beside them
+    for left in (None, 30):
+        got = K.window_attention(q, k, v, left=left)
+        assert torch.isfinite(got).all()
+        assert_attends(got, q, k, v, left=left)
+    big = torch.full_like(q, 2.0**62)
+    k = torch.where(torch.arange(n_kv, device="cuda")[:, None] % 7 == 0, 2.0**62, -(2.0**62)).to(BF16).expand(1, kv, n_kv, dim).contiguous()
+    v = normal(3, 1, kv, n_kv, dim, dtype=BF16)
+    # scores of +- dim 2^124 (2^130 or 2^131 unscaled): the keys of the larger one share the row
+    got = K.window_attention(big, k, v, right=None, scale=2.0**-10)
+    mean = v[:, :, ::7].double().mean(dim=2, keepdim=True).repeat_interleave(heads // kv, dim=1).expand(1, heads, n, dim)
+    off = (got.double().view(1, n, heads, dim).transpose(1, 2) - mean).abs()
+    assert torch.all(off <= 2.0**-8 * mean.abs() + (n_kv + 8) * 2.0**-23 * v.double().abs().amax())
