@@ -598,7 +598,8 @@ def window_attention(
     returns ``[B, N, H * D]`` (``out``, or a new tensor).
 
     Query ``i`` of sample ``b`` is at position ``p = starts[b] + i`` (int32 ``[B]``;
-    default ``N_kv - N + i``) and sees the keys ``j < lengths[b]`` (int32 ``[B]``, clamped
+    default ``N_kv - N + i``, ``lengths`` or not: a chunk over a partly filled cache needs
+    its starts) and sees the keys ``j < lengths[b]`` (int32 ``[B]``, clamped
     to ``[0, N_kv]``; default ``N_kv``) with ``j <= p + right`` and ``j >= p - left`` or ``j <
     sinks``; ``None`` is no bound, the default is causal. A query that sees no key
     gives 0. Other keys' rows may hold anything. Heads and samples may be expanded,

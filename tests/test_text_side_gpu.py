@@ -700,3 +700,58 @@ def test_values_near_the_end_of_the_range(K, dim, n, n_kv, heads, kv):
     mean = v[:, :, ::7].double().mean(dim=2, keepdim=True).repeat_interleave(heads // kv, dim=1).expand(1, heads, n, dim)
     off = (got.double().view(1, n, heads, dim).transpose(1, 2) - mean).abs()
     assert torch.all(off <= 2.0**-8 * mean.abs() + (n_kv + 8) * 2.0**-23 * v.double().abs().amax())
+
+
+@pytest.mark.parametrize("n, n_kv", [(1, 60), (5, 60), (40, 2000), (200, 500), (10, 4), (300, 100)])
+def test_positions_by_default_count_from_the_last_key(K, n, n_kv):
+    """Without `starts` the last query is at the last key, whatever `lengths` say: a chunk over a partly filled cache needs
+    its starts. With more queries than keys the first ones see nothing."""
+    q = normal(1, 3, 4, n, 64, dtype=BF16)
+    k, v = normal(2, 3, 2, n_kv, 64, dtype=BF16), normal(3, 3, 2, n_kv, 64, dtype=BF16)
+    lengths = int32([n_kv, max(1, n_kv // 2), max(0, n_kv - 3)])
+    for left, right in [(None, 0), (20, 0), (20, 3), (None, None)]:
+        got = K.window_attention(q, k, v, left=left, right=right, lengths=lengths)
+        assert_attends(got, q, k, v, left=left, right=right, lengths=lengths)
+        assert torch.equal(got, K.window_attention(q, k, v, left=left, right=right, lengths=lengths, starts=int32([n_kv - n] * 3)))
+        if n > n_kv and right == 0:
+            assert torch.all(got[:, : n - n_kv] == 0)
+
+
+def test_captured_with_streams_that_fork_and_join(K):
+    """Calls that each wait for two others, on several streams inside one capture; the predecessors of a call in its
+    stream are a kernel, a copy and a fill in turn."""
+    w = K.pack_q4(normal(7, 12 * 128, 256), 64)
+    out = K.pack_q4(normal(8, 200, 1024), 128)
+    cos, sin = table(128, 4000)
+    x, caches = normal(1, 2, 256, dtype=BF16), normal(2, 2, 2, 2, 1500, 128, dtype=BF16)
+    starts, lengths, room = int32([3000, 700]), int32([3001, 701]), torch.empty(2, 256, device="cuda", dtype=BF16)
+
+    def step(x, caches, side):
+        main = torch.cuda.current_stream()
+        room.copy_(x)
+        heads = K.gemv_q4(room, *w).view(2, 1, 12, 128).transpose(1, 2)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            turned = K.rope(heads[:, :8], cos, sin, starts[:, None].contiguous())
+        q = K.rope_append(heads[:, :8], heads[:, 8:10], heads[:, 10:], cos, sin, starts, caches[0], caches[1], sinks=4)
+        main.wait_stream(side)
+        o = K.window_attention(q, caches[0], caches[1], right=None, lengths=lengths)
+        o = o + K.window_attention(turned, caches[0], caches[1], right=None, lengths=lengths)
+        room.zero_()
+        return K.gemv_q4(o.view(2, -1), *out), q, turned
+
+    side = torch.cuda.Stream()
+    expected = step(x, caches.clone(), side)
+    assert torch.equal(expected[1], expected[2])
+    held = caches.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(x, held, side)
+    for _ in range(5):
+        held.copy_(caches)
+        for t in got:
+            t.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, expected))
