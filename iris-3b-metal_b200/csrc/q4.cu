@@ -351,6 +351,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(COLS8)) gemv_q4_kernel(co
   int at_slot = 0;  // the step's slot and its phase
   uint32_t phase = 0;
   uint32_t now[2 * TILES][HELD];
+  uint32_t zeros_seen = 0;
 #pragma unroll 1
   for (int t = 0; t < steps; ++t) {
     if (chunk_t == chunk_steps) {  // uniform over the CTA
@@ -363,10 +364,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(COLS8)) gemv_q4_kernel(co
 #pragma unroll
       for (int r = 0; r < 2 * TILES; ++r)
 #pragma unroll
-        for (int h = 0; h < HELD; ++h) {  // scale, 16 zero, zero; a zero point of more than 4 bits makes its row NaN
-          const bool fits = sz_zero[r][h] < 16u;
-          now[r][h] = fits ? static_cast<uint32_t>(sz_scale[r][h]) << 16 | sz_zero[r][h] * 0x1001u : 0x7fc00000u;
-          if (!fits) atomicOr(&g_device_error, kErrBadArgument);
+        for (int h = 0; h < HELD; ++h) {  // scale, 16 zero, zero
+          now[r][h] = static_cast<uint32_t>(sz_scale[r][h]) << 16 | sz_zero[r][h] * 0x1001u;
+          zeros_seen |= sz_zero[r][h];
         }
       fetch();
     }
@@ -462,6 +462,20 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(COLS8)) gemv_q4_kernel(co
       for (int c = 0; c < COLS8; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) total[r][c][e] = __int_as_float(0x7fc00000);
+  }
+  if (__any_sync(0xffffffffu, zeros_seen > 15u)) {  // a zero point of more than 4 bits: its weight row is NaN
+    const int from = k0 / G, groups_here = k1 / G - from;
+#pragma unroll
+    for (int r = 0; r < 2 * TILES; ++r) {
+      bool bad = false;
+      for (int i = quad; r < real_rows && i < groups_here; i += 4)
+        bad = bad || p.zero[static_cast<int64_t>(n0 + row_g + 8 * r) * groups + from + i] > 15;
+      const unsigned row_bad = __ballot_sync(0xffffffffu, bad) >> (lane & ~3) & 0xfu;  // the row's four lanes
+      if (row_bad == 0u) continue;
+      if (quad == 0) atomicOr(&g_device_error, kErrBadArgument);
+#pragma unroll
+      for (int c = 0; c < COLS8; ++c) total[r / 2][c][r % 2 * 2] = total[r / 2][c][r % 2 * 2 + 1] = __int_as_float(0x7fc00000);
+    }
   }
   if (p.parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the cluster's CTAs have begun
   // sums [part][row][COLS8 * 8] of the rows that a CTA owns, 128 / parts of them
