@@ -5,7 +5,8 @@
 // HBM-bound on N K / 2 bytes of weights, as long as few instructions are spent per
 // weight: the products run on mma.sync m16n8k16 with the weights as the 16-row
 // operand and x's rows as its 8 columns, so that a weight costs its unpacking alone
-// (and / or, subtract, half an instruction each) whatever M is.
+// (and / or, subtract, half an instruction each), once for up to 32 rows of 16 bits or 16
+// of fp32. More rows are passes of those, and each reads and unpacks every weight again.
 //  - q - zero is exact in the operand type: q is put into the mantissa of 128 (bf16)
 //    or 1024 (f16) and 128 + zero or 1024 + zero subtracted. Scales are applied in
 //    fp32 to each group's fp32 sum, so weights are never rounded.
@@ -15,7 +16,8 @@
 //    weight row split a group's words, so that every product of an mma has one scale.
 //  - x in 16 bits goes in as it is. FP32 (and act_in's results) go in as three bf16
 //    columns, 8 bits each of the 24, cut off rather than rounded: their sum is x, and
-//    the columns are free up to 8 of them.
+//    the columns are free up to 8 of them. (To 2^-133, bf16's last bit: rows that lie
+//    below 1e-33 throughout keep fewer than 24 bits.)
 // A CTA owns 128 weight rows, 32 a warp, and, in a cluster, one part of K, whose x it
 // lays out once for all of them; a warp streams 256-wide pieces of its rows through
 // its own ring of TMA copies (one instruction for 32 rows; filled before x is laid
@@ -23,12 +25,12 @@
 // row (no CTA waits on another's memory: reading the sums from there instead took 2 to
 // 4 us of a call's 12 to 21), which adds them in a fixed order.
 //
-// Measured: 8192 -> 32768, groups of 128, one bf16 row 40 us (3.4 TB/s, 0.53 of a plain
-// copy). The unpacking (7 and / shift operations a word at half rate, 3 more per mma)
+// Measured: 8192 -> 32768, groups of 128, one bf16 row 41 us (3.4 TB/s, 0.52 of a plain
+// copy), 8 rows 61, 16 rows 87, 32 rows 139, 64 rows (two passes) 278. The unpacking (7 and / shift operations a word at half rate, 3 more per mma)
 // alone takes about 19 us, the copies alone 25, the start (launch, cluster, first
-// copies, x) 5; they overlap in part. 2560 -> 15360, groups of 64, one fp32 row 12.5 us
-// (1.7 TB/s); 6848 -> 2561, groups of 32 with zeros, 16 f16 rows 16.0 us: an SM has four
-// warps or eight, each a chain of shared memory -> unpacking -> mma -> scale. Deeper rings,
+// copies, x) 5; they overlap in part. 2560 -> 15360, groups of 64, one fp32 row 12.7 us
+// (1.7 TB/s), 8 rows 21, 16 rows 42, 64 rows (four passes) 149; 6848 -> 2561, groups of
+// 32 with zeros, 16 f16 rows 16.1 us: an SM has four warps or eight, each a chain of shared memory -> unpacking -> mma -> scale. Deeper rings,
 // scales prefetched into L2, two accumulators a sum: no gain; eight warps of 16 rows in place
 // of four 15.0 us there, but 7.6 instead of 6.8 for 2560 -> 2560, one row; three CTAs an
 // SM for one row instead of four 47.7 us; twice the parts 43.9 us, 18.5 the 2560 -> 15360.
@@ -67,6 +69,8 @@ struct Params {
   int stages;     // ring slots of a warp
 };
 
+// With the fast exponential, as iris_gemv has it: its relative error is |v| 2^-24 for
+// negative v, 2^-18 at -64 where silu is -1e-26.
 IRIS_DEVICE float silu(float v) { return v / (1.f + __expf(-v)); }
 
 // (v & mask) | bits in one instruction

@@ -139,7 +139,7 @@ __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, fl
 // of the first `sinks` keys, then the window's), two CTAs to an SM. Warp 0 brings Q once
 // and K and V through two-slot rings by TMA; warp 1 issues the MMAs; warps 2 to 5 do
 // the softmax, a thread per row (TMEM lane), its 64 scores in registers: no exchange
-// between threads. Exponentials (4096 a quarter and block at 4 a clock) take as long as
+// between threads. Exponentials (2048 a quarter and block at 4 a clock) take as long as
 // the MMAs, so what costs is waiting: S alternates between two buffers and runs a block
 // ahead of P V, so that a block's scores are there when the softmax of the one before
 // ends, and the other CTA fills what waits are left (its start and its epilogue too).
@@ -152,12 +152,12 @@ __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, fl
 // which reads visible keys alone (also rows that see no key: 0 / 0 here).
 //
 // Measured, 128 wide, FLOP of visible pairs: 16384 tokens, 20 over 5 heads, window 1024
-// 204 us (0.82 PFLOP/s; 238 inside long runs under the power cap), 2 x 4352 f16 rows of
-// 24 heads, 512 to each side 151 us (0.84); 8192 tokens 1.0 unmasked, 1.12 causal. Tensor
+// 205 us (0.82 PFLOP/s; 239 inside long runs under the power cap), 2 x 4352 f16 rows of
+// 24 heads, 512 to each side 154 us (0.82; 180 in long runs); 8192 tokens 1.0 unmasked, 1.12 causal. Tensor
 // pipe and exponentials 45% busy each: a block takes a warp about 1730 cycles, 870 of them
 // weights, 320 the wait for S. Two row tiles a CTA 281 us, one tile with 128-key blocks
 // 262, eight softmax warps 465 (registers spill), a part of the exponentials as
-// polynomials 213 to 219, against 204.
+// polynomials 213 to 219, against 204 on that box.
 constexpr int BQ = 128, BKV = 64, KV = 2;  // rows, keys of a block, slots of the K and V rings
 constexpr int TILE_THREADS = 192;
 constexpr int Q_HALF = BQ * 128, KV_HALF = BKV * 128;  // bytes of 64 columns of a tile
@@ -429,8 +429,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 2)
         }
       }
       m_run = m_new;
-      // weights 2^(s * scale - m), rounded once to the operand type of the P V product
-      // (their fp32 values go into the sum); masked keys give exact zeros
+      // weights 2^(s * scale - m), rounded once to the operand type of the P V product:
+      // the tensor cores take 16 bits, and the remainders would be a second product beside
+      // two that already share the pipe. The rounding is relative to each weight and
+      // averages out over the keys (bf16 rows 0.0020-0.0023 off the 64-bit ones, 0.0016 with
+      // fp32 weights); the sum takes the fp32 values. Masked keys give exact zeros
       const float shift = m_new == -INFINITY ? 0.f : -m_new;
       const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(shift, shift);
       float2 sum2 = make_float2(0.f, 0.f);
@@ -748,7 +751,8 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
       l_run[0] *= corr[0];
       l_run[1] *= corr[1];
     }
-    // weights, rounded once to the operand type (the fp32 values go into the totals)
+    // weights, rounded once to the operand type (the fp32 values go into the totals): as in
+    // tiles_kernel, so that a row is as accurate in either form
     uint32_t pa[4];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
