@@ -157,7 +157,7 @@ __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, fl
 // pipe and exponentials 45% busy each: a block takes a warp about 1730 cycles, 870 of them
 // weights, 320 the wait for S. Two row tiles a CTA 281 us, one tile with 128-key blocks
 // 262, eight softmax warps 465 (registers spill), a part of the exponentials as
-// polynomials 213 to 219, against 204 on that box.
+// polynomials 213 to 219, against 204 in the same runs.
 constexpr int BQ = 128, BKV = 64, KV = 2;  // rows, keys of a block, slots of the K and V rings
 constexpr int TILE_THREADS = 192;
 constexpr int Q_HALF = BQ * 128, KV_HALF = BKV * 128;  // bytes of 64 columns of a tile
