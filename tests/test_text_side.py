@@ -272,7 +272,7 @@ def test_outputs_that_would_race_are_refused(K):
 
     refused("CUDA", K.rope, x, cos, sin, out=x)  # in place is allowed: it gets as far as the device
     refused("CUDA", K.rope, x, cos, sin, out=x.view(2, 4, 3, 64))
-    refused("CUDA", K.rope, x, cos, sin, out=buf[1536:3072].view(2, 4, 3, 64))
+    refused("CUDA", K.rope, x, cos, sin, out=buf[2048:3584].view(2, 4, 3, 64))
     refused("x itself", K.rope, x, cos, sin, out=buf[64:1600].view(2, 4, 3, 64))
     refused("x itself", K.rope, x, cos, sin, out=buf[:1536].view(2, 3, 4, 64).transpose(1, 2))
     refused("CUDA", K.rope, buf[:0].view(2, 4, 0, 64), cos, sin, out=buf[:0].view(2, 4, 0, 64))
