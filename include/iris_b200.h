@@ -37,6 +37,7 @@ extern "C" {
 #define IRIS_F32 0
 #define IRIS_BF16 1
 #define IRIS_F16 2
+#define IRIS_I8 3 /* rows that iris_quantize_i8 wrote (iris_gemm_i8 alone) */
 
 /* GEMM epilogues */
 #define IRIS_EPI_STORE 0  /* out = acc (+ bias)                        */
@@ -441,6 +442,40 @@ typedef struct iris_q4_problem {
   int64_t M, K, N, ldx, group, x_dtype, out_dtype, silu_in, silu_out;
 } iris_q4_problem;
 int iris_gemv_q4(const iris_q4_problem* problem, void* stream);
+
+/* Rows to 8 bits with a scale each: top = max_k |x[m, k]|, scale[m] = top / 127 (fp32),
+ * q[m, k] = the whole number nearest 127 x[m, k] / top, halves to even, of the exact
+ * quotient. A row of zeros has scale 0; one that holds an infinity or NaN has scale
+ * NaN and zeros. x fp32, bf16 or f16 with row stride ldx (elements), 1 <= K <= 131071;
+ * q int8 with row stride ldq, a multiple of 8 (of 16 where iris_gemm_i8 reads it). */
+typedef struct iris_quantize_problem {
+  const void* x;
+  void* q;
+  float* scale;
+  int64_t M, K, ldx, ldq, x_dtype;
+} iris_quantize_problem;
+int iris_quantize_i8(const iris_quantize_problem* problem, void* stream);
+
+/* The linear over 8-bit weights with a scale for each token and channel:
+ * out[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] + bias[n], the sum exact in
+ * int32 (1 <= K <= 131071), out [M, N] contiguous in out_dtype. w int8 [N, K] (iris_quantize_i8
+ * of the weights' rows), row stride ldw; 8-bit x (x_dtype IRIS_I8) with x_scale: 16-byte
+ * aligned rows, as w's (the stride of a single row is not read). x in IRIS_F32, IRIS_BF16 or
+ * IRIS_F16 (x_scale unused) is quantised first, into workspace (iris_gemm_i8_workspace bytes,
+ * 16-byte aligned; calls that may run at the same time need one each). bias fp32 or null. */
+typedef struct iris_i8_problem {
+  const void* x;
+  const float* x_scale;
+  const void* w;
+  const float* w_scale;
+  const float* bias;
+  void* out;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t M, N, K, ldx, ldw, x_dtype, out_dtype;
+} iris_i8_problem;
+int iris_gemm_i8(const iris_i8_problem* problem, void* stream);
+int iris_gemm_i8_workspace(const iris_i8_problem* problem, int64_t* bytes);
 
 /* Per-block modulation rows, SharedCoreBias.forward (src/iris3b/nn/modulation.py:284-285):
  * out[j, b, :] = core[b, :] + bias[j, :] for j < n_blocks. */

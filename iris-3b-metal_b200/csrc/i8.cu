@@ -1,0 +1,526 @@
+// Linear over 8-bit weights with a scale for each token and channel:
+//   x_scale[m] = max_k |x[m, k]| / 127,   q[m, k] = the whole number nearest 127 x[m, k] / max_k |x[m, k]|
+//   out[m, n] = x_scale[m] w_scale[n] sum_k q[m, k] w[n, k] + bias[n]
+// The sum is of whole numbers and exact in int32 (K <= 131071: 128 * 128 * K < 2^31),
+// so how K is split changes nothing.
+#include <algorithm>
+
+#include "common.cuh"
+#include "iris_abi_internal.h"
+
+namespace iris {
+namespace i8 {
+
+// ------------------------------------------------------------------ rows to 8 bits
+// HBM-bound: one read of x, one byte written per value. A team of warps takes a row and
+// keeps it in registers between the maximum and the rounding (what does not fit is read again).
+//
+// q is the correctly rounded quotient, halves to even: y = x (127 / max) is off by at
+// most 127 (2^-24 + 2^-24) < 2^-16, so y's nearest whole number is the quotient's
+// unless y is within 2^-15 of a half; such a value (one of 2^14) is divided in 64 bits,
+// where 127 x is exact and a quotient of two 24-bit numbers that is no half stays 2^-26
+// of itself away from one. So the 8-bit values are the formula's, whatever order or unit computes them.
+struct QuantizeParams {
+  const void* x;
+  int8_t* q;
+  float* scale;
+  int64_t ldx, ldq;
+  int M, K;
+};
+
+template <typename T>
+struct Vec {  // values of a 16-byte vector
+  static constexpr int N = 16 / sizeof(T);
+};
+
+template <typename T>
+IRIS_DEVICE float value_of(const uint4& v, int e);
+template <>
+IRIS_DEVICE float value_of<float>(const uint4& v, int e) {
+  return __uint_as_float(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w);
+}
+template <>
+IRIS_DEVICE float value_of<__nv_bfloat16>(const uint4& v, int e) {
+  const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
+  return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+}
+template <>
+IRIS_DEVICE float value_of<__half>(const uint4& v, int e) {
+  const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return e & 1 ? f.y : f.x;
+}
+
+// Largest magnitude of a vector as the bits of its type: they order like magnitudes,
+// infinities and NaN above all others.
+template <typename T>
+IRIS_DEVICE uint32_t top_of(const uint4& v, uint32_t top) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    top = sizeof(T) == 4 ? max(top, w[i] & 0x7fffffffu) : __vmaxu2(top, w[i] & 0x7fff7fffu);
+  return top;
+}
+
+template <typename T, bool ALIGNED>
+IRIS_DEVICE uint4 load_vec(const T* row, int v, int K) {
+  constexpr int N = Vec<T>::N;
+  if (ALIGNED && (v + 1) * N <= K) return *reinterpret_cast<const uint4*>(row + v * N);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const int k = v * N + e;
+    if (k >= K) continue;
+    if (sizeof(T) == 4) w[e % 4] = reinterpret_cast<const uint32_t*>(row)[k];
+    else w[e / 2 % 4] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[k]) << (16 * (e & 1));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+IRIS_DEVICE void store_vec(int8_t* out, const uint4& v, int at, int K, float inv, float top, bool slow) {
+  constexpr int N = Vec<T>::N;
+  uint32_t packed[2] = {0u, 0u};
+  float worst = 0.f;
+  constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: the sum's last bit is 1
+#pragma unroll
+  for (int g = 0; g < N / 4; ++g) {
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = value_of<T>(v, 4 * g + e);
+      const float t = fmaf(x, inv, kWhole);
+      worst = fmaxf(worst, fabsf(fmaf(x, inv, -(t - kWhole))));
+      b[e] = __float_as_uint(t);
+    }
+    packed[g] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  }
+  if (slow || worst > 0.5f - 1.f / 32768) {
+#pragma unroll 1
+    for (int e = 0; e < N; ++e) {
+      const float x = value_of<T>(v, e);
+      const int q = top == 0.f ? 0 : __double2int_rn(127.0 * x / static_cast<double>(top));
+      packed[e >> 2] = (packed[e >> 2] & ~(0xffu << (8 * (e & 3)))) | (static_cast<uint32_t>(q) & 0xffu) << (8 * (e & 3));
+    }
+  }
+  if ((at + 1) * N <= K) {
+    if (N == 8) *reinterpret_cast<uint2*>(out + at * N) = make_uint2(packed[0], packed[1]);
+    else *reinterpret_cast<uint32_t*>(out + at * N) = packed[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (at * N + e < K) out[at * N + e] = static_cast<int8_t>(packed[e >> 2] >> (8 * (e & 3)) & 0xffu);
+  }
+}
+
+constexpr int KEPT = 4;  // vectors of a row that a thread keeps
+
+template <typename T, int WARPS, bool ALIGNED>
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) quantize_kernel(const QuantizeParams p) {
+  constexpr int TEAM = WARPS * 32, N = Vec<T>::N;
+  __shared__ uint32_t tops[WARPS];
+  grid_wait();
+  grid_trigger();
+  const int t = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int m = WARPS == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (m >= p.M) return;  // a warp of its own team
+  const T* row = reinterpret_cast<const T*>(p.x) + m * p.ldx;
+  const int vecs = (p.K + N - 1) / N;
+  uint4 kept[KEPT];
+#pragma unroll
+  for (int i = 0; i < KEPT; ++i) {
+    const int v = t + i * TEAM;
+    kept[i] = v < vecs ? load_vec<T, ALIGNED>(row, v, p.K) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  uint32_t top = 0u;
+#pragma unroll
+  for (int i = 0; i < KEPT; ++i) top = top_of<T>(kept[i], top);
+  for (int v = t + KEPT * TEAM; v < vecs; v += TEAM) top = top_of<T>(load_vec<T, ALIGNED>(row, v, p.K), top);
+  if (sizeof(T) == 2) top = max(top & 0xffffu, top >> 16);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (WARPS > 1) {
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = max(top, tops[w]);
+  }
+  uint4 bits = make_uint4(top, 0u, 0u, 0u);
+  float size = value_of<T>(bits, 0);
+  const bool finite = size < INFINITY;  // not so for NaN
+  if (t == 0) p.scale[m] = finite ? __fdiv_rn(size, 127.f) : NAN;
+  if (!finite) size = 0.f;
+  // below 2^-100 the reciprocal leaves fp32 or 127 x loses bits; 0 has none
+  const bool slow = size < 7.9e-31f;
+  const float inv = slow ? 0.f : __fdiv_rn(127.f, size);
+  int8_t* out = p.q + m * p.ldq;
+  auto store = [&](const uint4& v, int at) {
+    if (finite) store_vec<T>(out, v, at, p.K, inv, size, slow);
+    else store_vec<T>(out, make_uint4(0u, 0u, 0u, 0u), at, p.K, 0.f, 0.f, false);
+  };
+#pragma unroll
+  for (int i = 0; i < KEPT; ++i)
+    if (t + i * TEAM < vecs) store(kept[i], t + i * TEAM);
+  for (int v = t + KEPT * TEAM; v < vecs; v += TEAM) store(load_vec<T, ALIGNED>(row, v, p.K), v);
+}
+
+template <typename T, bool ALIGNED>
+int launch_quantize(const QuantizeParams& p, cudaStream_t st) {
+  const int vecs = (p.K + Vec<T>::N - 1) / Vec<T>::N;
+  const unsigned rows = static_cast<unsigned>(p.M);
+  // the smallest team that keeps a row
+  if (vecs <= KEPT * 32)
+    IRIS_CUDA(launch_early(quantize_kernel<T, 1, ALIGNED>, dim3((rows + 3) / 4), 128, 0, st, 1, p));
+  else if (vecs <= KEPT * 128)
+    IRIS_CUDA(launch_early(quantize_kernel<T, 4, ALIGNED>, dim3(rows), 128, 0, st, 1, p));
+  else
+    IRIS_CUDA(launch_early(quantize_kernel<T, 8, ALIGNED>, dim3(rows), 256, 0, st, 1, p));
+  return IRIS_OK;
+}
+
+template <typename T>
+int quantize(const QuantizeParams& p, cudaStream_t st) {
+  const bool aligned = aligned16(p.x) && p.ldx * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+  return aligned ? launch_quantize<T, true>(p, st) : launch_quantize<T, false>(p, st);
+}
+
+// ------------------------------------------------------------------- the product
+// A tile is 128 weight rows (TMEM lanes) by T tokens (columns): the weights are the
+// tensor cores' first operand, whatever the number of tokens, so that few tokens waste
+// none of it and the lanes of a warp write neighbouring channels of out, at any N.
+constexpr int BN = 128, SLAB = 128;  // weight rows of a CTA, k of a ring slot (bytes)
+constexpr int THREADS = 192;
+
+struct Params {
+  const float* x_scale;
+  const float* w_scale;
+  const float* bias;
+  void* out;
+  int M, N, K, out_dtype;
+  int splits;         // parts of K, the CTAs of a cluster
+  int token_tiles;
+  int early;          // the weights are there before the kernel's predecessor ends
+};
+
+__host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
+  return (2u << 4)                                // D format: S32
+         | (1u << 7)                              // A format: signed 8-bit
+         | (1u << 10)                             // B format: signed 8-bit
+         | (static_cast<uint32_t>(n >> 3) << 17)  // N / 8
+         | (static_cast<uint32_t>(m >> 4) << 24); // M / 16
+}
+IRIS_DEVICE void umma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// sum * x_scale * w_scale: the smaller scale first, so that no step leaves fp32 where
+// the product does not. A NaN scale stays.
+IRIS_DEVICE float scaled(int sum, float xs, float ws, float bias) {
+  const bool less = fabsf(xs) < fabsf(ws);
+  return fmaf(static_cast<float>(sum) * (less ? xs : ws), less ? ws : xs, bias);
+}
+IRIS_DEVICE void store_out(const Params& p, int64_t at, float y) { store_elem(p.out, at, p.out_dtype, y); }
+
+template <int T>
+struct Rows {
+  static constexpr int X_BYTES = T * SLAB, W_BYTES = BN * SLAB, STAGE = X_BYTES + W_BYTES;
+  static constexpr int STAGES = T == 16 ? 6 : T == 32 ? 5 : T == 64 ? 4 : 3;
+  static constexpr int COLS = T < 32 ? 32 : T;
+  static constexpr int RING = STAGES * STAGE;
+  static constexpr int SMEM = 1024 + RING + 256;
+  static_assert(T * BN * 4 <= RING, "the parts of a tile lie in the ring");
+};
+
+template <int T>
+struct RowsSmem {
+  uint64_t full[Rows<T>::STAGES], empty[Rows<T>::STAGES], done;
+  uint32_t tmem_base;
+  int abort, bad[8];
+};
+
+template <int T>
+__global__ void __launch_bounds__(THREADS, 2)
+    rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
+                const __grid_constant__ Params p) {
+  using R = Rows<T>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  RowsSmem<T>* s = reinterpret_cast<RowsSmem<T>*>(ring + R::RING);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int part = static_cast<int>(blockIdx.x % p.splits), unit = static_cast<int>(blockIdx.x / p.splits);
+  const int m0 = unit % p.token_tiles * T, n0 = unit / p.token_tiles * BN;
+  const int slabs = (p.K + SLAB - 1) / SLAB;
+  const int first = static_cast<int>(static_cast<int64_t>(slabs) * part / p.splits);
+  const int count = static_cast<int>(static_cast<int64_t>(slabs) * (part + 1) / p.splits) - first;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < R::STAGES; ++i) {
+      mbar_init(&s->full[i], 1);
+      mbar_init(&s->empty[i], 1);
+    }
+    mbar_init(&s->done, 1);
+    s->abort = 0;
+    for (int i = 0; i < 8; ++i) s->bad[i] = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tw);
+    tma_prefetch_desc(&tx);
+  }
+  if (warp == 1) tmem_alloc(&s->tmem_base, R::COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s->tmem_base;
+  volatile int* abort = &s->abort;
+
+  if (warp == 0) {
+    // ----------------------------------------------------------------- TMA
+    if (lane == 0) {
+      const int ahead = p.early ? min(count, R::STAGES) : 0;
+      auto load_w = [&](int i) {
+        const int st = i % R::STAGES;
+        mbar_arrive_expect_tx(&s->full[st], R::STAGE);
+        tma_load_2d(&tw, &s->full[st], ring + st * R::STAGE, (first + i) * SLAB, n0);
+      };
+      auto load_x = [&](int i) {
+        const int st = i % R::STAGES;
+        tma_load_2d(&tx, &s->full[st], ring + st * R::STAGE + R::W_BYTES, (first + i) * SLAB, m0);
+      };
+      for (int i = 0; i < ahead; ++i) load_w(i);
+      grid_wait();
+      grid_trigger();
+      for (int i = 0; i < ahead; ++i) load_x(i);
+      bool ok = true;
+      int issued = ahead;
+      for (; issued < count; ++issued) {
+        ok = mbar_wait(&s->empty[issued % R::STAGES], static_cast<uint32_t>((issued / R::STAGES) & 1) ^ 1u, abort);
+        if (!ok) break;
+        load_w(issued);
+        load_x(issued);
+      }
+      if (!ok) {  // no copy may land after the CTA is gone
+        int dummy = 0;
+        for (int i = max(0, issued - R::STAGES); i < issued; ++i)
+          mbar_wait(&s->full[i % R::STAGES], static_cast<uint32_t>((i / R::STAGES) & 1), &dummy);
+      }
+    }
+  } else if (warp == 1) {
+    // ----------------------------------------------------------------- MMA
+    grid_wait();
+    grid_trigger();
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_i8(BN, T);
+      for (int i = 0; i < count; ++i) {
+        const int st = i % R::STAGES;
+        if (!mbar_wait(&s->full[st], static_cast<uint32_t>((i / R::STAGES) & 1), abort)) break;
+        tc_fence_after();
+        const uint32_t w_addr = smem_addr(ring + st * R::STAGE), x_addr = w_addr + R::W_BYTES;
+#pragma unroll
+        for (int k = 0; k < SLAB / 32; ++k)
+          umma_i8(tmem, umma_desc(w_addr + k * 32, 16, 1024, kLayoutSw128), umma_desc(x_addr + k * 32, 16, 1024, kLayoutSw128),
+                  idesc, (i | k) != 0 ? 1u : 0u);
+        umma_commit(&s->empty[st]);
+      }
+      umma_commit(&s->done);  // also after a wait that gave up: all that was issued ends before TMEM is freed
+      int dummy = 0;
+      mbar_wait(&s->done, 0, &dummy);
+    }
+  }
+  __syncwarp();
+  // ------------------------------------------------------------- epilogue
+  if (warp >= 2) {
+    grid_wait();
+    grid_trigger();
+  }
+  bool ok = true;
+  if (warp >= 2) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&s->done, 0, abort));
+    ok = ok && *abort == 0;
+    tc_fence_after();
+  }
+  const int quarter = warp & 3;
+  const int n = n0 + quarter * 32 + lane;
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const bool real = n < p.N;
+  if (p.splits == 1) {
+    if (warp >= 2) {
+      const float ws = real ? p.w_scale[n] : 0.f, bias = real && p.bias ? p.bias[n] : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < T; c += 16) {
+        if (m0 + c >= p.M) break;
+        uint32_t r[16];
+        tmem_ld16(lanes + c, r);
+        const float mine = m0 + c + (lane & 15) < p.M ? p.x_scale[m0 + c + (lane & 15)] : 0.f;
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float xs = __shfl_sync(0xffffffffu, mine, e);
+          const int m = m0 + c + e;
+          if (real && m < p.M) store_out(p, static_cast<int64_t>(m) * p.N + n, ok ? scaled(static_cast<int>(r[e]), xs, ws, bias) : NAN);
+        }
+      }
+    }
+  } else {
+    // each part's sums go to the CTA that owns the columns, into its ring, which no
+    // copy and no MMA of that CTA uses any more
+    cluster_sync();
+    const int own = T / p.splits, log_own = __ffs(own) - 1;  // columns of a CTA: a power of two
+    int* parts = reinterpret_cast<int*>(ring);  // [part][column][128]
+    if (warp >= 2) {
+#pragma unroll 1
+      for (int c = 0; c < T; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(lanes + c, r);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int col = c + e, owner = col >> log_own;
+          const uint32_t to = map_to_cta(parts + (part * own + (col & (own - 1))) * BN + quarter * 32 + lane, static_cast<uint32_t>(owner));
+          asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(r[e]) : "memory");
+        }
+      }
+      if (!ok && lane < p.splits) {
+        const uint32_t to = map_to_cta(&s->bad[part], static_cast<uint32_t>(lane));
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(1) : "memory");
+      }
+    }
+    cluster_sync();
+    if (warp >= 2) {
+      bool bad = false;
+      for (int i = 0; i < p.splits; ++i) bad = bad || s->bad[i] != 0;
+      const float ws = real ? p.w_scale[n] : 0.f, bias = real && p.bias ? p.bias[n] : 0.f;
+      for (int c = 0; c < own; ++c) {
+        const int m = m0 + part * own + c;
+        if (m >= p.M) break;
+        int sum = 0;
+        for (int i = 0; i < p.splits; ++i) sum += parts[(i * own + c) * BN + quarter * 32 + lane];
+        if (real) store_out(p, static_cast<int64_t>(m) * p.N + n, bad ? NAN : scaled(sum, p.x_scale[m], ws, bias));
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, R::COLS);
+}
+
+template <int T>
+int launch_rows(const CUtensorMap& tw, const CUtensorMap& tx, Params p, cudaStream_t st) {
+  auto kernel = rows_kernel<T>;
+  static bool configured[64] = {false};
+  int dev = 0;
+  IRIS_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !configured[dev]) {
+    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows<T>::SMEM));
+    if (dev < 64) configured[dev] = true;
+  }
+  p.token_tiles = (p.M + T - 1) / T;
+  const int64_t units = static_cast<int64_t>(p.token_tiles) * ((p.N + BN - 1) / BN);
+  const int64_t slabs = (p.K + SLAB - 1) / SLAB;
+  p.splits = 1;
+  while (p.splits < 8 && units * p.splits * 2 <= 2 * num_sms() && 4 * p.splits <= slabs) p.splits *= 2;
+  IRIS_REQUIRE(units * p.splits < (1ll << 31), "gemm_i8: too many rows");
+  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(units * p.splits)), THREADS, Rows<T>::SMEM, st,
+                         static_cast<unsigned>(p.splits), tw, tx, p));
+  return IRIS_OK;
+}
+
+inline int check_rows(int64_t M, int64_t K, int64_t ldx) {
+  IRIS_REQUIRE(M >= 0 && M < (1ll << 31) - 256 && K >= 1 && K <= 131071, "quantize_i8: M rows of 1 to 131071 values");
+  IRIS_REQUIRE(ldx >= 0, "quantize_i8: the row stride must not be negative");
+  return IRIS_OK;
+}
+
+inline int64_t row_bytes(int64_t K) { return (K + 15) / 16 * 16; }
+inline int64_t workspace_bytes(const iris_i8_problem& q) {
+  return q.x_dtype == IRIS_I8 ? 0 : q.M * row_bytes(q.K) + (q.M + 3) / 4 * 16;
+}
+
+inline int launch_quantize_any(const QuantizeParams& p, int64_t dtype, cudaStream_t st) {
+  return dtype == IRIS_F32 ? quantize<float>(p, st) : dtype == IRIS_BF16 ? quantize<__nv_bfloat16>(p, st) : quantize<__half>(p, st);
+}
+
+int check_product(const iris_i8_problem& q) {
+  IRIS_REQUIRE(q.x_dtype >= IRIS_F32 && q.x_dtype <= IRIS_I8 && q.out_dtype >= IRIS_F32 && q.out_dtype <= IRIS_F16,
+               "gemm_i8: unsupported dtype");
+  IRIS_REQUIRE(q.M >= 0 && q.M < (1ll << 31) - 256 && q.N >= 0 && q.N < (1ll << 31) - 256, "gemm_i8: sizes");
+  IRIS_REQUIRE(q.K >= 1 && q.K <= 131071, "gemm_i8: 1 <= K <= 131071 (longer sums could leave int32)");
+  return IRIS_OK;
+}
+
+}  // namespace i8
+}  // namespace iris
+
+using namespace iris;
+
+extern "C" int iris_quantize_i8(const iris_quantize_problem* q, void* stream) {
+  using namespace iris::i8;
+  IRIS_REQUIRE(q != nullptr, "quantize_i8: null pointer");
+  IRIS_REQUIRE(q->x_dtype >= IRIS_F32 && q->x_dtype <= IRIS_F16, "quantize_i8: unsupported dtype");
+  IRIS_CHECK_STATUS(check_rows(q->M, q->K, q->ldx));
+  IRIS_REQUIRE(q->ldq >= q->K && q->ldq % 8 == 0, "quantize_i8: rows of q at multiples of 8 bytes, at least K");
+  if (q->M == 0) return IRIS_OK;
+  IRIS_REQUIRE(q->x && q->q && q->scale, "quantize_i8: null pointer");
+  IRIS_REQUIRE(aligned_n(q->q, 8) && aligned_n(q->scale, 4) && aligned_n(q->x, q->x_dtype == IRIS_F32 ? 4 : 2),
+               "quantize_i8: misaligned pointer");
+  const QuantizeParams p = {q->x, static_cast<int8_t*>(q->q), q->scale, q->ldx, q->ldq, static_cast<int>(q->M),
+                            static_cast<int>(q->K)};
+  return launch_quantize_any(p, q->x_dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int iris_gemm_i8_workspace(const iris_i8_problem* q, int64_t* bytes) {
+  using namespace iris::i8;
+  IRIS_REQUIRE(q != nullptr && bytes != nullptr, "gemm_i8_workspace: null pointer");
+  IRIS_CHECK_STATUS(check_product(*q));
+  *bytes = workspace_bytes(*q);
+  return IRIS_OK;
+}
+
+extern "C" int iris_gemm_i8(const iris_i8_problem* q, void* stream) {
+  using namespace iris::i8;
+  IRIS_REQUIRE(q != nullptr, "gemm_i8: null pointer");
+  IRIS_CHECK_STATUS(check_product(*q));
+  if (q->M == 0 || q->N == 0) return IRIS_OK;
+  const bool fresh = q->x_dtype != IRIS_I8;
+  IRIS_REQUIRE(q->x && q->w && q->w_scale && q->out && (fresh || q->x_scale), "gemm_i8: null pointer");
+  IRIS_REQUIRE(aligned16(q->w) && q->ldw % 16 == 0 && q->ldw >= q->K, "gemm_i8: weight rows at multiples of 16 bytes");
+  IRIS_REQUIRE(aligned_n(q->w_scale, 4) && aligned_n(q->bias, 4) && aligned_n(q->x_scale, 4) &&
+                   aligned_n(q->out, q->out_dtype == IRIS_F32 ? 4 : 2) && aligned_n(q->x, q->x_dtype == IRIS_F32 ? 4 : fresh ? 2 : 1),
+               "gemm_i8: misaligned pointer");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const void* x = q->x;
+  int64_t ldx = q->ldx;
+  Params p = {};
+  p.x_scale = q->x_scale;
+  if (fresh) {
+    IRIS_CHECK_STATUS(check_rows(q->M, q->K, q->ldx));
+    IRIS_REQUIRE(q->workspace && aligned16(q->workspace) && q->workspace_bytes >= workspace_bytes(*q), "gemm_i8: workspace too small");
+    ldx = row_bytes(q->K);
+    float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(q->workspace) + q->M * ldx);
+    const QuantizeParams rows = {q->x, static_cast<int8_t*>(q->workspace), scale, q->ldx, ldx, static_cast<int>(q->M),
+                                 static_cast<int>(q->K)};
+    IRIS_CHECK_STATUS(launch_quantize_any(rows, q->x_dtype, st));
+    x = q->workspace;
+    p.x_scale = scale;
+  } else {
+    if (q->M == 1) ldx = row_bytes(q->K);  // a lone row's stride says nothing
+    IRIS_REQUIRE(aligned16(x) && ldx % 16 == 0 && ldx >= q->K, "gemm_i8: 8-bit rows of x at multiples of 16 bytes");
+  }
+  p.w_scale = q->w_scale, p.bias = q->bias, p.out = q->out;
+  p.M = static_cast<int>(q->M), p.N = static_cast<int>(q->N), p.K = static_cast<int>(q->K);
+  p.out_dtype = static_cast<int>(q->out_dtype);
+  p.early = fresh;
+  const int tokens = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+  CUtensorMap tw, tx;
+  IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tw, q->w, q->K, q->N, q->ldw, SLAB, BN));
+  IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tx, x, q->K, q->M, ldx, SLAB, tokens));
+  switch (tokens) {
+    case 16: return launch_rows<16>(tw, tx, p, st);
+    case 32: return launch_rows<32>(tw, tx, p, st);
+    case 64: return launch_rows<64>(tw, tx, p, st);
+    default: return launch_rows<128>(tw, tx, p, st);
+  }
+}

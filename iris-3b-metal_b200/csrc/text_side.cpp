@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <cstring>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -36,6 +37,9 @@ struct Entries {
   decltype(&iris_window_attn_fwd) window_attn_fwd;
   decltype(&iris_window_attn_workspace) window_attn_workspace;
   decltype(&iris_gemv_q4) gemv_q4;
+  decltype(&iris_quantize_i8) quantize_i8;
+  decltype(&iris_gemm_i8) gemm_i8;
+  decltype(&iris_gemm_i8_workspace) gemm_i8_workspace;
   decltype(&iris_last_error) last_error;
 } entries = {};
 long long launches = 0;
@@ -345,6 +349,78 @@ PyObject* gemv_q4(PyObject* const* a) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// 8-bit rows that TMA reads: each starts at a multiple of 16 bytes.
+at::Tensor byte_rows(int64_t rows, int64_t width, const at::Tensor& like) {
+  const auto options = like.options().dtype(at::kChar);
+  const int64_t stride = (width + 15) / 16 * 16;
+  if (stride == width) return at::empty({rows, width}, options);
+  return at::empty({rows, stride}, options).narrow(1, 0, width);
+}
+
+PyObject* quantize_i8(PyObject* const* a) {
+  const at::Tensor& x = tensor(a[0], "quantize_i8 needs x [M, K]");
+  require(x.dim() == 2, "quantize_i8 needs x [M, K]");
+  iris_quantize_problem q = {};
+  q.M = x.size(0), q.K = x.size(1), q.x_dtype = type_code(x.scalar_type());
+  require(x.stride(1) == 1 || q.K == 1, "quantize_i8: x rows must be contiguous");
+  q.ldx = q.M > 1 ? x.stride(0) : q.K;
+  const On on(x, {});
+  at::Tensor packed = byte_rows(q.M, q.K, x), scale = at::empty({q.M}, x.options().dtype(at::kFloat));
+  q.ldq = (q.K + 15) / 16 * 16;
+  q.x = x.data_ptr(), q.q = packed.data_ptr(), q.scale = static_cast<float*>(scale.data_ptr());
+  on.check("iris_quantize_i8", entries.quantize_i8(&q, on.stream()), q.M > 0);
+  PyObject* first = THPVariable_Wrap(std::move(packed));
+  PyObject* second = first ? THPVariable_Wrap(std::move(scale)) : nullptr;
+  PyObject* both = second ? PyTuple_Pack(2, first, second) : nullptr;
+  Py_XDECREF(first);
+  Py_XDECREF(second);
+  if (both == nullptr) throw Raised{};
+  return both;
+}
+
+PyObject* gemm_i8(PyObject* const* a) {
+  const char* need = "gemm_i8 needs x [M, K], packed [N, K], scale [N]";
+  const at::Tensor &x = tensor(a[0], need), &packed = tensor(a[1], need), &scale = tensor(a[2], need);
+  const at::Tensor* bias = maybe(a[3], "gemm_i8: bias must be a tensor");
+  const at::Tensor* x_scale = maybe(a[4], "gemm_i8: x_scale must be a tensor");
+  require(x.dim() == 2 && packed.dim() == 2, need);
+  iris_i8_problem q = {};
+  q.M = x.size(0), q.K = x.size(1), q.N = packed.size(0);
+  require(packed.scalar_type() == at::kChar && packed.size(1) == q.K, "gemm_i8: packed must be int8 [N, K]");
+  require((packed.stride(1) == 1 || q.K == 1) && (x.stride(1) == 1 || q.K == 1), "gemm_i8: rows must be contiguous");
+  const auto row_of = [](const at::Tensor* t, int64_t n) {
+    return t->scalar_type() == at::kFloat && t->dim() == 1 && t->size(0) == n && t->is_contiguous();
+  };
+  require(row_of(&scale, q.N), "gemm_i8: scale must be contiguous FP32 [N]");
+  require(bias == nullptr || row_of(bias, q.N), "gemm_i8: bias must be contiguous FP32 [N]");
+  const bool eight = x.scalar_type() == at::kChar;
+  require(eight == (x_scale != nullptr), "gemm_i8: x_scale goes with int8 x, and with it alone");
+  require(x_scale == nullptr || row_of(x_scale, q.M), "gemm_i8: x_scale must be contiguous FP32 [M]");
+  at::ScalarType out_type = eight ? at::kBFloat16 : x.scalar_type();
+  q.x_dtype = eight ? IRIS_I8 : type_code(out_type);
+  if (a[5] != Py_None) {
+    require(THPDtype_Check(a[5]), "gemm_i8: out_dtype must be a dtype");
+    out_type = reinterpret_cast<THPDtype*>(a[5])->scalar_type;
+  }
+  q.out_dtype = type_code(out_type);
+  q.ldx = q.M > 1 ? x.stride(0) : (q.K + 15) / 16 * 16;
+  q.ldw = q.N > 1 ? packed.stride(0) : (q.K + 15) / 16 * 16;  // a lone row's stride says nothing
+  const On on(x, {&packed, &scale, bias, x_scale});
+  at::Tensor out = at::empty({q.M, q.N}, x.options().dtype(out_type));
+  q.x = x.data_ptr(), q.w = packed.data_ptr(), q.out = out.data_ptr();
+  q.w_scale = static_cast<const float*>(scale.data_ptr());
+  q.x_scale = x_scale ? static_cast<const float*>(x_scale->data_ptr()) : nullptr;
+  q.bias = bias ? static_cast<const float*>(bias->data_ptr()) : nullptr;
+  on.check("iris_gemm_i8_workspace", entries.gemm_i8_workspace(&q, &q.workspace_bytes), 0);
+  at::Tensor workspace;  // of this call's own
+  if (q.workspace_bytes > 0) {
+    workspace = at::empty({q.workspace_bytes}, x.options().dtype(at::kByte));
+    q.workspace = workspace.data_ptr();
+  }
+  on.check("iris_gemm_i8", entries.gemm_i8(&q, on.stream()), q.M * q.N == 0 ? 0 : eight ? 1 : 2);
+  return THPVariable_Wrap(std::move(out));
+}
+
 // No C++ exception leaves the module.
 template <PyObject* (*Call)(PyObject* const*), int Args>
 PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -364,24 +440,20 @@ PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // Addresses of the entry points, in the order of Entries.
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  void* at[6] = {};
-  if (n != 6) {
-    PyErr_SetString(PyExc_ValueError, "bind takes six addresses");
+  constexpr int count = sizeof(Entries) / sizeof(void*);
+  void* at[count] = {};
+  if (n != count) {
+    PyErr_SetString(PyExc_ValueError, "bind takes an address for each entry point");
     return nullptr;
   }
-  for (int i = 0; i < 6; ++i) {
+  for (int i = 0; i < count; ++i) {
     at[i] = PyLong_AsVoidPtr(args[i]);
     if (at[i] == nullptr) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: null address");
       return nullptr;
     }
   }
-  entries.rope = reinterpret_cast<decltype(entries.rope)>(at[0]);
-  entries.rope_append = reinterpret_cast<decltype(entries.rope_append)>(at[1]);
-  entries.window_attn_fwd = reinterpret_cast<decltype(entries.window_attn_fwd)>(at[2]);
-  entries.window_attn_workspace = reinterpret_cast<decltype(entries.window_attn_workspace)>(at[3]);
-  entries.gemv_q4 = reinterpret_cast<decltype(entries.gemv_q4)>(at[4]);
-  entries.last_error = reinterpret_cast<decltype(entries.last_error)>(at[5]);
+  std::memcpy(&entries, at, sizeof(entries));
   Py_RETURN_NONE;
 }
 
@@ -397,6 +469,8 @@ PyMethodDef methods[] = {
     method<rope_append, 12>("rope_append"),
     method<window_attention, 10>("window_attention"),
     method<gemv_q4, 8>("gemv_q4"),
+    method<quantize_i8, 1>("quantize_i8"),
+    method<gemm_i8, 6>("gemm_i8"),
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind)), METH_FASTCALL, ""},
     {"launched", launched, METH_NOARGS, "Kernels that these calls enqueued."},
     {nullptr, nullptr, 0, nullptr},

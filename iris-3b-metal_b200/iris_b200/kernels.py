@@ -651,6 +651,35 @@ def gemv_q4(
     return (_lib._text_side or _lib.text_side()).gemv_q4(x, packed, scale, zero, bias, silu_in, silu_out, out_dtype)
 
 
+def quantize_i8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows ``[M, K]`` (FP32, BF16 or FP16, ``K`` up to 131071; the row stride may exceed ``K``) to 8 bits with
+    a scale each, for :func:`gemm_i8`: ``(packed, scale)``, int8 ``[M, K]`` whose rows
+    start at multiples of 16 bytes, and FP32 ``[M]``, a row's largest magnitude over 127.
+    Each value is the whole number nearest ``127 x / max|x|`` (halves to even). Weights
+    ``[N, K]`` are packed by the same call, once; a token's row quantised once serves several
+    products. A row that holds an infinity or NaN has scale NaN and zeros."""
+    return (_lib._text_side or _lib.text_side()).quantize_i8(x)
+
+
+def gemm_i8(
+    x: torch.Tensor,
+    packed: torch.Tensor,
+    scale: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    x_scale: torch.Tensor | None = None,
+    out_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """``x @ w.T + bias`` for any number of rows over 8-bit weights with a scale for each
+    channel (``packed`` int8 ``[N, K]``, ``scale`` FP32 ``[N]``, from :func:`quantize_i8`) and one for
+    each token: ``x`` ``[M, K]`` in FP32, BF16 or FP16 is quantised by rows within the call, int8
+    rows with their ``x_scale`` (FP32 ``[M]``) are taken as they are. Sums are exact (int32),
+    scales and ``bias`` (FP32 ``[N]``) FP32; the result is ``[M, N]`` of ``out_dtype`` (default:
+    the input's; BF16 for int8 rows). int8 rows start at multiples of 16 bytes. A row of ``x`` that
+    holds an infinity or NaN gives a row of NaN."""
+    return (_lib._text_side or _lib.text_side()).gemm_i8(x, packed, scale, bias, x_scale, out_dtype)
+
+
 def block_copy(
     dst: torch.Tensor,
     dst_strides: tuple[int, int, int],
