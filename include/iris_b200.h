@@ -332,6 +332,36 @@ int iris_window_attn_fwd(const iris_window_problem* problem, void* stream);
  * at the same time need one each. */
 int iris_window_attn_workspace(const iris_window_problem* problem, int64_t* bytes);
 
+/* Attention of a batch that shares a long prefix, read once for all (no reference
+ * counterpart; the mask and the rows as for iris_window_attn_fwd): samples
+ * [g * batch / groups, (g + 1) * batch / groups) have the keys prefix_k / prefix_v[g] in
+ * common and k / v[b] of their own behind them. Query i of sample b sees the prefix's
+ * keys j < prefix_lengths[g] (null: n_prefix; clamped to [0, n_prefix]) and its own keys
+ * j < lengths[b] (null: n_kv; clamped) with j <= starts[b] + i + right (starts null: n_kv
+ * - n; right -1: no bound), all in one softmax; 0 where there is none. q [batch, heads_q, n, head_dim],
+ * prefix_k / prefix_v [groups, heads_kv, n_prefix, head_dim], k / v [batch, heads_kv,
+ * n_kv, head_dim], bf16 or f16, strides multiples of 8 (0 repeats a head, group or sample),
+ * head_dim 64 or 128; out shares no memory with the keys, and with q only as its own
+ * rows in place. workspace: iris_prefix_attn_workspace bytes. */
+typedef struct iris_prefix_problem {
+  iris_head_rows q, prefix_k, prefix_v, k, v;
+  void* out;
+  int64_t out_stride_b, out_stride_n;
+  const int* prefix_lengths;
+  const int* starts;
+  const int* lengths;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t dtype, batch, groups, heads_q, heads_kv, n, n_prefix, n_kv, head_dim, right;
+  double scale;
+} iris_prefix_problem;
+int iris_prefix_attn_fwd(const iris_prefix_problem* problem, void* stream);
+
+/* Bytes of workspace (16-byte aligned; null for 0) that iris_prefix_attn_fwd needs for a
+ * problem's sizes, type and right (its pointers and strides are not read). Two calls that
+ * may run at the same time need one each. */
+int iris_prefix_attn_workspace(const iris_prefix_problem* problem, int64_t* bytes);
+
 /* ---- peer memory (sequence parallelism across processes) ---------------- */
 /* No reference counterpart. iris_ipc_export: the IPC handle (IRIS_IPC_HANDLE_BYTES)
  * of the allocation holding device pointer ptr and ptr's offset in it;

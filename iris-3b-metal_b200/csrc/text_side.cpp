@@ -40,6 +40,8 @@ struct Entries {
   decltype(&iris_quantize_i8) quantize_i8;
   decltype(&iris_gemm_i8) gemm_i8;
   decltype(&iris_gemm_i8_workspace) gemm_i8_workspace;
+  decltype(&iris_prefix_attn_fwd) prefix_attn_fwd;
+  decltype(&iris_prefix_attn_workspace) prefix_attn_workspace;
   decltype(&iris_last_error) last_error;
 } entries = {};
 long long launches = 0;
@@ -250,6 +252,15 @@ PyObject* rope_append(PyObject* const* a) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// Whether out [B, N, H * D] lies onto q's [B, H, N, D] rows: a row is read by the CTAs
+// that write it, before they do.
+bool own_rows(const at::Tensor& out, const at::Tensor& q) {
+  const int64_t batch = q.size(0), heads = q.size(1), n = q.size(2), dim = q.size(3);
+  return out.dim() == 3 && out.data_ptr() == q.data_ptr() && out.size(0) == batch && out.size(1) == n &&
+         out.size(2) == heads * dim && out.stride(2) == 1 && (batch <= 1 || out.stride(0) == q.stride(0)) &&
+         (n <= 1 || out.stride(1) == q.stride(2)) && (heads <= 1 || q.stride(1) == dim);
+}
+
 PyObject* window_attention(PyObject* const* a) {
   const char* need = "window_attention: q [B, H, N, D], k/v [B, H_kv, N_kv, D]";
   const at::Tensor &qt = tensor(a[0], need), &k = tensor(a[1], need), &v = tensor(a[2], need);
@@ -282,12 +293,7 @@ PyObject* window_attention(PyObject* const* a) {
   }
   const int64_t width = q.heads_q * q.head_dim;
   if (given) {
-    // onto q's own rows: a row is read by the CTAs that write it, before they do
-    const bool own = given->dim() == 3 && given->data_ptr() == qt.data_ptr() && given->size(0) == q.batch &&
-                     given->size(1) == q.n && given->size(2) == width && given->stride(2) == 1 &&
-                     (q.batch <= 1 || given->stride(0) == qt.stride(0)) && (q.n <= 1 || given->stride(1) == qt.stride(2)) &&
-                     (q.heads_q <= 1 || qt.stride(1) == q.head_dim);
-    require(own || !share(*given, qt), "window_attention: out must be q's own rows or share no memory with q");
+    require(own_rows(*given, qt) || !share(*given, qt), "window_attention: out must be q's own rows or share no memory with q");
     require(!share(*given, k) && !share(*given, v), "window_attention: out must not share memory with k or v");
   }
   const On on(qt, {&k, &v, starts, lengths, given});
@@ -309,6 +315,67 @@ PyObject* window_attention(PyObject* const* a) {
     q.workspace = workspace.data_ptr();
   }
   on.check("iris_window_attn_fwd", entries.window_attn_fwd(&q, on.stream()), q.batch * q.n == 0 ? 0 : q.workspace ? 2 : 1);
+  return THPVariable_Wrap(std::move(out));
+}
+
+PyObject* prefix_attention(PyObject* const* a) {
+  const char* need = "prefix_attention: q [B, H, N, D], prefix_k/v [G, H_kv, P, D], k/v [B, H_kv, N_kv, D]";
+  const at::Tensor &qt = tensor(a[0], need), &pk = tensor(a[1], need), &pv = tensor(a[2], need);
+  const at::Tensor &k = tensor(a[3], need), &v = tensor(a[4], need);
+  const at::Tensor* prefix_lengths = maybe(a[5], "prefix_lengths must be contiguous int32 [G]");
+  const at::Tensor* starts = maybe(a[6], "starts must be contiguous int32 [B]");
+  const at::Tensor* lengths = maybe(a[7], "lengths must be contiguous int32 [B]");
+  const at::Tensor* given = maybe(a[10], "prefix_attention: out must be a tensor");
+  require(qt.dim() == 4 && pk.dim() == 4 && k.dim() == 4, need);
+  iris_prefix_problem q = {};
+  q.batch = qt.size(0), q.heads_q = qt.size(1), q.n = qt.size(2), q.head_dim = qt.size(3);
+  q.groups = pk.size(0), q.heads_kv = pk.size(1), q.n_prefix = pk.size(2), q.n_kv = k.size(2);
+  const at::ScalarType type = qt.scalar_type();
+  require(type == at::kBFloat16 || type == at::kHalf, "prefix_attention: q, keys and values in one of bf16, f16");
+  for (const at::Tensor* t : {&pk, &pv, &k, &v})
+    require(t->scalar_type() == type, "prefix_attention: q, keys and values in one of bf16, f16");
+  q.dtype = type_code(type);
+  require(q.head_dim == 128 || q.head_dim == 64, "prefix_attention: head_dim must be 64 or 128");
+  require(q.groups >= 1 && q.batch % q.groups == 0, "prefix_attention: the batch must be a multiple of the prefixes");
+  q.q = head_rows(qt, q.batch, q.heads_q, q.n, q.head_dim, need);
+  q.prefix_k = head_rows(pk, q.groups, q.heads_kv, q.n_prefix, q.head_dim, "prefix_attention: prefix_k must be [G, H_kv, P, D]");
+  q.prefix_v = head_rows(pv, q.groups, q.heads_kv, q.n_prefix, q.head_dim, "prefix_attention: prefix_v must be [G, H_kv, P, D]");
+  q.k = head_rows(k, q.batch, q.heads_kv, q.n_kv, q.head_dim, "prefix_attention: k must be [B, H_kv, N_kv, D]");
+  q.v = head_rows(v, q.batch, q.heads_kv, q.n_kv, q.head_dim, "prefix_attention: v must be [B, H_kv, N_kv, D]");
+  q.right = a[8] == Py_None ? -1 : whole(a[8]);
+  require(q.right >= 0 || a[8] == Py_None, "prefix_attention: right must not be negative");
+  q.prefix_lengths = int32_rows(prefix_lengths, q.groups, "prefix_lengths must be contiguous int32 [G]");
+  q.starts = int32_rows(starts, q.batch, "starts must be contiguous int32 [B]");
+  q.lengths = int32_rows(lengths, q.batch, "lengths must be contiguous int32 [B]");
+  q.scale = 1.0 / std::sqrt(static_cast<double>(q.head_dim));
+  if (a[9] != Py_None) {
+    q.scale = PyFloat_AsDouble(a[9]);
+    if (q.scale == -1.0 && PyErr_Occurred()) throw Raised{};
+  }
+  const int64_t width = q.heads_q * q.head_dim;
+  if (given) {
+    require(own_rows(*given, qt) || !share(*given, qt), "prefix_attention: out must be q's own rows or share no memory with q");
+    for (const at::Tensor* t : {&pk, &pv, &k, &v})
+      require(!share(*given, *t), "prefix_attention: out must not share memory with keys or values");
+  }
+  const On on(qt, {&pk, &pv, &k, &v, prefix_lengths, starts, lengths, given});
+  if (given) {
+    require(given->dim() == 3 && given->size(0) == q.batch && given->size(1) == q.n && given->size(2) == width &&
+                given->scalar_type() == type && given->stride(2) == 1,
+            "prefix_attention: out must be [B, N, H * D] rows of the input's type");
+    writable(*given);
+  }
+  at::Tensor out = given ? *given : at::empty({q.batch, q.n, width}, qt.options());
+  q.out = out.data_ptr();
+  q.out_stride_b = q.batch > 1 ? out.stride(0) : 0;
+  q.out_stride_n = q.n > 1 ? out.stride(1) : 0;
+  on.check("iris_prefix_attn_workspace", entries.prefix_attn_workspace(&q, &q.workspace_bytes), 0);
+  at::Tensor workspace;  // of this call's own: two graphs or streams never share one
+  if (q.workspace_bytes > 0) {
+    workspace = at::empty({q.workspace_bytes}, qt.options().dtype(at::kByte));
+    q.workspace = workspace.data_ptr();
+  }
+  on.check("iris_prefix_attn_fwd", entries.prefix_attn_fwd(&q, on.stream()), q.batch * q.n == 0 ? 0 : q.workspace ? 2 : 1);
   return THPVariable_Wrap(std::move(out));
 }
 
@@ -468,6 +535,7 @@ PyMethodDef methods[] = {
     method<rope, 7>("rope"),
     method<rope_append, 12>("rope_append"),
     method<window_attention, 10>("window_attention"),
+    method<prefix_attention, 11>("prefix_attention"),
     method<gemv_q4, 8>("gemv_q4"),
     method<quantize_i8, 1>("quantize_i8"),
     method<gemm_i8, 6>("gemm_i8"),

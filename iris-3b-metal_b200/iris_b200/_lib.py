@@ -112,9 +112,10 @@ SIGNATURES["iris_ipc_close"] = [P]
 SIGNATURES["iris_peer_barrier"] = [P, P, I32, I32, ctypes.c_uint, I64, P]
 SIGNATURES["iris_flash_attn_fwd_split"] = [P, P, P, I64, I64, I64, I64, I64, I64, F, F, I64, P, P, P, P, I64, P]
 
-for _name in ("iris_rope", "iris_rope_append", "iris_window_attn_fwd", "iris_gemv_q4", "iris_quantize_i8", "iris_gemm_i8"):
+for _name in ("iris_rope", "iris_rope_append", "iris_window_attn_fwd", "iris_gemv_q4", "iris_quantize_i8", "iris_gemm_i8",
+              "iris_prefix_attn_fwd"):  # fmt: skip
     SIGNATURES[_name] = [P, P]  # a problem struct and the stream
-for _name in ("iris_window_attn_workspace", "iris_gemm_i8_workspace"):
+for _name in ("iris_window_attn_workspace", "iris_gemm_i8_workspace", "iris_prefix_attn_workspace"):
     SIGNATURES[_name] = [P, ctypes.POINTER(I64)]
 
 _lib: ctypes.CDLL | None = None
@@ -143,7 +144,8 @@ def load() -> ctypes.CDLL:
 
 # the text side's entry points, in the order of the module's bind()
 _TEXT_ENTRIES = ("iris_rope", "iris_rope_append", "iris_window_attn_fwd", "iris_window_attn_workspace", "iris_gemv_q4",
-                 "iris_quantize_i8", "iris_gemm_i8", "iris_gemm_i8_workspace", "iris_last_error")  # fmt: skip
+                 "iris_quantize_i8", "iris_gemm_i8", "iris_gemm_i8_workspace", "iris_prefix_attn_fwd",
+                 "iris_prefix_attn_workspace", "iris_last_error")  # fmt: skip
 _text_side = None
 
 
@@ -166,7 +168,8 @@ def text_side():
 _launches = 0
 # kernels each entry point enqueues (1 unless listed)
 _KERNELS_PER_CALL = {"iris_device_error": 0, "iris_all_finite": 2, "iris_ipc_export": 0, "iris_ipc_import": 0,
-                     "iris_ipc_close": 0, "iris_window_attn_workspace": 0, "iris_gemm_i8_workspace": 0}
+                     "iris_ipc_close": 0, "iris_window_attn_workspace": 0, "iris_gemm_i8_workspace": 0,
+                     "iris_prefix_attn_workspace": 0}
 
 
 def launch_count() -> int:

@@ -607,6 +607,39 @@ def window_attention(
     return (_lib._text_side or _lib.text_side()).window_attention(q, k, v, left, right, sinks, starts, lengths, scale, out)
 
 
+def prefix_attention(
+    q: torch.Tensor,
+    prefix_k: torch.Tensor,
+    prefix_v: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    prefix_lengths: torch.Tensor | None = None,
+    starts: torch.Tensor | None = None,
+    lengths: torch.Tensor | None = None,
+    right: int | None = 0,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``softmax(q k^T * scale) v`` of a batch that shares a long prefix, which is read once
+    for all of it, over the prefix's keys and each sample's own, for prompts, chunks and
+    single tokens: ``q`` ``[B, H, N, D]``, ``prefix_k``/``prefix_v`` ``[G, H_kv, P, D]``, ``k``/``v``
+    ``[B, H_kv, N_kv, D]`` (BF16 or FP16, ``D`` 64 or 128, any strides of multiples of 8
+    elements with contiguous rows); returns ``[B, N, H * D]`` (``out``, or a new tensor).
+
+    ``B / G`` neighbouring samples share a prefix (``G`` 1: all of them). Query ``i`` of
+    sample ``b`` sees the prefix's keys ``j < prefix_lengths[g]`` (int32 ``[G]``, clamped to ``[0,
+    P]``; default ``P``), and of its own keys those with ``j < lengths[b]`` (int32 ``[B]``, clamped to ``[0,
+    N_kv]``; default ``N_kv``) and ``j <= starts[b] + i + right`` (``starts``: int32 ``[B]``, places in
+    ``k``, not counting the prefix; default ``N_kv - N``, ``lengths`` or not). ``right=None`` is no
+    bound, the default is causal. A query that sees no key gives 0. Other keys' rows may hold
+    anything. Heads, groups and samples may be expanded, tokens not. ``out`` shares no memory
+    with the inputs, or is ``q``'s own rows."""
+    return (_lib._text_side or _lib.text_side()).prefix_attention(
+        q, prefix_k, prefix_v, k, v, prefix_lengths, starts, lengths, right, scale, out
+    )
+
+
 def pack_q4(
     w: torch.Tensor, group: int = 64, symmetric: bool = True
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
