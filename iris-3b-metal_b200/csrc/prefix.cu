@@ -111,26 +111,819 @@ __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, fl
     acc[c] = count == 0 ? make_float2(0.f, 0.f) : l == 0.f ? make_float2(NAN, NAN) : acc[c];
 }
 
+// -------------------------------------------------------- 128-row tiles (tcgen05)
+// A tile is 128 query rows of one key head: tokens times query heads of `per` samples, row
+// r being sample r / (n group), token r / group % n, head r % group. The prefix is the
+// same for all samples of a group, so its rows are taken together (per = per_group): one
+// token of 32 samples and 4 heads each fills a tile that would hold 4 rows. Where one
+// sample's rows fill tiles (per = 1), they see its own keys too, in the same pass.
+//
+// A CTA takes a tile and a chunk of its blocks of 64 keys, two CTAs to an SM: warps 2 to 5
+// bring Q's rows, which lie anywhere, into the swizzled place that the tensor cores read;
+// warp 0 brings K and V through two-slot rings by TMA; warp 1 issues the MMAs; warps 2 to 5
+// do the softmax, a thread per row (TMEM lane). S alternates between two buffers and runs a
+// block ahead of P V. Chunks' states are joined by join_kernel.
+//
+// A block that every row of a warp sees in full takes no mask. Keys behind a length
+// are zeroed in shared memory (their K only reaches masked scores). A masked key's weight is
+// exactly 0, and 0 times a NaN or infinity of its V row is NaN: a row that comes out
+// not finite is computed again by attend_row, which reads visible keys alone.
+constexpr int BQ = 128, BKV = 64, KV = 2;  // rows, keys of a block, slots of the K and V rings
+constexpr int THREADS = 192;
+constexpr int Q_HALF = BQ * 128, KV_HALF = BKV * 128;  // bytes of 64 columns of a tile
+constexpr uint32_t COL_S = 0, COL_O = 2 * BKV, TILE_COLS = 256;
+
+struct TileSmem {
+  uint64_t q_full, k_full[KV], k_free[KV], v_full[KV], v_free[KV], v_tail;
+  uint64_t s_full[2], p_full[2], pv_done, o_final, teardown;
+  uint32_t tmem_base;
+  int abort;
+};
+
+template <int D>
+constexpr int tile_smem() {
+  return 1024 + (D / 64) * (Q_HALF + 2 * KV * KV_HALF) + static_cast<int>(sizeof(TileSmem));
+}
+
+// ------------------------------------------------- few rows over many keys
+// A sample's own keys where its rows fill no tile, and all of its keys where they are
+// few: a CTA takes 16 query rows of a sample and key head (read once for all of them) and a
+// chunk of the keys; its warps walk 16-key tiles of their own, each with its own softmax state
+// and its own ring of cp.async copies (no barrier until the end), scores and P V on
+// mma.sync m16n8k16: HBM-bound.
+constexpr int STEP_WARPS = 4, STEP_STAGES = 3, STEP_KEYS = 16, STEP_ROWS = 16;
+
+// How a call is cut up.
+struct Plan {
+  int per;           // samples whose rows share tiles; 1: tiles see the samples' own keys too
+  int tiles;         // 128-row tiles of a unit (per samples and a key head); 0: none
+  int tile_chunk;    // blocks of 64 keys a tile's CTA walks
+  int tile_splits;   // chunks of a tile
+  int tile_ctas;
+  int row_tiles;     // 16-row tiles of a sample and key head
+  int step_prefix;   // whether they see the prefix (no tiles do)
+  int step_chunk;    // keys of such a tile's CTA
+  int step_splits;   // chunks; 0: tiles see all keys
+  int step_ctas;
+  float* tile_sums;  // [unit, tile, split, 128, D], then maxima and totals [.., 128]; null: rows are finished by their tile
+  float2* tile_states;
+  float* step_sums;  // [sample, key head, row tile, split, 16, D], then [.., 16]; null: rows are finished by their CTA
+  float2* step_states;
+};
+
+template <int D>
+constexpr int step_smem() {
+  return STEP_WARPS * STEP_STAGES * 2 * STEP_KEYS * D * 2;
+}
+template <int D>
+constexpr int most_smem() {
+  return tile_smem<D>() > step_smem<D>() ? tile_smem<D>() : step_smem<D>();
+}
+
+struct Row {
+  int b, h, i;
+};
+// Row r of unit (u, hk).
+IRIS_DEVICE Row row_of(const Params& p, int per, int u, int hk, int r) {
+  const int group = p.heads_q / p.heads_kv;
+  const int token = r / group;
+  return Row{u * per + token / p.n, hk * group + r - token * group, token % p.n};
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ Params p) {
-  grid_wait();
-  grid_trigger();
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= static_cast<int64_t>(p.batch) * p.n * p.heads_q) return;
-  const int h = static_cast<int>(row % p.heads_q), i = static_cast<int>(row / p.heads_q % p.n);
-  const int b = static_cast<int>(row / p.heads_q / p.n);
-  float2 acc[D / 64];
-  attend_row<T, D>(p, b, h, i, acc);
+IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const CUtensorMap& tk, const CUtensorMap& tv,
+                          const Params& p, const Plan& plan, int cta, uint8_t* smem_raw) {
+  constexpr int HALVES = D / 64, KV_BYTES = HALVES * KV_HALF;
+  uint8_t* q_tile = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* k_tile = q_tile + HALVES * Q_HALF;
+  uint8_t* v_tile = k_tile + KV * KV_BYTES;
+  TileSmem* s = reinterpret_cast<TileSmem*>(v_tile + KV * KV_BYTES);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int group = p.heads_q / p.heads_kv, rows = plan.per * p.n * group;
+  const int split = cta % plan.tile_splits, unit_tile = cta / plan.tile_splits;
+  // later rows first: under a causal mask they see the most keys
+  const int units = p.batch / plan.per * p.heads_kv;
+  const int unit = unit_tile % units, tile = plan.tiles - 1 - unit_tile / units;
+  const int hk = unit % p.heads_kv, u = unit / p.heads_kv;
+  const int row0 = tile * BQ, last = min(row0 + BQ, rows) - 1;
+  const int b0 = u * plan.per, g = b0 / p.per_group;
+  const bool own = plan.per == 1 && plan.step_splits == 0;
+  const int early = prefix_length(p, b0);
+  const int length = own ? own_length(p, b0) : 0;
+  const int64_t start = own ? own_start(p, b0) : 0;
+  const int early_blocks = (early + BKV - 1) / BKV;
+  const int all_blocks = early_blocks + (own ? (own_keys(p, start + last / group, length) + BKV - 1) / BKV : 0);
+  const int first = min(split * plan.tile_chunk, all_blocks);
+  const int iters = min(plan.tile_chunk, all_blocks - first);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&s->q_full, 4);
+    for (int i = 0; i < KV; ++i) {
+      mbar_init(&s->k_full[i], 1);
+      mbar_init(&s->k_free[i], 1);
+      mbar_init(&s->v_full[i], 1);
+      mbar_init(&s->v_free[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s->s_full[i], 1);
+      mbar_init(&s->p_full[i], 4);
+    }
+    mbar_init(&s->pv_done, 1);
+    mbar_init(&s->o_final, 1);
+    mbar_init(&s->v_tail, 1);
+    mbar_init(&s->teardown, 1);
+    s->abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc(&s->tmem_base, TILE_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s->tmem_base;
+  volatile int* abort = &s->abort;
+
+  if (warp == 0) {
+    // ----------------------------------------------------------------- TMA
+    int issued_k[KV], issued_v[KV];
+    for (int i = 0; i < KV; ++i) issued_k[i] = issued_v[i] = -1;
+    int tails = 0;
+    bool ok = true;
+    if (lane == 0 && first < early_blocks) {
+      tma_prefetch_desc(&tpk);
+      tma_prefetch_desc(&tpv);
+    }
+    if (lane == 0 && all_blocks > early_blocks) {
+      tma_prefetch_desc(&tk);
+      tma_prefetch_desc(&tv);
+    }
+    // one block's 64 rows of keys or values into a slot
+    auto load = [&](const CUtensorMap& of_prefix, const CUtensorMap& of_own, uint64_t* bar, uint8_t* slot, int block, int ph, int pb,
+                    int oh, int ob) {
+      mbar_arrive_expect_tx(bar, KV_BYTES);
+      for (int c = 0; c < HALVES; ++c)
+        if (block < early_blocks) tma_load_4d(&of_prefix, bar, slot + c * KV_HALF, c * 64, block * BKV, ph, pb);
+        else tma_load_4d(&of_own, bar, slot + c * KV_HALF, c * 64, (block - early_blocks) * BKV, oh, ob);
+    };
+    auto load_k = [&](int it) {
+      const int st = it % KV;
+      const uint32_t ph = static_cast<uint32_t>((it / KV) & 1);
+      ok = mbar_wait(&s->k_free[st], ph ^ 1u, abort);
+      if (!ok) return;
+      load(tpk, tk, &s->k_full[st], k_tile + st * KV_BYTES, first + it, p.pkh != 0 ? hk : 0, p.pkb != 0 ? g : 0, p.kh != 0 ? hk : 0,
+           p.kb != 0 ? b0 : 0);
+      issued_k[st] = static_cast<int>(ph);
+    };
+    if (lane == 0 && iters > 0) load_k(0);
+    for (int it = 0; it < iters; ++it) {
+      const int st = it % KV;
+      const uint32_t ph = static_cast<uint32_t>((it / KV) & 1);
+      const int block = first + it;
+      // keys behind the length that the tensor map does not end before
+      const int left = block < early_blocks ? early - block * BKV : length - (block - early_blocks) * BKV;
+      const bool tail = left < BKV && (block < early_blocks ? early < p.n_prefix : length < p.n_kv);
+      if (lane == 0 && ok) {
+        if (it + 1 < iters) load_k(it + 1);  // scores run a block ahead
+        ok = ok && mbar_wait(&s->v_free[st], ph ^ 1u, abort);
+        if (ok) {
+          load(tpv, tv, tail ? &s->v_tail : &s->v_full[st], v_tile + st * KV_BYTES, block, p.pvh != 0 ? hk : 0, p.pvb != 0 ? g : 0,
+               p.vh != 0 ? hk : 0, p.vb != 0 ? b0 : 0);
+          issued_v[st] = tail ? -1 : static_cast<int>(ph);  // the copy before in this slot has been read
+        }
+      }
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      if (tail) {  // two blocks of the CTA at most: those that the lengths end in
+        ++tails;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s->v_tail, static_cast<uint32_t>(tails - 1) & 1u, abort));
+        if (!ok) break;
+        for (int e = left * 8 + lane; e < BKV * 8; e += 32)
+          for (int c = 0; c < HALVES; ++c)
+            *reinterpret_cast<uint4*>(v_tile + st * KV_BYTES + c * KV_HALF + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s->v_full[st]);
+      }
+    }
+    if (lane == 0 && iters > 0) {  // whichever warp gives up: no copy may land after the CTA is gone
+      int dummy = 0;
+      for (int i = 0; i < KV; ++i) {
+        if (issued_k[i] >= 0) mbar_wait(&s->k_full[i], static_cast<uint32_t>(issued_k[i]), &dummy);
+        if (issued_v[i] >= 0) mbar_wait(&s->v_full[i], static_cast<uint32_t>(issued_v[i]), &dummy);
+      }
+      if (tails > 0) mbar_wait(&s->v_tail, static_cast<uint32_t>(tails - 1) & 1u, &dummy);
+    }
+  } else if (warp == 1) {
+    // ----------------------------------------------------------------- MMA
+    if (lane == 0 && iters > 0) {
+      constexpr uint32_t f16 = (1u << 7) | (1u << 10);  // the BF16 bits of idesc_bf16_f32; F16 is 0
+      constexpr uint32_t clear = IsHalf<T>::value ? f16 : 0u;
+      const uint32_t idesc_s = idesc_bf16_f32(BQ, BKV) & ~clear;
+      const uint32_t idesc_o = idesc_bf16_f32(BQ, D, false, true) & ~clear;  // V is MN-major (columns contiguous)
+      bool ok = mbar_wait(&s->q_full, 0, abort);
+      // scores of block `it` into buffer it % 2
+      auto issue_s = [&](int it) {
+        ok = ok && mbar_wait(&s->k_full[it % KV], static_cast<uint32_t>((it / KV) & 1), abort);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t q_addr = smem_addr(q_tile), k_addr = smem_addr(k_tile + (it % KV) * KV_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_ss(tmem + COL_S + (it & 1) * BKV, umma_desc(q_addr + (kk >> 2) * Q_HALF + (kk & 3) * 32, 16, 1024, kLayoutSw128),
+                  umma_desc(k_addr + (kk >> 2) * KV_HALF + (kk & 3) * 32, 16, 1024, kLayoutSw128), idesc_s, kk > 0 ? 1u : 0u);
+        umma_commit(&s->s_full[it & 1]);
+        umma_commit(&s->k_free[it % KV]);
+      };
+      issue_s(0);
+      if (iters > 1) issue_s(1);
+      for (int it = 0; it < iters && ok; ++it) {
+        const int st = it % KV;
+        ok = mbar_wait(&s->v_full[st], static_cast<uint32_t>((it / KV) & 1), abort) &&
+             mbar_wait(&s->p_full[it & 1], static_cast<uint32_t>((it >> 1) & 1), abort);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t v_addr = smem_addr(v_tile + st * KV_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < BKV / 16; ++kk)  // P lies packed over the first half of its scores
+          umma_ts(tmem + COL_O, tmem + COL_S + (it & 1) * BKV + kk * 8,
+                  umma_desc(v_addr + kk * 16 * 128, KV_HALF, 1024, kLayoutSw128), idesc_o, (it > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&s->pv_done);
+        umma_commit(&s->v_free[st]);
+        // into the buffer of the P just read: one thread's MMAs run in order
+        if (it + 2 < iters) issue_s(it + 2);
+      }
+      if (ok) umma_commit(&s->o_final);
+      umma_commit(&s->teardown);
+      int dummy = 0;
+      mbar_wait(&s->teardown, 0, &dummy);
+    }
+  } else {
+    // ------------------------------------------------------------- softmax
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane, r = row0 + row;  // of the tile, of the unit
+    const Row at = row_of(p, plan.per, u, hk, min(r, rows - 1));
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    auto place = [&](int row, int piece) { return row * 128 + ((piece ^ (row & 7)) * 16); };
+    // Q: the warp's 32 rows, each by D / 8 lanes; rows from the unit's end on are zeros
+    if (iters > 0) {
+      constexpr int LANES = D / 8, STEP = 32 / LANES;
+      const int piece = lane % LANES;
+      const int64_t mine = at.b * p.qb + at.h * p.qh + at.i * p.qn;
+#pragma unroll 8
+      for (int x = 0; x < 32; x += STEP) {
+        const int w = x + lane / LANES;
+        const int64_t from = __shfl_sync(0xffffffffu, mine, w);
+        const uint4 v = row0 + quarter * 32 + w < rows
+                            ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + from + piece * 8)
+                            : make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(q_tile + (piece >> 3) * Q_HALF + place(quarter * 32 + w, piece & 7)) = v;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s->q_full);
+    }
+    const int own_hi = own ? own_keys(p, start + at.i, length) : 0;
+    // what every row of the warp sees
+    const int hi_all = __shfl_sync(0xffffffffu, own_hi, 0);
+    float m_run = -INFINITY, l_run = 0.f;
+    bool ok = true;
+    for (int it = 0; it < iters; ++it) {
+      const int block = first + it;
+      const int key0 = (block < early_blocks ? block : block - early_blocks) * BKV;
+      const int seen = (block < early_blocks ? early : own_hi) - key0;  // leading keys of the block that the row sees
+      const bool full = (block < early_blocks ? early : hi_all) - key0 >= BKV;
+      const uint32_t s_at = lanes + COL_S + (it & 1) * BKV;
+      ok = __all_sync(0xffffffffu, mbar_wait(&s->s_full[it & 1], static_cast<uint32_t>((it >> 1) & 1), abort));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t r[2][32];
+      tmem_ld32(s_at, r[0]);
+      tmem_ld32(s_at + 32, r[1]);
+      tmem_wait_ld();
+      if (!full) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c * 32 + e >= seen) r[c][e] = __float_as_uint(-INFINITY);
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+          top[e / 2 % 4] = max3(top[e / 2 % 4], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+      const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.scale_log2;
+      // the maximum is kept until a row exceeds it by 2^8 (O and l share it: exact); a row
+      // that has seen nothing yet (-inf) has weights and sums of 0
+      const bool grow = mx > m_run + RESCALE;
+      const float m_new = grow ? mx : m_run;
+      const bool rescale = grow && m_run != -INFINITY;
+      if (__any_sync(0xffffffffu, rescale)) {
+        const float corr = rescale ? ex2(m_run - m_new) : 1.f;
+        l_run *= corr;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s->pv_done, static_cast<uint32_t>((it - 1) & 1), abort));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld16(lanes + COL_O + c * 16, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+          tmem_st16(lanes + COL_O + c * 16, o);
+        }
+      }
+      m_run = m_new;
+      // weights 2^(s * scale - m), rounded once to the operand type of the P V product:
+      // the tensor cores take 16 bits. The rounding is relative to each weight and averages
+      // out over the keys; the sum takes the fp32 values. Masked keys give exact zeros
+      const float shift = m_new == -INFINITY ? 0.f : -m_new;
+      const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(shift, shift);
+      float2 sum2 = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float2 x =
+              __ffma2_rn(make_float2(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])), scale2, shift2);
+          const float2 w = make_float2(ex2(x.x), ex2(x.y));
+          sum2 = __fadd2_rn(sum2, w);
+          pk[e] = pack2<T>(w.x, w.y);
+        }
+        tmem_st16(s_at + c * 16, pk);
+      }
+      l_run += sum2.x + sum2.y;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s->p_full[it & 1]);
+    }
+    if (iters > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&s->o_final, 0, abort));
+    ok = ok && *abort == 0;
+    tc_fence_after();
+    if (plan.tile_sums != nullptr) {
+      // this chunk's state; a wait that gave up (device error word) makes the row NaN
+      const int64_t part = ((static_cast<int64_t>(unit) * plan.tiles + tile) * plan.tile_splits + split) * BQ + row;
+      if (r < rows) plan.tile_states[part] = ok ? make_float2(m_run, l_run) : make_float2(NAN, NAN);
+      if (ok && iters > 0) {
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(lanes + COL_O + c * 32, o);
+          tmem_wait_ld();
+          if (r >= rows) continue;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<uint4*>(plan.tile_sums + part * D + c * 32 + e * 4) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+      }
+    } else {
+      const float inv = ok ? 1.f / l_run : NAN;
+      bool finite = true;
+      // the rows into Q's place (every score is computed)
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (iters > 0) {
+          tmem_ld32(lanes + COL_O + c * 32, o);
+          tmem_wait_ld();
+        }
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = iters > 0 ? __uint_as_float(o[2 * e]) * inv : 0.f;
+          const float z = iters > 0 ? __uint_as_float(o[2 * e + 1]) * inv : 0.f;
+          finite = finite && isfinite(x) && isfinite(z);
+          pk[e] = pack2<T>(x, z);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<uint4*>(q_tile + (c >> 1) * Q_HALF + place(row, (c & 1) * 4 + e)) =
+              make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+      }
+      __syncwarp();  // a row that is computed again comes after what was written of it
+      for (uint32_t again = __ballot_sync(0xffffffffu, ok && !finite && r < rows); again != 0; again &= again - 1) {
+        const int from = __ffs(again) - 1, w = quarter * 32 + from;
+        float2 acc[D / 64];
+        attend_row<T, D>(p, __shfl_sync(0xffffffffu, at.b, from), __shfl_sync(0xffffffffu, at.h, from),
+                         __shfl_sync(0xffffffffu, at.i, from), acc);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          *reinterpret_cast<uint32_t*>(q_tile + c * Q_HALF + place(w, lane >> 2) + (lane & 3) * 4) = pack2<T>(acc[c].x, acc[c].y);
+      }
+      __syncwarp();
+      constexpr int LANES = D / 8, STEP = 32 / LANES;
+      const int piece = lane % LANES;
+      const int64_t mine = at.b * p.ob + at.i * p.on + static_cast<int64_t>(at.h) * D;
+#pragma unroll 4
+      for (int x = 0; x < 32; x += STEP) {
+        const int w = x + lane / LANES;
+        const int64_t to = __shfl_sync(0xffffffffu, mine, w);
+        if (row0 + quarter * 32 + w < rows)
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + to + piece * 8) =
+              *reinterpret_cast<const uint4*>(q_tile + (piece >> 3) * Q_HALF + place(quarter * 32 + w, piece & 7));
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, TILE_COLS);
+}
+
+// Writes row (b, h, i), columns [64 c + 2 lane, + 2); rows that are not finite again
+// from visible keys alone (a masked key's V may be NaN or infinite: 0 times it is NaN).
+template <typename T, int D>
+IRIS_DEVICE void finish_row(const Params& p, int b, int h, int i, float2 (&acc)[D / 64], float total) {
+  const float inv = 1.f / total;
+  bool finite = true;
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) {
+    acc[c] = make_float2(acc[c].x * inv, acc[c].y * inv);
+    finite = finite && isfinite(acc[c].x) && isfinite(acc[c].y);
+  }
+  if (!__all_sync(0xffffffffu, finite)) attend_row<T, D>(p, b, h, i, acc);
   T* o = reinterpret_cast<T*>(p.out) + b * p.ob + i * p.on + static_cast<int64_t>(h) * D + 2 * (threadIdx.x & 31);
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) *reinterpret_cast<uint32_t*>(o + 64 * c) = pack2<T>(acc[c].x, acc[c].y);
 }
 
+// 16 rows of a sample and key head over a chunk of their keys: the prefix's (where
+// plan.step_prefix) and then the sample's own. Four warps; the block's others leave at once.
+template <typename T, int D>
+IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* smem_raw) {
+  constexpr int TILE = STEP_KEYS * D * 2;  // bytes of one K or V tile
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = cta % plan.step_splits, unit = cta / plan.step_splits;  // (b, hk, row tile)
+  const int rt = unit % plan.row_tiles, hk = unit / plan.row_tiles % p.heads_kv, b = unit / plan.row_tiles / p.heads_kv;
+  const int group = p.heads_q / p.heads_kv, rows = p.n * group;
+  const int r0 = rt * STEP_ROWS, r_last = min(r0 + STEP_ROWS, rows) - 1;
+  const int early = plan.step_prefix ? prefix_length(p, b) : 0;
+  const int length = own_length(p, b);
+  const int64_t start = own_start(p, b);
+  const int count = early + own_keys(p, start + r_last / group, length);  // some row of the tile sees them
+  const bool same = r0 / group == r_last / group;  // one token: every row sees all of them
+  const int c_begin = min(split * plan.step_chunk, count), c_end = min(c_begin + plan.step_chunk, count);
+
+  const T* pk = reinterpret_cast<const T*>(p.pk) + b / p.per_group * p.pkb + hk * p.pkh;
+  const T* pv = reinterpret_cast<const T*>(p.pv) + b / p.per_group * p.pvb + hk * p.pvh;
+  const T* k = reinterpret_cast<const T*>(p.k) + b * p.kb + hk * p.kh;
+  const T* v = reinterpret_cast<const T*>(p.v) + b * p.vb + hk * p.vh;
+  const uint32_t ring = smem_addr(smem_raw) + warp * (STEP_STAGES * 2 * TILE);
+  const int tiles = (c_end - c_begin + STEP_KEYS - 1) / STEP_KEYS;
+  const int mine = tiles > warp ? (tiles - warp + STEP_WARPS - 1) / STEP_WARPS : 0;
+  // tile t of the warp into its slot: rows of D / 8 16-byte pieces, piece x of row r at x ^ (r & 7)
+  constexpr int PIECES = D / 8;
+  auto load = [&](int t) {
+    if (t < mine) {
+      const int c0 = c_begin + (warp + t * STEP_WARPS) * STEP_KEYS;
+      const uint32_t slot = ring + (t % STEP_STAGES) * 2 * TILE;
+#pragma unroll
+      for (int e = 0; e < STEP_KEYS * PIECES / 32; ++e) {
+        const int at = e * 32 + lane, r = at / PIECES, x = at % PIECES;
+        const int c = c0 + r;
+        const bool real = c < c_end;
+        const T* from_k = real ? (c < early ? pk + c * p.pkn : k + (c - early) * p.kn) + x * 8 : reinterpret_cast<const T*>(p.q);
+        const T* from_v = real ? (c < early ? pv + c * p.pvn : v + (c - early) * p.vn) + x * 8 : reinterpret_cast<const T*>(p.q);
+        const uint32_t dst = slot + r * (D * 2) + ((x ^ (r & 7)) * 16);
+        copy16(dst, from_k, real);
+        copy16(dst + TILE, from_v, real);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int g = lane >> 2, quad = lane & 3;
+  float o[D / 8][4];
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  if (warp < STEP_WARPS) {
+#pragma unroll
+    for (int t = 0; t < STEP_STAGES - 1; ++t) load(t);
+
+    // Q rows as the A operand: this lane's rows g and g + 8, columns 2 (lane % 4) + {0, 1} of each 8
+    uint32_t qa[D / 16][4];
+    int seen[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = min(r0 + g + 8 * u, rows - 1);
+      const int i = r / group, h = hk * group + r % group;
+      seen[u] = early + own_keys(p, start + i, length);
+      const T* q = reinterpret_cast<const T*>(p.q) + b * p.qb + h * p.qh + static_cast<int64_t>(i) * p.qn + 2 * quad;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        qa[d][u] = *reinterpret_cast<const uint32_t*>(q + 16 * d);
+        qa[d][u + 2] = *reinterpret_cast<const uint32_t*>(q + 16 * d + 8);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+
+    for (int t = 0; t < mine; ++t) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STEP_STAGES - 2) : "memory");
+      __syncwarp();  // every lane's copies of the tile have landed; the slot refilled next was read by all
+      load(t + STEP_STAGES - 1);
+      const uint32_t slot = ring + (t % STEP_STAGES) * 2 * TILE;
+      const int c0 = c_begin + (warp + t * STEP_WARPS) * STEP_KEYS;
+      // S: keys [8 j, 8 j + 8) in s[j]
+      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, odd[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) {  // two k steps per load: pieces 4 d .. 4 d + 3 of the 8 key rows
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t kb[4];
+          const int r = 8 * j + (lane & 7), x = 4 * d + (lane >> 3);
+          ldmatrix4(kb, slot + r * (D * 2) + ((x ^ (r & 7)) * 16));
+          mma_16816<T>(s[j], qa[2 * d], kb[0], kb[1]);
+          mma_16816<T>(odd[j], qa[2 * d + 1], kb[2], kb[3]);  // two chains: half the wait for the last
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[j][e] += odd[j][e];
+      if (!same || c0 + STEP_KEYS > c_end) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = c0 + 8 * j + 2 * quad + (e & 1);
+            if (c >= c_end || c >= seen[e >> 1]) s[j][e] = -INFINITY;
+          }
+      }
+      bool rescale = false;
+      float corr[2], shift[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float mx = fmaxf(fmaxf(s[0][2 * u], s[0][2 * u + 1]), fmaxf(s[1][2 * u], s[1][2 * u + 1])) * p.scale_log2;
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const bool grow = mx > m_run[u] + RESCALE;
+        const float m_new = grow ? mx : m_run[u];
+        corr[u] = grow && m_run[u] != -INFINITY ? ex2(m_run[u] - m_new) : 1.f;
+        rescale = rescale || corr[u] != 1.f;
+        m_run[u] = m_new;
+        shift[u] = m_new == -INFINITY ? 0.f : -m_new;
+      }
+      if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][e] *= corr[e >> 1];
+        l_run[0] *= corr[0];
+        l_run[1] *= corr[1];
+      }
+      // weights, rounded once to the operand type (the fp32 values go into the totals): as in
+      // tile_cta, so that a row is as accurate in either form
+      uint32_t pa[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float w0 = ex2(fmaf(s[j][2 * u], p.scale_log2, shift[u]));
+          const float w1 = ex2(fmaf(s[j][2 * u + 1], p.scale_log2, shift[u]));
+          l_run[u] += w0 + w1;
+          pa[2 * j + u] = pack2<T>(w0, w1);
+        }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {  // 16 columns per load: key rows 0-7 and 8-15, pieces 2 d and 2 d + 1
+        uint32_t vb[4];
+        const int r = lane & 15, x = 2 * d + (lane >> 4);
+        ldmatrix4_trans(vb, slot + TILE + r * (D * 2) + ((x ^ (r & 7)) * 16));
+        mma_16816<T>(o[2 * d], pa, vb[0], vb[1]);
+        mma_16816<T>(o[2 * d + 1], pa, vb[2], vb[3]);
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      l_run[u] += __shfl_xor_sync(0xffffffffu, l_run[u], 1);
+      l_run[u] += __shfl_xor_sync(0xffffffffu, l_run[u], 2);
+    }
+  }
+  // the warps' states, joined per row: warp w finishes rows w, w + 4, ...
+  __syncthreads();  // the rings are done with
+  float* sums = reinterpret_cast<float*>(smem_raw);  // [warp][16][D]
+  __shared__ float tops[STEP_WARPS][STEP_ROWS], totals[STEP_WARPS][STEP_ROWS];
+  if (warp < STEP_WARPS) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float* dst = sums + (warp * STEP_ROWS + g + 8 * u) * D + 2 * quad;
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(dst + 8 * d) = make_float2(o[d][2 * u], o[d][2 * u + 1]);
+      if (quad == 0) {
+        tops[warp][g + 8 * u] = m_run[u];
+        totals[warp][g + 8 * u] = l_run[u];
+      }
+    }
+  }
+  __syncthreads();
+  if (warp >= STEP_WARPS) return;
+  for (int r = warp; r <= r_last - r0; r += STEP_WARPS) {
+    float top = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < STEP_WARPS; ++w) top = fmaxf(top, tops[w][r]);
+    float2 acc[D / 64];
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < STEP_WARPS; ++w) {
+      // a warp that saw nothing has sums of 0 (or NaN, from a masked V: kept, it marks the row)
+      const float f = tops[w][r] == -INFINITY ? 1.f : ex2(tops[w][r] - top);
+      total += f * totals[w][r];
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        const float2 x = *reinterpret_cast<const float2*>(sums + (w * STEP_ROWS + r) * D + 64 * c + 2 * lane);
+        acc[c] = make_float2(fmaf(f, x.x, acc[c].x), fmaf(f, x.y, acc[c].y));
+      }
+    }
+    if (plan.step_sums == nullptr) {
+      finish_row<T, D>(p, b, hk * group + (r0 + r) % group, (r0 + r) / group, acc, total);
+    } else {
+      const int64_t part = (static_cast<int64_t>(unit) * plan.step_splits + split) * STEP_ROWS + r;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) *reinterpret_cast<float2*>(plan.step_sums + part * D + 64 * c + 2 * lane) = acc[c];
+      if (lane == 0) plan.step_states[part] = make_float2(top, total);
+    }
+  }
+}
+
+// Both kinds of CTA in one launch, mixed evenly: tiles are bound by the tensor cores and
+// exponentials, the others by memory.
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 2)
+    attend_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ CUtensorMap tpv,
+                  const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                  const __grid_constant__ Params p, const __grid_constant__ Plan plan) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  grid_wait();
+  grid_trigger();
+  const int64_t all = static_cast<int64_t>(plan.tile_ctas) + plan.step_ctas;
+  const int before = static_cast<int>(blockIdx.x * static_cast<int64_t>(plan.tile_ctas) / all);
+  const bool tile = (blockIdx.x + 1) * static_cast<int64_t>(plan.tile_ctas) / all > before;
+  if (tile) tile_cta<T, D>(tpk, tpv, tk, tv, p, plan, before, smem_raw);
+  else step_cta<T, D>(p, plan, static_cast<int>(blockIdx.x) - before, smem_raw);
+}
+
+// A row's chunks joined by a warp.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Params p, const __grid_constant__ Plan plan) {
+  const int lane = threadIdx.x & 31;
+  const int group = p.heads_q / p.heads_kv;
+  const int64_t rows = static_cast<int64_t>(p.batch) * p.n * p.heads_q;
+  const int64_t index = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  grid_wait();
+  grid_trigger();
+  if (index >= rows) return;
+  const int h = static_cast<int>(index % p.heads_q), i = static_cast<int>(index / p.heads_q % p.n);
+  const int b = static_cast<int>(index / p.heads_q / p.n);
+  const int hk = h / group;
+  int64_t tile0 = 0, step0 = 0;  // of its states: first place, and how many there are, BQ or STEP_ROWS apart
+  int tile_parts = 0, step_parts = 0;
+  if (plan.tile_sums != nullptr) {
+    const int64_t r = (static_cast<int64_t>(b % plan.per) * p.n + i) * group + h % group;
+    const int64_t unit = static_cast<int64_t>(b / plan.per) * p.heads_kv + hk;
+    tile0 = (unit * plan.tiles + r / BQ) * plan.tile_splits * BQ + r % BQ;
+    tile_parts = plan.tile_splits;
+  }
+  if (plan.step_sums != nullptr) {
+    const int64_t r = static_cast<int64_t>(i) * group + h % group;
+    const int64_t unit = (static_cast<int64_t>(b) * p.heads_kv + hk) * plan.row_tiles + r / STEP_ROWS;
+    step0 = unit * plan.step_splits * STEP_ROWS + r % STEP_ROWS;
+    step_parts = plan.step_splits;
+  }
+  const int parts = tile_parts + step_parts;
+  auto state_of = [&](int c) {
+    return c < tile_parts ? plan.tile_states[tile0 + static_cast<int64_t>(c) * BQ]
+                          : plan.step_states[step0 + static_cast<int64_t>(c - tile_parts) * STEP_ROWS];
+  };
+  float top = -INFINITY;
+  for (int c = lane; c < parts; c += 32) top = fmaxf(top, state_of(c).x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float total = 0.f;
+  bool lost = false;  // a wait gave up
+  float2 acc[D / 64];
+#pragma unroll
+  for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
+#pragma unroll 4
+  for (int c = 0; c < parts; ++c) {
+    const float2 st = state_of(c);
+    lost = lost || (isnan(st.x) && isnan(st.y));
+    if (st.x == -INFINITY && st.y == 0.f) continue;  // it saw nothing; a tile without keys wrote no sums
+    const float f = st.x == -INFINITY ? 1.f : ex2(st.x - top);
+    total = fmaf(f, st.y, total);
+    const float* from = c < tile_parts ? plan.tile_sums + (tile0 + static_cast<int64_t>(c) * BQ) * D
+                                       : plan.step_sums + (step0 + static_cast<int64_t>(c - tile_parts) * STEP_ROWS) * D;
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d) {
+      const float2 x = *reinterpret_cast<const float2*>(from + 64 * d + 2 * lane);
+      acc[d] = make_float2(fmaf(f, x.x, acc[d].x), fmaf(f, x.y, acc[d].y));
+    }
+  }
+  if (lost) {
+    T* o = reinterpret_cast<T*>(p.out) + b * p.ob + i * p.on + static_cast<int64_t>(h) * D + 2 * lane;
+    for (int c = 0; c < D / 64; ++c) *reinterpret_cast<uint32_t*>(o + 64 * c) = pack2<T>(NAN, NAN);
+    return;
+  }
+  finish_row<T, D>(p, b, h, i, acc, total);
+}
+
+// How a call is cut up, from its sizes alone (lengths are on the device: n_prefix and
+// n_kv bound them).
+struct Sizes {
+  int64_t batch, groups, heads_q, heads_kv, n, n_prefix, n_kv, right;
+};
+
+int make_plan(const Sizes& z, Plan* out) {
+  Plan plan = {};
+  const int64_t group = z.heads_q / z.heads_kv, rows = z.n * group, per_group = z.batch / z.groups;
+  const int64_t slots = 2 * num_sms();
+  const bool whole = rows >= 64;  // a sample's rows fill tiles
+  const bool shared = !whole && z.n_prefix >= 256 && per_group > 1;
+  plan.per = static_cast<int>(whole ? 1 : per_group);
+  if (whole || shared) {
+    const int64_t units = z.batch / plan.per * z.heads_kv, tiles = (plan.per * rows + BQ - 1) / BQ;
+    const int64_t blocks = (z.n_prefix + BKV - 1) / BKV + (whole ? (z.n_kv + BKV - 1) / BKV : 0);
+    const int64_t splits = std::max<int64_t>(1, std::min((slots + units * tiles - 1) / (units * tiles), blocks / 4));
+    plan.tiles = static_cast<int>(tiles);
+    plan.tile_chunk = static_cast<int>(std::max<int64_t>(1, (blocks + splits - 1) / splits));
+    plan.tile_splits = static_cast<int>(std::max<int64_t>(1, (blocks + plan.tile_chunk - 1) / plan.tile_chunk));
+    IRIS_REQUIRE(units * tiles * plan.tile_splits < (1ll << 30), "prefix_attn_fwd: too many rows");
+    plan.tile_ctas = static_cast<int>(units * tiles * plan.tile_splits);
+  }
+  if (!whole) {
+    plan.row_tiles = static_cast<int>((rows + STEP_ROWS - 1) / STEP_ROWS);
+    plan.step_prefix = !shared;
+    const int64_t units = z.batch * z.heads_kv * plan.row_tiles, keys = z.n_kv + (shared ? 0 : z.n_prefix);
+    const int64_t splits = std::max<int64_t>(1, std::min((slots + units - 1) / units, keys / 128));
+    plan.step_chunk = static_cast<int>(std::max<int64_t>(64, ((keys + splits - 1) / splits + 63) / 64 * 64));
+    plan.step_splits = static_cast<int>(std::max<int64_t>(1, (keys + plan.step_chunk - 1) / plan.step_chunk));
+    IRIS_REQUIRE(units * plan.step_splits < (1ll << 30), "prefix_attn_fwd: too many rows");
+    plan.step_ctas = static_cast<int>(units * plan.step_splits);
+  }
+  *out = plan;
+  return IRIS_OK;
+}
+
+// Floats of the parts' sums, and as many pairs of a maximum and a total as rows of them.
+struct Room {
+  int64_t tile_rows, step_rows;
+};
+inline Room room_of(const Plan& plan) {
+  Room x = {};
+  const bool parts = (plan.tiles > 0 && plan.step_splits > 0) || plan.tile_splits > 1 || plan.step_splits > 1;
+  if (parts) x = {static_cast<int64_t>(plan.tile_ctas) * BQ, static_cast<int64_t>(plan.step_ctas) * STEP_ROWS};
+  return x;
+}
+inline int64_t room_bytes(const Room& x, int64_t d) { return (x.tile_rows + x.step_rows) * (d + 2) * 4; }
+
 template <typename T, int D>
 int launch(const Params& p, int dtype, void* workspace, int64_t workspace_bytes, cudaStream_t st) {
   const int64_t rows = static_cast<int64_t>(p.batch) * p.n * p.heads_q;
   IRIS_REQUIRE(rows < (1ll << 31), "prefix_attn_fwd: too many rows");
-  IRIS_CUDA(launch_early(rows_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, 1, p));
+  Plan plan;
+  IRIS_CHECK_STATUS(make_plan(Sizes{p.batch, p.batch / p.per_group, p.heads_q, p.heads_kv, p.n, p.n_prefix, p.n_kv, p.right}, &plan));
+  const Room room = room_of(plan);
+  if (room.tile_rows + room.step_rows > 0) {
+    IRIS_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= room_bytes(room, D),
+                 "prefix_attn_fwd: workspace too small");
+    float* at = static_cast<float*>(workspace);
+    if (room.tile_rows > 0) plan.tile_sums = at;
+    at += room.tile_rows * D;
+    if (room.step_rows > 0) plan.step_sums = at;
+    at += room.step_rows * D;
+    plan.tile_states = reinterpret_cast<float2*>(at);
+    plan.step_states = plan.tile_states + room.tile_rows;
+  }
+  CUtensorMap tpk = {}, tpv = {}, tk = {}, tv = {};
+  if (plan.tiles > 0) {
+    if (p.n_prefix > 0) {
+      const int groups = p.batch / p.per_group;
+      IRIS_CHECK_STATUS(make_tmap_heads(&tpk, p.pk, dtype, D, p.n_prefix, p.heads_kv, groups, p.pkn, p.pkh, p.pkb, BKV));
+      IRIS_CHECK_STATUS(make_tmap_heads(&tpv, p.pv, dtype, D, p.n_prefix, p.heads_kv, groups, p.pvn, p.pvh, p.pvb, BKV));
+    }
+    if (plan.step_splits == 0 && p.n_kv > 0) {
+      IRIS_CHECK_STATUS(make_tmap_heads(&tk, p.k, dtype, D, p.n_kv, p.heads_kv, p.batch, p.kn, p.kh, p.kb, BKV));
+      IRIS_CHECK_STATUS(make_tmap_heads(&tv, p.v, dtype, D, p.n_kv, p.heads_kv, p.batch, p.vn, p.vh, p.vb, BKV));
+    }
+  }
+  auto kernel = attend_kernel<T, D>;
+  static bool configured[64] = {false};
+  int dev = 0;
+  IRIS_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !configured[dev]) {
+    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem<D>()));
+    if (dev < 64) configured[dev] = true;
+  }
+  const int smem = plan.tiles == 0 ? step_smem<D>() : plan.step_splits == 0 ? tile_smem<D>() : most_smem<D>();
+  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(plan.tile_ctas + plan.step_ctas)), THREADS, smem, st, 1, tpk, tpv, tk,
+                         tv, p, plan));
+  if (room.tile_rows + room.step_rows == 0) return IRIS_OK;
+  IRIS_CUDA(launch_early(join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, 1, p, plan));
   return IRIS_OK;
 }
 
@@ -166,6 +959,10 @@ extern "C" int iris_prefix_attn_workspace(const iris_prefix_problem* q, int64_t*
   IRIS_REQUIRE(q != nullptr && bytes != nullptr, "prefix_attn_workspace: null pointer");
   IRIS_CHECK_STATUS(check_sizes(*q));
   *bytes = 0;
+  if (q->batch * q->n == 0) return IRIS_OK;
+  Plan plan;
+  IRIS_CHECK_STATUS(make_plan(Sizes{q->batch, q->groups, q->heads_q, q->heads_kv, q->n, q->n_prefix, q->n_kv, bound(q->right)}, &plan));
+  *bytes = room_bytes(room_of(plan), q->head_dim);
   return IRIS_OK;
 }
 
