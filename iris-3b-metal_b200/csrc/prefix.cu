@@ -130,6 +130,9 @@ __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, fl
 // not finite is computed again by attend_row, which reads visible keys alone.
 constexpr int BQ = 128, BKV = 64, KV = 2;  // rows, keys of a block, slots of the K and V rings
 constexpr int THREADS = 192;
+// Two CTAs to an SM: warp w of each sits in quarter w % 4 of the SM, whose registers hold
+// four such warps (two of either CTA) at 128 each, not at the 168 that 2 x 192 threads would share
+constexpr int BOUND_THREADS = 256;
 constexpr int Q_HALF = BQ * 128, KV_HALF = BKV * 128;  // bytes of 64 columns of a tile
 constexpr uint32_t COL_S = 0, COL_O = 2 * BKV, TILE_COLS = 256;
 
@@ -201,22 +204,6 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int group = p.heads_q / p.heads_kv, rows = plan.per * p.n * group;
-  const int split = cta % plan.tile_splits, unit_tile = cta / plan.tile_splits;
-  // later rows first: under a causal mask they see the most keys
-  const int units = p.batch / plan.per * p.heads_kv;
-  const int unit = unit_tile % units, tile = plan.tiles - 1 - unit_tile / units;
-  const int hk = unit % p.heads_kv, u = unit / p.heads_kv;
-  const int row0 = tile * BQ, last = min(row0 + BQ, rows) - 1;
-  const int b0 = u * plan.per, g = b0 / p.per_group;
-  const bool own = plan.per == 1 && plan.step_splits == 0;
-  const int early = prefix_length(p, b0);
-  const int length = own ? own_length(p, b0) : 0;
-  const int64_t start = own ? own_start(p, b0) : 0;
-  const int early_blocks = (early + BKV - 1) / BKV;
-  const int all_blocks = early_blocks + (own ? (own_keys(p, start + last / group, length) + BKV - 1) / BKV : 0);
-  const int first = min(split * plan.tile_chunk, all_blocks);
-  const int iters = min(plan.tile_chunk, all_blocks - first);
-
   if (threadIdx.x == 0) {
     mbar_init(&s->q_full, 4);
     for (int i = 0; i < KV; ++i) {
@@ -242,6 +229,24 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
   tc_fence_after();
   const uint32_t tmem = s->tmem_base;
   volatile int* abort = &s->abort;
+
+  grid_wait();
+  grid_trigger();
+  const int split = cta % plan.tile_splits, unit_tile = cta / plan.tile_splits;
+  // later rows first: under a causal mask they see the most keys
+  const int units = p.batch / plan.per * p.heads_kv;
+  const int unit = unit_tile % units, tile = plan.tiles - 1 - unit_tile / units;
+  const int hk = unit % p.heads_kv, u = unit / p.heads_kv;
+  const int row0 = tile * BQ, last = min(row0 + BQ, rows) - 1;
+  const int b0 = u * plan.per, g = b0 / p.per_group;
+  const bool own = plan.per == 1 && plan.step_splits == 0;
+  const int early = prefix_length(p, b0);
+  const int length = own ? own_length(p, b0) : 0;
+  const int64_t start = own ? own_start(p, b0) : 0;
+  const int early_blocks = (early + BKV - 1) / BKV;
+  const int all_blocks = early_blocks + (own ? (own_keys(p, start + last / group, length) + BKV - 1) / BKV : 0);
+  const int first = min(split * plan.tile_chunk, all_blocks);
+  const int iters = min(plan.tile_chunk, all_blocks - first);
 
   if (warp == 0) {
     // ----------------------------------------------------------------- TMA
@@ -368,15 +373,14 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
       constexpr int LANES = D / 8, STEP = 32 / LANES;
       const int piece = lane % LANES;
       const int64_t mine = at.b * p.qb + at.h * p.qh + at.i * p.qn;
-#pragma unroll 8
+      const uint32_t to = smem_addr(q_tile) + (piece >> 3) * Q_HALF;
+#pragma unroll
       for (int x = 0; x < 32; x += STEP) {
         const int w = x + lane / LANES;
-        const int64_t from = __shfl_sync(0xffffffffu, mine, w);
-        const uint4 v = row0 + quarter * 32 + w < rows
-                            ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + from + piece * 8)
-                            : make_uint4(0u, 0u, 0u, 0u);
-        *reinterpret_cast<uint4*>(q_tile + (piece >> 3) * Q_HALF + place(quarter * 32 + w, piece & 7)) = v;
+        const T* from = reinterpret_cast<const T*>(p.q) + __shfl_sync(0xffffffffu, mine, w) + piece * 8;
+        copy16(to + place(quarter * 32 + w, piece & 7), from, row0 + quarter * 32 + w < rows);
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s->q_full);
@@ -463,26 +467,31 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
     if (iters > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&s->o_final, 0, abort));
     ok = ok && *abort == 0;
     tc_fence_after();
+    // rows leave from the place of Q and the rings (every product is computed), each as one
+    // bulk copy; 16 bytes of padding spread a piece of 8 rows over the banks
     if (plan.tile_sums != nullptr) {
       // this chunk's state; a wait that gave up (device error word) makes the row NaN
       const int64_t part = ((static_cast<int64_t>(unit) * plan.tiles + tile) * plan.tile_splits + split) * BQ + row;
       if (r < rows) plan.tile_states[part] = ok ? make_float2(m_run, l_run) : make_float2(NAN, NAN);
       if (ok && iters > 0) {
-#pragma unroll 1
+        uint8_t* mine = q_tile + row * (D * 4 + 16);
+#pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tmem_ld32(lanes + COL_O + c * 32, o);
           tmem_wait_ld();
-          if (r >= rows) continue;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<uint4*>(plan.tile_sums + part * D + c * 32 + e * 4) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            *reinterpret_cast<uint4*>(mine + c * 128 + e * 16) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
         }
+        fence_proxy_async_smem();
+        if (r < rows) bulk_store(plan.tile_sums + part * D, mine, D * 4);
+        tma_store_wait();
       }
     } else {
       const float inv = ok ? 1.f / l_run : NAN;
       bool finite = true;
-      // the rows into Q's place (every score is computed)
+      uint8_t* mine = q_tile + row * (D * 2 + 16);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -500,31 +509,22 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<uint4*>(q_tile + (c >> 1) * Q_HALF + place(row, (c & 1) * 4 + e)) =
-              make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+          *reinterpret_cast<uint4*>(mine + c * 64 + e * 16) = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
       }
       __syncwarp();  // a row that is computed again comes after what was written of it
       for (uint32_t again = __ballot_sync(0xffffffffu, ok && !finite && r < rows); again != 0; again &= again - 1) {
-        const int from = __ffs(again) - 1, w = quarter * 32 + from;
+        const int from = __ffs(again) - 1;
         float2 acc[D / 64];
         attend_row<T, D>(p, __shfl_sync(0xffffffffu, at.b, from), __shfl_sync(0xffffffffu, at.h, from),
                          __shfl_sync(0xffffffffu, at.i, from), acc);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          *reinterpret_cast<uint32_t*>(q_tile + c * Q_HALF + place(w, lane >> 2) + (lane & 3) * 4) = pack2<T>(acc[c].x, acc[c].y);
+          *reinterpret_cast<uint32_t*>(q_tile + (quarter * 32 + from) * (D * 2 + 16) + c * 128 + lane * 4) = pack2<T>(acc[c].x, acc[c].y);
       }
+      fence_proxy_async_smem();
       __syncwarp();
-      constexpr int LANES = D / 8, STEP = 32 / LANES;
-      const int piece = lane % LANES;
-      const int64_t mine = at.b * p.ob + at.i * p.on + static_cast<int64_t>(at.h) * D;
-#pragma unroll 4
-      for (int x = 0; x < 32; x += STEP) {
-        const int w = x + lane / LANES;
-        const int64_t to = __shfl_sync(0xffffffffu, mine, w);
-        if (row0 + quarter * 32 + w < rows)
-          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + to + piece * 8) =
-              *reinterpret_cast<const uint4*>(q_tile + (piece >> 3) * Q_HALF + place(quarter * 32 + w, piece & 7));
-      }
+      if (r < rows) bulk_store(reinterpret_cast<T*>(p.out) + at.b * p.ob + at.i * p.on + static_cast<int64_t>(at.h) * D, mine, D * 2);
+      tma_store_wait();
     }
   }
 
@@ -551,12 +551,27 @@ IRIS_DEVICE void finish_row(const Params& p, int b, int h, int i, float2 (&acc)[
   for (int c = 0; c < D / 64; ++c) *reinterpret_cast<uint32_t*>(o + 64 * c) = pack2<T>(acc[c].x, acc[c].y);
 }
 
+// Rows of keys or values: row c at `at` + 16 stride c, which is row c - first of the tensor.
+struct KeyRows {
+  uint64_t at;
+  uint32_t stride;  // 16-byte pieces: strides are below 2^34 elements
+};
+template <typename T>
+IRIS_DEVICE KeyRows key_rows(const void* data, int64_t offset, int64_t stride, int first) {
+  return KeyRows{reinterpret_cast<uint64_t>(reinterpret_cast<const T*>(data) + offset - first * stride), static_cast<uint32_t>(stride / 8)};
+}
+
 // 16 rows of a sample and key head over a chunk of their keys: the prefix's (where
 // plan.step_prefix) and then the sample's own. Four warps; the block's others leave at once.
 template <typename T, int D>
 IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* smem_raw) {
   constexpr int TILE = STEP_KEYS * D * 2;  // bytes of one K or V tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // no second CTA starts on the SM while one of a kernel that allocates TMEM may still do so
+  // (measured: step CTAs alone ran one at a time, 41 us instead of 23)
+  if (warp == STEP_WARPS) tmem_relinquish();
+  grid_wait();
+  grid_trigger();
   const int split = cta % plan.step_splits, unit = cta / plan.step_splits;  // (b, hk, row tile)
   const int rt = unit % plan.row_tiles, hk = unit / plan.row_tiles % p.heads_kv, b = unit / plan.row_tiles / p.heads_kv;
   const int group = p.heads_q / p.heads_kv, rows = p.n * group;
@@ -568,10 +583,10 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
   const bool same = r0 / group == r_last / group;  // one token: every row sees all of them
   const int c_begin = min(split * plan.step_chunk, count), c_end = min(c_begin + plan.step_chunk, count);
 
-  const T* pk = reinterpret_cast<const T*>(p.pk) + b / p.per_group * p.pkb + hk * p.pkh;
-  const T* pv = reinterpret_cast<const T*>(p.pv) + b / p.per_group * p.pvb + hk * p.pvh;
-  const T* k = reinterpret_cast<const T*>(p.k) + b * p.kb + hk * p.kh;
-  const T* v = reinterpret_cast<const T*>(p.v) + b * p.vb + hk * p.vh;
+  // where key c of each lot would start, and its rows' stride in 16-byte pieces: one multiplication a copy
+  const int pb = b / p.per_group;
+  const KeyRows pk = key_rows<T>(p.pk, pb * p.pkb + hk * p.pkh, p.pkn, 0), pv = key_rows<T>(p.pv, pb * p.pvb + hk * p.pvh, p.pvn, 0);
+  const KeyRows k = key_rows<T>(p.k, b * p.kb + hk * p.kh, p.kn, early), v = key_rows<T>(p.v, b * p.vb + hk * p.vh, p.vn, early);
   const uint32_t ring = smem_addr(smem_raw) + warp * (STEP_STAGES * 2 * TILE);
   const int tiles = (c_end - c_begin + STEP_KEYS - 1) / STEP_KEYS;
   const int mine = tiles > warp ? (tiles - warp + STEP_WARPS - 1) / STEP_WARPS : 0;
@@ -586,11 +601,13 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
         const int at = e * 32 + lane, r = at / PIECES, x = at % PIECES;
         const int c = c0 + r;
         const bool real = c < c_end;
-        const T* from_k = real ? (c < early ? pk + c * p.pkn : k + (c - early) * p.kn) + x * 8 : reinterpret_cast<const T*>(p.q);
-        const T* from_v = real ? (c < early ? pv + c * p.pvn : v + (c - early) * p.vn) + x * 8 : reinterpret_cast<const T*>(p.q);
+        const bool of_prefix = c < early;
+        const uint64_t key = static_cast<uint32_t>(real ? c : c_begin);
+        const uint64_t from_k = (of_prefix ? pk.at : k.at) + key * (of_prefix ? pk.stride : k.stride) * 16 + x * 16;
+        const uint64_t from_v = (of_prefix ? pv.at : v.at) + key * (of_prefix ? pv.stride : v.stride) * 16 + x * 16;
         const uint32_t dst = slot + r * (D * 2) + ((x ^ (r & 7)) * 16);
-        copy16(dst, from_k, real);
-        copy16(dst + TILE, from_v, real);
+        copy16(dst, reinterpret_cast<const void*>(from_k), real);
+        copy16(dst + TILE, reinterpret_cast<const void*>(from_v), real);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -599,23 +616,30 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
   float o[D / 8][4];
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
   if (warp < STEP_WARPS) {
+    // Q's 16 rows into the slot that is filled last, then the first tiles
+    const uint32_t q_slot = ring + (STEP_STAGES - 1) * 2 * TILE;
+#pragma unroll
+    for (int e = 0; e < STEP_ROWS * PIECES / 32; ++e) {
+      const int at = e * 32 + lane, w = at / PIECES, x = at % PIECES;
+      const int r = min(r0 + w, rows - 1);
+      const T* q = reinterpret_cast<const T*>(p.q) + b * p.qb + (hk * group + r % group) * p.qh + static_cast<int64_t>(r / group) * p.qn;
+      copy16(q_slot + w * (D * 2) + ((x ^ (w & 7)) * 16), q + x * 8, r0 + w < rows);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
     for (int t = 0; t < STEP_STAGES - 1; ++t) load(t);
 
-    // Q rows as the A operand: this lane's rows g and g + 8, columns 2 (lane % 4) + {0, 1} of each 8
+    // as the A operand: this lane's rows g and g + 8, columns 2 (lane % 4) + {0, 1} of each 8
     uint32_t qa[D / 16][4];
     int seen[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int r = min(r0 + g + 8 * u, rows - 1);
-      const int i = r / group, h = hk * group + r % group;
-      seen[u] = early + own_keys(p, start + i, length);
-      const T* q = reinterpret_cast<const T*>(p.q) + b * p.qb + h * p.qh + static_cast<int64_t>(i) * p.qn + 2 * quad;
+    for (int u = 0; u < 2; ++u) seen[u] = early + own_keys(p, start + min(r0 + g + 8 * u, rows - 1) / group, length);
+    asm volatile("cp.async.wait_group %0;" ::"n"(STEP_STAGES - 1) : "memory");
+    __syncwarp();
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        qa[d][u] = *reinterpret_cast<const uint32_t*>(q + 16 * d);
-        qa[d][u + 2] = *reinterpret_cast<const uint32_t*>(q + 16 * d + 8);
-      }
+    for (int d = 0; d < D / 16; ++d) {  // matrices: rows 0-7 and 8-15 of piece 2 d, then of 2 d + 1
+      const int r = lane & 15, x = 2 * d + (lane >> 4);
+      ldmatrix4(qa[d], q_slot + r * (D * 2) + ((x ^ (r & 7)) * 16));
     }
 #pragma unroll
     for (int d = 0; d < D / 8; ++d)
@@ -754,13 +778,11 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
 // Both kinds of CTA in one launch, mixed evenly: tiles are bound by the tensor cores and
 // exponentials, the others by memory.
 template <typename T, int D>
-__global__ void __launch_bounds__(THREADS, 2)
+__global__ void __launch_bounds__(BOUND_THREADS, 2)
     attend_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ CUtensorMap tpv,
                   const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                   const __grid_constant__ Params p, const __grid_constant__ Plan plan) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  grid_wait();
-  grid_trigger();
   const int64_t all = static_cast<int64_t>(plan.tile_ctas) + plan.step_ctas;
   const int before = static_cast<int>(blockIdx.x * static_cast<int64_t>(plan.tile_ctas) / all);
   const bool tile = (blockIdx.x + 1) * static_cast<int64_t>(plan.tile_ctas) / all > before;
@@ -809,21 +831,30 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Param
   float2 acc[D / 64];
 #pragma unroll
   for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
-#pragma unroll 4
-  for (int c = 0; c < parts; ++c) {
-    const float2 st = state_of(c);
+  for (int c0 = 0; c0 < parts; c0 += 32) {
+    // a lane's part: its factor; one that saw nothing has none (a tile without keys wrote no sums)
+    const float2 st = c0 + lane < parts ? state_of(c0 + lane) : make_float2(-INFINITY, 0.f);
+    const bool real = st.x != -INFINITY || st.y != 0.f;
+    const float f = !real ? 0.f : st.x == -INFINITY ? 1.f : ex2(st.x - top);
+    total += real ? f * st.y : 0.f;
     lost = lost || (isnan(st.x) && isnan(st.y));
-    if (st.x == -INFINITY && st.y == 0.f) continue;  // it saw nothing; a tile without keys wrote no sums
-    const float f = st.x == -INFINITY ? 1.f : ex2(st.x - top);
-    total = fmaf(f, st.y, total);
-    const float* from = c < tile_parts ? plan.tile_sums + (tile0 + static_cast<int64_t>(c) * BQ) * D
-                                       : plan.step_sums + (step0 + static_cast<int64_t>(c - tile_parts) * STEP_ROWS) * D;
+    const uint32_t some = __ballot_sync(0xffffffffu, real);
+    const int most = min(32, parts - c0);
+#pragma unroll 4
+    for (int e = 0; e < most; ++e) {
+      const int c = c0 + e;
+      const float* from = c < tile_parts ? plan.tile_sums + (tile0 + static_cast<int64_t>(c) * BQ) * D
+                                         : plan.step_sums + (step0 + static_cast<int64_t>(c - tile_parts) * STEP_ROWS) * D;
+      const float fc = __shfl_sync(0xffffffffu, f, e);
 #pragma unroll
-    for (int d = 0; d < D / 64; ++d) {
-      const float2 x = *reinterpret_cast<const float2*>(from + 64 * d + 2 * lane);
-      acc[d] = make_float2(fmaf(f, x.x, acc[d].x), fmaf(f, x.y, acc[d].y));
+      for (int d = 0; d < D / 64; ++d) {
+        const float2 x = *reinterpret_cast<const float2*>(from + 64 * d + 2 * lane);
+        if (some >> e & 1u) acc[d] = make_float2(fmaf(fc, x.x, acc[d].x), fmaf(fc, x.y, acc[d].y));
+      }
     }
   }
+  total = warp_sum(total);
+  lost = __any_sync(0xffffffffu, lost);
   if (lost) {
     T* o = reinterpret_cast<T*>(p.out) + b * p.ob + i * p.on + static_cast<int64_t>(h) * D + 2 * lane;
     for (int c = 0; c < D / 64; ++c) *reinterpret_cast<uint32_t*>(o + 64 * c) = pack2<T>(NAN, NAN);
@@ -917,6 +948,7 @@ int launch(const Params& p, int dtype, void* workspace, int64_t workspace_bytes,
   IRIS_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !configured[dev]) {
     IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem<D>()));
+    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     if (dev < 64) configured[dev] = true;
   }
   const int smem = plan.tiles == 0 ? step_smem<D>() : plan.step_splits == 0 ? tile_smem<D>() : most_smem<D>();
@@ -978,6 +1010,7 @@ extern "C" int iris_prefix_attn_fwd(const iris_prefix_problem* q, void* stream) 
   for (int i = 0; i < 5; ++i) {
     IRIS_REQUIRE(rows_aligned(all[i]), "prefix_attn_fwd: pointers and strides must be multiples of 16 bytes");
     IRIS_REQUIRE(rows_apart(all[i], tokens[i]), "prefix_attn_fwd: rows must not repeat along the tokens");
+    IRIS_REQUIRE(all[i].stride_n < (1ll << 34), "prefix_attn_fwd: rows must lie less than 2^34 elements apart");
   }
   IRIS_REQUIRE(aligned16(q->out) && q->out_stride_b % 8 == 0 && q->out_stride_n % 8 == 0,
                "prefix_attn_fwd: pointers and strides must be multiples of 16 bytes");

@@ -45,7 +45,7 @@ def test_c_entries_refuse_bad_arguments(lib):  # noqa: F811
                          (dict(m=1 << 30), "sizes"), (dict(p=1 << 30), "sizes"), (dict(n=1 << 30), "sizes"), (dict(p=-1), "sizes"),
                          (dict(batch=65536), "sizes"), (dict(groups=0), "groups"), (dict(groups=4), "groups"), (dict(kv=0), "heads_kv"),
                          (dict(qn=0), "repeat"), (dict(pn=0), "repeat"), (dict(kn=0), "repeat"), (dict(vb=-128), "repeat"),
-                         (dict(q=0), "null"), (dict(out=0), "null")]:  # fmt: skip
+                         (dict(kn=1 << 34), "apart"), (dict(q=0), "null"), (dict(out=0), "null")]:  # fmt: skip
         assert message in _einval(lib, "iris_prefix_attn_fwd", attend(**bad), None), bad
     for name in ("iris_prefix_attn_fwd", "iris_prefix_attn_workspace"):
         assert "null" in _einval(lib, name, None, None)
