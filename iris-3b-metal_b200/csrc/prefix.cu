@@ -150,11 +150,14 @@ constexpr int tile_smem() {
 
 // ------------------------------------------------- few rows over many keys
 // A sample's own keys where its rows fill no tile, and all of its keys where they are
-// few: a CTA takes 16 query rows of a sample and key head (read once for all of them) and a
-// chunk of the keys; its warps walk 16-key tiles of their own, each with its own softmax state
-// and its own ring of cp.async copies (no barrier until the end), scores and P V on
-// mma.sync m16n8k16: HBM-bound.
-constexpr int STEP_WARPS = 4, STEP_STAGES = 3, STEP_KEYS = 16, STEP_ROWS = 16;
+// few: a CTA takes 8 or 16 query rows of a sample and key head (K and V are read once for all of
+// them) and a chunk of the keys; its warps walk 16-key tiles of their own, each with its own
+// softmax state and its own ring of cp.async copies (no barrier until the end). Scores and
+// P V on mma.sync m16n8k16 with the keys, then the columns of V, as the 16-row operand: S^T = K
+// Q^T, O^T = V^T P^T. So 8 rows (one token's query heads, mostly) need half the products and
+// registers that a 16-row operand of queries would: HBM-bound where the keys are many.
+constexpr int STEP_WARPS = 4, STEP_STAGES = 3, STEP_KEYS = 16;
+constexpr int MOST_CLUSTER = 8;
 
 // How a call is cut up.
 struct Plan {
@@ -163,24 +166,30 @@ struct Plan {
   int tile_chunk;    // blocks of 64 keys a tile's CTA walks
   int tile_splits;   // chunks of a tile
   int tile_ctas;
-  int row_tiles;     // 16-row tiles of a sample and key head
+  int row_tiles;     // tiles of 8 or 16 rows of a sample and key head
+  int step_rows;     // 8 or 16
   int step_prefix;   // whether they see the prefix (no tiles do)
+  int cluster;       // a row tile's chunks are a cluster and joined there (step_prefix alone)
   int step_chunk;    // keys of such a tile's CTA
   int step_splits;   // chunks; 0: tiles see all keys
   int step_ctas;
   float* tile_sums;  // [unit, tile, split, 128, D], then maxima and totals [.., 128]; null: rows are finished by their tile
   float2* tile_states;
-  float* step_sums;  // [sample, key head, row tile, split, 16, D], then [.., 16]; null: rows are finished by their CTA
+  float* step_sums;  // [sample, key head, row tile, split, step_rows, D], then [.., step_rows]; null: rows are finished by their CTA
   float2* step_states;
 };
 
 template <int D>
-constexpr int step_smem() {
-  return STEP_WARPS * STEP_STAGES * 2 * STEP_KEYS * D * 2;
+constexpr int STEP_RINGS = STEP_WARPS * STEP_STAGES * 2 * STEP_KEYS * D * 2;  // bytes
+// Rows that a cluster's CTA owns, and places behind the rings for the states of all chunks of them.
+IRIS_DEVICE int rows_owned(int rows, int splits) { return (rows + splits - 1) / splits; }
+template <int D>
+constexpr int cluster_smem() {
+  return STEP_RINGS<D> + (16 + MOST_CLUSTER) * (D + 2) * 4;  // at least splits * rows_owned(splits) of them
 }
 template <int D>
 constexpr int most_smem() {
-  return tile_smem<D>() > step_smem<D>() ? tile_smem<D>() : step_smem<D>();
+  return tile_smem<D>() > STEP_RINGS<D> ? tile_smem<D>() : STEP_RINGS<D>;
 }
 
 struct Row {
@@ -561,22 +570,28 @@ IRIS_DEVICE KeyRows key_rows(const void* data, int64_t offset, int64_t stride, i
   return KeyRows{reinterpret_cast<uint64_t>(reinterpret_cast<const T*>(data) + offset - first * stride), static_cast<uint32_t>(stride / 8)};
 }
 
-// 16 rows of a sample and key head over a chunk of their keys: the prefix's (where
-// plan.step_prefix) and then the sample's own. Four warps; the block's others leave at once.
-template <typename T, int D>
+// 8 x 8 16-bit elements of a warp's registers transposed.
+IRIS_DEVICE uint32_t movmatrix(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// 8 NQ rows of a sample and key head over a chunk of their keys: the prefix's (PREFIX) and
+// then the sample's own. Four warps; the block's others only meet the barriers.
+template <typename T, int D, int NQ, bool PREFIX>
 IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* smem_raw) {
-  constexpr int TILE = STEP_KEYS * D * 2;  // bytes of one K or V tile
+  constexpr int ROWS = 8 * NQ, TILE = STEP_KEYS * D * 2;  // bytes of one K or V tile
+  constexpr int PAD = D + 4;  // floats of a row of sums: the four lanes of a column pair in different banks
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // no second CTA starts on the SM while one of a kernel that allocates TMEM may still do so
-  // (measured: step CTAs alone ran one at a time, 41 us instead of 23)
-  if (warp == STEP_WARPS) tmem_relinquish();
-  grid_wait();
-  grid_trigger();
   const int split = cta % plan.step_splits, unit = cta / plan.step_splits;  // (b, hk, row tile)
   const int rt = unit % plan.row_tiles, hk = unit / plan.row_tiles % p.heads_kv, b = unit / plan.row_tiles / p.heads_kv;
   const int group = p.heads_q / p.heads_kv, rows = p.n * group;
-  const int r0 = rt * STEP_ROWS, r_last = min(r0 + STEP_ROWS, rows) - 1;
-  const int early = plan.step_prefix ? prefix_length(p, b) : 0;
+  const int r0 = rt * ROWS, r_last = min(r0 + ROWS, rows) - 1;
+  if (PREFIX && plan.cluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  grid_wait();
+  grid_trigger();
+  const int early = PREFIX ? prefix_length(p, b) : 0;
   const int length = own_length(p, b);
   const int64_t start = own_start(p, b);
   const int count = early + own_keys(p, start + r_last / group, length);  // some row of the tile sees them
@@ -601,7 +616,7 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
         const int at = e * 32 + lane, r = at / PIECES, x = at % PIECES;
         const int c = c0 + r;
         const bool real = c < c_end;
-        const bool of_prefix = c < early;
+        const bool of_prefix = PREFIX && c < early;
         const uint64_t key = static_cast<uint32_t>(real ? c : c_begin);
         const uint64_t from_k = (of_prefix ? pk.at : k.at) + key * (of_prefix ? pk.stride : k.stride) * 16 + x * 16;
         const uint64_t from_v = (of_prefix ? pv.at : v.at) + key * (of_prefix ? pv.stride : v.stride) * 16 + x * 16;
@@ -612,14 +627,15 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // this lane's queries: 8 j + 2 (lane % 4) + {0, 1}; its key of a tile's halves, column of O^T's: lane / 4
   const int g = lane >> 2, quad = lane & 3;
-  float o[D / 8][4];
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  float o[D / 16][NQ][4];
+  float m_run[NQ][2], l_run[NQ][2];
   if (warp < STEP_WARPS) {
-    // Q's 16 rows into the slot that is filled last, then the first tiles
+    // Q's rows into the slot that is filled last, then the first tiles
     const uint32_t q_slot = ring + (STEP_STAGES - 1) * 2 * TILE;
 #pragma unroll
-    for (int e = 0; e < STEP_ROWS * PIECES / 32; ++e) {
+    for (int e = 0; e < ROWS * PIECES / 32; ++e) {
       const int at = e * 32 + lane, w = at / PIECES, x = at % PIECES;
       const int r = min(r0 + w, rows - 1);
       const T* q = reinterpret_cast<const T*>(p.q) + b * p.qb + (hk * group + r % group) * p.qh + static_cast<int64_t>(r / group) * p.qn;
@@ -629,22 +645,33 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
 #pragma unroll
     for (int t = 0; t < STEP_STAGES - 1; ++t) load(t);
 
-    // as the A operand: this lane's rows g and g + 8, columns 2 (lane % 4) + {0, 1} of each 8
-    uint32_t qa[D / 16][4];
-    int seen[2];
+    uint32_t qb[D / 16][NQ][2];
+    int seen[NQ][2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) seen[u] = early + own_keys(p, start + min(r0 + g + 8 * u, rows - 1) / group, length);
+    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        seen[j][u] = early + own_keys(p, start + min(r0 + 8 * j + 2 * quad + u, rows - 1) / group, length);
+        m_run[j][u] = -INFINITY;
+        l_run[j][u] = 0.f;
+      }
     asm volatile("cp.async.wait_group %0;" ::"n"(STEP_STAGES - 1) : "memory");
     __syncwarp();
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) {  // matrices: rows 0-7 and 8-15 of piece 2 d, then of 2 d + 1
-      const int r = lane & 15, x = 2 * d + (lane >> 4);
-      ldmatrix4(qa[d], q_slot + r * (D * 2) + ((x ^ (r & 7)) * 16));
-    }
+    for (int j = 0; j < NQ; ++j)
 #pragma unroll
-    for (int d = 0; d < D / 8; ++d)
+      for (int d = 0; d < D / 32; ++d) {  // pieces 4 d .. 4 d + 3 of 8 query rows
+        uint32_t r4[4];
+        const int r = 8 * j + (lane & 7), x = 4 * d + (lane >> 3);
+        ldmatrix4(r4, q_slot + r * (D * 2) + ((x ^ (r & 7)) * 16));
+        qb[2 * d][j][0] = r4[0], qb[2 * d][j][1] = r4[1], qb[2 * d + 1][j][0] = r4[2], qb[2 * d + 1][j][1] = r4[3];
+      }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[d][e] = 0.f;
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][j][e] = 0.f;
 
     for (int t = 0; t < mine; ++t) {
       asm volatile("cp.async.wait_group %0;" ::"n"(STEP_STAGES - 2) : "memory");
@@ -652,132 +679,186 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
       load(t + STEP_STAGES - 1);
       const uint32_t slot = ring + (t % STEP_STAGES) * 2 * TILE;
       const int c0 = c_begin + (warp + t * STEP_WARPS) * STEP_KEYS;
-      // S: keys [8 j, 8 j + 8) in s[j]
-      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, odd[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      float s[NQ][4], odd[NQ][4];
 #pragma unroll
-      for (int d = 0; d < D / 32; ++d) {  // two k steps per load: pieces 4 d .. 4 d + 3 of the 8 key rows
+      for (int j = 0; j < NQ; ++j)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t kb[4];
-          const int r = 8 * j + (lane & 7), x = 4 * d + (lane >> 3);
-          ldmatrix4(kb, slot + r * (D * 2) + ((x ^ (r & 7)) * 16));
-          mma_16816<T>(s[j], qa[2 * d], kb[0], kb[1]);
-          mma_16816<T>(odd[j], qa[2 * d + 1], kb[2], kb[3]);  // two chains: half the wait for the last
-        }
+        for (int e = 0; e < 4; ++e) s[j][e] = odd[j][e] = 0.f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {  // 16 keys of pieces 2 d and 2 d + 1
+        uint32_t ka[4];
+        const int r = lane & 15, x = 2 * d + (lane >> 4);
+        ldmatrix4(ka, slot + r * (D * 2) + ((x ^ (r & 7)) * 16));
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) mma_16816<T>(d & 1 ? odd[j] : s[j], ka, qb[d][j][0], qb[d][j][1]);  // two chains
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NQ; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[j][e] += odd[j][e];
       if (!same || c0 + STEP_KEYS > c_end) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < NQ; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int c = c0 + 8 * j + 2 * quad + (e & 1);
-            if (c >= c_end || c >= seen[e >> 1]) s[j][e] = -INFINITY;
+            const int c = c0 + g + 8 * (e >> 1);
+            if (c >= c_end || c >= seen[j][e & 1]) s[j][e] = -INFINITY;
           }
       }
-      bool rescale = false;
-      float corr[2], shift[2];
+      // a row's maximum is kept until a score exceeds it by 2^8, seen by any lane
+      bool grow = false;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float mx = fmaxf(fmaxf(s[0][2 * u], s[0][2 * u + 1]), fmaxf(s[1][2 * u], s[1][2 * u + 1])) * p.scale_log2;
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const bool grow = mx > m_run[u] + RESCALE;
-        const float m_new = grow ? mx : m_run[u];
-        corr[u] = grow && m_run[u] != -INFINITY ? ex2(m_run[u] - m_new) : 1.f;
-        rescale = rescale || corr[u] != 1.f;
-        m_run[u] = m_new;
-        shift[u] = m_new == -INFINITY ? 0.f : -m_new;
-      }
-      if (__any_sync(0xffffffffu, rescale)) {
+      for (int j = 0; j < NQ; ++j)
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d)
+        for (int u = 0; u < 2; ++u) grow = grow || fmaxf(s[j][u], s[j][u + 2]) * p.scale_log2 > m_run[j][u] + RESCALE;
+      if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[d][e] *= corr[e >> 1];
-        l_run[0] *= corr[0];
-        l_run[1] *= corr[1];
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float mx = fmaxf(s[j][u], s[j][u + 2]) * p.scale_log2;
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const bool more = mx > m_run[j][u] + RESCALE;
+            const float corr = more && m_run[j][u] != -INFINITY ? ex2(m_run[j][u] - mx) : 1.f;
+            if (more) m_run[j][u] = mx;
+            l_run[j][u] *= corr;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              o[d][j][u] *= corr;
+              o[d][j][u + 2] *= corr;
+            }
+          }
       }
       // weights, rounded once to the operand type (the fp32 values go into the totals): as in
       // tile_cta, so that a row is as accurate in either form
-      uint32_t pa[4];
+      uint32_t pw[NQ][2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NQ; ++j) {
+        float w[4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float w0 = ex2(fmaf(s[j][2 * u], p.scale_log2, shift[u]));
-          const float w1 = ex2(fmaf(s[j][2 * u + 1], p.scale_log2, shift[u]));
-          l_run[u] += w0 + w1;
-          pa[2 * j + u] = pack2<T>(w0, w1);
+        for (int e = 0; e < 4; ++e) {
+          const float m = m_run[j][e & 1];
+          w[e] = ex2(fmaf(s[j][e], p.scale_log2, m == -INFINITY ? 0.f : -m));
+          l_run[j][e & 1] += w[e];
         }
+        pw[j][0] = movmatrix(pack2<T>(w[0], w[1]));
+        pw[j][1] = movmatrix(pack2<T>(w[2], w[3]));
+      }
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) {  // 16 columns per load: key rows 0-7 and 8-15, pieces 2 d and 2 d + 1
-        uint32_t vb[4];
-        const int r = lane & 15, x = 2 * d + (lane >> 4);
-        ldmatrix4_trans(vb, slot + TILE + r * (D * 2) + ((x ^ (r & 7)) * 16));
-        mma_16816<T>(o[2 * d], pa, vb[0], vb[1]);
-        mma_16816<T>(o[2 * d + 1], pa, vb[2], vb[3]);
+      for (int d = 0; d < D / 16; ++d) {  // 16 columns of V (pieces 2 d and 2 d + 1) as rows, by 16 keys
+        uint32_t va[4];
+        const int r = (lane & 7) + (lane >> 4) * 8, x = 2 * d + (lane >> 3 & 1);
+        ldmatrix4_trans(va, slot + TILE + r * (D * 2) + ((x ^ (r & 7)) * 16));
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) mma_16816<T>(o[d][j], va, pw[j][0], pw[j][1]);
       }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      l_run[u] += __shfl_xor_sync(0xffffffffu, l_run[u], 1);
-      l_run[u] += __shfl_xor_sync(0xffffffffu, l_run[u], 2);
-    }
+    for (int j = 0; j < NQ; ++j)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int x = 4; x <= 16; x *= 2) l_run[j][u] += __shfl_xor_sync(0xffffffffu, l_run[j][u], x);
   }
   // the warps' states, joined per row: warp w finishes rows w, w + 4, ...
   __syncthreads();  // the rings are done with
-  float* sums = reinterpret_cast<float*>(smem_raw);  // [warp][16][D]
-  __shared__ float tops[STEP_WARPS][STEP_ROWS], totals[STEP_WARPS][STEP_ROWS];
+  float* sums = reinterpret_cast<float*>(smem_raw);  // [warp][ROWS][PAD]
+  __shared__ float tops[STEP_WARPS][16], totals[STEP_WARPS][16];
   if (warp < STEP_WARPS) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float* dst = sums + (warp * STEP_ROWS + g + 8 * u) * D + 2 * quad;
+    for (int j = 0; j < NQ; ++j)
 #pragma unroll
-      for (int d = 0; d < D / 8; ++d) *reinterpret_cast<float2*>(dst + 8 * d) = make_float2(o[d][2 * u], o[d][2 * u + 1]);
-      if (quad == 0) {
-        tops[warp][g + 8 * u] = m_run[u];
-        totals[warp][g + 8 * u] = l_run[u];
+      for (int u = 0; u < 2; ++u) {
+        const int row = 8 * j + 2 * quad + u;
+        float* dst = sums + (warp * ROWS + row) * PAD + g;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          dst[16 * d] = o[d][j][u];
+          dst[16 * d + 8] = o[d][j][u + 2];
+        }
+        if (g == 0) {
+          tops[warp][row] = m_run[j][u];
+          totals[warp][row] = l_run[j][u];
+        }
+      }
+  }
+  __syncthreads();
+  // cluster: states [chunk][owned row], sums then {maximum, total}; other CTAs store here once all have begun
+  float* states = reinterpret_cast<float*>(smem_raw + STEP_RINGS<D>);
+  const int owned = rows_owned(ROWS, plan.step_splits);
+  if (PREFIX && plan.cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (warp < STEP_WARPS) {
+    for (int r = warp; r <= r_last - r0; r += STEP_WARPS) {
+      float top = -INFINITY, total = 0.f;
+#pragma unroll
+      for (int w = 0; w < STEP_WARPS; ++w) top = fmaxf(top, tops[w][r]);
+      float2 acc[D / 64];
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < STEP_WARPS; ++w) {
+        // a warp that saw nothing has sums of 0 (or NaN, from a masked V: kept, it marks the row)
+        const float f = tops[w][r] == -INFINITY ? 1.f : ex2(tops[w][r] - top);
+        total += f * totals[w][r];
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const float2 x = *reinterpret_cast<const float2*>(sums + (w * ROWS + r) * PAD + 64 * c + 2 * lane);
+          acc[c] = make_float2(fmaf(f, x.x, acc[c].x), fmaf(f, x.y, acc[c].y));
+        }
+      }
+      if (PREFIX && plan.cluster) {
+        float* at = states + (split * owned + r % owned) * (D + 2);
+        const uint32_t to = map_to_cta(at, static_cast<uint32_t>(r / owned));
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) store_remote(to + 4 * (64 * c + 2 * lane), acc[c]);
+        if (lane == 0) store_remote(to + 4 * D, make_float2(top, total));
+      } else if (plan.step_sums == nullptr) {
+        finish_row<T, D>(p, b, hk * group + (r0 + r) % group, (r0 + r) / group, acc, total);
+      } else {
+        const int64_t part = (static_cast<int64_t>(unit) * plan.step_splits + split) * ROWS + r;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) *reinterpret_cast<float2*>(plan.step_sums + part * D + 64 * c + 2 * lane) = acc[c];
+        if (lane == 0) plan.step_states[part] = make_float2(top, total);
       }
     }
   }
-  __syncthreads();
-  if (warp >= STEP_WARPS) return;
-  for (int r = warp; r <= r_last - r0; r += STEP_WARPS) {
-    float top = -INFINITY, total = 0.f;
+  if (PREFIX && plan.cluster) {
+    cluster_sync();
+    for (int local = warp; local < owned && split * owned + local <= r_last - r0; local += STEP_WARPS) {
+      const int r = r0 + split * owned + local;
+      float top = -INFINITY, total = 0.f;
+      for (int q = 0; q < plan.step_splits; ++q) top = fmaxf(top, states[(q * owned + local) * (D + 2) + D]);
+      float2 acc[D / 64];
 #pragma unroll
-    for (int w = 0; w < STEP_WARPS; ++w) top = fmaxf(top, tops[w][r]);
-    float2 acc[D / 64];
+      for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
+      for (int q = 0; q < plan.step_splits; ++q) {
+        const float* from = states + (q * owned + local) * (D + 2);
+        const float f = from[D] == -INFINITY ? 1.f : ex2(from[D] - top);
+        total = fmaf(f, from[D + 1], total);
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < STEP_WARPS; ++w) {
-      // a warp that saw nothing has sums of 0 (or NaN, from a masked V: kept, it marks the row)
-      const float f = tops[w][r] == -INFINITY ? 1.f : ex2(tops[w][r] - top);
-      total += f * totals[w][r];
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        const float2 x = *reinterpret_cast<const float2*>(sums + (w * STEP_ROWS + r) * D + 64 * c + 2 * lane);
-        acc[c] = make_float2(fmaf(f, x.x, acc[c].x), fmaf(f, x.y, acc[c].y));
+        for (int c = 0; c < D / 64; ++c) {
+          const float2 x = *reinterpret_cast<const float2*>(from + 64 * c + 2 * lane);
+          acc[c] = make_float2(fmaf(f, x.x, acc[c].x), fmaf(f, x.y, acc[c].y));
+        }
       }
-    }
-    if (plan.step_sums == nullptr) {
-      finish_row<T, D>(p, b, hk * group + (r0 + r) % group, (r0 + r) / group, acc, total);
-    } else {
-      const int64_t part = (static_cast<int64_t>(unit) * plan.step_splits + split) * STEP_ROWS + r;
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) *reinterpret_cast<float2*>(plan.step_sums + part * D + 64 * c + 2 * lane) = acc[c];
-      if (lane == 0) plan.step_states[part] = make_float2(top, total);
+      finish_row<T, D>(p, b, hk * group + r % group, r / group, acc, total);
     }
   }
 }
 
+// Few rows over few keys: no tiles.
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_constant__ Params p, const __grid_constant__ Plan plan) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  step_cta<T, D, NQ, true>(p, plan, static_cast<int>(blockIdx.x), smem_raw);
+}
+
 // Both kinds of CTA in one launch, mixed evenly: tiles are bound by the tensor cores and
 // exponentials, the others by memory.
-template <typename T, int D>
+template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(BOUND_THREADS, 2)
     attend_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ CUtensorMap tpv,
                   const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -786,8 +867,14 @@ __global__ void __launch_bounds__(BOUND_THREADS, 2)
   const int64_t all = static_cast<int64_t>(plan.tile_ctas) + plan.step_ctas;
   const int before = static_cast<int>(blockIdx.x * static_cast<int64_t>(plan.tile_ctas) / all);
   const bool tile = (blockIdx.x + 1) * static_cast<int64_t>(plan.tile_ctas) / all > before;
-  if (tile) tile_cta<T, D>(tpk, tpv, tk, tv, p, plan, before, smem_raw);
-  else step_cta<T, D>(p, plan, static_cast<int>(blockIdx.x) - before, smem_raw);
+  if (tile) {
+    tile_cta<T, D>(tpk, tpv, tk, tv, p, plan, before, smem_raw);
+  } else {
+    // no second CTA starts on the SM while one of a kernel that allocates TMEM may still do so
+    // (measured: step CTAs ran one at a time, 41 us instead of 30 for 512 of them)
+    if (threadIdx.x < 32) tmem_relinquish();
+    step_cta<T, D, NQ, false>(p, plan, static_cast<int>(blockIdx.x) - before, smem_raw);
+  }
 }
 
 // A row's chunks joined by a warp.
@@ -803,7 +890,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Param
   const int h = static_cast<int>(index % p.heads_q), i = static_cast<int>(index / p.heads_q % p.n);
   const int b = static_cast<int>(index / p.heads_q / p.n);
   const int hk = h / group;
-  int64_t tile0 = 0, step0 = 0;  // of its states: first place, and how many there are, BQ or STEP_ROWS apart
+  int64_t tile0 = 0, step0 = 0;  // of its states: first place, and how many there are, BQ or step_rows apart
   int tile_parts = 0, step_parts = 0;
   if (plan.tile_sums != nullptr) {
     const int64_t r = (static_cast<int64_t>(b % plan.per) * p.n + i) * group + h % group;
@@ -813,14 +900,14 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Param
   }
   if (plan.step_sums != nullptr) {
     const int64_t r = static_cast<int64_t>(i) * group + h % group;
-    const int64_t unit = (static_cast<int64_t>(b) * p.heads_kv + hk) * plan.row_tiles + r / STEP_ROWS;
-    step0 = unit * plan.step_splits * STEP_ROWS + r % STEP_ROWS;
+    const int64_t unit = (static_cast<int64_t>(b) * p.heads_kv + hk) * plan.row_tiles + r / plan.step_rows;
+    step0 = unit * plan.step_splits * plan.step_rows + r % plan.step_rows;
     step_parts = plan.step_splits;
   }
   const int parts = tile_parts + step_parts;
   auto state_of = [&](int c) {
     return c < tile_parts ? plan.tile_states[tile0 + static_cast<int64_t>(c) * BQ]
-                          : plan.step_states[step0 + static_cast<int64_t>(c - tile_parts) * STEP_ROWS];
+                          : plan.step_states[step0 + static_cast<int64_t>(c - tile_parts) * plan.step_rows];
   };
   float top = -INFINITY;
   for (int c = lane; c < parts; c += 32) top = fmaxf(top, state_of(c).x);
@@ -844,7 +931,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Param
     for (int e = 0; e < most; ++e) {
       const int c = c0 + e;
       const float* from = c < tile_parts ? plan.tile_sums + (tile0 + static_cast<int64_t>(c) * BQ) * D
-                                         : plan.step_sums + (step0 + static_cast<int64_t>(c - tile_parts) * STEP_ROWS) * D;
+                                         : plan.step_sums + (step0 + static_cast<int64_t>(c - tile_parts) * plan.step_rows) * D;
       const float fc = __shfl_sync(0xffffffffu, f, e);
 #pragma unroll
       for (int d = 0; d < D / 64; ++d) {
@@ -887,7 +974,8 @@ int make_plan(const Sizes& z, Plan* out) {
     plan.tile_ctas = static_cast<int>(units * tiles * plan.tile_splits);
   }
   if (!whole) {
-    plan.row_tiles = static_cast<int>((rows + STEP_ROWS - 1) / STEP_ROWS);
+    plan.step_rows = rows <= 8 ? 8 : 16;
+    plan.row_tiles = static_cast<int>((rows + plan.step_rows - 1) / plan.step_rows);
     plan.step_prefix = !shared;
     const int64_t units = z.batch * z.heads_kv * plan.row_tiles, keys = z.n_kv + (shared ? 0 : z.n_prefix);
     const int64_t splits = std::max<int64_t>(1, std::min((slots + units - 1) / units, keys / 128));
@@ -895,6 +983,7 @@ int make_plan(const Sizes& z, Plan* out) {
     plan.step_splits = static_cast<int>(std::max<int64_t>(1, (keys + plan.step_chunk - 1) / plan.step_chunk));
     IRIS_REQUIRE(units * plan.step_splits < (1ll << 30), "prefix_attn_fwd: too many rows");
     plan.step_ctas = static_cast<int>(units * plan.step_splits);
+    plan.cluster = plan.step_prefix && plan.step_splits > 1 && plan.step_splits <= MOST_CLUSTER;
   }
   *out = plan;
   return IRIS_OK;
@@ -906,11 +995,49 @@ struct Room {
 };
 inline Room room_of(const Plan& plan) {
   Room x = {};
-  const bool parts = (plan.tiles > 0 && plan.step_splits > 0) || plan.tile_splits > 1 || plan.step_splits > 1;
-  if (parts) x = {static_cast<int64_t>(plan.tile_ctas) * BQ, static_cast<int64_t>(plan.step_ctas) * STEP_ROWS};
+  const bool parts = (plan.tiles > 0 && plan.step_splits > 0) || plan.tile_splits > 1 || (plan.step_splits > 1 && !plan.cluster);
+  if (parts) x = {static_cast<int64_t>(plan.tile_ctas) * BQ, static_cast<int64_t>(plan.step_ctas) * plan.step_rows};
   return x;
 }
 inline int64_t room_bytes(const Room& x, int64_t d) { return (x.tile_rows + x.step_rows) * (d + 2) * 4; }
+
+template <typename... Params_>
+int allow_smem(void (*kernel)(Params_...), int bytes, bool (&configured)[64]) {
+  int dev = 0;
+  IRIS_CUDA(cudaGetDevice(&dev));
+  if (dev < 64 && configured[dev]) return IRIS_OK;
+  IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  if (dev < 64) configured[dev] = true;
+  return IRIS_OK;
+}
+
+template <typename T, int D, int NQ>
+int launch_rows(const Params& p, const Plan& plan, int dtype, cudaStream_t st) {
+  if (plan.tiles == 0) {
+    static bool configured[64] = {false};
+    IRIS_CHECK_STATUS(allow_smem(step_kernel<T, D, NQ>, cluster_smem<D>(), configured));
+    IRIS_CUDA(launch_early(step_kernel<T, D, NQ>, dim3(static_cast<unsigned>(plan.step_ctas)), STEP_WARPS * 32,
+                           plan.cluster ? cluster_smem<D>() : STEP_RINGS<D>, st,
+                           plan.cluster ? static_cast<unsigned>(plan.step_splits) : 1u, p, plan));
+    return IRIS_OK;
+  }
+  CUtensorMap tpk = {}, tpv = {}, tk = {}, tv = {};
+  if (p.n_prefix > 0) {
+    const int groups = p.batch / p.per_group;
+    IRIS_CHECK_STATUS(make_tmap_heads(&tpk, p.pk, dtype, D, p.n_prefix, p.heads_kv, groups, p.pkn, p.pkh, p.pkb, BKV));
+    IRIS_CHECK_STATUS(make_tmap_heads(&tpv, p.pv, dtype, D, p.n_prefix, p.heads_kv, groups, p.pvn, p.pvh, p.pvb, BKV));
+  }
+  if (plan.step_splits == 0 && p.n_kv > 0) {
+    IRIS_CHECK_STATUS(make_tmap_heads(&tk, p.k, dtype, D, p.n_kv, p.heads_kv, p.batch, p.kn, p.kh, p.kb, BKV));
+    IRIS_CHECK_STATUS(make_tmap_heads(&tv, p.v, dtype, D, p.n_kv, p.heads_kv, p.batch, p.vn, p.vh, p.vb, BKV));
+  }
+  static bool configured[64] = {false};
+  IRIS_CHECK_STATUS(allow_smem(attend_kernel<T, D, NQ>, most_smem<D>(), configured));
+  IRIS_CUDA(launch_early(attend_kernel<T, D, NQ>, dim3(static_cast<unsigned>(plan.tile_ctas + plan.step_ctas)), THREADS,
+                         plan.step_splits == 0 ? tile_smem<D>() : most_smem<D>(), st, 1, tpk, tpv, tk, tv, p, plan));
+  return IRIS_OK;
+}
 
 template <typename T, int D>
 int launch(const Params& p, int dtype, void* workspace, int64_t workspace_bytes, cudaStream_t st) {
@@ -919,7 +1046,8 @@ int launch(const Params& p, int dtype, void* workspace, int64_t workspace_bytes,
   Plan plan;
   IRIS_CHECK_STATUS(make_plan(Sizes{p.batch, p.batch / p.per_group, p.heads_q, p.heads_kv, p.n, p.n_prefix, p.n_kv, p.right}, &plan));
   const Room room = room_of(plan);
-  if (room.tile_rows + room.step_rows > 0) {
+  const bool parts = room.tile_rows + room.step_rows > 0;
+  if (parts) {
     IRIS_REQUIRE(workspace != nullptr && aligned16(workspace) && workspace_bytes >= room_bytes(room, D),
                  "prefix_attn_fwd: workspace too small");
     float* at = static_cast<float*>(workspace);
@@ -930,32 +1058,9 @@ int launch(const Params& p, int dtype, void* workspace, int64_t workspace_bytes,
     plan.tile_states = reinterpret_cast<float2*>(at);
     plan.step_states = plan.tile_states + room.tile_rows;
   }
-  CUtensorMap tpk = {}, tpv = {}, tk = {}, tv = {};
-  if (plan.tiles > 0) {
-    if (p.n_prefix > 0) {
-      const int groups = p.batch / p.per_group;
-      IRIS_CHECK_STATUS(make_tmap_heads(&tpk, p.pk, dtype, D, p.n_prefix, p.heads_kv, groups, p.pkn, p.pkh, p.pkb, BKV));
-      IRIS_CHECK_STATUS(make_tmap_heads(&tpv, p.pv, dtype, D, p.n_prefix, p.heads_kv, groups, p.pvn, p.pvh, p.pvb, BKV));
-    }
-    if (plan.step_splits == 0 && p.n_kv > 0) {
-      IRIS_CHECK_STATUS(make_tmap_heads(&tk, p.k, dtype, D, p.n_kv, p.heads_kv, p.batch, p.kn, p.kh, p.kb, BKV));
-      IRIS_CHECK_STATUS(make_tmap_heads(&tv, p.v, dtype, D, p.n_kv, p.heads_kv, p.batch, p.vn, p.vh, p.vb, BKV));
-    }
-  }
-  auto kernel = attend_kernel<T, D>;
-  static bool configured[64] = {false};
-  int dev = 0;
-  IRIS_CUDA(cudaGetDevice(&dev));
-  if (dev >= 64 || !configured[dev]) {
-    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most_smem<D>()));
-    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-    if (dev < 64) configured[dev] = true;
-  }
-  const int smem = plan.tiles == 0 ? step_smem<D>() : plan.step_splits == 0 ? tile_smem<D>() : most_smem<D>();
-  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(plan.tile_ctas + plan.step_ctas)), THREADS, smem, st, 1, tpk, tpv, tk,
-                         tv, p, plan));
-  if (room.tile_rows + room.step_rows == 0) return IRIS_OK;
-  IRIS_CUDA(launch_early(join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, 1, p, plan));
+  if (plan.step_rows == 16) IRIS_CHECK_STATUS((launch_rows<T, D, 2>(p, plan, dtype, st)));
+  else IRIS_CHECK_STATUS((launch_rows<T, D, 1>(p, plan, dtype, st)));
+  if (parts) IRIS_CUDA(launch_early(join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, 1, p, plan));
   return IRIS_OK;
 }
 
