@@ -128,6 +128,11 @@ __device__ __noinline__ void attend_row(const Params& p, int b, int h, int i, fl
 // are zeroed in shared memory (their K only reaches masked scores). A masked key's weight is
 // exactly 0, and 0 times a NaN or infinity of its V row is NaN: a row that comes out
 // not finite is computed again by attend_row, which reads visible keys alone.
+//
+// A commit holds the tensor pipe for about 90 cycles before the next product (measured: 8 + 4
+// products of a block 633 cycles, 989 with four commits), so a block has two: one
+// barrier tells the softmax of its scores and the TMA warp of its slot of K, another of
+// P V and its slot of V.
 constexpr int BQ = 128, BKV = 64, KV = 2;  // rows, keys of a block, slots of the K and V rings
 constexpr int THREADS = 192;
 // Two CTAs to an SM: warp w of each sits in quarter w % 4 of the SM, whose registers hold
@@ -137,8 +142,11 @@ constexpr int Q_HALF = BQ * 128, KV_HALF = BKV * 128;  // bytes of 64 columns of
 constexpr uint32_t COL_S = 0, COL_O = 2 * BKV, TILE_COLS = 256;
 
 struct TileSmem {
-  uint64_t q_full, k_full[KV], k_free[KV], v_full[KV], v_free[KV], v_tail;
-  uint64_t s_full[2], p_full[2], pv_done, o_final, teardown;
+  uint64_t q_full, k_full[KV], v_full[KV], v_tail;
+  uint64_t s_full[2];   // block it's scores are there, and its slot of K is free: [it % 2]
+  uint64_t p_full[2];
+  uint64_t pv_done[2];  // block it's products are in O, and its slot of V is free
+  uint64_t teardown;
   uint32_t tmem_base;
   int abort;
 };
@@ -217,16 +225,11 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
     mbar_init(&s->q_full, 4);
     for (int i = 0; i < KV; ++i) {
       mbar_init(&s->k_full[i], 1);
-      mbar_init(&s->k_free[i], 1);
       mbar_init(&s->v_full[i], 1);
-      mbar_init(&s->v_free[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
       mbar_init(&s->s_full[i], 1);
       mbar_init(&s->p_full[i], 4);
+      mbar_init(&s->pv_done[i], 1);
     }
-    mbar_init(&s->pv_done, 1);
-    mbar_init(&s->o_final, 1);
     mbar_init(&s->v_tail, 1);
     mbar_init(&s->teardown, 1);
     s->abort = 0;
@@ -282,7 +285,7 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
     auto load_k = [&](int it) {
       const int st = it % KV;
       const uint32_t ph = static_cast<uint32_t>((it / KV) & 1);
-      ok = mbar_wait(&s->k_free[st], ph ^ 1u, abort);
+      ok = mbar_wait(&s->s_full[st], ph ^ 1u, abort);
       if (!ok) return;
       load(tpk, tk, &s->k_full[st], k_tile + st * KV_BYTES, first + it, p.pkh != 0 ? hk : 0, p.pkb != 0 ? g : 0, p.kh != 0 ? hk : 0,
            p.kb != 0 ? b0 : 0);
@@ -298,7 +301,7 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
       const bool tail = left < BKV && (block < early_blocks ? early < p.n_prefix : length < p.n_kv);
       if (lane == 0 && ok) {
         if (it + 1 < iters) load_k(it + 1);  // scores run a block ahead
-        ok = ok && mbar_wait(&s->v_free[st], ph ^ 1u, abort);
+        ok = ok && mbar_wait(&s->pv_done[st], ph ^ 1u, abort);
         if (ok) {
           load(tpv, tv, tail ? &s->v_tail : &s->v_full[st], v_tile + st * KV_BYTES, block, p.pvh != 0 ? hk : 0, p.pvb != 0 ? g : 0,
                p.vh != 0 ? hk : 0, p.vb != 0 ? b0 : 0);
@@ -345,7 +348,6 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
           umma_ss(tmem + COL_S + (it & 1) * BKV, umma_desc(q_addr + (kk >> 2) * Q_HALF + (kk & 3) * 32, 16, 1024, kLayoutSw128),
                   umma_desc(k_addr + (kk >> 2) * KV_HALF + (kk & 3) * 32, 16, 1024, kLayoutSw128), idesc_s, kk > 0 ? 1u : 0u);
         umma_commit(&s->s_full[it & 1]);
-        umma_commit(&s->k_free[it % KV]);
       };
       issue_s(0);
       if (iters > 1) issue_s(1);
@@ -360,12 +362,10 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
         for (int kk = 0; kk < BKV / 16; ++kk)  // P lies packed over the first half of its scores
           umma_ts(tmem + COL_O, tmem + COL_S + (it & 1) * BKV + kk * 8,
                   umma_desc(v_addr + kk * 16 * 128, KV_HALF, 1024, kLayoutSw128), idesc_o, (it > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&s->pv_done);
-        umma_commit(&s->v_free[st]);
+        umma_commit(&s->pv_done[st]);
         // into the buffer of the P just read: one thread's MMAs run in order
         if (it + 2 < iters) issue_s(it + 2);
       }
-      if (ok) umma_commit(&s->o_final);
       umma_commit(&s->teardown);
       int dummy = 0;
       mbar_wait(&s->teardown, 0, &dummy);
@@ -434,7 +434,7 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
       if (__any_sync(0xffffffffu, rescale)) {
         const float corr = rescale ? ex2(m_run - m_new) : 1.f;
         l_run *= corr;
-        ok = __all_sync(0xffffffffu, mbar_wait(&s->pv_done, static_cast<uint32_t>((it - 1) & 1), abort));
+        ok = __all_sync(0xffffffffu, mbar_wait(&s->pv_done[(it - 1) & 1], static_cast<uint32_t>(((it - 1) >> 1) & 1), abort));
         if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
@@ -473,7 +473,8 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
       __syncwarp();
       if (lane == 0) mbar_arrive(&s->p_full[it & 1]);
     }
-    if (iters > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(&s->o_final, 0, abort));
+    if (iters > 0)
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&s->pv_done[(iters - 1) & 1], static_cast<uint32_t>(((iters - 1) >> 1) & 1), abort));
     ok = ok && *abort == 0;
     tc_fence_after();
     // rows leave from the place of Q and the rings (every product is computed), each as one
