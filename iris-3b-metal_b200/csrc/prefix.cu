@@ -170,9 +170,11 @@ constexpr int MOST_CLUSTER = 8;
 // How a call is cut up.
 struct Plan {
   int per;           // samples whose rows share tiles; 1: tiles see the samples' own keys too
-  int tiles;         // 128-row tiles of a unit (per samples and a key head); 0: none
-  int tile_chunk;    // blocks of 64 keys a tile's CTA walks
-  int tile_splits;   // chunks of a tile
+  int units;         // of `per` samples and a key head
+  int tiles;         // 128-row tiles of a unit
+  int whole_tiles;   // the first tiles (all units') have one CTA each, which finishes their rows
+  int tile_chunk;    // blocks of 64 keys that a CTA of the others walks
+  int tile_splits;   // chunks of such a tile
   int tile_ctas;
   int row_tiles;     // tiles of 8 or 16 rows of a sample and key head
   int step_rows;     // 8 or 16
@@ -181,7 +183,7 @@ struct Plan {
   int step_chunk;    // keys of such a tile's CTA
   int step_splits;   // chunks; 0: tiles see all keys
   int step_ctas;
-  float* tile_sums;  // [unit, tile, split, 128, D], then maxima and totals [.., 128]; null: rows are finished by their tile
+  float* tile_sums;  // [tile behind the whole ones, split, 128, D], then maxima and totals [.., 128]
   float2* tile_states;
   float* step_sums;  // [sample, key head, row tile, split, step_rows, D], then [.., step_rows]; null: rows are finished by their CTA
   float2* step_states;
@@ -208,6 +210,15 @@ IRIS_DEVICE Row row_of(const Params& p, int per, int u, int hk, int r) {
   const int group = p.heads_q / p.heads_kv;
   const int token = r / group;
   return Row{u * per + token / p.n, hk * group + r - token * group, token % p.n};
+}
+
+// Tile `index` of all units': later rows first, for under a causal mask they see the most keys.
+struct Place {
+  int u, hk, tile;
+};
+IRIS_DEVICE Place tile_place(const Params& p, const Plan& plan, int index) {
+  const int unit = index % plan.units;
+  return Place{unit / p.heads_kv, unit % p.heads_kv, plan.tiles - 1 - index / plan.units};
 }
 
 template <typename T, int D>
@@ -244,11 +255,11 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
 
   grid_wait();
   grid_trigger();
-  const int split = cta % plan.tile_splits, unit_tile = cta / plan.tile_splits;
-  // later rows first: under a causal mask they see the most keys
-  const int units = p.batch / plan.per * p.heads_kv;
-  const int unit = unit_tile % units, tile = plan.tiles - 1 - unit_tile / units;
-  const int hk = unit % p.heads_kv, u = unit / p.heads_kv;
+  const bool finish = cta < plan.whole_tiles;
+  const int split = finish ? 0 : (cta - plan.whole_tiles) % plan.tile_splits;
+  const int unit_tile = finish ? cta : plan.whole_tiles + (cta - plan.whole_tiles) / plan.tile_splits;
+  const Place place_of = tile_place(p, plan, unit_tile);
+  const int tile = place_of.tile, hk = place_of.hk, u = place_of.u;
   const int row0 = tile * BQ, last = min(row0 + BQ, rows) - 1;
   const int b0 = u * plan.per, g = b0 / p.per_group;
   const bool own = plan.per == 1 && plan.step_splits == 0;
@@ -257,8 +268,8 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
   const int64_t start = own ? own_start(p, b0) : 0;
   const int early_blocks = (early + BKV - 1) / BKV;
   const int all_blocks = early_blocks + (own ? (own_keys(p, start + last / group, length) + BKV - 1) / BKV : 0);
-  const int first = min(split * plan.tile_chunk, all_blocks);
-  const int iters = min(plan.tile_chunk, all_blocks - first);
+  const int first = finish ? 0 : min(split * plan.tile_chunk, all_blocks);
+  const int iters = finish ? all_blocks : min(plan.tile_chunk, all_blocks - first);
 
   if (warp == 0) {
     // ----------------------------------------------------------------- TMA
@@ -479,9 +490,9 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
     tc_fence_after();
     // rows leave from the place of Q and the rings (every product is computed), each as one
     // bulk copy; 16 bytes of padding spread a piece of 8 rows over the banks
-    if (plan.tile_sums != nullptr) {
+    if (!finish) {
       // this chunk's state; a wait that gave up (device error word) makes the row NaN
-      const int64_t part = ((static_cast<int64_t>(unit) * plan.tiles + tile) * plan.tile_splits + split) * BQ + row;
+      const int64_t part = (static_cast<int64_t>(unit_tile - plan.whole_tiles) * plan.tile_splits + split) * BQ + row;
       if (r < rows) plan.tile_states[part] = ok ? make_float2(m_run, l_run) : make_float2(NAN, NAN);
       if (ok && iters > 0) {
         uint8_t* mine = q_tile + row * (D * 4 + 16);
@@ -882,27 +893,26 @@ __global__ void __launch_bounds__(BOUND_THREADS, 2)
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Params p, const __grid_constant__ Plan plan) {
   const int lane = threadIdx.x & 31;
-  const int group = p.heads_q / p.heads_kv;
-  const int64_t rows = static_cast<int64_t>(p.batch) * p.n * p.heads_q;
-  const int64_t index = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int group = p.heads_q / p.heads_kv, rows = plan.per * p.n * group;
+  const int index = static_cast<int>(blockIdx.x / (BQ / 4));  // of the tiles behind the whole ones
+  const int in_tile = static_cast<int>(blockIdx.x % (BQ / 4)) * 4 + (threadIdx.x >> 5);
+  const Place at = tile_place(p, plan, plan.whole_tiles + index);
+  const int r = at.tile * BQ + in_tile;
+  if (r >= rows) return;
+  const Row row = row_of(p, plan.per, at.u, at.hk, r);
+  const int b = row.b, h = row.h, i = row.i;
   grid_wait();
   grid_trigger();
-  if (index >= rows) return;
-  const int h = static_cast<int>(index % p.heads_q), i = static_cast<int>(index / p.heads_q % p.n);
-  const int b = static_cast<int>(index / p.heads_q / p.n);
-  const int hk = h / group;
   int64_t tile0 = 0, step0 = 0;  // of its states: first place, and how many there are, BQ or step_rows apart
   int tile_parts = 0, step_parts = 0;
   if (plan.tile_sums != nullptr) {
-    const int64_t r = (static_cast<int64_t>(b % plan.per) * p.n + i) * group + h % group;
-    const int64_t unit = static_cast<int64_t>(b / plan.per) * p.heads_kv + hk;
-    tile0 = (unit * plan.tiles + r / BQ) * plan.tile_splits * BQ + r % BQ;
+    tile0 = static_cast<int64_t>(index) * plan.tile_splits * BQ + in_tile;
     tile_parts = plan.tile_splits;
   }
   if (plan.step_sums != nullptr) {
-    const int64_t r = static_cast<int64_t>(i) * group + h % group;
-    const int64_t unit = (static_cast<int64_t>(b) * p.heads_kv + hk) * plan.row_tiles + r / plan.step_rows;
-    step0 = unit * plan.step_splits * plan.step_rows + r % plan.step_rows;
+    const int of_sample = i * group + h % group;
+    const int64_t unit = (static_cast<int64_t>(b) * p.heads_kv + at.hk) * plan.row_tiles + of_sample / plan.step_rows;
+    step0 = unit * plan.step_splits * plan.step_rows + of_sample % plan.step_rows;
     step_parts = plan.step_splits;
   }
   const int parts = tile_parts + step_parts;
@@ -965,15 +975,25 @@ int make_plan(const Sizes& z, Plan* out) {
   const bool shared = !whole && z.n_prefix >= 256 && per_group > 1;
   plan.per = static_cast<int>(whole ? 1 : per_group);
   if (whole || shared) {
-    const int64_t units = z.batch / plan.per * z.heads_kv, tiles = (plan.per * rows + BQ - 1) / BQ;
+    const int64_t units = z.batch / plan.per * z.heads_kv, tiles = (plan.per * rows + BQ - 1) / BQ;  // int64: not yet checked
     const int64_t blocks = (z.n_prefix + BKV - 1) / BKV + (whole ? (z.n_kv + BKV - 1) / BKV : 0);
-    const int64_t splits = std::max<int64_t>(1, std::min((slots + units * tiles - 1) / (units * tiles), blocks / 4));
+    const int64_t all = units * tiles;
+    IRIS_REQUIRE(all < (1ll << 30), "prefix_attn_fwd: too many rows");
+    // tiles that fill the SMs are not split; the last of them, which would leave some idle, are
+    const int64_t rest = whole && all % slots != 0 ? all % slots : all;
+    const int64_t splits = std::max<int64_t>(1, std::min(slots / rest, blocks / 4));
     plan.tiles = static_cast<int>(tiles);
     plan.tile_chunk = static_cast<int>(std::max<int64_t>(1, (blocks + splits - 1) / splits));
     plan.tile_splits = static_cast<int>(std::max<int64_t>(1, (blocks + plan.tile_chunk - 1) / plan.tile_chunk));
-    IRIS_REQUIRE(units * tiles * plan.tile_splits < (1ll << 30), "prefix_attn_fwd: too many rows");
-    plan.tile_ctas = static_cast<int>(units * tiles * plan.tile_splits);
+    plan.whole_tiles = static_cast<int>(!whole ? 0 : plan.tile_splits == 1 ? all : all - rest);
+    const int64_t ctas = plan.whole_tiles + (all - plan.whole_tiles) * plan.tile_splits;
+    IRIS_REQUIRE(ctas < (1ll << 30), "prefix_attn_fwd: too many rows");
+    plan.tile_ctas = static_cast<int>(ctas);
+  } else {  // join_kernel takes the rows by tiles too
+    plan.per = 1;
+    plan.tiles = static_cast<int>((rows + BQ - 1) / BQ);
   }
+  plan.units = static_cast<int>(z.batch / plan.per * z.heads_kv);
   if (!whole) {
     plan.step_rows = rows <= 8 ? 8 : 16;
     plan.row_tiles = static_cast<int>((rows + plan.step_rows - 1) / plan.step_rows);
@@ -996,9 +1016,13 @@ struct Room {
 };
 inline Room room_of(const Plan& plan) {
   Room x = {};
-  const bool parts = (plan.tiles > 0 && plan.step_splits > 0) || plan.tile_splits > 1 || (plan.step_splits > 1 && !plan.cluster);
-  if (parts) x = {static_cast<int64_t>(plan.tile_ctas) * BQ, static_cast<int64_t>(plan.step_ctas) * plan.step_rows};
+  x.tile_rows = static_cast<int64_t>(plan.tile_ctas - plan.whole_tiles) * BQ;
+  if (x.tile_rows > 0 || (plan.step_splits > 1 && !plan.cluster)) x.step_rows = static_cast<int64_t>(plan.step_ctas) * plan.step_rows;
   return x;
+}
+// Tiles whose rows join_kernel takes.
+inline int64_t joined_tiles(const Plan& plan) {
+  return plan.tile_ctas > 0 ? (plan.tile_ctas - plan.whole_tiles) / plan.tile_splits : static_cast<int64_t>(plan.tiles) * plan.units;
 }
 inline int64_t room_bytes(const Room& x, int64_t d) { return (x.tile_rows + x.step_rows) * (d + 2) * 4; }
 
@@ -1015,7 +1039,7 @@ int allow_smem(void (*kernel)(Params_...), int bytes, bool (&configured)[64]) {
 
 template <typename T, int D, int NQ>
 int launch_rows(const Params& p, const Plan& plan, int dtype, cudaStream_t st) {
-  if (plan.tiles == 0) {
+  if (plan.tile_ctas == 0) {
     static bool configured[64] = {false};
     IRIS_CHECK_STATUS(allow_smem(step_kernel<T, D, NQ>, cluster_smem<D>(), configured));
     IRIS_CUDA(launch_early(step_kernel<T, D, NQ>, dim3(static_cast<unsigned>(plan.step_ctas)), STEP_WARPS * 32,
@@ -1061,7 +1085,11 @@ int launch(const Params& p, int dtype, void* workspace, int64_t workspace_bytes,
   }
   if (plan.step_rows == 16) IRIS_CHECK_STATUS((launch_rows<T, D, 2>(p, plan, dtype, st)));
   else IRIS_CHECK_STATUS((launch_rows<T, D, 1>(p, plan, dtype, st)));
-  if (parts) IRIS_CUDA(launch_early(join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, 1, p, plan));
+  if (parts) {
+    const int64_t blocks = joined_tiles(plan) * (BQ / 4);
+    IRIS_REQUIRE(blocks < (1ll << 31), "prefix_attn_fwd: too many rows");
+    IRIS_CUDA(launch_early(join_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), 128, 0, st, 1, p, plan));
+  }
   return IRIS_OK;
 }
 
