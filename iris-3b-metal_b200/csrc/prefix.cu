@@ -230,7 +230,7 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
   uint8_t* v_tile = k_tile + KV * KV_BYTES;
   TileSmem* s = reinterpret_cast<TileSmem*>(v_tile + KV * KV_BYTES);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int group = p.heads_q / p.heads_kv, rows = plan.per * p.n * group;
   if (threadIdx.x == 0) {
     mbar_init(&s->q_full, 4);
@@ -394,7 +394,7 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
       const int piece = lane % LANES;
       const int64_t mine = at.b * p.qb + at.h * p.qh + at.i * p.qn;
       const uint32_t to = smem_addr(q_tile) + (piece >> 3) * Q_HALF;
-#pragma unroll
+#pragma unroll 1
       for (int x = 0; x < 32; x += STEP) {
         const int w = x + lane / LANES;
         const T* from = reinterpret_cast<const T*>(p.q) + __shfl_sync(0xffffffffu, mine, w) + piece * 8;
@@ -496,14 +496,14 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
       if (r < rows) plan.tile_states[part] = ok ? make_float2(m_run, l_run) : make_float2(NAN, NAN);
       if (ok && iters > 0) {
         uint8_t* mine = q_tile + row * (D * 4 + 16);
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(lanes + COL_O + c * 32, o);
+#pragma unroll 1
+        for (int c = 0; c < D / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld16(lanes + COL_O + c * 16, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<uint4*>(mine + c * 128 + e * 16) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<uint4*>(mine + c * 64 + e * 16) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
         }
         fence_proxy_async_smem();
         if (r < rows) bulk_store(plan.tile_sums + part * D, mine, D * 4);
@@ -513,24 +513,24 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
       const float inv = ok ? 1.f / l_run : NAN;
       bool finite = true;
       uint8_t* mine = q_tile + row * (D * 2 + 16);
+#pragma unroll 1
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t o[16], pk[8];
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
+        for (int e = 0; e < 16; ++e) o[e] = 0u;
         if (iters > 0) {
-          tmem_ld32(lanes + COL_O + c * 32, o);
+          tmem_ld16(lanes + COL_O + c * 16, o);
           tmem_wait_ld();
         }
-        uint32_t pk[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < 8; ++e) {
           const float x = iters > 0 ? __uint_as_float(o[2 * e]) * inv : 0.f;
           const float z = iters > 0 ? __uint_as_float(o[2 * e + 1]) * inv : 0.f;
           finite = finite && isfinite(x) && isfinite(z);
           pk[e] = pack2<T>(x, z);
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          *reinterpret_cast<uint4*>(mine + c * 64 + e * 16) = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+        *reinterpret_cast<uint4*>(mine + c * 32) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+        *reinterpret_cast<uint4*>(mine + c * 32 + 16) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
       }
       __syncwarp();  // a row that is computed again comes after what was written of it
       for (uint32_t again = __ballot_sync(0xffffffffu, ok && !finite && r < rows); again != 0; again &= again - 1) {
@@ -595,7 +595,7 @@ template <typename T, int D, int NQ, bool PREFIX>
 IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* smem_raw) {
   constexpr int ROWS = 8 * NQ, TILE = STEP_KEYS * D * 2;  // bytes of one K or V tile
   constexpr int PAD = D + 4;  // floats of a row of sums: the four lanes of a column pair in different banks
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x & 31;
   const int split = cta % plan.step_splits, unit = cta / plan.step_splits;  // (b, hk, row tile)
   const int rt = unit % plan.row_tiles, hk = unit / plan.row_tiles % p.heads_kv, b = unit / plan.row_tiles / p.heads_kv;
   const int group = p.heads_q / p.heads_kv, rows = p.n * group;
@@ -623,7 +623,7 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
     if (t < mine) {
       const int c0 = c_begin + (warp + t * STEP_WARPS) * STEP_KEYS;
       const uint32_t slot = ring + (t % STEP_STAGES) * 2 * TILE;
-#pragma unroll
+#pragma unroll 1
       for (int e = 0; e < STEP_KEYS * PIECES / 32; ++e) {
         const int at = e * 32 + lane, r = at / PIECES, x = at % PIECES;
         const int c = c0 + r;
@@ -646,7 +646,7 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
   if (warp < STEP_WARPS) {
     // Q's rows into the slot that is filled last, then the first tiles
     const uint32_t q_slot = ring + (STEP_STAGES - 1) * 2 * TILE;
-#pragma unroll
+#pragma unroll 1
     for (int e = 0; e < ROWS * PIECES / 32; ++e) {
       const int at = e * 32 + lane, w = at / PIECES, x = at % PIECES;
       const int r = min(r0 + w, rows - 1);
@@ -654,7 +654,7 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
       copy16(q_slot + w * (D * 2) + ((x ^ (w & 7)) * 16), q + x * 8, r0 + w < rows);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-#pragma unroll
+#pragma unroll 1
     for (int t = 0; t < STEP_STAGES - 1; ++t) load(t);
 
     uint32_t qb[D / 16][NQ][2];
@@ -810,7 +810,7 @@ IRIS_DEVICE void step_cta(const Params& p, const Plan& plan, int cta, uint8_t* s
       float2 acc[D / 64];
 #pragma unroll
       for (int c = 0; c < D / 64; ++c) acc[c] = make_float2(0.f, 0.f);
-#pragma unroll
+#pragma unroll 1
       for (int w = 0; w < STEP_WARPS; ++w) {
         // a warp that saw nothing has sums of 0 (or NaN, from a masked V: kept, it marks the row)
         const float f = tops[w][r] == -INFINITY ? 1.f : ex2(tops[w][r] - top);
@@ -867,6 +867,9 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   step_cta<T, D, NQ, true>(p, plan, static_cast<int>(blockIdx.x), smem_raw);
 }
+
+// What a CTA runs once is kept in loops, here and in tile_cta: straight code waits for its
+// instructions (Q's 16 copies a lane unrolled took 4.9 us of a tile's 14).
 
 // Both kinds of CTA in one launch, mixed evenly: tiles are bound by the tensor cores and
 // exponentials, the others by memory.
