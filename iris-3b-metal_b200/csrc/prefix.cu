@@ -871,24 +871,22 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
 // What a CTA runs once is kept in loops, here and in tile_cta: straight code waits for its
 // instructions (Q's 16 copies a lane unrolled took 4.9 us of a tile's 14).
 
-// Both kinds of CTA in one launch, mixed evenly: tiles are bound by the tensor cores and
-// exponentials, the others by memory.
+// Both kinds of CTA in one launch, the longer ones first: tiles are bound by the tensor cores
+// and exponentials, the others by memory, and they share the SMs (mixed evenly, tiles that
+// started late ended last: 64 samples behind 32768 tokens 111 us).
 template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(BOUND_THREADS, 2)
     attend_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ CUtensorMap tpv,
                   const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                   const __grid_constant__ Params p, const __grid_constant__ Plan plan) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const int64_t all = static_cast<int64_t>(plan.tile_ctas) + plan.step_ctas;
-  const int before = static_cast<int>(blockIdx.x * static_cast<int64_t>(plan.tile_ctas) / all);
-  const bool tile = (blockIdx.x + 1) * static_cast<int64_t>(plan.tile_ctas) / all > before;
-  if (tile) {
-    tile_cta<T, D>(tpk, tpv, tk, tv, p, plan, before, smem_raw);
+  if (static_cast<int>(blockIdx.x) < plan.tile_ctas) {
+    tile_cta<T, D>(tpk, tpv, tk, tv, p, plan, static_cast<int>(blockIdx.x), smem_raw);
   } else {
     // no second CTA starts on the SM while one of a kernel that allocates TMEM may still do so
     // (measured: step CTAs ran one at a time, 41 us instead of 30 for 512 of them)
     if (threadIdx.x < 32) tmem_relinquish();
-    step_cta<T, D, NQ, false>(p, plan, static_cast<int>(blockIdx.x) - before, smem_raw);
+    step_cta<T, D, NQ, false>(p, plan, static_cast<int>(blockIdx.x) - plan.tile_ctas, smem_raw);
   }
 }
 
@@ -965,49 +963,121 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Param
 }
 
 // How a call is cut up, from its sizes alone (lengths are on the device: n_prefix and
-// n_kv bound them).
+// n_kv bound them). Three forms, and the one whose estimate is least:
+//  - joint: row tiles of a sample see all of its keys (step_kernel); few rows or short prefixes;
+//  - shared: a group's rows see the prefix by tiles, row tiles their own keys;
+//  - whole: a sample's rows see all keys by tiles; prompts.
+// Estimates in us, from the SMs' two slots each. A tile's CTA takes TILE_START and TILE_BLOCK
+// for each 64 keys, a row tile's STEP_START and, for each key, STEP_KEY alone on its SM or
+// STEP_PAIRED beside another (8 rows; 16 rows 1.3 times that, heads of 64 0.6 times); joining
+// parts takes JOIN and their bytes. Measured against the estimate, heads of 128, the form
+// taken and the next: 4 samples behind 300 tokens, 4 rows each, joint 4.4 (3.7), shared 9.4 (9.7);
+// 32 behind 2048 with 512 of their own, shared 20 (16), joint 36 (38); 8 behind 8192, shared
+// 20 (16), joint 31 (32); one of 256 rows behind 16384, whole 27 (24), joint 99 (98); 4 of 128 rows
+// behind 1000, whole 14 (13), joint 22 (16).
+constexpr float TILE_START = 5.3f, TILE_BLOCK = 0.95f, STEP_START = 2.5f, STEP_KEY = 0.0096f, STEP_PAIRED = 0.0139f;
+constexpr float JOIN = 2.5f, JOIN_BYTES = 5.0e6f;  // bytes per us, written and read
+
 struct Sizes {
-  int64_t batch, groups, heads_q, heads_kv, n, n_prefix, n_kv, right;
+  int64_t batch, groups, heads_q, heads_kv, n, n_prefix, n_kv, head_dim;
 };
 
+struct Estimate {
+  const Sizes& z;
+  int64_t sms = num_sms(), slots = 2 * sms;
+  int64_t group = z.heads_q / z.heads_kv, rows = z.n * group, all_rows = z.batch * z.heads_q * z.n;
+  float width = z.head_dim == 64 ? 0.6f : 1.f;
+
+  float tile(int64_t blocks) const { return TILE_START + TILE_BLOCK * (0.5f + 0.5f * width) * blocks; }
+  // a row tile's CTA over so many keys, one of `ctas`
+  float step(int64_t keys, int64_t ctas) const {
+    return STEP_START + (ctas <= sms ? STEP_KEY : STEP_PAIRED) * (rows > 8 ? 1.3f : 1.f) * width * keys;
+  }
+  float join(int64_t joined, int64_t parts) const { return JOIN + joined * parts * z.head_dim * 8 / JOIN_BYTES; }
+};
+
+// Chunks of `keys` in units of `unit`, so many or fewer.
+struct Cut {
+  int64_t chunk, splits;
+};
+inline Cut cut(int64_t keys, int64_t splits, int64_t unit) {
+  splits = std::max<int64_t>(1, std::min(splits, (keys + unit - 1) / unit));
+  const int64_t chunk = std::max(unit, ((keys + splits - 1) / splits + unit - 1) / unit * unit);
+  return Cut{chunk, std::max<int64_t>(1, (keys + chunk - 1) / chunk)};
+}
+
 int make_plan(const Sizes& z, Plan* out) {
+  const Estimate e{z};
+  const int64_t per_group = z.batch / z.groups;
+  const int64_t step_rows = e.rows <= 8 ? 8 : 16, row_tiles = (e.rows + step_rows - 1) / step_rows;
+  const int64_t step_units = z.batch * z.heads_kv * row_tiles, keys = z.n_prefix + z.n_kv;
+  constexpr int64_t STEP_UNIT = STEP_WARPS * STEP_KEYS;
+  float least = INFINITY;
   Plan plan = {};
-  const int64_t group = z.heads_q / z.heads_kv, rows = z.n * group, per_group = z.batch / z.groups;
-  const int64_t slots = 2 * num_sms();
-  const bool whole = rows >= 64;  // a sample's rows fill tiles
-  const bool shared = !whole && z.n_prefix >= 256 && per_group > 1;
-  plan.per = static_cast<int>(whole ? 1 : per_group);
-  if (whole || shared) {
-    const int64_t units = z.batch / plan.per * z.heads_kv, tiles = (plan.per * rows + BQ - 1) / BQ;  // int64: not yet checked
-    const int64_t blocks = (z.n_prefix + BKV - 1) / BKV + (whole ? (z.n_kv + BKV - 1) / BKV : 0);
-    const int64_t all = units * tiles;
-    IRIS_REQUIRE(all < (1ll << 30), "prefix_attn_fwd: too many rows");
+  plan.step_rows = static_cast<int>(step_rows);
+  plan.row_tiles = static_cast<int>(std::min<int64_t>(row_tiles, 1 << 30));
+  Cut tile_cut = {1, 1}, step_cut = {STEP_UNIT, 1};
+  int form = 0;  // 0 joint, 1 shared, 2 whole
+  // joint: up to eight chunks are joined in a cluster
+  for (int64_t s : {int64_t(1), int64_t(2), int64_t(4), int64_t(8), e.slots / std::max<int64_t>(1, step_units)}) {
+    const Cut c = cut(keys, s, STEP_UNIT);
+    const int64_t ctas = step_units * c.splits;
+    const float t = ((ctas + e.slots - 1) / e.slots) * e.step(std::min(c.chunk, keys), ctas) +
+                    (c.splits > MOST_CLUSTER ? e.join(e.all_rows, c.splits) : 0.f);
+    if (t < least) least = t, step_cut = c;
+  }
+  const int64_t prefix_blocks = (z.n_prefix + BKV - 1) / BKV;
+  if (per_group > 1 && z.n_prefix > 0) {
+    // the samples' own keys: split only where they leave SMs idle
+    const Cut own = cut(z.n_kv, step_units * 2 <= e.sms ? e.sms / step_units : 1, STEP_UNIT);
+    const int64_t steps = step_units * own.splits, units = z.groups * z.heads_kv;
+    const int64_t tiles = units * ((per_group * e.rows + BQ - 1) / BQ);
+    for (int64_t s : {int64_t(1), int64_t(2), int64_t(4), int64_t(8), int64_t(16), int64_t(32), e.sms / std::max<int64_t>(1, tiles),
+                      e.slots / std::max<int64_t>(1, tiles)}) {
+      const Cut c = cut(prefix_blocks, s, 1);
+      const int64_t ctas = tiles * c.splits;
+      const float tile = e.tile(c.chunk), step = e.step(std::min(own.chunk, z.n_kv), steps + ctas);
+      const int64_t beside = std::max<int64_t>(0, e.slots - ctas);  // slots that row tiles have from the start
+      float t;
+      if (ctas > e.slots) t = (ctas * tile + steps * step) / e.slots + 0.5f * tile;
+      else if (steps * step <= beside * tile) t = std::max(tile, (steps + beside - 1) / beside * step);
+      else t = tile + (steps * step - beside * tile) / e.slots + 0.5f * step;
+      t += e.join(e.all_rows, c.splits + own.splits);
+      if (t < least) least = t, form = 1, tile_cut = c, step_cut = own;
+    }
+  }
+  {
+    const int64_t blocks = prefix_blocks + (z.n_kv + BKV - 1) / BKV;
+    const int64_t tiles = z.batch * z.heads_kv * ((e.rows + BQ - 1) / BQ);
     // tiles that fill the SMs are not split; the last of them, which would leave some idle, are
-    const int64_t rest = whole && all % slots != 0 ? all % slots : all;
-    const int64_t splits = std::max<int64_t>(1, std::min(slots / rest, blocks / 4));
-    plan.tiles = static_cast<int>(tiles);
-    plan.tile_chunk = static_cast<int>(std::max<int64_t>(1, (blocks + splits - 1) / splits));
-    plan.tile_splits = static_cast<int>(std::max<int64_t>(1, (blocks + plan.tile_chunk - 1) / plan.tile_chunk));
-    plan.whole_tiles = static_cast<int>(!whole ? 0 : plan.tile_splits == 1 ? all : all - rest);
-    const int64_t ctas = plan.whole_tiles + (all - plan.whole_tiles) * plan.tile_splits;
+    const int64_t rest = tiles % e.slots != 0 ? tiles % e.slots : tiles;
+    const Cut c = cut(blocks, std::min(e.slots / std::max<int64_t>(1, rest), std::max<int64_t>(1, blocks / 4)), 1);
+    float t = ((tiles - 1) / e.slots) * e.tile(blocks) + e.tile(c.chunk);
+    if (c.splits > 1) t += e.join(rest * std::min<int64_t>(BQ, e.rows), c.splits);
+    if (t < least) least = t, form = 2, tile_cut = c;
+  }
+  plan.per = static_cast<int>(form == 1 ? per_group : 1);
+  const int64_t units = z.batch / plan.per * z.heads_kv, tiles = (plan.per * e.rows + BQ - 1) / BQ, all = units * tiles;
+  IRIS_REQUIRE(all < (1ll << 30) && step_units < (1ll << 30), "prefix_attn_fwd: too many rows");
+  plan.units = static_cast<int>(units);
+  plan.tiles = static_cast<int>(tiles);
+  plan.tile_splits = 1;
+  if (form != 0) {
+    const int64_t rest = form == 2 && all % e.slots != 0 ? all % e.slots : all;
+    plan.tile_chunk = static_cast<int>(tile_cut.chunk);
+    plan.tile_splits = static_cast<int>(tile_cut.splits);
+    plan.whole_tiles = static_cast<int>(form == 1 ? 0 : tile_cut.splits == 1 ? all : all - rest);
+    const int64_t ctas = plan.whole_tiles + (all - plan.whole_tiles) * tile_cut.splits;
     IRIS_REQUIRE(ctas < (1ll << 30), "prefix_attn_fwd: too many rows");
     plan.tile_ctas = static_cast<int>(ctas);
-  } else {  // join_kernel takes the rows by tiles too
-    plan.per = 1;
-    plan.tiles = static_cast<int>((rows + BQ - 1) / BQ);
   }
-  plan.units = static_cast<int>(z.batch / plan.per * z.heads_kv);
-  if (!whole) {
-    plan.step_rows = rows <= 8 ? 8 : 16;
-    plan.row_tiles = static_cast<int>((rows + plan.step_rows - 1) / plan.step_rows);
-    plan.step_prefix = !shared;
-    const int64_t units = z.batch * z.heads_kv * plan.row_tiles, keys = z.n_kv + (shared ? 0 : z.n_prefix);
-    const int64_t splits = std::max<int64_t>(1, std::min((slots + units - 1) / units, keys / 128));
-    plan.step_chunk = static_cast<int>(std::max<int64_t>(64, ((keys + splits - 1) / splits + 63) / 64 * 64));
-    plan.step_splits = static_cast<int>(std::max<int64_t>(1, (keys + plan.step_chunk - 1) / plan.step_chunk));
-    IRIS_REQUIRE(units * plan.step_splits < (1ll << 30), "prefix_attn_fwd: too many rows");
-    plan.step_ctas = static_cast<int>(units * plan.step_splits);
-    plan.cluster = plan.step_prefix && plan.step_splits > 1 && plan.step_splits <= MOST_CLUSTER;
+  if (form != 2) {
+    IRIS_REQUIRE(step_units * step_cut.splits < (1ll << 30), "prefix_attn_fwd: too many rows");
+    plan.step_prefix = form == 0;
+    plan.step_chunk = static_cast<int>(std::min<int64_t>(step_cut.chunk, 1ll << 30));
+    plan.step_splits = static_cast<int>(step_cut.splits);
+    plan.step_ctas = static_cast<int>(step_units * step_cut.splits);
+    plan.cluster = form == 0 && plan.step_splits > 1 && plan.step_splits <= MOST_CLUSTER;
   }
   *out = plan;
   return IRIS_OK;
@@ -1072,7 +1142,7 @@ int launch(const Params& p, int dtype, void* workspace, int64_t workspace_bytes,
   const int64_t rows = static_cast<int64_t>(p.batch) * p.n * p.heads_q;
   IRIS_REQUIRE(rows < (1ll << 31), "prefix_attn_fwd: too many rows");
   Plan plan;
-  IRIS_CHECK_STATUS(make_plan(Sizes{p.batch, p.batch / p.per_group, p.heads_q, p.heads_kv, p.n, p.n_prefix, p.n_kv, p.right}, &plan));
+  IRIS_CHECK_STATUS(make_plan(Sizes{p.batch, p.batch / p.per_group, p.heads_q, p.heads_kv, p.n, p.n_prefix, p.n_kv, D}, &plan));
   const Room room = room_of(plan);
   const bool parts = room.tile_rows + room.step_rows > 0;
   if (parts) {
@@ -1130,7 +1200,7 @@ extern "C" int iris_prefix_attn_workspace(const iris_prefix_problem* q, int64_t*
   *bytes = 0;
   if (q->batch * q->n == 0) return IRIS_OK;
   Plan plan;
-  IRIS_CHECK_STATUS(make_plan(Sizes{q->batch, q->groups, q->heads_q, q->heads_kv, q->n, q->n_prefix, q->n_kv, bound(q->right)}, &plan));
+  IRIS_CHECK_STATUS(make_plan(Sizes{q->batch, q->groups, q->heads_q, q->heads_kv, q->n, q->n_prefix, q->n_kv, q->head_dim}, &plan));
   *bytes = room_bytes(room_of(plan), q->head_dim);
   return IRIS_OK;
 }
