@@ -3,6 +3,7 @@
 //   out[m, n] = x_scale[m] w_scale[n] sum_k q[m, k] w[n, k] + bias[n]
 // The sum is of whole numbers and exact in int32 (K <= 131071: 128 * 128 * K < 2^31),
 // so how K is split changes nothing.
+#include <stdlib.h>
 #include <algorithm>
 
 #include "common.cuh"
@@ -17,9 +18,8 @@ namespace i8 {
 //
 // q is the correctly rounded quotient, halves to even: y = x (127 / max) is off by at
 // most 127 (2^-24 + 2^-24) < 2^-16, so y's nearest whole number is the quotient's
-// unless y is within 2^-15 of a half; such a value (one of 2^14) is divided in 64 bits,
-// where 127 x is exact and a quotient of two 24-bit numbers that is no half stays 2^-26
-// of itself away from one. So the 8-bit values are the formula's, whatever order or unit computes them.
+// unless y is within 2^-15 of a half h; then 254 x is compared with 2 h max, both exact in
+// 64 bits. So the 8-bit values are the formula's, whatever order or unit computes them.
 struct QuantizeParams {
   const void* x;
   int8_t* q;
@@ -77,8 +77,9 @@ IRIS_DEVICE uint4 load_vec(const T* row, int v, int K) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// up: a power of two that keeps rows of tiny values away from fp32's smallest steps; top and inv go with it.
 template <typename T>
-IRIS_DEVICE void store_vec(int8_t* out, const uint4& v, int at, int K, float inv, float top, bool slow) {
+IRIS_DEVICE void store_vec(int8_t* out, const uint4& v, int at, int K, float inv, float top, float up) {
   constexpr int N = Vec<T>::N;
   uint32_t packed[2] = {0u, 0u};
   float worst = 0.f;
@@ -88,18 +89,20 @@ IRIS_DEVICE void store_vec(int8_t* out, const uint4& v, int at, int K, float inv
     uint32_t b[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float x = value_of<T>(v, 4 * g + e);
+      const float x = value_of<T>(v, 4 * g + e) * up;
       const float t = fmaf(x, inv, kWhole);
       worst = fmaxf(worst, fabsf(fmaf(x, inv, -(t - kWhole))));
       b[e] = __float_as_uint(t);
     }
     packed[g] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
   }
-  if (slow || worst > 0.5f - 1.f / 32768) {
+  if (worst > 0.5f - 1.f / 32768) {
 #pragma unroll 1
     for (int e = 0; e < N; ++e) {
-      const float x = value_of<T>(v, e);
-      const int q = top == 0.f ? 0 : __double2int_rn(127.0 * x / static_cast<double>(top));
+      const float x = value_of<T>(v, e) * up;
+      const float lo = floorf(x * inv);
+      const double off = fma(254.0, static_cast<double>(x), -(2.0 * lo + 1.0) * top);
+      const int low = static_cast<int>(lo), q = off > 0.0 || (off == 0.0 && (low & 1)) ? low + 1 : low;
       packed[e >> 2] = (packed[e >> 2] & ~(0xffu << (8 * (e & 3)))) | (static_cast<uint32_t>(q) & 0xffu) << (8 * (e & 3));
     }
   }
@@ -148,14 +151,13 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) quantize_kernel
   float size = value_of<T>(bits, 0);
   const bool finite = size < INFINITY;  // not so for NaN
   if (t == 0) p.scale[m] = finite ? __fdiv_rn(size, 127.f) : NAN;
-  if (!finite) size = 0.f;
-  // below 2^-100 the reciprocal leaves fp32 or 127 x loses bits; 0 has none
-  const bool slow = size < 7.9e-31f;
-  const float inv = slow ? 0.f : __fdiv_rn(127.f, size);
+  // rows below 2^-100 are scaled up, exactly; a row that is not finite gives zeros
+  const float up = !finite ? 0.f : size < 7.9e-31f ? 1.2676506e30f : 1.f;
+  size *= up;
+  const float inv = finite && size > 0.f ? __fdiv_rn(127.f, size) : 0.f;
   int8_t* out = p.q + m * p.ldq;
   auto store = [&](const uint4& v, int at) {
-    if (finite) store_vec<T>(out, v, at, p.K, inv, size, slow);
-    else store_vec<T>(out, make_uint4(0u, 0u, 0u, 0u), at, p.K, 0.f, 0.f, false);
+    store_vec<T>(out, finite ? v : make_uint4(0u, 0u, 0u, 0u), at, p.K, inv, finite ? size : 0.f, up);
   };
 #pragma unroll
   for (int i = 0; i < KEPT; ++i)
@@ -225,6 +227,45 @@ IRIS_DEVICE float scaled(int sum, float xs, float ws, float bias) {
 }
 IRIS_DEVICE void store_out(const Params& p, int64_t at, float y) { store_elem(p.out, at, p.out_dtype, y); }
 
+template <typename O>
+IRIS_DEVICE O rounded(float y);
+template <>
+IRIS_DEVICE float rounded<float>(float y) { return y; }
+template <>
+IRIS_DEVICE __nv_bfloat16 rounded<__nv_bfloat16>(float y) { return __float2bfloat16_rn(y); }
+template <>
+IRIS_DEVICE __half rounded<__half>(float y) { return __float2half_rn(y); }
+
+// A warp's 32 channels (lane: channel n) of tokens [m0, m0 + count) from TMEM columns [at, at + count).
+template <typename O>
+IRIS_DEVICE void store_columns_as(const Params& p, uint32_t at, int m0, int count, int n, bool ok) {
+  const int lane = threadIdx.x & 31;
+  const bool real = n < p.N;
+  const float ws = real ? p.w_scale[n] : 0.f, bias = real && p.bias ? p.bias[n] : 0.f;
+  O* out = reinterpret_cast<O*>(p.out) + static_cast<int64_t>(m0) * p.N + n;
+#pragma unroll 1
+  for (int c = 0; c < count; c += 16) {
+    const int most = real ? p.M - m0 - c : 0;
+    if (m0 + c >= p.M) break;
+    uint32_t r[16];
+    tmem_ld16(at + c, r);
+    const float mine = m0 + c + (lane & 15) < p.M ? p.x_scale[m0 + c + (lane & 15)] : 0.f;
+    tmem_wait_ld();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float xs = __shfl_sync(0xffffffffu, mine, e);
+      const float y = ok ? scaled(static_cast<int>(r[e]), xs, ws, bias) : NAN;
+      if (e < most) *out = rounded<O>(y);
+      out += p.N;
+    }
+  }
+}
+IRIS_DEVICE void store_columns(const Params& p, uint32_t at, int m0, int count, int n, bool ok) {
+  if (p.out_dtype == IRIS_F32) store_columns_as<float>(p, at, m0, count, n, ok);
+  else if (p.out_dtype == IRIS_BF16) store_columns_as<__nv_bfloat16>(p, at, m0, count, n, ok);
+  else store_columns_as<__half>(p, at, m0, count, n, ok);
+}
+
 template <int T>
 struct Rows {
   static constexpr int X_BYTES = T * SLAB, W_BYTES = BN * SLAB, STAGE = X_BYTES + W_BYTES;
@@ -250,7 +291,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   RowsSmem<T>* s = reinterpret_cast<RowsSmem<T>*>(ring + R::RING);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int part = static_cast<int>(blockIdx.x % p.splits), unit = static_cast<int>(blockIdx.x / p.splits);
   const int m0 = unit % p.token_tiles * T, n0 = unit / p.token_tiles * BN;
   const int slabs = (p.K + SLAB - 1) / SLAB;
@@ -346,23 +387,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   const bool real = n < p.N;
   if (p.splits == 1) {
-    if (warp >= 2) {
-      const float ws = real ? p.w_scale[n] : 0.f, bias = real && p.bias ? p.bias[n] : 0.f;
-#pragma unroll 1
-      for (int c = 0; c < T; c += 16) {
-        if (m0 + c >= p.M) break;
-        uint32_t r[16];
-        tmem_ld16(lanes + c, r);
-        const float mine = m0 + c + (lane & 15) < p.M ? p.x_scale[m0 + c + (lane & 15)] : 0.f;
-        tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float xs = __shfl_sync(0xffffffffu, mine, e);
-          const int m = m0 + c + e;
-          if (real && m < p.M) store_out(p, static_cast<int64_t>(m) * p.N + n, ok ? scaled(static_cast<int>(r[e]), xs, ws, bias) : NAN);
-        }
-      }
-    }
+    if (warp >= 2) store_columns(p, lanes, m0, T, n, ok);
   } else {
     // each part's sums go to the CTA that owns the columns, into its ring, which no
     // copy and no MMA of that CTA uses any more
@@ -425,6 +450,238 @@ int launch_rows(const CUtensorMap& tw, const CUtensorMap& tx, Params p, cudaStre
   IRIS_REQUIRE(units * p.splits < (1ll << 31), "gemm_i8: too many rows");
   IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(units * p.splits)), THREADS, Rows<T>::SMEM, st,
                          static_cast<unsigned>(p.splits), tw, tx, p));
+  return IRIS_OK;
+}
+
+// ---------------------------------------------------------------- many tokens
+// CTA pairs (cta_group::2), persistent: a cluster of two CTAs on paired SMs computes 256
+// weight rows by up to 256 tokens. Each CTA brings its own 128 weight rows and half of the
+// tokens' rows by TMA, 256 wide in k (two slabs) into a three-stage ring; both CTAs' copies complete
+// on the leader's barrier. The leader's MMA thread issues tcgen05.mma.cta_group::2, which
+// leaves each CTA's 128 rows by all tokens in that CTA's TMEM, twice: the next tile's
+// products run under the epilogue. The tile's tokens (a multiple of 32) follow M, so that
+// the last tile is not mostly padding.
+namespace pair {
+constexpr int STAGES = 3, SLABS = 2;
+constexpr int W_BYTES = 128 * SLAB, X_BYTES = 128 * SLAB;  // of a slab, at most
+constexpr int STAGE = SLABS * (W_BYTES + X_BYTES);
+constexpr int GROUP = 16;  // neighbouring tiles: 16 of weight rows share their tokens, then tokens go on
+struct Smem {
+  uint64_t full[STAGES];  // used in the leader only: both CTAs' copies complete here
+  uint64_t empty[STAGES];
+  uint64_t tmem_full[2];
+  uint64_t tmem_empty[2];  // used in the leader only: 4 local + 4 peer epilogue warps
+  uint64_t teardown;
+  uint32_t tmem_base;
+  int abort;
+};
+constexpr int SMEM = 1024 + STAGES * STAGE + static_cast<int>(sizeof(Smem));
+static_assert(SMEM <= 232448, "pair kernel shared memory");
+
+struct Tile {
+  int nb, mb;
+};
+IRIS_DEVICE Tile locate(int t, int num_n, int num_m) {
+  const int group = t / (GROUP * num_m), first = group * GROUP;
+  const int in_group = t - group * GROUP * num_m, wide = min(GROUP, num_n - first);
+  return Tile{first + in_group % wide, in_group / wide};
+}
+IRIS_DEVICE void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+}  // namespace pair
+
+__global__ void __launch_bounds__(THREADS, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
+                const __grid_constant__ Params p, int tokens) {
+  using namespace pair;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  pair::Smem* s = reinterpret_cast<pair::Smem*>(ring + STAGES * STAGE);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const bool leader = rank == 0;
+  const int pair_id = static_cast<int>(blockIdx.x / 2), pairs = static_cast<int>(gridDim.x / 2);
+  const int num_n = (p.N + 255) / 256, num_m = (p.M + tokens - 1) / tokens, tiles = num_n * num_m;
+  const int slabs = (p.K + SLAB - 1) / SLAB, steps = (slabs + SLABS - 1) / SLABS;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&s->full[i], 1);
+      mbar_init(&s->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s->tmem_full[i], 1);
+      mbar_init(&s->tmem_empty[i], 8);
+    }
+    mbar_init(&s->teardown, 1);
+    s->abort = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tw);
+    tma_prefetch_desc(&tx);
+  }
+  if (warp == 1) tmem_alloc_pair(&s->tmem_base, 512);
+  tc_fence_before();
+  cluster_sync();  // every barrier of both CTAs exists before any remote arrival
+  tc_fence_after();
+  const uint32_t tmem = s->tmem_base;
+  volatile int* abort = &s->abort;
+  grid_wait();
+  grid_trigger();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer (both CTAs)
+    if (lane == 0) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const int half = tokens / 2;
+      for (int t = pair_id; t < tiles && ok; t += pairs) {
+        const Tile tl = locate(t, num_n, num_m);
+        for (int step = 0; step < steps; ++step) {
+          if (!mbar_wait(&s->empty[stage], phase ^ 1u, abort)) {
+            ok = false;
+            break;
+          }
+          const uint32_t full_leader = map_to_cta(&s->full[stage], 0);
+          const int n = min(SLABS, slabs - step * SLABS);
+          if (leader) mbar_arrive_expect_tx(&s->full[stage], 2 * n * (W_BYTES + half * SLAB));
+          for (int i = 0; i < n; ++i) {
+            const int k = (step * SLABS + i) * SLAB;
+            tma_load_2d_pair(&tw, full_leader, ring + stage * STAGE + i * W_BYTES, k, tl.nb * 256 + rank * 128);
+            tma_load_2d_pair(&tx, full_leader, ring + stage * STAGE + SLABS * W_BYTES + i * X_BYTES, k, tl.mb * tokens + rank * half);
+          }
+          ++issued;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok && issued > 0) {
+        // the loads in flight target both CTAs' shared memory: give them time to land
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader)
+    if (lane == 0 && leader) {
+      const uint32_t idesc = idesc_i8(256, tokens);
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair_id; t < tiles && ok; t += pairs, ++it) {
+        const int acc = it & 1;
+        if (!mbar_wait_cluster(&s->tmem_empty[acc], static_cast<uint32_t>((it >> 1) & 1) ^ 1u, abort)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem + static_cast<uint32_t>(acc * 256);
+        for (int step = 0; step < steps; ++step) {
+          if (!mbar_wait(&s->full[stage], phase, abort)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int n = min(SLABS, slabs - step * SLABS);
+          for (int i = 0; i < n; ++i) {
+            const uint32_t w_addr = smem_addr(ring + stage * STAGE + i * W_BYTES);
+            const uint32_t x_addr = smem_addr(ring + stage * STAGE + SLABS * W_BYTES + i * X_BYTES);
+#pragma unroll
+            for (int k = 0; k < SLAB / 32; ++k)
+              umma_i8_pair(d_tmem, umma_desc(w_addr + k * 32, 16, 1024, kLayoutSw128), umma_desc(x_addr + k * 32, 16, 1024, kLayoutSw128),
+                           idesc, (step | i | k) != 0 ? 1u : 0u);
+          }
+          umma_commit_pair(map_to_cta(&s->empty[stage], 0));
+          umma_commit_pair(map_to_cta(&s->empty[stage], 1));
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) {
+          umma_commit_pair(map_to_cta(&s->tmem_full[acc], 0));
+          umma_commit_pair(map_to_cta(&s->tmem_full[acc], 1));
+        }
+      }
+      umma_commit_pair(map_to_cta(&s->teardown, 0));
+      int dummy = 0;
+      mbar_wait(&s->teardown, 0, &dummy);
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int quarter = warp & 3;
+    const uint32_t empty_leader = map_to_cta(&s->tmem_empty[0], 0);
+    int it = 0;
+    bool ok = true;  // a wait gave up: NaN rather than wrong values
+    for (int t = pair_id; t < tiles; t += pairs, ++it) {
+      const Tile tl = locate(t, num_n, num_m);
+      const int acc = it & 1;
+      ok = ok && __all_sync(0xffffffffu, mbar_wait_cluster(&s->tmem_full[acc], static_cast<uint32_t>((it >> 1) & 1), abort));
+      tc_fence_after();
+      const int n = tl.nb * 256 + rank * 128 + quarter * 32 + lane;
+      store_columns(p, tmem + static_cast<uint32_t>(acc * 256) + (static_cast<uint32_t>(quarter * 32) << 16), tl.mb * tokens, tokens, n, ok);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(empty_leader + static_cast<uint32_t>(acc) * 8u);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();  // no CTA leaves while the other may still address its barriers or TMEM
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
+// Not every SM has a partner SM that a cluster of two can use: the persistent grid has the
+// clusters that are resident at once.
+int resident_pairs(int* pairs) {
+  static int cache[64] = {0};
+  int dev = 0;
+  IRIS_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || cache[dev] == 0) {
+    IRIS_CUDA(cudaFuncSetAttribute(pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pair::SMEM));
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(num_sms() / 2 * 2));
+    config.blockDim = dim3(THREADS);
+    config.dynamicSmemBytes = pair::SMEM;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    IRIS_CUDA(cudaOccupancyMaxActiveClusters(pairs, pair_kernel, &config));
+    IRIS_REQUIRE(*pairs > 0, "gemm_i8: no CTA pair fits on this device");
+    if (dev < 64) cache[dev] = *pairs;
+    return IRIS_OK;
+  }
+  *pairs = cache[dev];
+  return IRIS_OK;
+}
+
+// Tokens of a tile: as few tiles as 256 gives, evenly filled.
+inline int pair_tokens(int64_t M) {
+  const int64_t tiles = (M + 255) / 256;
+  return static_cast<int>(((M + tiles - 1) / tiles + 31) / 32 * 32);
+}
+
+int launch_pair(const void* w, int64_t ldw, const void* x, int64_t ldx, const Params& p, cudaStream_t st) {
+  const int tokens = pair_tokens(p.M);
+  CUtensorMap tw, tx;
+  IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tw, w, p.K, p.N, ldw, SLAB, 128));
+  IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tx, x, p.K, p.M, ldx, SLAB, tokens / 2));
+  int pairs = 0;
+  IRIS_CHECK_STATUS(resident_pairs(&pairs));
+  const int64_t tiles = static_cast<int64_t>((p.N + 255) / 256) * ((p.M + tokens - 1) / tokens);
+  IRIS_REQUIRE(tiles < (1ll << 30), "gemm_i8: too many tiles");
+  IRIS_CUDA(launch_early(pair_kernel, dim3(static_cast<unsigned>(2 * std::min<int64_t>(tiles, pairs))), THREADS, pair::SMEM, st, 2, tw, tx,
+                         p, tokens));
   return IRIS_OK;
 }
 
@@ -513,6 +770,8 @@ extern "C" int iris_gemm_i8(const iris_i8_problem* q, void* stream) {
   p.M = static_cast<int>(q->M), p.N = static_cast<int>(q->N), p.K = static_cast<int>(q->K);
   p.out_dtype = static_cast<int>(q->out_dtype);
   p.early = fresh;
+  const char* ev = getenv("I8_PAIR");
+  if (ev ? atoi(ev) : p.M > 256) return launch_pair(q->w, q->ldw, x, ldx, p, st);
   const int tokens = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
   CUtensorMap tw, tx;
   IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tw, q->w, q->K, q->N, q->ldw, SLAB, BN));
