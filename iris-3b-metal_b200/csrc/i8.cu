@@ -5,6 +5,7 @@
 // so how K is split changes nothing.
 #include <stdlib.h>
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "iris_abi_internal.h"
@@ -16,10 +17,17 @@ namespace i8 {
 // HBM-bound: one read of x, one byte written per value. A team of warps takes a row and
 // keeps it in registers between the maximum and the rounding (what does not fit is read again).
 //
-// q is the correctly rounded quotient, halves to even: y = x (127 / max) is off by at
-// most 127 (2^-24 + 2^-24) < 2^-16, so y's nearest whole number is the quotient's
-// unless y is within 2^-15 of a half h; then 254 x is compared with 2 h max, both exact in
-// 64 bits. So the 8-bit values are the formula's, whatever order or unit computes them.
+// q is the correctly rounded quotient y = 127 x / max, halves to even, so that the 8-bit
+// values are the formula's, whatever order or unit computes them.
+//  - Rows of 16 bits meet halves often (a quarter of a warp's vectors hold one). With 127 / max =
+//    hi + lo to 48 bits, fma(x, hi, x lo) is y rounded to fp32: a half comes out as
+//    itself, and any other y, a ratio of short numbers, stays on its side: it is at least 2^-19 of
+//    itself away (254 m - h M 2^j is a whole number, m and M below 2^11), fp32 rounds by 2^-24.
+//  - FP32 rows: x hi is off by at most 127 (2^-24 + 2^-24) < 2^-16, so its nearest whole number
+//    is y's unless it lies within 2^-15 of a half h; then 254 x is compared with 2 h max,
+//    both exact in 64 bits.
+//
+// Measured, bf16: 16384 rows of 8192 QUANT_LONG us (QUANT_RATE TB/s), 2400 of 2560 QUANT_SOME us.
 struct QuantizeParams {
   const void* x;
   int8_t* q;
@@ -77,34 +85,56 @@ IRIS_DEVICE uint4 load_vec(const T* row, int v, int K) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// up: a power of two that keeps rows of tiny values away from fp32's smallest steps; top and inv go with it.
+// What a row's values are multiplied by.
+struct Factors {
+  float hi, lo;  // 127 / (top up)
+  float top, up; // the largest magnitude, scaled by a power of two where it is extreme (extreme: up is not 1)
+};
+
+// A vector's 8-bit values from 64-bit comparisons: values next to halves, and rows of
+// extreme values, whose factors alone would leave fp32.
 template <typename T>
-IRIS_DEVICE void store_vec(int8_t* out, const uint4& v, int at, int K, float inv, float top, float up) {
+__device__ __noinline__ uint2 round_exactly(uint4 v, float hi, float top, float up) {
+  uint32_t packed[2] = {0u, 0u};
+#pragma unroll 1
+  for (int e = 0; e < Vec<T>::N; ++e) {
+    const float x = value_of<T>(v, e) * up;
+    const float low = floorf(x * hi);
+    const double off = fma(254.0, static_cast<double>(x), -(2.0 * low + 1.0) * top);
+    const int lo = static_cast<int>(low), q = off > 0 || (off == 0 && (lo & 1)) ? lo + 1 : lo;
+    packed[e >> 2] |= (static_cast<uint32_t>(q) & 0xffu) << (8 * (e & 3));
+  }
+  return make_uint2(packed[0], packed[1]);
+}
+
+template <typename T>
+IRIS_DEVICE void store_vec(int8_t* out, const uint4& v, int at, int K, const Factors& f) {
   constexpr int N = Vec<T>::N;
   uint32_t packed[2] = {0u, 0u};
-  float worst = 0.f;
+  bool again = f.up != 1.f;
   constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: the sum's last bit is 1
+  const float2 hi = make_float2(f.hi, f.hi), lo = make_float2(f.lo, f.lo), whole = make_float2(kWhole, kWhole);
 #pragma unroll
   for (int g = 0; g < N / 4; ++g) {
     uint32_t b[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x = value_of<T>(v, 4 * g + e) * up;
-      const float t = fmaf(x, inv, kWhole);
-      worst = fmaxf(worst, fabsf(fmaf(x, inv, -(t - kWhole))));
-      b[e] = __float_as_uint(t);
+    for (int e = 0; e < 4; e += 2) {
+      const float2 x = make_float2(value_of<T>(v, 4 * g + e), value_of<T>(v, 4 * g + e + 1));
+      float2 t;
+      if (sizeof(T) == 2) {
+        t = __fadd2_rn(__ffma2_rn(x, hi, __fmul2_rn(x, lo)), whole);
+      } else {
+        t = __ffma2_rn(x, hi, whole);
+        const float2 r = __ffma2_rn(x, hi, __ffma2_rn(t, make_float2(-1.f, -1.f), whole));  // minus the whole number
+        again = again || fmaxf(fabsf(r.x), fabsf(r.y)) > 0.5f - 1.f / 32768;
+      }
+      b[e] = __float_as_uint(t.x), b[e + 1] = __float_as_uint(t.y);
     }
     packed[g] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
   }
-  if (worst > 0.5f - 1.f / 32768) {
-#pragma unroll 1
-    for (int e = 0; e < N; ++e) {
-      const float x = value_of<T>(v, e) * up;
-      const float lo = floorf(x * inv);
-      const double off = fma(254.0, static_cast<double>(x), -(2.0 * lo + 1.0) * top);
-      const int low = static_cast<int>(lo), q = off > 0.0 || (off == 0.0 && (low & 1)) ? low + 1 : low;
-      packed[e >> 2] = (packed[e >> 2] & ~(0xffu << (8 * (e & 3)))) | (static_cast<uint32_t>(q) & 0xffu) << (8 * (e & 3));
-    }
+  if (again) {
+    const uint2 w = round_exactly<T>(v, f.hi, f.top, f.up);
+    packed[0] = w.x, packed[1] = w.y;
   }
   if ((at + 1) * N <= K) {
     if (N == 8) *reinterpret_cast<uint2*>(out + at * N) = make_uint2(packed[0], packed[1]);
@@ -119,63 +149,74 @@ IRIS_DEVICE void store_vec(int8_t* out, const uint4& v, int at, int K, float inv
 constexpr int KEPT = 4;  // vectors of a row that a thread keeps
 
 template <typename T, int WARPS, bool ALIGNED>
-__global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32) quantize_kernel(const QuantizeParams p) {
+__global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32, WARPS == 8 ? 4 : 8) quantize_kernel(const QuantizeParams p) {
   constexpr int TEAM = WARPS * 32, N = Vec<T>::N;
-  __shared__ uint32_t tops[WARPS];
+  __shared__ uint32_t tops[2][WARPS];
   grid_wait();
   grid_trigger();
   const int t = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
-  const int m = WARPS == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
-  if (m >= p.M) return;  // a warp of its own team
-  const T* row = reinterpret_cast<const T*>(p.x) + m * p.ldx;
   const int vecs = (p.K + N - 1) / N;
+  const int step = WARPS == 1 ? gridDim.x * 4 : gridDim.x;
+  const T* x = reinterpret_cast<const T*>(p.x);
   uint4 kept[KEPT];
+  auto load = [&](int64_t m) {
 #pragma unroll
-  for (int i = 0; i < KEPT; ++i) {
-    const int v = t + i * TEAM;
-    kept[i] = v < vecs ? load_vec<T, ALIGNED>(row, v, p.K) : make_uint4(0u, 0u, 0u, 0u);
-  }
-  uint32_t top = 0u;
-#pragma unroll
-  for (int i = 0; i < KEPT; ++i) top = top_of<T>(kept[i], top);
-  for (int v = t + KEPT * TEAM; v < vecs; v += TEAM) top = top_of<T>(load_vec<T, ALIGNED>(row, v, p.K), top);
-  if (sizeof(T) == 2) top = max(top & 0xffffu, top >> 16);
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (WARPS > 1) {
-    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) top = max(top, tops[w]);
-  }
-  uint4 bits = make_uint4(top, 0u, 0u, 0u);
-  float size = value_of<T>(bits, 0);
-  const bool finite = size < INFINITY;  // not so for NaN
-  if (t == 0) p.scale[m] = finite ? __fdiv_rn(size, 127.f) : NAN;
-  // rows below 2^-100 are scaled up, exactly; a row that is not finite gives zeros
-  const float up = !finite ? 0.f : size < 7.9e-31f ? 1.2676506e30f : 1.f;
-  size *= up;
-  const float inv = finite && size > 0.f ? __fdiv_rn(127.f, size) : 0.f;
-  int8_t* out = p.q + m * p.ldq;
-  auto store = [&](const uint4& v, int at) {
-    store_vec<T>(out, finite ? v : make_uint4(0u, 0u, 0u, 0u), at, p.K, inv, finite ? size : 0.f, up);
+    for (int i = 0; i < KEPT; ++i) {
+      const int v = t + i * TEAM;
+      kept[i] = m < p.M && v < vecs ? load_vec<T, ALIGNED>(x + m * p.ldx, v, p.K) : make_uint4(0u, 0u, 0u, 0u);
+    }
   };
+  int64_t m = WARPS == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  load(m);
+  for (int turn = 0; m < p.M; m += step, turn ^= 1) {
+    const T* row = x + m * p.ldx;
+    uint4 now[KEPT];
+    uint32_t top = 0u;
 #pragma unroll
-  for (int i = 0; i < KEPT; ++i)
-    if (t + i * TEAM < vecs) store(kept[i], t + i * TEAM);
-  for (int v = t + KEPT * TEAM; v < vecs; v += TEAM) store(load_vec<T, ALIGNED>(row, v, p.K), v);
+    for (int i = 0; i < KEPT; ++i) {
+      now[i] = kept[i];
+      top = top_of<T>(now[i], top);
+    }
+    load(m + step);  // the next row's values are on their way while this one's are rounded
+    for (int v = t + KEPT * TEAM; v < vecs; v += TEAM) top = top_of<T>(load_vec<T, ALIGNED>(row, v, p.K), top);
+    if (sizeof(T) == 2) top = max(top & 0xffffu, top >> 16);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (WARPS > 1) {
+      if ((threadIdx.x & 31) == 0) tops[turn][threadIdx.x >> 5] = top;
+      __syncthreads();  // and no warp is a row ahead of another's reading
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) top = max(top, tops[turn][w]);
+    }
+    const float size = value_of<T>(make_uint4(top, 0u, 0u, 0u), 0);
+    const bool finite = size < INFINITY;  // not so for NaN
+    if (t == 0) p.scale[m] = finite ? __fdiv_rn(size, 127.f) : NAN;
+    // extreme rows are scaled to where the factors are normal numbers, exactly but for values
+    // that round to 0; a row that is not finite gives zeros
+    Factors f;
+    f.up = !finite ? 0.f : size < 0x1p-100f ? 0x1p100f : size > 0x1p60f ? 0x1p-100f : 1.f;
+    f.top = finite ? size * f.up : 0.f;
+    f.hi = f.top > 0.f ? __fdiv_rn(127.f, f.top) : 0.f;
+    f.lo = f.top > 0.f ? __fdiv_rn(fmaf(-f.hi, f.top, 127.f), f.top) : 0.f;
+    int8_t* out = p.q + m * p.ldq;
+    auto store = [&](const uint4& v, int at) { store_vec<T>(out, finite ? v : make_uint4(0u, 0u, 0u, 0u), at, p.K, f); };
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i)
+      if (t + i * TEAM < vecs) store(now[i], t + i * TEAM);
+    for (int v = t + KEPT * TEAM; v < vecs; v += TEAM) store(load_vec<T, ALIGNED>(row, v, p.K), v);
+  }
 }
 
 template <typename T, bool ALIGNED>
 int launch_quantize(const QuantizeParams& p, cudaStream_t st) {
   const int vecs = (p.K + Vec<T>::N - 1) / Vec<T>::N;
-  const unsigned rows = static_cast<unsigned>(p.M);
-  // the smallest team that keeps a row
+  // the smallest team that keeps a row; no more CTAs than the SMs hold at once
+  const int64_t rows = p.M, sms = num_sms();
   if (vecs <= KEPT * 32)
-    IRIS_CUDA(launch_early(quantize_kernel<T, 1, ALIGNED>, dim3((rows + 3) / 4), 128, 0, st, 1, p));
+    IRIS_CUDA(launch_early(quantize_kernel<T, 1, ALIGNED>, dim3(static_cast<unsigned>(std::min((rows + 3) / 4, 8 * sms))), 128, 0, st, 1, p));
   else if (vecs <= KEPT * 128)
-    IRIS_CUDA(launch_early(quantize_kernel<T, 4, ALIGNED>, dim3(rows), 128, 0, st, 1, p));
+    IRIS_CUDA(launch_early(quantize_kernel<T, 4, ALIGNED>, dim3(static_cast<unsigned>(std::min(rows, 8 * sms))), 128, 0, st, 1, p));
   else
-    IRIS_CUDA(launch_early(quantize_kernel<T, 8, ALIGNED>, dim3(rows), 256, 0, st, 1, p));
+    IRIS_CUDA(launch_early(quantize_kernel<T, 8, ALIGNED>, dim3(static_cast<unsigned>(std::min(rows, 4 * sms))), 256, 0, st, 1, p));
   return IRIS_OK;
 }
 
@@ -392,7 +433,9 @@ __global__ void __launch_bounds__(THREADS, 2)
     // each part's sums go to the CTA that owns the columns, into its ring, which no
     // copy and no MMA of that CTA uses any more
     cluster_sync();
-    const int own = T / p.splits, log_own = __ffs(own) - 1;  // columns of a CTA: a power of two
+    const int own = T / p.splits, log_own = __ffs(own) - 1;  // columns of a CTA: a power of two, 2 at least
+    // a lane's sums in neighbouring words: 128 bytes a store (four columns of a lane as one
+    // 16-byte store each took a third longer: 64 rows 2560 -> 2560 8.8 -> 11.7 us)
     int* parts = reinterpret_cast<int*>(ring);  // [part][column][128]
     if (warp >= 2) {
 #pragma unroll 1
@@ -402,8 +445,9 @@ __global__ void __launch_bounds__(THREADS, 2)
         tmem_wait_ld();
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int col = c + e, owner = col >> log_own;
-          const uint32_t to = map_to_cta(parts + (part * own + (col & (own - 1))) * BN + quarter * 32 + lane, static_cast<uint32_t>(owner));
+          const int col = c + e;
+          const uint32_t to = map_to_cta(parts + (part * own + (col & (own - 1))) * BN + quarter * 32 + lane,
+                                         static_cast<uint32_t>(col >> log_own));
           asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(r[e]) : "memory");
         }
       }
@@ -417,12 +461,21 @@ __global__ void __launch_bounds__(THREADS, 2)
       bool bad = false;
       for (int i = 0; i < p.splits; ++i) bad = bad || s->bad[i] != 0;
       const float ws = real ? p.w_scale[n] : 0.f, bias = real && p.bias ? p.bias[n] : 0.f;
-      for (int c = 0; c < own; ++c) {
+      const int* from = parts + quarter * 32 + lane;
+#pragma unroll 1
+      for (int c = 0; c < own; c += 4) {
         const int m = m0 + part * own + c;
         if (m >= p.M) break;
-        int sum = 0;
-        for (int i = 0; i < p.splits; ++i) sum += parts[(i * own + c) * BN + quarter * 32 + lane];
-        if (real) store_out(p, static_cast<int64_t>(m) * p.N + n, bad ? NAN : scaled(sum, p.x_scale[m], ws, bias));
+        int sum[4] = {0, 0, 0, 0};
+#pragma unroll 2
+        for (int i = 0; i < p.splits; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e < 2 || own >= 4) sum[e] += from[(i * own + c + e) * BN];
+        const int most = real ? min(min(own, 4), p.M - m) : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < most) store_out(p, static_cast<int64_t>(m + e) * p.N + n, bad ? NAN : scaled(sum[e], p.x_scale[m + e], ws, bias));
       }
     }
   }
