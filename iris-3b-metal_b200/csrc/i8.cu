@@ -3,7 +3,6 @@
 //   out[m, n] = x_scale[m] w_scale[n] sum_k q[m, k] w[n, k] + bias[n]
 // The sum is of whole numbers and exact in int32 (K <= 131071: 128 * 128 * K < 2^31),
 // so how K is split changes nothing.
-#include <stdlib.h>
 #include <algorithm>
 #include <type_traits>
 
@@ -231,7 +230,8 @@ int quantize(const QuantizeParams& p, cudaStream_t st) {
 // tensor cores' first operand, whatever the number of tokens, so that few tokens waste
 // none of it and the lanes of a warp write neighbouring channels of out, at any N.
 constexpr int BN = 128, SLAB = 128;  // weight rows of a CTA, k of a ring slot (bytes)
-constexpr int THREADS = 192;
+constexpr int EPILOGUE = 8;  // warps: two for each quarter of the TMEM lanes, half of the tokens each
+constexpr int THREADS = 64 + 32 * EPILOGUE;
 
 struct Params {
   const float* x_scale;
@@ -307,37 +307,44 @@ IRIS_DEVICE void store_columns(const Params& p, uint32_t at, int m0, int count, 
   else store_columns_as<__half>(p, at, m0, count, n, ok);
 }
 
-template <int T>
+// Few tokens, or few weight rows: a CTA of T tokens, two CTAs to an SM or (DEEP) one with
+// twice the ring, filled and committed two slabs at a time.
+template <int T, bool DEEP>
 struct Rows {
-  static constexpr int X_BYTES = T * SLAB, W_BYTES = BN * SLAB, STAGE = X_BYTES + W_BYTES;
-  static constexpr int STAGES = T == 16 ? 6 : T == 32 ? 5 : T == 64 ? 4 : 3;
+  static constexpr int SLABS = DEEP ? 2 : 1;  // of a stage
+  static constexpr int X_BYTES = T * SLAB, W_BYTES = BN * SLAB, STAGE = SLABS * (X_BYTES + W_BYTES);
+  static constexpr int STAGES = T <= 32 ? 5 : T == 64 ? 4 : 3;
   static constexpr int COLS = T < 32 ? 32 : T;
   static constexpr int RING = STAGES * STAGE;
-  static constexpr int SMEM = 1024 + RING + 256;
-  static_assert(T * BN * 4 <= RING, "the parts of a tile lie in the ring");
+  // the parts' sums: few tokens' have a place of their own, many tokens' lie in the ring
+  static constexpr bool APART = T <= 16;
+  static constexpr int PARTS = T * BN * 4;
+  static constexpr int SMEM = 1024 + RING + (APART ? PARTS : 0) + 256;
+  static_assert(PARTS <= RING && SMEM <= 232448, "the parts of a tile lie in the ring");
 };
 
-template <int T>
+template <int T, bool DEEP>
 struct RowsSmem {
-  uint64_t full[Rows<T>::STAGES], empty[Rows<T>::STAGES], done;
+  uint64_t full[Rows<T, DEEP>::STAGES], empty[Rows<T, DEEP>::STAGES], done;
   uint32_t tmem_base;
   int abort, bad[8];
 };
 
-template <int T>
-__global__ void __launch_bounds__(THREADS, 2)
+template <int T, bool DEEP>
+__global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2)
     rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
                 const __grid_constant__ Params p) {
-  using R = Rows<T>;
+  using R = Rows<T, DEEP>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  RowsSmem<T>* s = reinterpret_cast<RowsSmem<T>*>(ring + R::RING);
+  auto* s = reinterpret_cast<RowsSmem<T, DEEP>*>(ring + R::RING + (R::APART ? R::PARTS : 0));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int part = static_cast<int>(blockIdx.x % p.splits), unit = static_cast<int>(blockIdx.x / p.splits);
   const int m0 = unit % p.token_tiles * T, n0 = unit / p.token_tiles * BN;
   const int slabs = (p.K + SLAB - 1) / SLAB;
   const int first = static_cast<int>(static_cast<int64_t>(slabs) * part / p.splits);
   const int count = static_cast<int>(static_cast<int64_t>(slabs) * (part + 1) / p.splits) - first;
+  const int steps = (count + R::SLABS - 1) / R::SLABS;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < R::STAGES; ++i) {
@@ -357,19 +364,23 @@ __global__ void __launch_bounds__(THREADS, 2)
   tc_fence_after();
   const uint32_t tmem = s->tmem_base;
   volatile int* abort = &s->abort;
+  if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
   if (warp == 0) {
     // ----------------------------------------------------------------- TMA
     if (lane == 0) {
-      const int ahead = p.early ? min(count, R::STAGES) : 0;
+      const int ahead = p.early ? min(steps, R::STAGES) : 0;
       auto load_w = [&](int i) {
-        const int st = i % R::STAGES;
-        mbar_arrive_expect_tx(&s->full[st], R::STAGE);
-        tma_load_2d(&tw, &s->full[st], ring + st * R::STAGE, (first + i) * SLAB, n0);
+        const int st = i % R::STAGES, n = min(R::SLABS, count - i * R::SLABS);
+        mbar_arrive_expect_tx(&s->full[st], n * (R::W_BYTES + R::X_BYTES));
+        for (int j = 0; j < n; ++j)
+          tma_load_2d(&tw, &s->full[st], ring + st * R::STAGE + j * R::W_BYTES, (first + i * R::SLABS + j) * SLAB, n0);
       };
       auto load_x = [&](int i) {
-        const int st = i % R::STAGES;
-        tma_load_2d(&tx, &s->full[st], ring + st * R::STAGE + R::W_BYTES, (first + i) * SLAB, m0);
+        const int st = i % R::STAGES, n = min(R::SLABS, count - i * R::SLABS);
+        for (int j = 0; j < n; ++j)
+          tma_load_2d(&tx, &s->full[st], ring + st * R::STAGE + R::SLABS * R::W_BYTES + j * R::X_BYTES,
+                      (first + i * R::SLABS + j) * SLAB, m0);
       };
       for (int i = 0; i < ahead; ++i) load_w(i);
       grid_wait();
@@ -377,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       for (int i = 0; i < ahead; ++i) load_x(i);
       bool ok = true;
       int issued = ahead;
-      for (; issued < count; ++issued) {
+      for (; issued < steps; ++issued) {
         ok = mbar_wait(&s->empty[issued % R::STAGES], static_cast<uint32_t>((issued / R::STAGES) & 1) ^ 1u, abort);
         if (!ok) break;
         load_w(issued);
@@ -395,15 +406,18 @@ __global__ void __launch_bounds__(THREADS, 2)
     grid_trigger();
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_i8(BN, T);
-      for (int i = 0; i < count; ++i) {
-        const int st = i % R::STAGES;
+      for (int i = 0; i < steps; ++i) {
+        const int st = i % R::STAGES, n = min(R::SLABS, count - i * R::SLABS);
         if (!mbar_wait(&s->full[st], static_cast<uint32_t>((i / R::STAGES) & 1), abort)) break;
         tc_fence_after();
-        const uint32_t w_addr = smem_addr(ring + st * R::STAGE), x_addr = w_addr + R::W_BYTES;
+        for (int j = 0; j < n; ++j) {
+          const uint32_t w_addr = smem_addr(ring + st * R::STAGE + j * R::W_BYTES);
+          const uint32_t x_addr = smem_addr(ring + st * R::STAGE + R::SLABS * R::W_BYTES + j * R::X_BYTES);
 #pragma unroll
-        for (int k = 0; k < SLAB / 32; ++k)
-          umma_i8(tmem, umma_desc(w_addr + k * 32, 16, 1024, kLayoutSw128), umma_desc(x_addr + k * 32, 16, 1024, kLayoutSw128),
-                  idesc, (i | k) != 0 ? 1u : 0u);
+          for (int k = 0; k < SLAB / 32; ++k)
+            umma_i8(tmem, umma_desc(w_addr + k * 32, 16, 1024, kLayoutSw128), umma_desc(x_addr + k * 32, 16, 1024, kLayoutSw128),
+                    idesc, (i | j | k) != 0 ? 1u : 0u);
+        }
         umma_commit(&s->empty[st]);
       }
       umma_commit(&s->done);  // also after a wait that gave up: all that was issued ends before TMEM is freed
@@ -418,28 +432,36 @@ __global__ void __launch_bounds__(THREADS, 2)
     grid_trigger();
   }
   bool ok = true;
+  float my_scale = 0.f, my_bias = 0.f;
   if (warp >= 2) {
+    if (n0 + (warp & 3) * 32 + lane < p.N) {
+      my_scale = p.w_scale[n0 + (warp & 3) * 32 + lane];
+      if (p.bias) my_bias = p.bias[n0 + (warp & 3) * 32 + lane];
+    }
     ok = __all_sync(0xffffffffu, mbar_wait(&s->done, 0, abort));
     ok = ok && *abort == 0;
     tc_fence_after();
   }
-  const int quarter = warp & 3;
+  const int quarter = warp & 3, half = warp >= 6;
   const int n = n0 + quarter * 32 + lane;
   const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   const bool real = n < p.N;
+  constexpr int SHARE = T >= 32 ? T / 2 : T;  // a warp's tokens; fewer than 32 are one warp's
+  const int c_first = half * SHARE, c_end = min(T, c_first + SHARE);
   if (p.splits == 1) {
-    if (warp >= 2) store_columns(p, lanes, m0, T, n, ok);
+    if (warp >= 2 && c_first < T) store_columns(p, lanes + c_first, m0 + c_first, SHARE, n, ok);
   } else {
-    // each part's sums go to the CTA that owns the columns, into its ring, which no
-    // copy and no MMA of that CTA uses any more
-    cluster_sync();
+    // each part's sums go to the CTA that owns the columns: as soon as it has begun, or, where
+    // they lie in its ring, when no copy and no MMA of that CTA uses it any more
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (!R::APART) cluster_sync();
     const int own = T / p.splits, log_own = __ffs(own) - 1;  // columns of a CTA: a power of two, 2 at least
     // a lane's sums in neighbouring words: 128 bytes a store (four columns of a lane as one
     // 16-byte store each took a third longer: 64 rows 2560 -> 2560 8.8 -> 11.7 us)
-    int* parts = reinterpret_cast<int*>(ring);  // [part][column][128]
+    int* parts = reinterpret_cast<int*>(ring + (R::APART ? R::RING : 0));  // [part][column][128]
     if (warp >= 2) {
 #pragma unroll 1
-      for (int c = 0; c < T; c += 16) {
+      for (int c = c_first; c < c_end; c += 16) {
         uint32_t r[16];
         tmem_ld16(lanes + c, r);
         tmem_wait_ld();
@@ -460,10 +482,9 @@ __global__ void __launch_bounds__(THREADS, 2)
     if (warp >= 2) {
       bool bad = false;
       for (int i = 0; i < p.splits; ++i) bad = bad || s->bad[i] != 0;
-      const float ws = real ? p.w_scale[n] : 0.f, bias = real && p.bias ? p.bias[n] : 0.f;
       const int* from = parts + quarter * 32 + lane;
 #pragma unroll 1
-      for (int c = 0; c < own; c += 4) {
+      for (int c = 4 * half; c < own; c += 8) {
         const int m = m0 + part * own + c;
         if (m >= p.M) break;
         int sum[4] = {0, 0, 0, 0};
@@ -475,7 +496,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         const int most = real ? min(min(own, 4), p.M - m) : 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (e < most) store_out(p, static_cast<int64_t>(m + e) * p.N + n, bad ? NAN : scaled(sum[e], p.x_scale[m + e], ws, bias));
+          if (e < most) store_out(p, static_cast<int64_t>(m + e) * p.N + n, bad ? NAN : scaled(sum[e], p.x_scale[m + e], my_scale, my_bias));
       }
     }
   }
@@ -485,24 +506,22 @@ __global__ void __launch_bounds__(THREADS, 2)
   if (warp == 1) tmem_dealloc(tmem, R::COLS);
 }
 
-template <int T>
-int launch_rows(const CUtensorMap& tw, const CUtensorMap& tx, Params p, cudaStream_t st) {
-  auto kernel = rows_kernel<T>;
+template <int T, bool DEEP>
+int launch_rows(const CUtensorMap& tw, const CUtensorMap& tx, Params p, int splits, cudaStream_t st) {
+  auto kernel = rows_kernel<T, DEEP>;
   static bool configured[64] = {false};
   int dev = 0;
   IRIS_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !configured[dev]) {
-    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows<T>::SMEM));
+    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Rows<T, DEEP>::SMEM));
     if (dev < 64) configured[dev] = true;
   }
   p.token_tiles = (p.M + T - 1) / T;
-  const int64_t units = static_cast<int64_t>(p.token_tiles) * ((p.N + BN - 1) / BN);
-  const int64_t slabs = (p.K + SLAB - 1) / SLAB;
-  p.splits = 1;
-  while (p.splits < 8 && units * p.splits * 2 <= 2 * num_sms() && 4 * p.splits <= slabs) p.splits *= 2;
-  IRIS_REQUIRE(units * p.splits < (1ll << 31), "gemm_i8: too many rows");
-  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(units * p.splits)), THREADS, Rows<T>::SMEM, st,
-                         static_cast<unsigned>(p.splits), tw, tx, p));
+  p.splits = splits;
+  const int64_t ctas = static_cast<int64_t>(p.token_tiles) * ((p.N + BN - 1) / BN) * splits;
+  IRIS_REQUIRE(ctas < (1ll << 31), "gemm_i8: too many rows");
+  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(ctas)), THREADS, Rows<T, DEEP>::SMEM, st, static_cast<unsigned>(splits), tw,
+                         tx, p));
   return IRIS_OK;
 }
 
@@ -523,7 +542,7 @@ struct Smem {
   uint64_t full[STAGES];  // used in the leader only: both CTAs' copies complete here
   uint64_t empty[STAGES];
   uint64_t tmem_full[2];
-  uint64_t tmem_empty[2];  // used in the leader only: 4 local + 4 peer epilogue warps
+  uint64_t tmem_empty[2];  // used in the leader only: both CTAs' epilogue warps
   uint64_t teardown;
   uint32_t tmem_base;
   int abort;
@@ -570,7 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s->tmem_full[i], 1);
-      mbar_init(&s->tmem_empty[i], 8);
+      mbar_init(&s->tmem_empty[i], 2 * EPILOGUE);
     }
     mbar_init(&s->teardown, 1);
     s->abort = 0;
@@ -668,7 +687,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
-    const int quarter = warp & 3;
+    const int quarter = warp & 3, first = warp >= 6 ? tokens / 2 : 0;
     const uint32_t empty_leader = map_to_cta(&s->tmem_empty[0], 0);
     int it = 0;
     bool ok = true;  // a wait gave up: NaN rather than wrong values
@@ -678,7 +697,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       ok = ok && __all_sync(0xffffffffu, mbar_wait_cluster(&s->tmem_full[acc], static_cast<uint32_t>((it >> 1) & 1), abort));
       tc_fence_after();
       const int n = tl.nb * 256 + rank * 128 + quarter * 32 + lane;
-      store_columns(p, tmem + static_cast<uint32_t>(acc * 256) + (static_cast<uint32_t>(quarter * 32) << 16), tl.mb * tokens, tokens, n, ok);
+      store_columns(p, tmem + static_cast<uint32_t>(acc * 256 + first) + (static_cast<uint32_t>(quarter * 32) << 16), tl.mb * tokens + first,
+                    tokens / 2, n, ok);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(empty_leader + static_cast<uint32_t>(acc) * 8u);
@@ -736,6 +756,48 @@ int launch_pair(const void* w, int64_t ldw, const void* x, int64_t ldx, const Pa
   IRIS_CUDA(launch_early(pair_kernel, dim3(static_cast<unsigned>(2 * std::min<int64_t>(tiles, pairs))), THREADS, pair::SMEM, st, 2, tw, tx,
                          p, tokens));
   return IRIS_OK;
+}
+
+// ------------------------------------------------------------------- which form
+// By an estimate of its time in us. A rows_kernel CTA of T tokens takes START and, for each
+// of its slabs, what its ring of stages gives (SLAB_US alone on its SM; two on one 1.45 times that,
+// 0.85 of it for a deep ring), the weights' bytes HBM_RATE or L2_RATE at most; parts of K cost their exchange. A pair's
+// tile takes its tokens' products. Measured, us, (tokens, K -> N): 64, 2560 -> 2560: T 32
+// in 4 parts 6.6, 64 in 4 parts 6.7, 64 whole 8.7, pair 9.2; 16, 8192 -> 8192: 4 parts 10.2, deep
+// 2 parts 11.6, whole 19.7; 256, 8192 -> 8192: T 128 deep 20.6, 64 23.8, 128 24.4, pair
+// 25.6; 1024, 2560 -> 2560: T 128 13.3, pair 13.7; 301, 2560 -> 15360: pair 18.1, T 128 21.7.
+struct Choice {
+  int tokens, splits;  // 0 tokens: CTA pairs
+  bool deep;
+};
+
+Choice choose(int64_t M, int64_t N, int64_t K) {
+  constexpr float START = 2.6f, START_TOKEN = 0.0115f, SLAB_US = 0.24f, SLAB_TOKEN = 0.0006f, HBM_RATE = 6.3e6f, L2_RATE = 9.0e6f;
+  constexpr int64_t IN_L2 = 96 << 20;  // weights that L2 may hold from the last step
+  constexpr float EXCHANGE = 0.3f, EXCHANGE_TOKEN = 0.024f;
+  constexpr float PAIR_START = 6.3f, PAIR_TILE = 1.2f, PAIR_SLAB = 0.08f, PAIR_TOKEN = 0.0009f;
+  const int64_t sms = num_sms(), slabs = (K + SLAB - 1) / SLAB, wide = (N + BN - 1) / BN;
+  const int64_t per = pair_tokens(M), tiles = (M + per - 1) / per * ((N + 255) / 256), waves = (tiles + sms / 2 - 1) / (sms / 2);
+  Choice best = {0, 1, false};
+  if (waves > 4) return best;
+  const float hbm = N * K / (N * K > IN_L2 ? HBM_RATE : L2_RATE);
+  float least = PAIR_START + std::max(hbm, waves * (PAIR_TILE + slabs * (PAIR_SLAB + PAIR_TOKEN * per)));
+  for (int T = 16; T <= 128 && T < 2 * M + 16; T *= 2) {
+    const int64_t units = (M + T - 1) / T * wide;
+    if (units > 4 * sms) continue;
+    const float start = START + START_TOKEN * T, slab = SLAB_US + SLAB_TOKEN * T;
+    for (int splits = 1; splits <= 8 && splits <= slabs; splits *= 2) {
+      const int64_t ctas = units * splits, mine = (slabs + splits - 1) / splits;
+      const float exchange = splits > 1 ? EXCHANGE + EXCHANGE_TOKEN * T : 0.f;
+      for (int deep = 0; deep < 2; ++deep) {
+        const int64_t slots = deep ? sms : 2 * sms, turns = (ctas + slots - 1) / slots;
+        const float each = mine * slab * (deep ? 0.85f : ctas > sms ? 1.45f : 1.f);
+        const float t = start + exchange + std::max(hbm, turns * each + (turns - 1) * (start + exchange - 1.f));
+        if (t < least) least = t, best = Choice{T, splits, deep != 0};
+      }
+    }
+  }
+  return best;
 }
 
 inline int check_rows(int64_t M, int64_t K, int64_t ldx) {
@@ -823,16 +885,19 @@ extern "C" int iris_gemm_i8(const iris_i8_problem* q, void* stream) {
   p.M = static_cast<int>(q->M), p.N = static_cast<int>(q->N), p.K = static_cast<int>(q->K);
   p.out_dtype = static_cast<int>(q->out_dtype);
   p.early = fresh;
-  const char* ev = getenv("I8_PAIR");
-  if (ev ? atoi(ev) : p.M > 256) return launch_pair(q->w, q->ldw, x, ldx, p, st);
-  const int tokens = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
+  const Choice c = choose(p.M, p.N, p.K);
+  if (c.tokens == 0) return launch_pair(q->w, q->ldw, x, ldx, p, st);
   CUtensorMap tw, tx;
   IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tw, q->w, q->K, q->N, q->ldw, SLAB, BN));
-  IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tx, x, q->K, q->M, ldx, SLAB, tokens));
-  switch (tokens) {
-    case 16: return launch_rows<16>(tw, tx, p, st);
-    case 32: return launch_rows<32>(tw, tx, p, st);
-    case 64: return launch_rows<64>(tw, tx, p, st);
-    default: return launch_rows<128>(tw, tx, p, st);
+  IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tx, x, q->K, q->M, ldx, SLAB, c.tokens));
+  switch (c.tokens + c.deep) {
+    case 16: return launch_rows<16, false>(tw, tx, p, c.splits, st);
+    case 32: return launch_rows<32, false>(tw, tx, p, c.splits, st);
+    case 64: return launch_rows<64, false>(tw, tx, p, c.splits, st);
+    case 128: return launch_rows<128, false>(tw, tx, p, c.splits, st);
+    case 17: return launch_rows<16, true>(tw, tx, p, c.splits, st);
+    case 33: return launch_rows<32, true>(tw, tx, p, c.splits, st);
+    case 65: return launch_rows<64, true>(tw, tx, p, c.splits, st);
+    default: return launch_rows<128, true>(tw, tx, p, c.splits, st);
   }
 }
