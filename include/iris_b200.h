@@ -491,8 +491,9 @@ int iris_quantize_i8(const iris_quantize_problem* problem, void* stream);
  * int32 (1 <= K <= 131071), out [M, N] contiguous in out_dtype. w int8 [N, K] (iris_quantize_i8
  * of the weights' rows), row stride ldw; 8-bit x (x_dtype IRIS_I8) with x_scale: 16-byte
  * aligned rows, as w's (the stride of a single row is not read). x in IRIS_F32, IRIS_BF16 or
- * IRIS_F16 (x_scale unused) is quantised first, into workspace (iris_gemm_i8_workspace bytes,
- * 16-byte aligned; calls that may run at the same time need one each). bias fp32 or null. */
+ * IRIS_F16 (x_scale unused) is quantised first, a few rows by the product itself, more into
+ * workspace (iris_gemm_i8_workspace bytes for the problem, x and ldx among it; 16-byte
+ * aligned; calls that may run at the same time need one each). bias fp32 or null. */
 typedef struct iris_i8_problem {
   const void* x;
   const float* x_scale;

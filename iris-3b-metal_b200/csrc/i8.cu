@@ -107,7 +107,7 @@ __device__ __noinline__ uint2 round_exactly(uint4 v, float hi, float top, float 
 }
 
 template <typename T>
-IRIS_DEVICE void store_vec(int8_t* out, const uint4& v, int at, int K, const Factors& f) {
+IRIS_DEVICE uint2 round_vec(const uint4& v, const Factors& f) {
   constexpr int N = Vec<T>::N;
   uint32_t packed[2] = {0u, 0u};
   bool again = f.up != 1.f;
@@ -131,18 +131,38 @@ IRIS_DEVICE void store_vec(int8_t* out, const uint4& v, int at, int K, const Fac
     }
     packed[g] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
   }
-  if (again) {
-    const uint2 w = round_exactly<T>(v, f.hi, f.top, f.up);
-    packed[0] = w.x, packed[1] = w.y;
-  }
+  return again ? round_exactly<T>(v, f.hi, f.top, f.up) : make_uint2(packed[0], packed[1]);
+}
+
+template <typename T>
+IRIS_DEVICE void store_vec(int8_t* out, const uint4& v, int at, int K, const Factors& f) {
+  constexpr int N = Vec<T>::N;
+  const uint2 w = round_vec<T>(v, f);
   if ((at + 1) * N <= K) {
-    if (N == 8) *reinterpret_cast<uint2*>(out + at * N) = make_uint2(packed[0], packed[1]);
-    else *reinterpret_cast<uint32_t*>(out + at * N) = packed[0];
+    if (N == 8) *reinterpret_cast<uint2*>(out + at * N) = w;
+    else *reinterpret_cast<uint32_t*>(out + at * N) = w.x;
   } else {
+    const uint32_t packed[2] = {w.x, w.y};
 #pragma unroll
     for (int e = 0; e < N; ++e)
       if (at * N + e < K) out[at * N + e] = static_cast<int8_t>(packed[e >> 2] >> (8 * (e & 3)) & 0xffu);
   }
+}
+
+// From the bits of a row's largest magnitude. Extreme rows are scaled to where the factors are
+// normal numbers, exactly but for values that round to 0; a row that is not finite gives
+// zeros (its values are to be taken as such).
+template <typename T>
+IRIS_DEVICE Factors factors_of(uint32_t top, float* scale) {
+  const float size = value_of<T>(make_uint4(top, 0u, 0u, 0u), 0);
+  const bool finite = size < INFINITY;  // not so for NaN
+  *scale = finite ? __fdiv_rn(size, 127.f) : NAN;
+  Factors f;
+  f.up = !finite ? 0.f : size < 0x1p-100f ? 0x1p100f : size > 0x1p60f ? 0x1p-100f : 1.f;
+  f.top = finite ? size * f.up : 0.f;
+  f.hi = f.top > 0.f ? __fdiv_rn(127.f, f.top) : 0.f;
+  f.lo = f.top > 0.f ? __fdiv_rn(fmaf(-f.hi, f.top, 127.f), f.top) : 0.f;
+  return f;
 }
 
 constexpr int KEPT = 4;  // vectors of a row that a thread keeps
@@ -186,16 +206,10 @@ __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32, WARPS == 8 ? 4 
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) top = max(top, tops[turn][w]);
     }
-    const float size = value_of<T>(make_uint4(top, 0u, 0u, 0u), 0);
-    const bool finite = size < INFINITY;  // not so for NaN
-    if (t == 0) p.scale[m] = finite ? __fdiv_rn(size, 127.f) : NAN;
-    // extreme rows are scaled to where the factors are normal numbers, exactly but for values
-    // that round to 0; a row that is not finite gives zeros
-    Factors f;
-    f.up = !finite ? 0.f : size < 0x1p-100f ? 0x1p100f : size > 0x1p60f ? 0x1p-100f : 1.f;
-    f.top = finite ? size * f.up : 0.f;
-    f.hi = f.top > 0.f ? __fdiv_rn(127.f, f.top) : 0.f;
-    f.lo = f.top > 0.f ? __fdiv_rn(fmaf(-f.hi, f.top, 127.f), f.top) : 0.f;
+    float scale;
+    const Factors f = factors_of<T>(top, &scale);
+    const bool finite = f.up != 0.f;
+    if (t == 0) p.scale[m] = scale;
     int8_t* out = p.q + m * p.ldq;
     auto store = [&](const uint4& v, int at) { store_vec<T>(out, finite ? v : make_uint4(0u, 0u, 0u, 0u), at, p.K, f); };
 #pragma unroll
@@ -525,6 +539,209 @@ int launch_rows(const CUtensorMap& tw, const CUtensorMap& tx, Params p, int spli
   return IRIS_OK;
 }
 
+// A few tokens in fp32 or 16 bits: rows_kernel for 16 tokens that rounds them itself. Every CTA
+// reads the rows whole for their largest magnitudes and lays its own part of K out in shared
+// memory, as TMA would have; one launch instead of two, which take longer than what they do.
+namespace few {
+constexpr int T = 16, STAGES = 4, MOST_SLABS = 16;  // slabs of a CTA
+constexpr int RING = STAGES * BN * SLAB, X_SLAB = T * SLAB, X = MOST_SLABS * X_SLAB, PARTS = T * BN * 4;
+constexpr int64_t MOST_VALUES = 10240;  // of the rows (4 of 2560: 6.6 us, as in two launches; 8 of 2560 7.7 against 7.0)
+struct Smem {
+  uint64_t full[STAGES], empty[STAGES], x_full, done;
+  uint32_t tmem_base;
+  int abort, bad[8];
+  uint32_t top[T];
+  float scale[T];
+};
+constexpr int SMEM = 1024 + RING + X + PARTS + static_cast<int>(sizeof(Smem));
+}  // namespace few
+
+template <typename V>
+__global__ void __launch_bounds__(THREADS, 2)
+    few_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ Params p, const V* x, int64_t ldx) {
+  using namespace few;
+  constexpr int N = Vec<V>::N;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* rows = ring + RING;
+  int* parts = reinterpret_cast<int*>(rows + X);  // [part][column][128]
+  few::Smem* s = reinterpret_cast<few::Smem*>(rows + X + PARTS);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+  const int part = static_cast<int>(blockIdx.x % p.splits), n0 = static_cast<int>(blockIdx.x / p.splits) * BN;
+  const int slabs = (p.K + SLAB - 1) / SLAB;
+  const int first = slabs * part / p.splits, count = slabs * (part + 1) / p.splits - first;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&s->full[i], 1);
+      mbar_init(&s->empty[i], 1);
+    }
+    mbar_init(&s->x_full, EPILOGUE);
+    mbar_init(&s->done, 1);
+    s->abort = 0;
+    for (int i = 0; i < 8; ++i) s->bad[i] = 0;
+    for (int i = 0; i < T; ++i) s->top[i] = 0u;
+    fence_barrier_init();
+    tma_prefetch_desc(&tw);
+  }
+  if (warp == 1) tmem_alloc(&s->tmem_base, 32);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s->tmem_base;
+  volatile int* abort = &s->abort;
+  if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  grid_wait();
+  grid_trigger();
+
+  bool ok = true;
+  float my_scale = 0.f, my_bias = 0.f;
+  const int quarter = warp & 3, half = warp >= 6;
+  const int n = n0 + quarter * 32 + lane;
+  if (warp == 0) {
+    // ----------------------------------------------------------------- TMA
+    if (lane == 0) {
+      int issued = 0;
+      for (; issued < count; ++issued) {
+        const int st = issued % STAGES;
+        ok = mbar_wait(&s->empty[st], static_cast<uint32_t>((issued / STAGES) & 1) ^ 1u, abort);
+        if (!ok) break;
+        mbar_arrive_expect_tx(&s->full[st], BN * SLAB);
+        tma_load_2d(&tw, &s->full[st], ring + st * BN * SLAB, (first + issued) * SLAB, n0);
+      }
+      if (!ok) {  // no copy may land after the CTA is gone
+        int dummy = 0;
+        for (int i = max(0, issued - STAGES); i < issued; ++i)
+          mbar_wait(&s->full[i % STAGES], static_cast<uint32_t>((i / STAGES) & 1), &dummy);
+      }
+    }
+  } else if (warp == 1) {
+    // ----------------------------------------------------------------- MMA
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_i8(BN, T);
+      ok = mbar_wait(&s->x_full, 0, abort);
+      for (int i = 0; i < count && ok; ++i) {
+        const int st = i % STAGES;
+        ok = mbar_wait(&s->full[st], static_cast<uint32_t>((i / STAGES) & 1), abort);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t w_addr = smem_addr(ring + st * BN * SLAB), x_addr = smem_addr(rows + i * X_SLAB);
+#pragma unroll
+        for (int k = 0; k < SLAB / 32; ++k)
+          umma_i8(tmem, umma_desc(w_addr + k * 32, 16, 1024, kLayoutSw128), umma_desc(x_addr + k * 32, 16, 1024, kLayoutSw128),
+                  idesc, (i | k) != 0 ? 1u : 0u);
+        umma_commit(&s->empty[st]);
+      }
+      umma_commit(&s->done);  // also after a wait that gave up: all that was issued ends before TMEM is freed
+      int dummy = 0;
+      mbar_wait(&s->done, 0, &dummy);
+    }
+  } else {
+    // ------------------------------------------------------------- the rows
+    if (n < p.N) {
+      my_scale = p.w_scale[n];
+      if (p.bias) my_bias = p.bias[n];
+    }
+    const int w = warp - 2, share = p.M == 1 ? 8 : p.M == 2 ? 4 : p.M <= 4 ? 2 : 1;  // warps of a row
+    const int vecs = (p.K + N - 1) / N;
+    for (int m = w / share; m < p.M; m += EPILOGUE / share) {
+      uint32_t top = 0u;
+#pragma unroll 2
+      for (int v = w % share * 32 + lane; v < vecs; v += share * 32) top = top_of<V>(load_vec<V, true>(x + m * ldx, v, p.K), top);
+      if (sizeof(V) == 2) top = max(top & 0xffffu, top >> 16);
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) atomicMax(&s->top[m], top);
+    }
+    // rows that are not there are zeros
+    for (int i = threadIdx.x - 64; i < count * (T - p.M) * (SLAB / 16); i += 32 * EPILOGUE) {
+      const int piece = i % (SLAB / 16), row = p.M + i / (SLAB / 16) % (T - p.M), slab = i / (SLAB / 16) / (T - p.M);
+      *reinterpret_cast<uint4*>(rows + slab * X_SLAB + row * SLAB + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * EPILOGUE) : "memory");
+    // this part's values, in the swizzled places of each slab: 16-byte piece c of row r at c ^ (r & 7)
+    constexpr int OF_SLAB = SLAB / N;
+    for (int m = w / share; m < p.M; m += EPILOGUE / share) {
+      float scale;
+      const Factors f = factors_of<V>(s->top[m], &scale);
+      if (lane == 0) s->scale[m] = scale;
+#pragma unroll 1
+      for (int i = w % share * 32 + lane; i < count * OF_SLAB; i += share * 32) {
+        const int v = first * OF_SLAB + i;
+        const uint4 value = v < vecs && f.up != 0.f ? load_vec<V, true>(x + m * ldx, v, p.K) : make_uint4(0u, 0u, 0u, 0u);
+        const uint2 q = round_vec<V>(value, f);
+        const int byte = i % OF_SLAB * N;
+        uint8_t* to = rows + i / OF_SLAB * X_SLAB + m * SLAB + (((byte >> 4) ^ (m & 7)) * 16) + (byte & 15);
+        if (N == 8) *reinterpret_cast<uint2*>(to) = q;
+        else *reinterpret_cast<uint32_t*>(to) = q.x;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s->x_full);
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * EPILOGUE) : "memory");  // every row's scale is there
+    ok = __all_sync(0xffffffffu, mbar_wait(&s->done, 0, abort));
+    ok = ok && *abort == 0;
+    tc_fence_after();
+  }
+  __syncwarp();
+  // ------------------------------------------------------------- epilogue
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const int own = T / p.splits, log_own = __ffs(own) - 1;  // columns of a CTA: a power of two, 2 at least
+  if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (warp >= 2 && !half) {
+    uint32_t r[16];
+    tmem_ld16(lanes, r);
+    tmem_wait_ld();
+#pragma unroll
+    for (int col = 0; col < 16; ++col) {
+      const uint32_t to = map_to_cta(parts + (part * own + (col & (own - 1))) * BN + quarter * 32 + lane,
+                                     static_cast<uint32_t>(col >> log_own));
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(r[col]) : "memory");
+    }
+  }
+  if (warp >= 2 && !ok && lane < p.splits) {
+    const uint32_t to = map_to_cta(&s->bad[part], static_cast<uint32_t>(lane));
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(1) : "memory");
+  }
+  if (p.splits > 1) cluster_sync();
+  else __syncthreads();
+  if (warp >= 2) {
+    bool bad = false;
+    for (int i = 0; i < p.splits; ++i) bad = bad || s->bad[i] != 0;
+#pragma unroll 1
+    for (int c = half; c < own; c += 2) {
+      const int m = part * own + c;
+      if (m >= p.M) break;
+      int sum = 0;
+#pragma unroll 2
+      for (int i = 0; i < p.splits; ++i) sum += parts[(i * own + c) * BN + quarter * 32 + lane];
+      if (n < p.N) store_out(p, static_cast<int64_t>(m) * p.N + n, bad ? NAN : scaled(sum, s->scale[m], my_scale, my_bias));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 32);
+}
+
+template <typename V>
+int launch_few(const CUtensorMap& tw, Params p, int splits, const void* x, int64_t ldx, cudaStream_t st) {
+  auto kernel = few_kernel<V>;
+  static bool configured[64] = {false};
+  int dev = 0;
+  IRIS_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !configured[dev]) {
+    IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, few::SMEM));
+    if (dev < 64) configured[dev] = true;
+  }
+  p.splits = splits;
+  const int64_t ctas = static_cast<int64_t>((p.N + BN - 1) / BN) * splits;
+  IRIS_REQUIRE(ctas < (1ll << 31), "gemm_i8: too many rows");
+  IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(ctas)), THREADS, few::SMEM, st, static_cast<unsigned>(splits), tw, p,
+                         static_cast<const V*>(x), ldx));
+  return IRIS_OK;
+}
+
 // ---------------------------------------------------------------- many tokens
 // CTA pairs (cta_group::2), persistent: a cluster of two CTAs on paired SMs computes 256
 // weight rows by up to 256 tokens. Each CTA brings its own 128 weight rows and half of the
@@ -800,6 +1017,13 @@ Choice choose(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 
+// Whether few_kernel takes a call's rows.
+inline bool rounds_itself(const iris_i8_problem& q, const Choice& c) {
+  const int64_t slabs = (q.K + SLAB - 1) / SLAB, size = q.x_dtype == IRIS_F32 ? 4 : 2;
+  return q.x_dtype != IRIS_I8 && c.tokens == few::T && q.M <= few::T && q.M * q.K <= few::MOST_VALUES &&
+         (slabs + c.splits - 1) / c.splits <= few::MOST_SLABS && aligned16(q.x) && (q.M <= 1 || q.ldx * size % 16 == 0);
+}
+
 inline int check_rows(int64_t M, int64_t K, int64_t ldx) {
   IRIS_REQUIRE(M >= 0 && M < (1ll << 31) - 256 && K >= 1 && K <= 131071, "quantize_i8: M rows of 1 to 131071 values");
   IRIS_REQUIRE(ldx >= 0, "quantize_i8: the row stride must not be negative");
@@ -847,7 +1071,7 @@ extern "C" int iris_gemm_i8_workspace(const iris_i8_problem* q, int64_t* bytes) 
   using namespace iris::i8;
   IRIS_REQUIRE(q != nullptr && bytes != nullptr, "gemm_i8_workspace: null pointer");
   IRIS_CHECK_STATUS(check_product(*q));
-  *bytes = workspace_bytes(*q);
+  *bytes = q->M * q->N == 0 || rounds_itself(*q, choose(q->M, q->N, q->K)) ? 0 : workspace_bytes(*q);
   return IRIS_OK;
 }
 
@@ -867,8 +1091,19 @@ extern "C" int iris_gemm_i8(const iris_i8_problem* q, void* stream) {
   int64_t ldx = q->ldx;
   Params p = {};
   p.x_scale = q->x_scale;
+  p.w_scale = q->w_scale, p.bias = q->bias, p.out = q->out;
+  p.M = static_cast<int>(q->M), p.N = static_cast<int>(q->N), p.K = static_cast<int>(q->K);
+  p.out_dtype = static_cast<int>(q->out_dtype);
+  const Choice c = choose(p.M, p.N, p.K);
+  CUtensorMap tw, tx;
   if (fresh) {
     IRIS_CHECK_STATUS(check_rows(q->M, q->K, q->ldx));
+    if (rounds_itself(*q, c)) {
+      IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tw, q->w, q->K, q->N, q->ldw, SLAB, BN));
+      return q->x_dtype == IRIS_F32    ? launch_few<float>(tw, p, c.splits, x, ldx, st)
+             : q->x_dtype == IRIS_BF16 ? launch_few<__nv_bfloat16>(tw, p, c.splits, x, ldx, st)
+                                       : launch_few<__half>(tw, p, c.splits, x, ldx, st);
+    }
     IRIS_REQUIRE(q->workspace && aligned16(q->workspace) && q->workspace_bytes >= workspace_bytes(*q), "gemm_i8: workspace too small");
     ldx = row_bytes(q->K);
     float* scale = reinterpret_cast<float*>(static_cast<uint8_t*>(q->workspace) + q->M * ldx);
@@ -881,13 +1116,8 @@ extern "C" int iris_gemm_i8(const iris_i8_problem* q, void* stream) {
     if (q->M == 1) ldx = row_bytes(q->K);  // a lone row's stride says nothing
     IRIS_REQUIRE(aligned16(x) && ldx % 16 == 0 && ldx >= q->K, "gemm_i8: 8-bit rows of x at multiples of 16 bytes");
   }
-  p.w_scale = q->w_scale, p.bias = q->bias, p.out = q->out;
-  p.M = static_cast<int>(q->M), p.N = static_cast<int>(q->N), p.K = static_cast<int>(q->K);
-  p.out_dtype = static_cast<int>(q->out_dtype);
   p.early = fresh;
-  const Choice c = choose(p.M, p.N, p.K);
   if (c.tokens == 0) return launch_pair(q->w, q->ldw, x, ldx, p, st);
-  CUtensorMap tw, tx;
   IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tw, q->w, q->K, q->N, q->ldw, SLAB, BN));
   IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tx, x, q->K, q->M, ldx, SLAB, c.tokens));
   switch (c.tokens + c.deep) {

@@ -484,7 +484,7 @@ PyObject* gemm_i8(PyObject* const* a) {
     workspace = at::empty({q.workspace_bytes}, x.options().dtype(at::kByte));
     q.workspace = workspace.data_ptr();
   }
-  on.check("iris_gemm_i8", entries.gemm_i8(&q, on.stream()), q.M * q.N == 0 ? 0 : eight ? 1 : 2);
+  on.check("iris_gemm_i8", entries.gemm_i8(&q, on.stream()), q.M * q.N == 0 ? 0 : q.workspace ? 2 : 1);
   return THPVariable_Wrap(std::move(out));
 }
 

@@ -121,6 +121,24 @@ def test_product_wide(K, m):
         check(K, m, n, k, torch.bfloat16, bias=False, seed=m)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 8, 9, 15, 16])
+def test_a_few_rows_that_the_product_rounds(K, m, dtype):
+    """Against the same rows quantised before: bit for bit, in each number of parts of K, extreme rows among them."""
+    for k in (1, 7, 8, 127, 128, 129, 520, 1000, 1280, 2560, 10240 // m):
+        x = rows(k, m, k, dtype)
+        if m > 4:
+            x[0], x[1] = 0, x[1] * torch.finfo(dtype).smallest_normal * 2.0**9
+            x[2, k // 2], x[3, 0], x[4, -1] = math.inf, math.nan, torch.finfo(dtype).max
+        for n in (1, 130, 2561):
+            packed, scale = K.quantize_i8(rows(n, n, k, torch.float32, False))
+            q, x_scale = K.quantize_i8(x)
+            want = K.gemm_i8(q, packed, scale, x_scale=x_scale, out_dtype=dtype)
+            for view in (x, torch.cat([x, x], dim=1)[:, :k] if k % 8 == 0 else x):
+                got = K.gemm_i8(view, packed, scale)
+                assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(got.isnan(), want.isnan())
+
+
 def test_longest_sums(K):
     """K = 131071 of the type's lowest value: the sum is 2^31 - 16384."""
     for m, n in ((1, 3), (18, 130), (300, 300)):
@@ -233,7 +251,8 @@ def test_kernels_are_counted(K):
 
     packed, scale = K.quantize_i8(rows(50, 40, 64, torch.float32))
     x = rows(51, 3, 64)
-    for call, count in [(lambda: K.quantize_i8(x), 1), (lambda: K.gemm_i8(x, packed, scale), 2),
+    for call, count in [(lambda: K.quantize_i8(x), 1), (lambda: K.gemm_i8(x, packed, scale), 1),
+                        (lambda: K.gemm_i8(rows(52, 30, 64), packed, scale), 2),
                         (lambda: K.gemm_i8(packed[:2], packed, scale, x_scale=scale[:2]), 1),
                         (lambda: K.gemm_i8(x[:0], packed, scale), 0)]:  # fmt: skip
         before = _lib.launch_count()
