@@ -372,6 +372,19 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2)
     tma_prefetch_desc(&tw);
     tma_prefetch_desc(&tx);
   }
+  auto load_w = [&](int i) {
+    const int st = i % R::STAGES, n = min(R::SLABS, count - i * R::SLABS);
+    mbar_arrive_expect_tx(&s->full[st], n * (R::W_BYTES + R::X_BYTES));
+    for (int j = 0; j < n; ++j)
+      tma_load_2d(&tw, &s->full[st], ring + st * R::STAGE + j * R::W_BYTES, (first + i * R::SLABS + j) * SLAB, n0);
+  };
+  const int ahead = p.early ? min(steps, R::STAGES) : 0;
+  if (threadIdx.x == 0)
+    for (int i = 0; i < ahead; ++i) load_w(i);
+  // TMEM only after the wait: a CTA that held some while it waits could keep its predecessor's,
+  // which still have to allocate theirs, from ever ending
+  grid_wait();
+  grid_trigger();
   if (warp == 1) tmem_alloc(&s->tmem_base, R::COLS);
   tc_fence_before();
   __syncthreads();
@@ -383,22 +396,12 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2)
   if (warp == 0) {
     // ----------------------------------------------------------------- TMA
     if (lane == 0) {
-      const int ahead = p.early ? min(steps, R::STAGES) : 0;
-      auto load_w = [&](int i) {
-        const int st = i % R::STAGES, n = min(R::SLABS, count - i * R::SLABS);
-        mbar_arrive_expect_tx(&s->full[st], n * (R::W_BYTES + R::X_BYTES));
-        for (int j = 0; j < n; ++j)
-          tma_load_2d(&tw, &s->full[st], ring + st * R::STAGE + j * R::W_BYTES, (first + i * R::SLABS + j) * SLAB, n0);
-      };
       auto load_x = [&](int i) {
         const int st = i % R::STAGES, n = min(R::SLABS, count - i * R::SLABS);
         for (int j = 0; j < n; ++j)
           tma_load_2d(&tx, &s->full[st], ring + st * R::STAGE + R::SLABS * R::W_BYTES + j * R::X_BYTES,
                       (first + i * R::SLABS + j) * SLAB, m0);
       };
-      for (int i = 0; i < ahead; ++i) load_w(i);
-      grid_wait();
-      grid_trigger();
       for (int i = 0; i < ahead; ++i) load_x(i);
       bool ok = true;
       int issued = ahead;
@@ -416,8 +419,6 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2)
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMA
-    grid_wait();
-    grid_trigger();
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_i8(BN, T);
       for (int i = 0; i < steps; ++i) {
@@ -441,10 +442,6 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2)
   }
   __syncwarp();
   // ------------------------------------------------------------- epilogue
-  if (warp >= 2) {
-    grid_wait();
-    grid_trigger();
-  }
   bool ok = true;
   float my_scale = 0.f, my_bias = 0.f;
   if (warp >= 2) {
@@ -584,15 +581,15 @@ __global__ void __launch_bounds__(THREADS, 2)
     fence_barrier_init();
     tma_prefetch_desc(&tw);
   }
-  if (warp == 1) tmem_alloc(&s->tmem_base, 32);
+  grid_wait();
+  grid_trigger();
+  if (warp == 1) tmem_alloc(&s->tmem_base, 32);  // after the wait, as in rows_kernel
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s->tmem_base;
   volatile int* abort = &s->abort;
   if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  grid_wait();
-  grid_trigger();
 
   bool ok = true;
   float my_scale = 0.f, my_bias = 0.f;
@@ -814,14 +811,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     tma_prefetch_desc(&tw);
     tma_prefetch_desc(&tx);
   }
-  if (warp == 1) tmem_alloc_pair(&s->tmem_base, 512);
+  grid_wait();
+  grid_trigger();
+  if (warp == 1) tmem_alloc_pair(&s->tmem_base, 512);  // after the wait, as in rows_kernel
   tc_fence_before();
   cluster_sync();  // every barrier of both CTAs exists before any remote arrival
   tc_fence_after();
   const uint32_t tmem = s->tmem_base;
   volatile int* abort = &s->abort;
-  grid_wait();
-  grid_trigger();
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (both CTAs)

@@ -246,15 +246,11 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
     s->abort = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(&s->tmem_base, TILE_COLS);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = s->tmem_base;
-  volatile int* abort = &s->abort;
-
+  // TMEM only after the wait: a CTA that held some while it waits could keep its predecessor's,
+  // which still have to allocate theirs, from ever ending
   grid_wait();
   grid_trigger();
+  if (warp == 1) tmem_alloc(&s->tmem_base, TILE_COLS);
   const bool finish = cta < plan.whole_tiles;
   const int split = finish ? 0 : (cta - plan.whole_tiles) % plan.tile_splits;
   const int unit_tile = finish ? cta : plan.whole_tiles + (cta - plan.whole_tiles) / plan.tile_splits;
@@ -270,6 +266,12 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
   const int all_blocks = early_blocks + (own ? (own_keys(p, start + last / group, length) + BKV - 1) / BKV : 0);
   const int first = finish ? 0 : min(split * plan.tile_chunk, all_blocks);
   const int iters = finish ? all_blocks : min(plan.tile_chunk, all_blocks - first);
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s->tmem_base;
+  volatile int* abort = &s->abort;
 
   if (warp == 0) {
     // ----------------------------------------------------------------- TMA
