@@ -381,17 +381,11 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2)
   const int ahead = p.early ? min(steps, R::STAGES) : 0;
   if (threadIdx.x == 0)
     for (int i = 0; i < ahead; ++i) load_w(i);
-  // TMEM only after the wait: a CTA that held some while it waits could keep its predecessor's,
-  // which still have to allocate theirs, from ever ending
+  __syncthreads();
+  if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  volatile int* abort = &s->abort;
   grid_wait();
   grid_trigger();
-  if (warp == 1) tmem_alloc(&s->tmem_base, R::COLS);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = s->tmem_base;
-  volatile int* abort = &s->abort;
-  if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
   if (warp == 0) {
     // ----------------------------------------------------------------- TMA
@@ -419,6 +413,13 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2)
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMA
+    // TMEM only after the wait: a CTA that held some while it waits could keep its predecessor's,
+    // which still have to allocate theirs, from ever ending
+    tmem_alloc(&s->tmem_base, R::COLS);
+    tc_fence_before();
+    __syncwarp();
+    barrier_tell<1, 32 + 32 * EPILOGUE>();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s->tmem_base);
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_i8(BN, T);
       for (int i = 0; i < steps; ++i) {
@@ -444,11 +445,14 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2)
   // ------------------------------------------------------------- epilogue
   bool ok = true;
   float my_scale = 0.f, my_bias = 0.f;
+  uint32_t tmem = 0;
   if (warp >= 2) {
     if (n0 + (warp & 3) * 32 + lane < p.N) {
       my_scale = p.w_scale[n0 + (warp & 3) * 32 + lane];
       if (p.bias) my_bias = p.bias[n0 + (warp & 3) * 32 + lane];
     }
+    barrier_wait<1, 32 + 32 * EPILOGUE>();
+    tmem = s->tmem_base;
     ok = __all_sync(0xffffffffu, mbar_wait(&s->done, 0, abort));
     ok = ok && *abort == 0;
     tc_fence_after();
@@ -514,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, R::COLS);
+  if (warp == 1) tmem_dealloc(s->tmem_base, R::COLS);
 }
 
 template <int T, bool DEEP>
@@ -581,18 +585,15 @@ __global__ void __launch_bounds__(THREADS, 2)
     fence_barrier_init();
     tma_prefetch_desc(&tw);
   }
-  grid_wait();
-  grid_trigger();
-  if (warp == 1) tmem_alloc(&s->tmem_base, 32);  // after the wait, as in rows_kernel
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = s->tmem_base;
   volatile int* abort = &s->abort;
   if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  grid_wait();
+  grid_trigger();
 
   bool ok = true;
   float my_scale = 0.f, my_bias = 0.f;
+  uint32_t tmem = 0;
   const int quarter = warp & 3, half = warp >= 6;
   const int n = n0 + quarter * 32 + lane;
   if (warp == 0) {
@@ -614,6 +615,11 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMA
+    tmem_alloc(&s->tmem_base, 32);  // after the wait, as in rows_kernel
+    tc_fence_before();
+    __syncwarp();
+    barrier_tell<2, 32 + 32 * EPILOGUE>();
+    tmem = *reinterpret_cast<volatile uint32_t*>(&s->tmem_base);
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_i8(BN, T);
       ok = mbar_wait(&s->x_full, 0, abort);
@@ -654,7 +660,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       const int piece = i % (SLAB / 16), row = p.M + i / (SLAB / 16) % (T - p.M), slab = i / (SLAB / 16) / (T - p.M);
       *reinterpret_cast<uint4*>(rows + slab * X_SLAB + row * SLAB + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * EPILOGUE) : "memory");
+    barrier_wait<1, 32 * EPILOGUE>();
     // this part's values, in the swizzled places of each slab: 16-byte piece c of row r at c ^ (r & 7)
     constexpr int OF_SLAB = SLAB / N;
     for (int m = w / share; m < p.M; m += EPILOGUE / share) {
@@ -675,7 +681,8 @@ __global__ void __launch_bounds__(THREADS, 2)
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&s->x_full);
-    asm volatile("bar.sync 1, %0;" ::"n"(32 * EPILOGUE) : "memory");  // every row's scale is there
+    barrier_wait<2, 32 + 32 * EPILOGUE>();  // every row's scale is there, and TMEM
+    tmem = s->tmem_base;
     ok = __all_sync(0xffffffffu, mbar_wait(&s->done, 0, abort));
     ok = ok && *abort == 0;
     tc_fence_after();
@@ -718,7 +725,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, 32);
+  if (warp == 1) tmem_dealloc(s->tmem_base, 32);
 }
 
 template <typename V>
@@ -811,14 +818,18 @@ __global__ void __launch_bounds__(THREADS, 1)
     tma_prefetch_desc(&tw);
     tma_prefetch_desc(&tx);
   }
+  cluster_sync();  // every barrier of both CTAs exists before any remote arrival
+  volatile int* abort = &s->abort;
   grid_wait();
   grid_trigger();
   if (warp == 1) tmem_alloc_pair(&s->tmem_base, 512);  // after the wait, as in rows_kernel
+  // both CTAs' TMEM before any product; the producers go on meanwhile
   tc_fence_before();
-  cluster_sync();  // every barrier of both CTAs exists before any remote arrival
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if (warp != 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   tc_fence_after();
-  const uint32_t tmem = s->tmem_base;
-  volatile int* abort = &s->abort;
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s->tmem_base);
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (both CTAs)
@@ -856,6 +867,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
     }
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader)
     if (lane == 0 && leader) {

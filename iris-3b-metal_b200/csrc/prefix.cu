@@ -246,11 +246,10 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
     s->abort = 0;
     fence_barrier_init();
   }
-  // TMEM only after the wait: a CTA that held some while it waits could keep its predecessor's,
-  // which still have to allocate theirs, from ever ending
+  __syncthreads();
+  volatile int* abort = &s->abort;
   grid_wait();
   grid_trigger();
-  if (warp == 1) tmem_alloc(&s->tmem_base, TILE_COLS);
   const bool finish = cta < plan.whole_tiles;
   const int split = finish ? 0 : (cta - plan.whole_tiles) % plan.tile_splits;
   const int unit_tile = finish ? cta : plan.whole_tiles + (cta - plan.whole_tiles) / plan.tile_splits;
@@ -266,12 +265,6 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
   const int all_blocks = early_blocks + (own ? (own_keys(p, start + last / group, length) + BKV - 1) / BKV : 0);
   const int first = finish ? 0 : min(split * plan.tile_chunk, all_blocks);
   const int iters = finish ? all_blocks : min(plan.tile_chunk, all_blocks - first);
-
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = s->tmem_base;
-  volatile int* abort = &s->abort;
 
   if (warp == 0) {
     // ----------------------------------------------------------------- TMA
@@ -344,6 +337,13 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMA
+    // TMEM only after the wait: a CTA that held some while it waits could keep its predecessor's,
+    // which still have to allocate theirs, from ever ending
+    tmem_alloc(&s->tmem_base, TILE_COLS);
+    tc_fence_before();
+    __syncwarp();
+    barrier_tell<1, 32 + BQ>();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s->tmem_base);
     if (lane == 0 && iters > 0) {
       constexpr uint32_t f16 = (1u << 7) | (1u << 10);  // the BF16 bits of idesc_bf16_f32; F16 is 0
       constexpr uint32_t clear = IsHalf<T>::value ? f16 : 0u;
@@ -388,7 +388,6 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane, r = row0 + row;  // of the tile, of the unit
     const Row at = row_of(p, plan.per, u, hk, min(r, rows - 1));
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     auto place = [&](int row, int piece) { return row * 128 + ((piece ^ (row & 7)) * 16); };
     // Q: the warp's 32 rows, each by D / 8 lanes; rows from the unit's end on are zeros
     if (iters > 0) {
@@ -407,6 +406,9 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
       __syncwarp();
       if (lane == 0) mbar_arrive(&s->q_full);
     }
+    barrier_wait<1, 32 + BQ>();
+    tc_fence_after();
+    const uint32_t lanes = s->tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const int own_hi = own ? own_keys(p, start + at.i, length) : 0;
     // what every row of the warp sees
     const int hi_all = __shfl_sync(0xffffffffu, own_hi, 0);
@@ -554,7 +556,7 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, TILE_COLS);
+  if (warp == 1) tmem_dealloc(s->tmem_base, TILE_COLS);
 }
 
 // Writes row (b, h, i), columns [64 c + 2 lane, + 2); rows that are not finite again
