@@ -26,7 +26,8 @@ namespace i8 {
 //    is y's unless it lies within 2^-15 of a half h; then 254 x is compared with 2 h max,
 //    both exact in 64 bits.
 //
-// Measured, bf16: 16384 rows of 8192 QUANT_LONG us (QUANT_RATE TB/s), 2400 of 2560 QUANT_SOME us.
+// Measured, bf16: 16384 rows of 8192 92 us (4.4 TB/s; 110 without the next row's loads under this
+// one's rounding, 170 with halves looked at again), 2400 of 2560 5.2, 8 of 2560 1.8.
 struct QuantizeParams {
   const void* x;
   int8_t* q;
@@ -243,6 +244,13 @@ int quantize(const QuantizeParams& p, cudaStream_t st) {
 // A tile is 128 weight rows (TMEM lanes) by T tokens (columns): the weights are the
 // tensor cores' first operand, whatever the number of tokens, so that few tokens waste
 // none of it and the lanes of a warp write neighbouring channels of out, at any N.
+//
+// Measured, us, rows in bf16 and their rounding included (tokens, K -> N): 1, 2560 -> 2560 5.6
+// (launch, the cluster's exchange and two round trips to memory); 64, 8192 -> 32768 51 (5.3
+// TB/s of weights, 0.81 of a plain copy); 2400, 2560 -> 6848 42 (2.0 POP/s: 270 tiles are 3.65
+// waves of 74 pairs, and 6 us start and end them); 4096, 8192 -> 8192 191; 16384, 8192 -> 8192
+// 780, of which the product 680 (3.2 POP/s, twice the bf16 rate that a library reaches here;
+// tensor pipe 82% busy at 4096 tokens).
 constexpr int BN = 128, SLAB = 128;  // weight rows of a CTA, k of a ring slot (bytes)
 constexpr int EPILOGUE = 8;  // warps: two for each quarter of the TMEM lanes, half of the tokens each
 constexpr int THREADS = 64 + 32 * EPILOGUE;
