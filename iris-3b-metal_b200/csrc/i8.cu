@@ -995,12 +995,14 @@ int launch_pair(const void* w, int64_t ldw, const void* x, int64_t ldx, const Pa
 
 // ------------------------------------------------------------------- which form
 // By an estimate of its time in us. A rows_kernel CTA of T tokens takes START and, for each
-// of its slabs, what its ring of stages gives (SLAB_US alone on its SM; two on one 1.45 times that,
-// 0.85 of it for a deep ring), the weights' bytes HBM_RATE or L2_RATE at most; parts of K cost their exchange. A pair's
-// tile takes its tokens' products. Measured, us, (tokens, K -> N): 64, 2560 -> 2560: T 32
-// in 4 parts 6.6, 64 in 4 parts 6.7, 64 whole 8.7, pair 9.2; 16, 8192 -> 8192: 4 parts 10.2, deep
-// 2 parts 11.6, whole 19.7; 256, 8192 -> 8192: T 128 deep 20.6, 64 23.8, 128 24.4, pair
-// 25.6; 1024, 2560 -> 2560: T 128 13.3, pair 13.7; 301, 2560 -> 15360: pair 18.1, T 128 21.7.
+// of its slabs, what its ring of stages gives (SLAB_US alone on its SM; two on one PAIRED times
+// that, DEEP_SLAB of it for a deep ring), the weights' bytes HBM_RATE or L2_RATE at most; parts of K
+// cost their exchange; an SM's second CTA begins SECOND later. A pair's tile takes its tokens'
+// products. Measured, us, (tokens, K -> N): 64, 2560 -> 2560: T 64 deep in 4 parts 7.0, T 32 in 4
+// parts 7.9, T 64 whole 8.7, pair 9.2; 16, 8192 -> 8192: 4 parts 10.2, deep 2 parts 11.6,
+// whole 19.7; 256, 8192 -> 8192: T 128 deep 20.6, T 64 23.8, T 128 24.4, pair 25.6; 1024, 2560 ->
+// 2560: T 128 13.3, pair 13.7; 301, 2560 -> 15360: pair 18.1, T 128 21.7; 64, 8192 -> 32768: T 64
+// 49, deep 52, pair 53.
 struct Choice {
   int tokens, splits;  // 0 tokens: CTA pairs
   bool deep;
@@ -1009,7 +1011,7 @@ struct Choice {
 Choice choose(int64_t M, int64_t N, int64_t K) {
   constexpr float START = 2.6f, START_TOKEN = 0.0115f, SLAB_US = 0.24f, SLAB_TOKEN = 0.0006f, HBM_RATE = 6.3e6f, L2_RATE = 9.0e6f;
   constexpr int64_t IN_L2 = 96 << 20;  // weights that L2 may hold from the last step
-  constexpr float EXCHANGE = 0.3f, EXCHANGE_TOKEN = 0.024f;
+  constexpr float EXCHANGE = 0.3f, EXCHANGE_TOKEN = 0.024f, SECOND = 1.2f, DEEP_SLAB = 0.85f, DEEP_HBM = 1.07f, PAIRED = 1.45f;
   constexpr float PAIR_START = 6.3f, PAIR_TILE = 1.2f, PAIR_SLAB = 0.08f, PAIR_TOKEN = 0.0009f;
   const int64_t sms = num_sms(), slabs = (K + SLAB - 1) / SLAB, wide = (N + BN - 1) / BN;
   const int64_t per = pair_tokens(M), tiles = (M + per - 1) / per * ((N + 255) / 256), waves = (tiles + sms / 2 - 1) / (sms / 2);
@@ -1026,8 +1028,10 @@ Choice choose(int64_t M, int64_t N, int64_t K) {
       const float exchange = splits > 1 ? EXCHANGE + EXCHANGE_TOKEN * T : 0.f;
       for (int deep = 0; deep < 2; ++deep) {
         const int64_t slots = deep ? sms : 2 * sms, turns = (ctas + slots - 1) / slots;
-        const float each = mine * slab * (deep ? 0.85f : ctas > sms ? 1.45f : 1.f);
-        const float t = start + exchange + std::max(hbm, turns * each + (turns - 1) * (start + exchange - 1.f));
+        const float each = mine * slab * (deep ? DEEP_SLAB : ctas > sms ? PAIRED : 1.f);
+        // an SM's second CTA starts when the first has its TMEM, which is after the wait for the predecessor
+        const float late = !deep && ctas > sms ? SECOND : 0.f;
+        const float t = start + exchange + late + std::max(deep ? DEEP_HBM * hbm : hbm, turns * each + (turns - 1) * (start + exchange - 1.f));
         if (t < least) least = t, best = Choice{T, splits, deep != 0};
       }
     }

@@ -314,3 +314,40 @@ def test_a_layers_step(K):
         y = K.gemm_i8(o[:, 0], *w_out)
         assert_i8(y, *quantized(o[:, 0]), *w_out)
         positions = positions + 1
+
+
+def test_behind_one_another(K):
+    """Kernels with TMEM of different sizes in a chain, each starting while the one before ends."""
+    b, n, h, kv, d = 4, 300, 20, 5, 64
+    q, pk, pv, k, v = inputs(40, b, 1, h, kv, n, 500, n, d)
+    one = inputs(41, 16, 2, 8, 2, 1, 2000, 90, d)
+    packed, scale = K.quantize_i8(normal(42, 700, h * d, dtype=torch.float32))
+    many, many_scale = K.quantize_i8(normal(43, 2600, 900, dtype=torch.float32))
+    x8, x_scale = K.quantize_i8(normal(44, 16, h * d))
+    y8, y_scale = K.quantize_i8(normal(45, 600, 900))
+
+    def chain():
+        a = K.window_attention(q, k, v)
+        first = K.gemm_i8(x8, packed, scale, x_scale=x_scale)
+        p = K.prefix_attention(q, pk, pv, k, v)
+        second = K.gemm_i8(p.view(b * n, h * d)[:40], packed, scale)
+        t = K.prefix_attention(*one)
+        third = K.gemm_i8(y8, many, many_scale, x_scale=y_scale)
+        w = K.window_attention(q, k, v, left=100)
+        last = K.gemm_i8(w.view(b * n, h * d)[:1], packed, scale)
+        return a, first, p, second, t, third, w, last
+
+    want = chain()
+    assert_attends(want[0], q, k, v)
+    assert_prefix(want[2], q, pk, pv, k, v)
+    assert_i8(want[5], y8, y_scale, many, many_scale)
+    torch.cuda.synchronize()
+    for _ in range(60):
+        for got, x in zip(chain(), want):
+            assert torch.equal(got, x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = [chain() for _ in range(3)]
+    for _ in range(20):
+        graph.replay()
+    assert all(torch.equal(got, x) for outs in held for got, x in zip(outs, want))
