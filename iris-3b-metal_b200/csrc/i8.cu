@@ -548,28 +548,31 @@ int launch_rows(const CUtensorMap& tw, const CUtensorMap& tx, Params p, int spli
   return IRIS_OK;
 }
 
-// A few tokens in fp32 or 16 bits: rows_kernel for 16 tokens that rounds them itself. Every CTA
-// reads the rows whole for their largest magnitudes and lays its own part of K out in shared
+// A few values in fp32 or 16 bits (MOST_VALUES): rows_kernel that rounds its tokens itself. Every
+// CTA reads the rows whole for their largest magnitudes and lays its own part of K out in shared
 // memory, as TMA would have; one launch instead of two, which take longer than what they do.
+// Up to 16 tokens may have K in parts, and all warps take part in a row; more have it whole, in
+// few slabs, and a few lanes a row, all rows at once (a row after the other: 64 tokens 160 ->
+// 2560 10.5 us instead of 5.7). In two launches 4.6 us, but 7.7 of host time instead of 4.3.
 namespace few {
-constexpr int T = 16, STAGES = 4, MOST_SLABS = 16;  // slabs of a CTA
-constexpr int RING = STAGES * BN * SLAB, X_SLAB = T * SLAB, X = MOST_SLABS * X_SLAB, PARTS = T * BN * 4;
+constexpr int STAGES = 4, RING = STAGES * BN * SLAB, X = 32768, PARTS = 16 * BN * 4;
+constexpr int most_slabs(int T) { return X / (T * SLAB); }  // slabs of a CTA
 constexpr int64_t MOST_VALUES = 10240;  // of the rows (4 of 2560: 6.6 us, as in two launches; 8 of 2560 7.7 against 7.0)
 struct Smem {
   uint64_t full[STAGES], empty[STAGES], x_full, done;
   uint32_t tmem_base;
   int abort, bad[8];
-  uint32_t top[T];
-  float scale[T];
+  uint32_t top[16];
+  float scale[128];
 };
 constexpr int SMEM = 1024 + RING + X + PARTS + static_cast<int>(sizeof(Smem));
 }  // namespace few
 
-template <typename V>
+template <typename V, int T, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS, 2)
     few_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ Params p, const V* x, int64_t ldx) {
   using namespace few;
-  constexpr int N = Vec<V>::N;
+  constexpr int N = Vec<V>::N, X_SLAB = T * SLAB, COLS = T < 32 ? 32 : T;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* rows = ring + RING;
@@ -589,10 +592,10 @@ __global__ void __launch_bounds__(THREADS, 2)
     mbar_init(&s->done, 1);
     s->abort = 0;
     for (int i = 0; i < 8; ++i) s->bad[i] = 0;
-    for (int i = 0; i < T; ++i) s->top[i] = 0u;
     fence_barrier_init();
     tma_prefetch_desc(&tw);
   }
+  if (threadIdx.x < 16) s->top[threadIdx.x] = 0u;
   __syncthreads();
   volatile int* abort = &s->abort;
   if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -623,7 +626,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMA
-    tmem_alloc(&s->tmem_base, 32);  // after the wait, as in rows_kernel
+    tmem_alloc(&s->tmem_base, COLS);  // after the wait, as in rows_kernel
     tc_fence_before();
     __syncwarp();
     barrier_tell<2, 32 + 32 * EPILOGUE>();
@@ -653,37 +656,60 @@ __global__ void __launch_bounds__(THREADS, 2)
       my_scale = p.w_scale[n];
       if (p.bias) my_bias = p.bias[n];
     }
-    const int w = warp - 2, share = p.M == 1 ? 8 : p.M == 2 ? 4 : p.M <= 4 ? 2 : 1;  // warps of a row
     const int vecs = (p.K + N - 1) / N;
-    for (int m = w / share; m < p.M; m += EPILOGUE / share) {
-      uint32_t top = 0u;
-#pragma unroll 2
-      for (int v = w % share * 32 + lane; v < vecs; v += share * 32) top = top_of<V>(load_vec<V, true>(x + m * ldx, v, p.K), top);
-      if (sizeof(V) == 2) top = max(top & 0xffffu, top >> 16);
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) atomicMax(&s->top[m], top);
-    }
+    constexpr int OF_SLAB = SLAB / N;
+    // the 8-bit values of vector i of this part, of row m, in their swizzled place: 16-byte piece c of row r at c ^ (r & 7)
+    auto place = [&](int m, int i, const Factors& f) {
+      const int v = first * OF_SLAB + i;
+      const uint4 value = v < vecs && f.up != 0.f ? load_vec<V, ALIGNED>(x + m * ldx, v, p.K) : make_uint4(0u, 0u, 0u, 0u);
+      const uint2 q = round_vec<V>(value, f);
+      const int byte = i % OF_SLAB * N;
+      uint8_t* to = rows + i / OF_SLAB * X_SLAB + m * SLAB + (((byte >> 4) ^ (m & 7)) * 16) + (byte & 15);
+      if (N == 8) *reinterpret_cast<uint2*>(to) = q;
+      else *reinterpret_cast<uint32_t*>(to) = q.x;
+    };
     // rows that are not there are zeros
     for (int i = threadIdx.x - 64; i < count * (T - p.M) * (SLAB / 16); i += 32 * EPILOGUE) {
       const int piece = i % (SLAB / 16), row = p.M + i / (SLAB / 16) % (T - p.M), slab = i / (SLAB / 16) / (T - p.M);
       *reinterpret_cast<uint4*>(rows + slab * X_SLAB + row * SLAB + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
-    barrier_wait<1, 32 * EPILOGUE>();
-    // this part's values, in the swizzled places of each slab: 16-byte piece c of row r at c ^ (r & 7)
-    constexpr int OF_SLAB = SLAB / N;
-    for (int m = w / share; m < p.M; m += EPILOGUE / share) {
-      float scale;
-      const Factors f = factors_of<V>(s->top[m], &scale);
-      if (lane == 0) s->scale[m] = scale;
+    if (T > 16) {
+      // all rows at once, a few lanes each
+      constexpr int LANES = 32 * EPILOGUE / T;
+      const int m = (threadIdx.x - 64) / LANES, l = threadIdx.x % LANES;
+      uint32_t top = 0u;
+      if (m < p.M) {
+#pragma unroll 4
+        for (int v = l; v < vecs; v += LANES) top = top_of<V>(load_vec<V, ALIGNED>(x + m * ldx, v, p.K), top);
+      }
+      if (sizeof(V) == 2) top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+      for (int o = 1; o < LANES; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (m < p.M) {
+        float scale;
+        const Factors f = factors_of<V>(top, &scale);
+        if (l == 0) s->scale[m] = scale;
+#pragma unroll 2
+        for (int i = l; i < count * OF_SLAB; i += LANES) place(m, i, f);
+      }
+    } else {
+      const int w = warp - 2, share = p.M == 1 ? 8 : p.M == 2 ? 4 : p.M <= 4 ? 2 : 1;  // warps of a row
+      for (int m = w / share; m < p.M; m += EPILOGUE / share) {
+        uint32_t top = 0u;
+#pragma unroll 2
+        for (int v = w % share * 32 + lane; v < vecs; v += share * 32)
+          top = top_of<V>(load_vec<V, ALIGNED>(x + m * ldx, v, p.K), top);
+        if (sizeof(V) == 2) top = max(top & 0xffffu, top >> 16);
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) atomicMax(&s->top[m], top);
+      }
+      barrier_wait<1, 32 * EPILOGUE>();
+      for (int m = w / share; m < p.M; m += EPILOGUE / share) {
+        float scale;
+        const Factors f = factors_of<V>(s->top[m], &scale);
+        if (lane == 0) s->scale[m] = scale;
 #pragma unroll 1
-      for (int i = w % share * 32 + lane; i < count * OF_SLAB; i += share * 32) {
-        const int v = first * OF_SLAB + i;
-        const uint4 value = v < vecs && f.up != 0.f ? load_vec<V, true>(x + m * ldx, v, p.K) : make_uint4(0u, 0u, 0u, 0u);
-        const uint2 q = round_vec<V>(value, f);
-        const int byte = i % OF_SLAB * N;
-        uint8_t* to = rows + i / OF_SLAB * X_SLAB + m * SLAB + (((byte >> 4) ^ (m & 7)) * 16) + (byte & 15);
-        if (N == 8) *reinterpret_cast<uint2*>(to) = q;
-        else *reinterpret_cast<uint32_t*>(to) = q.x;
+        for (int i = w % share * 32 + lane; i < count * OF_SLAB; i += share * 32) place(m, i, f);
       }
     }
     fence_proxy_async_smem();
@@ -698,6 +724,17 @@ __global__ void __launch_bounds__(THREADS, 2)
   __syncwarp();
   // ------------------------------------------------------------- epilogue
   const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  if (T > 16) {
+    Params mine = p;
+    mine.x_scale = s->scale;
+    constexpr int SHARE = T / 2;
+    if (warp >= 2) store_columns(mine, lanes + half * SHARE, half * SHARE, SHARE, n, ok);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(s->tmem_base, COLS);
+    return;
+  }
   const int own = T / p.splits, log_own = __ffs(own) - 1;  // columns of a CTA: a power of two, 2 at least
   if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (warp >= 2 && !half) {
@@ -733,12 +770,12 @@ __global__ void __launch_bounds__(THREADS, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(s->tmem_base, 32);
+  if (warp == 1) tmem_dealloc(s->tmem_base, COLS);
 }
 
-template <typename V>
-int launch_few(const CUtensorMap& tw, Params p, int splits, const void* x, int64_t ldx, cudaStream_t st) {
-  auto kernel = few_kernel<V>;
+template <typename V, int T, bool ALIGNED>
+int launch_few_as(const CUtensorMap& tw, Params p, int splits, const void* x, int64_t ldx, cudaStream_t st) {
+  auto kernel = few_kernel<V, T, ALIGNED>;
   static bool configured[64] = {false};
   int dev = 0;
   IRIS_CUDA(cudaGetDevice(&dev));
@@ -752,6 +789,21 @@ int launch_few(const CUtensorMap& tw, Params p, int splits, const void* x, int64
   IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(ctas)), THREADS, few::SMEM, st, static_cast<unsigned>(splits), tw, p,
                          static_cast<const V*>(x), ldx));
   return IRIS_OK;
+}
+
+template <typename V>
+int launch_few(const CUtensorMap& tw, const Params& p, int tokens, int splits, const void* x, int64_t ldx, cudaStream_t st) {
+  const bool aligned = aligned16(x) && (p.M <= 1 || ldx * static_cast<int64_t>(sizeof(V)) % 16 == 0);
+  switch (tokens + aligned) {
+    case 16: return launch_few_as<V, 16, false>(tw, p, splits, x, ldx, st);
+    case 17: return launch_few_as<V, 16, true>(tw, p, splits, x, ldx, st);
+    case 32: return launch_few_as<V, 32, false>(tw, p, 1, x, ldx, st);
+    case 33: return launch_few_as<V, 32, true>(tw, p, 1, x, ldx, st);
+    case 64: return launch_few_as<V, 64, false>(tw, p, 1, x, ldx, st);
+    case 65: return launch_few_as<V, 64, true>(tw, p, 1, x, ldx, st);
+    case 128: return launch_few_as<V, 128, false>(tw, p, 1, x, ldx, st);
+    default: return launch_few_as<V, 128, true>(tw, p, 1, x, ldx, st);
+  }
 }
 
 // ---------------------------------------------------------------- many tokens
@@ -1039,11 +1091,12 @@ Choice choose(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 
-// Whether few_kernel takes a call's rows.
-inline bool rounds_itself(const iris_i8_problem& q, const Choice& c) {
-  const int64_t slabs = (q.K + SLAB - 1) / SLAB, size = q.x_dtype == IRIS_F32 ? 4 : 2;
-  return q.x_dtype != IRIS_I8 && c.tokens == few::T && q.M <= few::T && q.M * q.K <= few::MOST_VALUES &&
-         (slabs + c.splits - 1) / c.splits <= few::MOST_SLABS && aligned16(q.x) && (q.M <= 1 || q.ldx * size % 16 == 0);
+// The tokens of few_kernel's tile that takes a call's rows; 0: none does.
+inline int few_tokens(const iris_i8_problem& q, const Choice& c) {
+  if (q.x_dtype == IRIS_I8 || q.M > 128 || q.M * q.K > few::MOST_VALUES) return 0;
+  const int tokens = q.M <= 16 ? 16 : q.M <= 32 ? 32 : q.M <= 64 ? 64 : 128;
+  const int64_t slabs = (q.K + SLAB - 1) / SLAB, splits = tokens == 16 && c.tokens == 16 ? c.splits : 1;
+  return (slabs + splits - 1) / splits <= few::most_slabs(tokens) ? tokens : 0;
 }
 
 inline int check_rows(int64_t M, int64_t K, int64_t ldx) {
@@ -1093,7 +1146,7 @@ extern "C" int iris_gemm_i8_workspace(const iris_i8_problem* q, int64_t* bytes) 
   using namespace iris::i8;
   IRIS_REQUIRE(q != nullptr && bytes != nullptr, "gemm_i8_workspace: null pointer");
   IRIS_CHECK_STATUS(check_product(*q));
-  *bytes = q->M * q->N == 0 || rounds_itself(*q, choose(q->M, q->N, q->K)) ? 0 : workspace_bytes(*q);
+  *bytes = q->M * q->N == 0 || few_tokens(*q, choose(q->M, q->N, q->K)) != 0 ? 0 : workspace_bytes(*q);
   return IRIS_OK;
 }
 
@@ -1120,11 +1173,12 @@ extern "C" int iris_gemm_i8(const iris_i8_problem* q, void* stream) {
   CUtensorMap tw, tx;
   if (fresh) {
     IRIS_CHECK_STATUS(check_rows(q->M, q->K, q->ldx));
-    if (rounds_itself(*q, c)) {
+    if (const int tokens = few_tokens(*q, c)) {
+      const int splits = c.tokens == 16 ? c.splits : 1;
       IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tw, q->w, q->K, q->N, q->ldw, SLAB, BN));
-      return q->x_dtype == IRIS_F32    ? launch_few<float>(tw, p, c.splits, x, ldx, st)
-             : q->x_dtype == IRIS_BF16 ? launch_few<__nv_bfloat16>(tw, p, c.splits, x, ldx, st)
-                                       : launch_few<__half>(tw, p, c.splits, x, ldx, st);
+      return q->x_dtype == IRIS_F32    ? launch_few<float>(tw, p, tokens, splits, x, ldx, st)
+             : q->x_dtype == IRIS_BF16 ? launch_few<__nv_bfloat16>(tw, p, tokens, splits, x, ldx, st)
+                                       : launch_few<__half>(tw, p, tokens, splits, x, ldx, st);
     }
     IRIS_REQUIRE(q->workspace && aligned16(q->workspace) && q->workspace_bytes >= workspace_bytes(*q), "gemm_i8: workspace too small");
     ldx = row_bytes(q->K);

@@ -52,8 +52,8 @@ def test_c_entries_refuse_bad_arguments(lib):  # noqa: F811
                          (dict(w=24), "16 bytes"), (dict(x=24), "16 bytes"), (dict(ldx=56), "16 bytes"), (dict(ldx=32), "16 bytes"),
                          (dict(x_dtype=4), "dtype"), (dict(out_dtype=3), "dtype"), (dict(w_scale=18), "misaligned"),
                          (dict(bias=18), "misaligned"), (dict(out=17), "misaligned"), (dict(out=18, out_dtype=0), "misaligned"),
-                         (dict(x_dtype=1, m=30, workspace=0), "workspace"), (dict(x_dtype=1, m=30, workspace=24), "workspace"),
-                         (dict(x_dtype=1, m=30, room=1567), "workspace"), (dict(x_dtype=1, ldx=-1), "stride"),
+                         (dict(x_dtype=1, m=300, workspace=0), "workspace"), (dict(x_dtype=1, m=300, workspace=24), "workspace"),
+                         (dict(x_dtype=1, m=300, room=15599), "workspace"), (dict(x_dtype=1, ldx=-1), "stride"),
                          (dict(x_dtype=0, x=18), "misaligned")]:  # fmt: skip
         assert message in _einval(lib, "iris_gemm_i8", product(**bad), None), bad
     for name in ("iris_gemm_i8", "iris_gemm_i8_workspace"):
@@ -70,11 +70,13 @@ def test_workspace_is_for_rows_that_are_quantised(lib):  # noqa: F811
 
     assert need() == 0
     for dtype in (0, 1, 2):  # rows at 16 bytes, then their scales
-        assert need(x_dtype=dtype, m=30) == 30 * 48 + 128
+        assert need(x_dtype=dtype, m=300) == 300 * 48 + 1200
         assert need(x_dtype=dtype, m=1000, k=16) == 16000 + 4000
-        assert need(x_dtype=dtype, x=24) == 3 * 48 + 16  # a few rows at 16 bytes are rounded by the product itself
         assert need(x_dtype=dtype, k=7000, ldx=7008, ldw=7008) == 3 * 7008 + 16
-        assert need(x_dtype=dtype) == need(x_dtype=dtype, m=0) == need(x_dtype=dtype, n=0, m=1000) == 0
+        # a few rows are rounded by the product itself
+        for m in (3, 30, 100, 128):
+            assert need(x_dtype=dtype, m=m) == 0
+        assert need(x_dtype=dtype, m=0) == need(x_dtype=dtype, n=0, m=1000) == 0
 
 
 def test_wrappers_refuse_before_any_launch(K):

@@ -122,7 +122,7 @@ def test_product_wide(K, m):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 8, 9, 15, 16])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 8, 9, 15, 16, 17, 31, 32, 33, 64, 65, 100, 128])
 def test_a_few_rows_that_the_product_rounds(K, m, dtype):
     """Against the same rows quantised before: bit for bit, in each number of parts of K, extreme rows among them."""
     for k in (1, 7, 8, 127, 128, 129, 520, 1000, 1280, 2560, 10240 // m):
@@ -134,7 +134,7 @@ def test_a_few_rows_that_the_product_rounds(K, m, dtype):
             packed, scale = K.quantize_i8(rows(n, n, k, torch.float32, False))
             q, x_scale = K.quantize_i8(x)
             want = K.gemm_i8(q, packed, scale, x_scale=x_scale, out_dtype=dtype)
-            for view in (x, torch.cat([x, x], dim=1)[:, :k] if k % 8 == 0 else x):
+            for view in (x, torch.cat([x, x], dim=1)[:, :k], torch.cat([x[:, :1], x], dim=1)[:, 1:]):  # rows anywhere
                 got = K.gemm_i8(view, packed, scale)
                 assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(got.isnan(), want.isnan())
 
@@ -252,7 +252,7 @@ def test_kernels_are_counted(K):
     packed, scale = K.quantize_i8(rows(50, 40, 64, torch.float32))
     x = rows(51, 3, 64)
     for call, count in [(lambda: K.quantize_i8(x), 1), (lambda: K.gemm_i8(x, packed, scale), 1),
-                        (lambda: K.gemm_i8(rows(52, 30, 64), packed, scale), 2),
+                        (lambda: K.gemm_i8(rows(52, 30, 640), *K.quantize_i8(rows(53, 40, 640))), 3),
                         (lambda: K.gemm_i8(packed[:2], packed, scale, x_scale=scale[:2]), 1),
                         (lambda: K.gemm_i8(x[:0], packed, scale), 0)]:  # fmt: skip
         before = _lib.launch_count()
