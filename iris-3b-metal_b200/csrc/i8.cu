@@ -393,7 +393,6 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2)
   if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   volatile int* abort = &s->abort;
   grid_wait();
-  grid_trigger();
 
   if (warp == 0) {
     // ----------------------------------------------------------------- TMA
@@ -421,9 +420,10 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2)
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMA
-    // TMEM only after the wait: a CTA that held some while it waits could keep its predecessor's,
-    // which still have to allocate theirs, from ever ending
+    // TMEM only after the wait (a CTA that held some while it waits could keep its predecessor's,
+    // which still have to allocate theirs, from ever ending), and the successor only after TMEM
     tmem_alloc(&s->tmem_base, R::COLS);
+    grid_trigger();
     tc_fence_before();
     __syncwarp();
     barrier_tell<1, 32 + 32 * EPILOGUE>();
@@ -600,7 +600,6 @@ __global__ void __launch_bounds__(THREADS, 2)
   volatile int* abort = &s->abort;
   if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   grid_wait();
-  grid_trigger();
 
   bool ok = true;
   float my_scale = 0.f, my_bias = 0.f;
@@ -626,7 +625,8 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMA
-    tmem_alloc(&s->tmem_base, COLS);  // after the wait, as in rows_kernel
+    tmem_alloc(&s->tmem_base, COLS);  // after the wait and before the successor, as in rows_kernel
+    grid_trigger();
     tc_fence_before();
     __syncwarp();
     barrier_tell<2, 32 + 32 * EPILOGUE>();
@@ -881,8 +881,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   cluster_sync();  // every barrier of both CTAs exists before any remote arrival
   volatile int* abort = &s->abort;
   grid_wait();
-  grid_trigger();
-  if (warp == 1) tmem_alloc_pair(&s->tmem_base, 512);  // after the wait, as in rows_kernel
+  if (warp == 1) {
+    tmem_alloc_pair(&s->tmem_base, 512);  // after the wait and before the successor, as in rows_kernel
+    grid_trigger();
+  }
   // both CTAs' TMEM before any product; the producers go on meanwhile
   tc_fence_before();
   __syncwarp();

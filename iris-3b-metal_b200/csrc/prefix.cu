@@ -268,7 +268,6 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
   __syncthreads();
   volatile int* abort = &s->abort;
   grid_wait();
-  grid_trigger();
   const bool finish = cta < plan.whole_tiles;
   const int split = finish ? 0 : (cta - plan.whole_tiles) % plan.tile_splits;
   const int unit_tile = finish ? cta : plan.whole_tiles + (cta - plan.whole_tiles) / plan.tile_splits;
@@ -356,9 +355,10 @@ IRIS_DEVICE void tile_cta(const CUtensorMap& tpk, const CUtensorMap& tpv, const 
     }
   } else if (warp == 1) {
     // ----------------------------------------------------------------- MMA
-    // TMEM only after the wait: a CTA that held some while it waits could keep its predecessor's,
-    // which still have to allocate theirs, from ever ending
+    // TMEM only after the wait (a CTA that held some while it waits could keep its predecessor's,
+    // which still have to allocate theirs, from ever ending), and the successor only after TMEM
     tmem_alloc(&s->tmem_base, TILE_COLS);
+    grid_trigger();
     tc_fence_before();
     __syncwarp();
     barrier_tell<1, 32 + BQ>();

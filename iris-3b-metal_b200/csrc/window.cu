@@ -196,7 +196,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 2)
   const int b = blockIdx.x % per_row / p.heads_q, h = blockIdx.x % p.heads_q;
   const int hk = h / (p.heads_q / p.heads_kv);
   grid_wait();
-  grid_trigger();
   const int length = sample_length(p, b);
   const int64_t start = sample_start(p, b);
   const Blocks blocks = key_blocks(p, start + row0, min(BQ, p.n - row0), length);
@@ -221,7 +220,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 2)
     s->abort = 0;
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc(&s->tmem_base, TILE_COLS);
+  if (warp == 1) {
+    tmem_alloc(&s->tmem_base, TILE_COLS);
+    grid_trigger();  // behind TMEM: a successor that takes some could keep a CTA from ever getting its own
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
