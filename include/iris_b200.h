@@ -148,7 +148,8 @@ int iris_qkv_heads(const void* qkv, int64_t batch, int64_t tokens, int64_t row_s
                    int head_major, void* stream);
 
 /* Head rows [batch, heads, n, head_dim]: element strides of the first three
- * dimensions, head_dim contiguous. */
+ * dimensions, head_dim contiguous. The attentions below do not read the stride of a
+ * dimension with one entry. */
 typedef struct iris_head_rows {
   void* data;
   int64_t stride_b, stride_h, stride_n;

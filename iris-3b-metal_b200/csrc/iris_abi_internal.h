@@ -16,6 +16,14 @@ int set_error(int code, const char* fmt, ...);
 int num_sms();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Rows whose strides can all be used: that of a dimension with one entry says nothing and becomes 0.
+inline iris_head_rows used_strides(iris_head_rows r, int64_t batch, int64_t heads, int64_t tokens) {
+  if (batch <= 1) r.stride_b = 0;
+  if (heads <= 1) r.stride_h = 0;
+  if (tokens <= 1) r.stride_n = 0;
+  return r;
+}
+
 inline bool aligned_n(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
 
 // 2-D bf16 tensor map (inner dim first) with 128-byte swizzle and the given box.

@@ -1235,7 +1235,11 @@ extern "C" int iris_prefix_attn_fwd(const iris_prefix_problem* q, void* stream) 
   const float scale = static_cast<float>(q->scale);
   // and so must its product with log2(e) be: 0 times infinity is NaN
   IRIS_REQUIRE(scale > 0.f && scale * 1.4426950408889634f < INFINITY, "prefix_attn_fwd: scale must be positive and finite");
-  const iris_head_rows all[5] = {q->q, q->prefix_k, q->prefix_v, q->k, q->v};
+  const iris_head_rows all[5] = {used_strides(q->q, q->batch, q->heads_q, q->n),
+                                 used_strides(q->prefix_k, q->groups, q->heads_kv, q->n_prefix),
+                                 used_strides(q->prefix_v, q->groups, q->heads_kv, q->n_prefix),
+                                 used_strides(q->k, q->batch, q->heads_kv, q->n_kv),
+                                 used_strides(q->v, q->batch, q->heads_kv, q->n_kv)};
   const int64_t tokens[5] = {q->n, q->n_prefix, q->n_prefix, q->n_kv, q->n_kv};
   for (int i = 0; i < 5; ++i) {
     IRIS_REQUIRE(rows_aligned(all[i]), "prefix_attn_fwd: pointers and strides must be multiples of 16 bytes");
@@ -1248,12 +1252,12 @@ extern "C" int iris_prefix_attn_fwd(const iris_prefix_problem* q, void* stream) 
   IRIS_REQUIRE(q->out, "prefix_attn_fwd: null pointer");
   for (int i = 0; i < 5; ++i) IRIS_REQUIRE(all[i].data || tokens[i] == 0, "prefix_attn_fwd: null pointer");
   Params p = {};
-  p.q = q->q.data, p.pk = q->prefix_k.data, p.pv = q->prefix_v.data, p.k = q->k.data, p.v = q->v.data, p.out = q->out;
-  p.qb = q->q.stride_b, p.qh = q->q.stride_h, p.qn = q->q.stride_n;
-  p.pkb = q->prefix_k.stride_b, p.pkh = q->prefix_k.stride_h, p.pkn = q->prefix_k.stride_n;
-  p.pvb = q->prefix_v.stride_b, p.pvh = q->prefix_v.stride_h, p.pvn = q->prefix_v.stride_n;
-  p.kb = q->k.stride_b, p.kh = q->k.stride_h, p.kn = q->k.stride_n;
-  p.vb = q->v.stride_b, p.vh = q->v.stride_h, p.vn = q->v.stride_n;
+  p.q = all[0].data, p.pk = all[1].data, p.pv = all[2].data, p.k = all[3].data, p.v = all[4].data, p.out = q->out;
+  p.qb = all[0].stride_b, p.qh = all[0].stride_h, p.qn = all[0].stride_n;
+  p.pkb = all[1].stride_b, p.pkh = all[1].stride_h, p.pkn = all[1].stride_n;
+  p.pvb = all[2].stride_b, p.pvh = all[2].stride_h, p.pvn = all[2].stride_n;
+  p.kb = all[3].stride_b, p.kh = all[3].stride_h, p.kn = all[3].stride_n;
+  p.vb = all[4].stride_b, p.vh = all[4].stride_h, p.vn = all[4].stride_n;
   p.ob = q->out_stride_b, p.on = q->out_stride_n;
   p.batch = static_cast<int>(q->batch), p.per_group = static_cast<int>(q->batch / q->groups);
   p.heads_q = static_cast<int>(q->heads_q), p.heads_kv = static_cast<int>(q->heads_kv);

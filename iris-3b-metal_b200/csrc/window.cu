@@ -1021,18 +1021,20 @@ extern "C" int iris_window_attn_fwd(const iris_window_problem* q, void* stream) 
   const float scale = static_cast<float>(q->scale);
   // and so must its product with log2(e) be: 0 times infinity is NaN
   IRIS_REQUIRE(scale > 0.f && scale * 1.4426950408889634f < INFINITY, "window_attn_fwd: scale must be positive and finite");
-  IRIS_REQUIRE(rows_aligned(q->q) && rows_aligned(q->k) && rows_aligned(q->v) && aligned16(q->out) &&
+  const iris_head_rows rows = used_strides(q->q, q->batch, q->heads_q, q->n);
+  const iris_head_rows k = used_strides(q->k, q->batch, q->heads_kv, q->n_kv), v = used_strides(q->v, q->batch, q->heads_kv, q->n_kv);
+  IRIS_REQUIRE(rows_aligned(rows) && rows_aligned(k) && rows_aligned(v) && aligned16(q->out) &&
                    q->out_stride_b % 8 == 0 && q->out_stride_n % 8 == 0,
                "window_attn_fwd: pointers and strides must be multiples of 16 bytes");
-  IRIS_REQUIRE(rows_apart(q->q, q->n) && rows_apart(q->k, q->n_kv) && rows_apart(q->v, q->n_kv),
+  IRIS_REQUIRE(rows_apart(rows, q->n) && rows_apart(k, q->n_kv) && rows_apart(v, q->n_kv),
                "window_attn_fwd: rows must not repeat along the tokens");
   if (q->batch * q->n == 0) return IRIS_OK;
-  IRIS_REQUIRE(q->q.data && q->out && ((q->k.data && q->v.data) || q->n_kv == 0), "window_attn_fwd: null pointer");
+  IRIS_REQUIRE(rows.data && q->out && ((k.data && v.data) || q->n_kv == 0), "window_attn_fwd: null pointer");
   Params p = {};
-  p.q = q->q.data, p.k = q->k.data, p.v = q->v.data, p.out = q->out;
-  p.qb = q->q.stride_b, p.qh = q->q.stride_h, p.qn = q->q.stride_n;
-  p.kb = q->k.stride_b, p.kh = q->k.stride_h, p.kn = q->k.stride_n;
-  p.vb = q->v.stride_b, p.vh = q->v.stride_h, p.vn = q->v.stride_n;
+  p.q = rows.data, p.k = k.data, p.v = v.data, p.out = q->out;
+  p.qb = rows.stride_b, p.qh = rows.stride_h, p.qn = rows.stride_n;
+  p.kb = k.stride_b, p.kh = k.stride_h, p.kn = k.stride_n;
+  p.vb = v.stride_b, p.vh = v.stride_h, p.vn = v.stride_n;
   p.ob = q->out_stride_b, p.on = q->out_stride_n;
   p.batch = static_cast<int>(q->batch), p.heads_q = static_cast<int>(q->heads_q);
   p.heads_kv = static_cast<int>(q->heads_kv), p.n = static_cast<int>(q->n), p.n_kv = static_cast<int>(q->n_kv);

@@ -99,3 +99,12 @@ def test_wrapper_refuses_before_any_launch(K):
             K.prefix_attention(**good, out=good[name].view(-1)[: 6 * 64].view(6, 1, 64))
     with pytest.raises(TypeError):
         K.prefix_attention(**good, scale="x")
+
+
+def test_strides_of_lone_entries_are_not_looked_at(lib):  # noqa: F811
+    """Up to the check that refuses a missing output, which comes after those of the strides."""
+    for stride in (1 << 34, -(1 << 40), 12, -128):
+        assert "null" in _einval(lib, "iris_prefix_attn_fwd", attend(m=1, kn=stride, out=0), None), stride
+        assert "null" in _einval(lib, "iris_prefix_attn_fwd", attend(p=1, pn=stride, out=0), None), stride
+        assert "null" in _einval(lib, "iris_prefix_attn_fwd", attend(n=1, qn=stride, out=0), None), stride
+        assert "null" in _einval(lib, "iris_prefix_attn_fwd", attend(batch=1, groups=1, vb=stride, out=0), None), stride

@@ -351,3 +351,35 @@ def test_behind_one_another(K):
     for _ in range(20):
         graph.replay()
     assert all(torch.equal(got, x) for outs in held for got, x in zip(outs, want))
+
+
+@pytest.mark.parametrize("n, p", [(1, 300), (3, 77), (150, 300), (1, 0)])
+def test_the_stride_of_a_lone_token_is_not_read(K, n, p):
+    """Through the C ABI, where any value may stand in it."""
+    import ctypes
+
+    from iris_b200 import _lib
+    from test_prefix import PREFIX
+
+    lib, d = _lib.load(), 64
+    q, pk, pv, k, v = inputs(50, 2, 1, 4, 2, n, p, 1, d)
+    starts = int32([n, n])  # the one key is seen by every row
+    want = K.prefix_attention(q, pk, pv, k, v, starts=starts)
+    assert_prefix(want, q, pk, pv, k, v, starts=starts)
+    for stride in (0, -8, -(1 << 20), 1 << 34, 1 << 45):
+        def rows(t, n_stride=None):
+            return t.data_ptr(), t.stride(0), t.stride(1), t.stride(2) if n_stride is None else n_stride
+
+        out = torch.full_like(want, 7.0)
+
+        def problem(workspace=0, room=0):
+            return PREFIX.pack(*rows(q), *rows(pk), *rows(pv), *rows(k, stride), *rows(v, -stride), out.data_ptr(), n * 4 * d, 4 * d, 0,
+                               starts.data_ptr(), 0, workspace, room, 1, 2, 1, 4, 2, n, p, 1, d, 0, d**-0.5)  # fmt: skip
+
+        need = ctypes.c_int64(-1)
+        assert lib.iris_prefix_attn_workspace(problem(), ctypes.byref(need)) == 0
+        workspace = torch.empty(max(need.value, 16), device="cuda", dtype=torch.uint8)
+        stream = torch.cuda.current_stream().cuda_stream
+        assert lib.iris_prefix_attn_fwd(problem(workspace.data_ptr(), need.value), stream) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)

@@ -376,3 +376,12 @@ def test_the_module_is_for_one_python_and_torch(lib, monkeypatch):  # noqa: F811
             m.setattr(_lib, "_text_side", None)
             with pytest.raises(RuntimeError, match="not built"):
                 _lib.text_side()
+
+
+def test_strides_of_lone_entries_are_not_looked_at(lib):  # noqa: F811
+    """Up to the check that refuses a missing output, which comes after those of the strides."""
+    for stride in (12, -128, 1 << 45):
+        for q, k, n, m in [((16, 0, 0, stride), (16, 0, 0, 128), 1, 5), ((16, stride, 0, 128), (16, stride, 0, 128), 3, 5),
+                           ((16, 0, 0, 128), (16, 0, stride, stride), 3, 1)]:  # fmt: skip
+            problem = WINDOW.pack(*q, *k, *k, 0, 0, 0, 0, 0, 0, 0, 1, 1, 4, 1, n, m, 128, -1, 0, 0, 0.1)
+            assert "null" in _einval(lib, "iris_window_attn_fwd", problem, None), (q, k)
