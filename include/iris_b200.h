@@ -342,7 +342,7 @@ int iris_window_attn_workspace(const iris_window_problem* problem, int64_t* byte
  * - n; right -1: no bound), all in one softmax; 0 where there is none. q [batch, heads_q, n, head_dim],
  * prefix_k / prefix_v [groups, heads_kv, n_prefix, head_dim], k / v [batch, heads_kv,
  * n_kv, head_dim], bf16 or f16, strides multiples of 8 (0 repeats a head, group or sample),
- * head_dim 64 or 128; out shares no memory with the keys, and with q only as its own
+ * head_dim 64 or 128, n_prefix + n_kv below 2^30; out shares no memory with the keys, and with q only as its own
  * rows in place. workspace: iris_prefix_attn_workspace bytes. */
 typedef struct iris_prefix_problem {
   iris_head_rows q, prefix_k, prefix_v, k, v;

@@ -1097,7 +1097,7 @@ int make_plan(const Sizes& z, Plan* out) {
   if (form != 2) {
     IRIS_REQUIRE(step_units * step_cut.splits < (1ll << 30), "prefix_attn_fwd: too many rows");
     plan.step_prefix = form == 0;
-    plan.step_chunk = static_cast<int>(std::min<int64_t>(step_cut.chunk, 1ll << 30));
+    plan.step_chunk = static_cast<int>(step_cut.chunk);  // at most the keys (below 2^30) and 63
     plan.step_splits = static_cast<int>(step_cut.splits);
     plan.step_ctas = static_cast<int>(step_units * step_cut.splits);
     plan.cluster = form == 0 && plan.step_splits > 1 && plan.step_splits <= MOST_CLUSTER;
@@ -1197,7 +1197,7 @@ inline int check_sizes(const iris_prefix_problem& q) {
   IRIS_REQUIRE(q.heads_q > 0 && q.heads_kv > 0 && q.heads_q % q.heads_kv == 0,
                "prefix_attn_fwd: heads_q must be a positive multiple of heads_kv");
   IRIS_REQUIRE(q.batch >= 0 && q.n >= 0 && q.n_prefix >= 0 && q.n_kv >= 0 && q.batch <= 65535 && q.heads_q <= 65535 &&
-                   q.n < (1ll << 30) && q.n_prefix < (1ll << 30) && q.n_kv < (1ll << 30),
+                   q.n < (1ll << 30) && q.n_prefix < (1ll << 30) && q.n_kv < (1ll << 30) && q.n_prefix + q.n_kv < (1ll << 30),
                "prefix_attn_fwd: sizes");
   IRIS_REQUIRE(q.groups >= 1 && q.batch % q.groups == 0, "prefix_attn_fwd: the batch must be a multiple of the groups");
   IRIS_REQUIRE(q.right >= -1, "prefix_attn_fwd: right is -1 (no bound) or more");

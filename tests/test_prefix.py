@@ -108,3 +108,12 @@ def test_strides_of_lone_entries_are_not_looked_at(lib):  # noqa: F811
         assert "null" in _einval(lib, "iris_prefix_attn_fwd", attend(p=1, pn=stride, out=0), None), stride
         assert "null" in _einval(lib, "iris_prefix_attn_fwd", attend(n=1, qn=stride, out=0), None), stride
         assert "null" in _einval(lib, "iris_prefix_attn_fwd", attend(batch=1, groups=1, vb=stride, out=0), None), stride
+
+
+def test_keys_that_32_bits_do_not_count_are_refused(lib):  # noqa: F811
+    """A row tile's place among all keys, and one chunk of them, are held in 32 bits."""
+    out = ctypes.c_int64(-1)
+    for p, m in [(1 << 29, 1 << 29), ((1 << 30) - 1, 1), ((1 << 30) - 1, (1 << 30) - 1), (5, (1 << 30) - 5)]:
+        assert "sizes" in _einval(lib, "iris_prefix_attn_fwd", attend(p=p, m=m), None)
+        assert "sizes" in _einval(lib, "iris_prefix_attn_workspace", attend(p=p, m=m), ctypes.byref(out))
+    assert lib.iris_prefix_attn_workspace(attend(p=1 << 29, m=(1 << 29) - 1), ctypes.byref(out)) == 0
