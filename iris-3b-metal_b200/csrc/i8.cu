@@ -548,21 +548,22 @@ int launch_rows(const CUtensorMap& tw, const CUtensorMap& tx, Params p, int spli
   return IRIS_OK;
 }
 
-// A few values in fp32 or 16 bits (MOST_VALUES): rows_kernel that rounds its tokens itself. Every
-// CTA reads the rows whole for their largest magnitudes and lays its own part of K out in shared
-// memory, as TMA would have; one launch instead of two, which take longer than what they do.
-// Up to 16 tokens may have K in parts, and all warps take part in a row; more have it whole, in
-// few slabs, and a few lanes a row, all rows at once (a row after the other: 64 tokens 160 ->
-// 2560 10.5 us instead of 5.7). In two launches 4.6 us, but 7.7 of host time instead of 4.3.
+// rows_kernel that rounds its tokens itself, one launch instead of two: every CTA reads its rows
+// whole for their largest magnitudes and lays its own part of K out in shared memory, as TMA
+// would have. It is taken (few_tokens) where the device is done as early as with two launches or
+// earlier; the host is, by some 3 us, in any case.
+//  - T 32, 64 or 128, rows of one slab (SHORT_ROW bytes): all rows of a tile at once, a few lanes
+//    each. More lanes a row are faster, so T 32 while its tiles have an SM each.
+//  - T 16, up to MOST_ROWS longer rows: K in parts, a warp or more a row.
 namespace few {
 constexpr int STAGES = 4, RING = STAGES * BN * SLAB, X = 32768, PARTS = 16 * BN * 4;
 constexpr int most_slabs(int T) { return X / (T * SLAB); }  // slabs of a CTA
-constexpr int64_t MOST_VALUES = 10240;  // of the rows (4 of 2560: 6.6 us, as in two launches; 8 of 2560 7.7 against 7.0)
+constexpr int64_t SHORT_ROW = 256, MOST_TOKENS = 128, MOST_ROWS = 8;
 struct Smem {
   uint64_t full[STAGES], empty[STAGES], x_full, done;
   uint32_t tmem_base;
   int abort, bad[8];
-  uint32_t top[16];
+  uint32_t top[MOST_ROWS];
   float scale[128];
 };
 constexpr int SMEM = 1024 + RING + X + PARTS + static_cast<int>(sizeof(Smem));
@@ -579,7 +580,9 @@ __global__ void __launch_bounds__(THREADS, 2)
   int* parts = reinterpret_cast<int*>(rows + X);  // [part][column][128]
   few::Smem* s = reinterpret_cast<few::Smem*>(rows + X + PARTS);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
-  const int part = static_cast<int>(blockIdx.x % p.splits), n0 = static_cast<int>(blockIdx.x / p.splits) * BN;
+  const int part = static_cast<int>(blockIdx.x % p.splits), unit = static_cast<int>(blockIdx.x / p.splits);
+  const int m0 = unit % p.token_tiles * T, n0 = unit / p.token_tiles * BN;
+  const int tokens = min(T, p.M - m0);
   const int slabs = (p.K + SLAB - 1) / SLAB;
   const int first = slabs * part / p.splits, count = slabs * (part + 1) / p.splits - first;
 
@@ -595,7 +598,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     fence_barrier_init();
     tma_prefetch_desc(&tw);
   }
-  if (threadIdx.x < 16) s->top[threadIdx.x] = 0u;
+  if (threadIdx.x < MOST_ROWS) s->top[threadIdx.x] = 0u;
   __syncthreads();
   volatile int* abort = &s->abort;
   if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -658,10 +661,11 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
     const int vecs = (p.K + N - 1) / N;
     constexpr int OF_SLAB = SLAB / N;
+    const V* row0 = x + m0 * ldx;
     // the 8-bit values of vector i of this part, of row m, in their swizzled place: 16-byte piece c of row r at c ^ (r & 7)
     auto place = [&](int m, int i, const Factors& f) {
       const int v = first * OF_SLAB + i;
-      const uint4 value = v < vecs && f.up != 0.f ? load_vec<V, ALIGNED>(x + m * ldx, v, p.K) : make_uint4(0u, 0u, 0u, 0u);
+      const uint4 value = v < vecs && f.up != 0.f ? load_vec<V, ALIGNED>(row0 + m * ldx, v, p.K) : make_uint4(0u, 0u, 0u, 0u);
       const uint2 q = round_vec<V>(value, f);
       const int byte = i % OF_SLAB * N;
       uint8_t* to = rows + i / OF_SLAB * X_SLAB + m * SLAB + (((byte >> 4) ^ (m & 7)) * 16) + (byte & 15);
@@ -669,8 +673,8 @@ __global__ void __launch_bounds__(THREADS, 2)
       else *reinterpret_cast<uint32_t*>(to) = q.x;
     };
     // rows that are not there are zeros
-    for (int i = threadIdx.x - 64; i < count * (T - p.M) * (SLAB / 16); i += 32 * EPILOGUE) {
-      const int piece = i % (SLAB / 16), row = p.M + i / (SLAB / 16) % (T - p.M), slab = i / (SLAB / 16) / (T - p.M);
+    for (int i = threadIdx.x - 64; i < count * (T - tokens) * (SLAB / 16); i += 32 * EPILOGUE) {
+      const int piece = i % (SLAB / 16), row = tokens + i / (SLAB / 16) % (T - tokens), slab = i / (SLAB / 16) / (T - tokens);
       *reinterpret_cast<uint4*>(rows + slab * X_SLAB + row * SLAB + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
     if (T > 16) {
@@ -678,14 +682,14 @@ __global__ void __launch_bounds__(THREADS, 2)
       constexpr int LANES = 32 * EPILOGUE / T;
       const int m = (threadIdx.x - 64) / LANES, l = threadIdx.x % LANES;
       uint32_t top = 0u;
-      if (m < p.M) {
+      if (m < tokens) {
 #pragma unroll 4
-        for (int v = l; v < vecs; v += LANES) top = top_of<V>(load_vec<V, ALIGNED>(x + m * ldx, v, p.K), top);
+        for (int v = l; v < vecs; v += LANES) top = top_of<V>(load_vec<V, ALIGNED>(row0 + m * ldx, v, p.K), top);
       }
       if (sizeof(V) == 2) top = max(top & 0xffffu, top >> 16);
 #pragma unroll
       for (int o = 1; o < LANES; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (m < p.M) {
+      if (m < tokens) {
         float scale;
         const Factors f = factors_of<V>(top, &scale);
         if (l == 0) s->scale[m] = scale;
@@ -693,18 +697,18 @@ __global__ void __launch_bounds__(THREADS, 2)
         for (int i = l; i < count * OF_SLAB; i += LANES) place(m, i, f);
       }
     } else {
-      const int w = warp - 2, share = p.M == 1 ? 8 : p.M == 2 ? 4 : p.M <= 4 ? 2 : 1;  // warps of a row
-      for (int m = w / share; m < p.M; m += EPILOGUE / share) {
+      const int w = warp - 2, share = tokens == 1 ? 8 : tokens == 2 ? 4 : tokens <= 4 ? 2 : 1, m = w / share;  // warps of a row
+      if (m < tokens) {
         uint32_t top = 0u;
 #pragma unroll 2
         for (int v = w % share * 32 + lane; v < vecs; v += share * 32)
-          top = top_of<V>(load_vec<V, ALIGNED>(x + m * ldx, v, p.K), top);
+          top = top_of<V>(load_vec<V, ALIGNED>(row0 + m * ldx, v, p.K), top);
         if (sizeof(V) == 2) top = max(top & 0xffffu, top >> 16);
         top = __reduce_max_sync(0xffffffffu, top);
         if (lane == 0) atomicMax(&s->top[m], top);
       }
       barrier_wait<1, 32 * EPILOGUE>();
-      for (int m = w / share; m < p.M; m += EPILOGUE / share) {
+      if (m < tokens) {
         float scale;
         const Factors f = factors_of<V>(s->top[m], &scale);
         if (lane == 0) s->scale[m] = scale;
@@ -725,8 +729,10 @@ __global__ void __launch_bounds__(THREADS, 2)
   // ------------------------------------------------------------- epilogue
   const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
   if (T > 16) {
-    Params mine = p;
+    Params mine = p;  // of the tile's tokens
     mine.x_scale = s->scale;
+    mine.M = tokens;
+    mine.out = static_cast<uint8_t*>(p.out) + static_cast<int64_t>(m0) * p.N * (p.out_dtype == IRIS_F32 ? 4 : 2);
     constexpr int SHARE = T / 2;
     if (warp >= 2) store_columns(mine, lanes + half * SHARE, half * SHARE, SHARE, n, ok);
     tc_fence_before();
@@ -783,8 +789,9 @@ int launch_few_as(const CUtensorMap& tw, Params p, int splits, const void* x, in
     IRIS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, few::SMEM));
     if (dev < 64) configured[dev] = true;
   }
+  p.token_tiles = (p.M + T - 1) / T;
   p.splits = splits;
-  const int64_t ctas = static_cast<int64_t>((p.N + BN - 1) / BN) * splits;
+  const int64_t ctas = static_cast<int64_t>(p.token_tiles) * ((p.N + BN - 1) / BN) * splits;
   IRIS_REQUIRE(ctas < (1ll << 31), "gemm_i8: too many rows");
   IRIS_CUDA(launch_early(kernel, dim3(static_cast<unsigned>(ctas)), THREADS, few::SMEM, st, static_cast<unsigned>(splits), tw, p,
                          static_cast<const V*>(x), ldx));
@@ -1093,12 +1100,33 @@ Choice choose(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 
-// The tokens of few_kernel's tile that takes a call's rows; 0: none does.
+// The tokens of few_kernel's tile that takes a call's rows; 0: two launches do, `c` being the
+// product's form. us of graph replays over weights that come from memory, one launch against
+// two (rows x K -> N, bf16 unless said):
+//  - short rows: 1 x 16 -> 2560 3.0 / 3.9, 16 x 128 -> 2560 3.3 / 3.7, 128 x 40 -> 2560 3.3 / 4.4. T 32 where its
+//    tiles have an SM each, 33 x 128 -> 9000 3.6 / 4.4 (T 64 4.5); T 64, 128 x 80 -> 6848 4.6 / 5.2 (T 32 5.2, T 128
+//    6.4), 64 x 128 -> 15360 4.8 / 5.0 (T 32 5.1), -> 40000 9.5 / 8.8, 64 x 80 -> 70000 11.4 / 13.7; T 128, 128 x 80
+//    -> 15360 6.5 / 7.5 (T 64 6.6), 128 x 128 -> 15360 7.4 / 6.1, 128 x 40 -> 40000 12.6 / 13.2 (T 64 13.7), 128 x 64
+//    -> 40000 13.1 / 11.4.
+//  - K in parts: 1 x 2560 -> 2560 5.6 / 7.2, 4 x 2560 -> 2560 6.4 / 7.3, 8 x 1280 -> 2560 5.8 / 6.4; 10 KB a CTA
+//    level: fp32, 1 x 10240 -> 2560 11.8 / 11.9. Few long rows cost the rounding kernel most: fp32, 1 x 10240
+//    -> 256 8.1 / 9.2, 3 x 3000 -> 256 6.5 / 6.3, 4 x 2560 -> 2560 7.5 / 7.3.
+//  - K whole: 5 KB a CTA about level (4 x 640 -> 2560 5.6 / 5.3; fp32 5.8 / 5.2; 8 x 640 6.0 / 5.2). CTAs in
+//    turn: 4 x 640 -> 40000 13.1 / 10.4, 1 x 1280 -> 70000 18.6 / 19.4; where the product would have a
+//    deep ring, one CTA an SM, in three turns, 3 x 1280 -> 40000 17.7 / 20.6.
 inline int few_tokens(const iris_i8_problem& q, const Choice& c) {
-  if (q.x_dtype == IRIS_I8 || q.M > 128 || q.M * q.K > few::MOST_VALUES) return 0;
-  const int tokens = q.M <= 16 ? 16 : q.M <= 32 ? 32 : q.M <= 64 ? 64 : 128;
-  const int64_t slabs = (q.K + SLAB - 1) / SLAB, splits = tokens == 16 && c.tokens == 16 ? c.splits : 1;
-  return (slabs + splits - 1) / splits <= few::most_slabs(tokens) ? tokens : 0;
+  if (q.x_dtype == IRIS_I8 || q.M > few::MOST_TOKENS) return 0;
+  const int64_t row = q.K * (q.x_dtype == IRIS_F32 ? 4 : 2), wide = (q.N + BN - 1) / BN, sms = num_sms();
+  if (row <= few::SHORT_ROW) {
+    if (q.M <= 32 || (q.M + 31) / 32 * wide <= sms) return 32;
+    const int tokens = q.M <= 64 || 2 * wide <= sms ? 64 : 128;
+    const bool resident = (q.M + tokens - 1) / tokens * wide <= 2 * sms;
+    return row <= (tokens == 64 ? resident ? few::SHORT_ROW : 192 : resident ? 192 : 96) ? tokens : 0;
+  }
+  if (q.M > few::MOST_ROWS || c.tokens != 16 || (q.M - 1) * row > 20480) return 0;
+  const int64_t slabs = (q.K + SLAB - 1) / SLAB, part = q.M * row / c.splits;
+  const int64_t most = c.splits > 1 ? 10240 : q.M > 4 ? 0 : wide <= 2 * sms ? 5120 : c.deep ? 10240 : 4096;
+  return part <= most && (slabs + c.splits - 1) / c.splits <= few::most_slabs(16) ? 16 : 0;
 }
 
 inline int check_rows(int64_t M, int64_t K, int64_t ldx) {
@@ -1176,11 +1204,10 @@ extern "C" int iris_gemm_i8(const iris_i8_problem* q, void* stream) {
   if (fresh) {
     IRIS_CHECK_STATUS(check_rows(q->M, q->K, q->ldx));
     if (const int tokens = few_tokens(*q, c)) {
-      const int splits = c.tokens == 16 ? c.splits : 1;
       IRIS_CHECK_STATUS(make_tmap_2d_bytes(&tw, q->w, q->K, q->N, q->ldw, SLAB, BN));
-      return q->x_dtype == IRIS_F32    ? launch_few<float>(tw, p, tokens, splits, x, ldx, st)
-             : q->x_dtype == IRIS_BF16 ? launch_few<__nv_bfloat16>(tw, p, tokens, splits, x, ldx, st)
-                                       : launch_few<__half>(tw, p, tokens, splits, x, ldx, st);
+      return q->x_dtype == IRIS_F32    ? launch_few<float>(tw, p, tokens, c.splits, x, ldx, st)
+             : q->x_dtype == IRIS_BF16 ? launch_few<__nv_bfloat16>(tw, p, tokens, c.splits, x, ldx, st)
+                                       : launch_few<__half>(tw, p, tokens, c.splits, x, ldx, st);
     }
     IRIS_REQUIRE(q->workspace && aligned16(q->workspace) && q->workspace_bytes >= workspace_bytes(*q), "gemm_i8: workspace too small");
     ldx = row_bytes(q->K);

@@ -113,3 +113,25 @@ def test_wrappers_refuse_before_any_launch(K):
     ]:
         with pytest.raises(ValueError, match=message):
             K.gemm_i8(*args, **kw)
+
+
+def test_which_rows_the_product_rounds(lib):  # noqa: F811
+    """Calls of one launch need no workspace; where the device is done earlier with two, there are two."""
+
+    def rounds(m, n, k, dtype):
+        out, ld = ctypes.c_int64(-1), (k + 15) // 16 * 16
+        assert lib.iris_gemm_i8_workspace(product(m=m, n=n, k=k, ldx=k, ldw=ld, x_dtype=dtype), ctypes.byref(out)) == 0
+        assert out.value in (0, m * ld + (m + 3) // 4 * 16)
+        return out.value == 0
+
+    for dtype in (1, 2):  # 16 bits
+        for m, n, k in [(1, 2560, 2560), (4, 2560, 2560), (8, 2560, 1280), (1, 256, 10240), (3, 40000, 1280), (1, 40000, 16), (32, 150000, 128),
+                        (128, 2560, 128), (64, 15360, 128), (64, 70000, 80), (128, 15360, 80), (128, 70000, 40)]:  # fmt: skip
+            assert rounds(m, n, k, dtype), (m, n, k)
+        for m, n, k in [(16, 2560, 640), (8, 2560, 640), (5, 2560, 300), (64, 2560, 160), (17, 256, 600), (4, 40000, 640),
+                        (1, 150000, 1280), (128, 15360, 128), (64, 40000, 128), (128, 40000, 64), (129, 5, 16), (2, 2560, 20000)]:  # fmt: skip
+            assert not rounds(m, n, k, dtype), (m, n, k)
+    for m, n, k in [(1, 2560, 4096), (4, 6848, 1280), (32, 2560, 64), (1, 256, 10240)]:  # fp32
+        assert rounds(m, n, k, 0), (m, n, k)
+    for m, n, k in [(4, 2560, 640), (4, 256, 2560), (3, 2560, 3000), (17, 256, 128), (128, 15360, 64)]:
+        assert not rounds(m, n, k, 0), (m, n, k)

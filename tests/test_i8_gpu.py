@@ -270,3 +270,23 @@ def test_error_against_the_unquantised_product(K):
     most = dx * b.abs().sum(1) + (a.abs().sum(1, keepdim=True) + dx * 2560) * dw.T
     assert torch.all((got - a @ b.T).abs() <= 1.001 * most)
     assert HALF_STEP[torch.float32] < 0.001
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m, n", [(1, 75776 + 130), (32, 40000), (33, 2561), (33, 12000), (64, 15360), (65, 9473), (100, 19000), (128, 6848),
+                                  (128, 40000)])  # fmt: skip
+def test_short_rows_that_the_product_rounds(K, dtype, m, n):
+    """Tiles of 32, 64 and 128 tokens, several of them, against rows quantised before: bit for bit."""
+    packed, scale = K.quantize_i8(rows(n, n, 128, torch.float32, False))
+    bias = rows(m, 1, n, torch.float32)[0]
+    for k in (1, 16, 31, 48, 64, 80, 96, 128):
+        x = rows(m + k, m, k, dtype)
+        if m > 4:
+            x[0], x[1] = 0, x[1] * torch.finfo(dtype).smallest_normal * 2.0**9
+            x[2, k // 2], x[-2, 0], x[-1, -1] = math.inf, math.nan, torch.finfo(dtype).max
+        q, x_scale = K.quantize_i8(x)
+        for out_dtype in (dtype, torch.float32):
+            want = K.gemm_i8(q, packed[:, :k], scale, bias, x_scale=x_scale, out_dtype=out_dtype)
+            for view in (x, torch.cat([x[:, :1], x], dim=1)[:, 1:]):
+                got = K.gemm_i8(view, packed[:, :k], scale, bias, out_dtype=out_dtype)
+                assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(got.isnan(), want.isnan())
