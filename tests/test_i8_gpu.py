@@ -290,3 +290,62 @@ def test_short_rows_that_the_product_rounds(K, dtype, m, n):
             for view in (x, torch.cat([x[:, :1], x], dim=1)[:, 1:]):
                 got = K.gemm_i8(view, packed[:, :k], scale, bias, out_dtype=out_dtype)
                 assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(got.isnan(), want.isnan())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m, k", [(10000, 300), (9600, 512), (3000, 1300), (3000, 2560), (2500, 4096), (1500, 8192), (1500, 20011)])
+def test_rows_to_8_bits_in_several_turns(K, dtype, m, k):
+    """More rows than teams of one, four and eight warps: the next row's values are on their way under this
+    one's rounding. Rows that are not ordinary lie between the others."""
+    x = rows(m, m, k, dtype)
+    info = torch.finfo(dtype)
+    x[5::97] = 0
+    x[7::331, k // 3], x[8::331, 0], x[9::331, k - 1] = math.inf, math.nan, -math.inf
+    x[10::331, k // 2], x[11::331] = info.max, info.tiny
+    x[12::331] *= info.smallest_normal * 2.0**6
+    assert_quantized(K, x)
+    assert_quantized(K, x[:, 1:])  # rows at any value
+    assert_quantized(K, x[::2])
+
+
+@pytest.mark.parametrize("m", [1, 3, 40, 129, 300])
+def test_a_few_tokens_by_a_vocabulary(K, m):
+    """So many channels that no form gives every tile an SM's slot."""
+    for n, k in [(75777, 640), (90001, 1280), (150001, 320)]:
+        check(K, m, n, k, torch.bfloat16, bias=m % 2 == 1, seed=m)
+
+
+def test_results_past_32_bits(K):
+    m, n, k = 70001, 32768, 48
+    x, w, _ = product(70, m, n, k, torch.bfloat16, False)
+    packed, scale = K.quantize_i8(w)
+    got = K.gemm_i8(x, packed, scale)
+    assert got.numel() > 2**31
+    for first in (0, 65400, m - 300):  # element 2^31 lies in row 65536
+        assert torch.equal(got[first : first + 300], K.gemm_i8(x[first : first + 300], packed, scale))
+    assert_i8(got[m - 300 :], *quantized(x[m - 300 :]), packed, scale)
+
+
+def test_rows_and_weights_past_32_bits(K):
+    gen = torch.Generator(device="cuda").manual_seed(71)
+    m, k = 17000, 131071
+    x = torch.randn(m, k, device="cuda", generator=gen, dtype=torch.bfloat16)
+    packed, scale = K.quantize_i8(rows(72, 40, k, torch.float32, False))
+    q, x_scale = K.quantize_i8(x)
+    assert q.stride(0) * m > 2**31
+    got = K.gemm_i8(x, packed, scale)
+    assert torch.equal(got, K.gemm_i8(q, packed, scale, x_scale=x_scale, out_dtype=x.dtype))
+    for first in (0, 16300, m - 100):  # byte 2^31 of q lies in row 16384
+        want, want_scale = quantized(x[first : first + 100])
+        assert torch.equal(q[first : first + 100].double(), want) and torch.equal(x_scale[first : first + 100], want_scale)
+        assert_i8(got[first : first + 100], want, want_scale, packed, scale)
+    del x, q
+    n, k = 140000, 16384
+    w = torch.randint(-127, 128, (n, k), device="cuda", generator=gen, dtype=torch.int8)
+    scale = torch.rand(n, device="cuda", generator=gen) + 0.5
+    for m in (1, 20, 300):
+        x = rows(m, m, k)
+        got = K.gemm_i8(x, w, scale)
+        want = quantized(x)
+        for first in (0, 131000, n - 100):  # byte 2^31 of w lies in row 131072
+            assert_i8(got[:, first : first + 100], *want, w[first : first + 100], scale[first : first + 100])
