@@ -79,7 +79,8 @@ IRIS_DEVICE uint64_t global_timer_ns() {
 // A kernel launched with launch_early (iris_abi_internal.h) may start while the one
 // before it in the stream ends: it touches global memory only after grid_wait
 // (that kernel complete and its writes visible; no wait where it was launched
-// otherwise), and lets its own successor start with grid_trigger, after its wait. A CTA that
+// otherwise; the one exception is a kernel whose predecessor is of the same call and has itself
+// waited before it triggers: all that lay before that one is complete, i8.cu), and lets its own successor start with grid_trigger, after its wait. A CTA that
 // needs TMEM triggers (its allocating warp alone) once it holds it: an allocation waits without a
 // limit, and a successor that takes TMEM before its own wait would hold it until this kernel ends.
 // What it reads may have been written while it already ran: no __ldg or ld.global.nc in

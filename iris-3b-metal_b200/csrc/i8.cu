@@ -26,7 +26,7 @@ namespace i8 {
 //    is y's unless it lies within 2^-15 of a half h; then 254 x is compared with 2 h max,
 //    both exact in 64 bits.
 //
-// Measured, bf16: 16384 rows of 8192 92 us (4.4 TB/s; 110 without the next row's loads under this
+// Measured, bf16: 16384 rows of 8192 92 to 94 us (4.4 TB/s; 110 without the next row's loads under this
 // one's rounding, 170 with halves looked at again), 2400 of 2560 5.2, 8 of 2560 1.8.
 struct QuantizeParams {
   const void* x;
@@ -172,6 +172,8 @@ template <typename T, int WARPS, bool ALIGNED>
 __global__ void __launch_bounds__(WARPS == 1 ? 128 : WARPS * 32, WARPS == 8 ? 4 : 8) quantize_kernel(const QuantizeParams p) {
   constexpr int TEAM = WARPS * 32, N = Vec<T>::N;
   __shared__ uint32_t tops[2][WARPS];
+  // in this order: the product behind this kernel copies weights before its own wait (Params::early),
+  // which are there because every CTA here has waited for what may have written them
   grid_wait();
   grid_trigger();
   const int t = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
@@ -245,12 +247,12 @@ int quantize(const QuantizeParams& p, cudaStream_t st) {
 // tensor cores' first operand, whatever the number of tokens, so that few tokens waste
 // none of it and the lanes of a warp write neighbouring channels of out, at any N.
 //
-// Measured, us, rows in bf16 and their rounding included (tokens, K -> N): 1, 2560 -> 2560 5.6
-// (launch, the cluster's exchange and two round trips to memory); 64, 8192 -> 32768 51 (5.3
-// TB/s of weights, 0.81 of a plain copy); 2400, 2560 -> 6848 42 (2.0 POP/s: 270 tiles are 3.65
-// waves of 74 pairs, and 6 us start and end them); 4096, 8192 -> 8192 191; 16384, 8192 -> 8192
-// 780, of which the product 680 (3.2 POP/s, twice the bf16 rate that a library reaches here;
-// tensor pipe 82% busy at 4096 tokens).
+// Measured in graph replays, us, rows in bf16 and their rounding included (tokens, K -> N): 1, 2560 ->
+// 2560 5.5 (the product alone 4.5; x is read twice, a barrier between, then the cluster's exchange);
+// 64, 8192 -> 32768 51.5 (5.3 TB/s of weights, 0.81 of a plain copy; 53 among other work); 2400, 2560 ->
+// 6848 42 (2.0 POP/s: 270 tiles are 3.65 waves of 74 pairs, and 6 us start and end them); 4096, 8192 ->
+// 8192 193, 174 of them the product (tensor pipe 82% busy); 16384, 8192 -> 8192 770 to 780 in short
+// runs, the product 680 to 725 (2.9 to 3.2 POP/s), 843 in long ones under the power cap.
 constexpr int BN = 128, SLAB = 128;  // weight rows of a CTA, k of a ring slot (bytes)
 constexpr int EPILOGUE = 8;  // warps: two for each quarter of the TMEM lanes, half of the tokens each
 constexpr int THREADS = 64 + 32 * EPILOGUE;
@@ -263,7 +265,7 @@ struct Params {
   int M, N, K, out_dtype;
   int splits;         // parts of K, the CTAs of a cluster
   int token_tiles;
-  int early;          // the weights are there before the kernel's predecessor ends
+  int early;          // the predecessor is this call's quantize_kernel: the weights are there before it ends
 };
 
 __host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {

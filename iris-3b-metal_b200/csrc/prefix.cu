@@ -10,11 +10,11 @@
 // maxima and totals. Prompts, whose rows fill tiles by themselves, see all keys in one pass; few
 // rows over a short prefix take all keys by step_cta. make_plan chooses.
 //
-// Measured, 128 wide, us: one token of 4 samples behind 300 tokens, 20 over 5 heads 4.9; of 32
-// behind 2048 with up to 512 of their own, 32 over 8 heads 16.5; of 64 behind 32768 with 1024
-// 80 (402 MB, 5.0 TB/s, 0.77 of a plain copy: the tiles' start, the uneven end and the join take
-// the rest); 8 prompts of 300 behind 4096 113 (0.92 PFLOP/s); 2 x 1024 rows of 24 heads behind
-// 16384 392 (1.12 PFLOP/s; 476 in long runs under the power cap).
+// Measured in graph replays, 128 wide, caches full, us: one token of 4 samples behind 300 tokens, 20
+// over 5 heads 4.9; of 32 behind 2048 with 512 of their own, 32 over 8 heads 16.4; of 64 behind 32768
+// with 1024 80 (402 MB, 5.0 TB/s, 0.77 of a plain copy: the tiles' start, the uneven end and the join
+// take the rest); 8 prompts of 300 behind 4096 113 (0.92 PFLOP/s; 131, 0.79, in long runs under the
+// power cap); 2 x 1024 rows of 24 heads behind 16384 392 to 403 (1.1 PFLOP/s; 476, 0.92, in long runs).
 #include <math.h>
 
 #include <algorithm>
@@ -897,6 +897,9 @@ __global__ void __launch_bounds__(STEP_WARPS * 32) step_kernel(const __grid_cons
 // Both kinds of CTA in one launch, the longer ones first: tiles are bound by the tensor cores
 // and exponentials, the others by memory, and they share the SMs (mixed evenly, tiles that
 // started late ended last: 64 samples behind 32768 tokens 111 us).
+//
+// 128 registers a thread hold both kinds of CTA but for 16 rows of 128 columns (NQ 2), where the compiler
+// spills 140 bytes; that instance also runs where there are tiles alone.
 template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(BOUND_THREADS, 2)
     attend_kernel(const __grid_constant__ CUtensorMap tpk, const __grid_constant__ CUtensorMap tpv,
@@ -986,7 +989,9 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Param
 }
 
 // How a call is cut up, from its sizes alone (lengths are on the device: n_prefix and
-// n_kv bound them). Three forms, and the one whose estimate is least:
+// n_kv bound them, and are taken for them: caches with much room to spare are cut as if they were
+// full, one token of 32 samples behind 2048 with 256 of their own 15.9 us in a room of 256, 32.8 in
+// 2048, 166 in 8192). Three forms, and the one whose estimate is least:
 //  - joint: row tiles of a sample see all of its keys (step_kernel); few rows or short prefixes;
 //  - shared: a group's rows see the prefix by tiles, row tiles their own keys;
 //  - whole: a sample's rows see all keys by tiles; prompts.

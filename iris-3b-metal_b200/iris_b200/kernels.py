@@ -633,7 +633,8 @@ def prefix_attention(
     N_kv]``; default ``N_kv``) and ``j <= starts[b] + i + right`` (``starts``: int32 ``[B]``, places in
     ``k``, not counting the prefix; default ``N_kv - N``, ``lengths`` or not). ``right=None`` is no
     bound, the default is causal. A query that sees no key gives 0. Other keys' rows may hold
-    anything. ``P + N_kv`` is below ``2^30``. Heads, groups and samples may be expanded, tokens
+    anything, but the work is cut up by ``P`` and ``N_kv``: of caches with much room to spare pass the
+    filled part (``k[:, :, :longest]``). ``P + N_kv`` is below ``2^30``. Heads, groups and samples may be expanded, tokens
     not. ``out`` shares no memory with the inputs, or is ``q``'s own rows."""
     return (_lib._text_side or _lib.text_side()).prefix_attention(
         q, prefix_k, prefix_v, k, v, prefix_lengths, starts, lengths, right, scale, out
